@@ -581,6 +581,80 @@ int ti_opt_decoder_layers_decode(const TiOptDecodeLayer* const* layers, int64_t 
                                  int8_t* const* k_bufs, int8_t* const* v_bufs, int64_t B, int64_t cap, int64_t S, float* carry,
                                  void* scratch, int64_t scratch_bytes, void* stream);
 
+/* ---- A KV cache in pages: sequences of any lengths in one batch, no padding and no mask. ----
+ * No counterpart in the reference, whose caches are one growing tensor per batch (torch_int/models/opt.py:128-133).
+ *
+ * The pool: `pages` pages of `page_size` positions (a power of two, 16 or more) for each of `heads` key/value heads of
+ * `head_dim` int8 values (a multiple of 16 up to 128; the innermost dimension contiguous).  Strides are bytes, multiples of
+ * 16 that do not overlap; k and v are 16-byte aligned.  [pages, heads, page_size, head_dim] and [pages, page_size, heads,
+ * head_dim] are both such pools. */
+typedef struct {
+  int8_t *k, *v;
+  int64_t pages, page_size, heads, head_dim;
+  int64_t k_page, k_head, k_token;
+  int64_t v_page, v_head, v_token;
+} TiPagedCache;
+
+/* The batch, device arrays of int32 that are read when the kernel runs: `cu_new` [seqs + 1] holds where each sequence's new
+ * tokens begin among the `rows` rows (ascending, from 0; the last entry is their end, rows behind it belong to nobody),
+ * `context_lens` [seqs] how many positions each sequence has, its new tokens counted, and `block_table` [seqs,
+ * pages_per_seq] its pages, of which only those that hold a position are read.  New token i of T is at position
+ * context_len - T + i.  Whatever the arrays hold, nothing outside the tensors is accessed: lengths are cut off at
+ * pages_per_seq * page_size, rows at `rows`; nothing is written to a page that the pool does not have, its keys take no
+ * part in an attention, and a new token at a negative position is not appended and sees no key. */
+typedef struct {
+  const int32_t *block_table, *context_lens, *cu_new;
+  int64_t pages_per_seq, seqs, rows;
+} TiPagedBatch;
+
+#define TI_TYPE_F32 0
+#define TI_TYPE_F16 1
+#define TI_TYPE_BF16 2
+#define TI_TYPE_S8 3
+
+/* Appends the new tokens' keys and values [rows, heads, head_dim] to their pages:
+ *   cache = s8(rint(clamp(alpha * y, -128, 127))), y = x or x rotated; NaN -> 0; round-half-to-even of the fp64 result.
+ * `type` (TI_TYPE_*) is that of key, value and query; row and head strides count elements, rows begin at multiples of 16
+ * bytes.  With `cos_sin` fp32 [positions, rot] (rot a multiple of 16 up to head_dim; cosines, then sines) the first rot
+ * elements of a key are rotated by their position: pairs (j, j + rot/2), or with `neighbours` (2j, 2j + 1), become
+ * (x1 c - x2 s, x2 c + x1 s).  A token whose position the table does not reach is not appended.  `query` [rows,
+ * q_heads, head_dim], if given, is rotated and quantised the same way into `q_out`, packed; its rows that are not appended
+ * become zeros, rows of no sequence only with `fill`.  Two tokens of a batch that share a slot of the pool leave one of the
+ * two, in pieces, in it. */
+typedef struct {
+  const void *key, *value, *query;
+  int64_t k_row, k_head, v_row, v_head, q_row, q_head;
+  int8_t* q_out;
+  int64_t q_heads;
+  const float* cos_sin;
+  int64_t rot, positions;
+  int32_t type, neighbours, fill;
+  float alpha_q, alpha_k, alpha_v;
+} TiPagedAppend;
+int ti_paged_kv_append_s8(const TiPagedCache* cache, const TiPagedBatch* batch, const TiPagedAppend* what, void* stream);
+
+/* Attention of the new tokens over their sequences' pages, each token over the positions up to its own:
+ *   out[row, h] = alpha_pv * sum_j w_j v_j,  w = softmax(alpha_qk * q . k_j),  0 where there is no position.
+ * q int8 [rows, q_heads, head_dim] with row and head strides in bytes, multiples of 16; q_heads a multiple of the cache's
+ * heads, q head h reads key head h / (q_heads / heads).  out [rows, q_heads, head_dim] packed, of `out_type`: TI_TYPE_S8
+ * (rint, clamp to [-128, 127]), TI_TYPE_F16 or TI_TYPE_BF16.  Rows of no sequence become zeros with `fill` and stay as they
+ * are without.  alpha_qk in [1e-30, 0.25] (scores reach 2^21 alpha_qk).  Probabilities are not quantised to int8 (the whole-cache attentions above do
+ * that): a row's largest counts 2^8 to 2^15 in fp16, and where little else bounds the kernel they have 22 bits.
+ * `workspace` (16-byte aligned, private to the stream, contents irrelevant) of ti_paged_attn_workspace_bytes lets long
+ * sequences be cut into slices; with less, or NULL, each is read by one workgroup.  `capacity` there: pages_per_seq *
+ * page_size. */
+typedef struct {
+  const int8_t* q;
+  int64_t q_row, q_head, q_heads;
+  void* out;
+  int32_t out_type, fill;
+  float alpha_qk, alpha_pv;
+} TiPagedAttn;
+int64_t ti_paged_attn_workspace_bytes(int64_t rows, int64_t seqs, int64_t q_heads, int64_t heads, int64_t head_dim,
+                                      int64_t capacity);
+int ti_paged_attn_s8(const TiPagedCache* cache, const TiPagedBatch* batch, const TiPagedAttn* what, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -301,6 +301,64 @@ static PyObject* fc_plan_current(PyObject* self, PyObject* const* a, Py_ssize_t 
   Py_RETURN_TRUE;
 }
 
+/* The cache and the batch that both calls begin with: k, v, pages, page_size, heads, head_dim, k strides (page, head, token),
+ * v strides, block_table, context_lens, cu_new, pages_per_seq, seqs, rows */
+enum { PAGED_ARGS = 18 };
+static void paged_args(PyObject* const* a, TiPagedCache* c, TiPagedBatch* b) {
+  c->k = as_ptr(a[0]), c->v = as_ptr(a[1]);
+  c->pages = as_i64(a[2]), c->page_size = as_i64(a[3]), c->heads = as_i64(a[4]), c->head_dim = as_i64(a[5]);
+  c->k_page = as_i64(a[6]), c->k_head = as_i64(a[7]), c->k_token = as_i64(a[8]);
+  c->v_page = as_i64(a[9]), c->v_head = as_i64(a[10]), c->v_token = as_i64(a[11]);
+  b->block_table = as_ptr(a[12]), b->context_lens = as_ptr(a[13]), b->cu_new = as_ptr(a[14]);
+  b->pages_per_seq = as_i64(a[15]), b->seqs = as_i64(a[16]), b->rows = as_i64(a[17]);
+}
+
+/* paged_append(..., key, value, query, k_row, k_head, v_row, v_head, q_row, q_head, q_out, q_heads, cos_sin, rot, positions, type,
+ * neighbours, fill, alpha_q, alpha_k, alpha_v, stream) -> status */
+static PyObject* fc_paged_append(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (n != PAGED_ARGS + 21) {
+    PyErr_SetString(PyExc_TypeError, "paged_append expects 39 arguments");
+    return NULL;
+  }
+  TiPagedCache c;
+  TiPagedBatch b;
+  TiPagedAppend w;
+  paged_args(a, &c, &b);
+  a += PAGED_ARGS;
+  w.key = as_ptr(a[0]), w.value = as_ptr(a[1]), w.query = as_ptr(a[2]);
+  w.k_row = as_i64(a[3]), w.k_head = as_i64(a[4]), w.v_row = as_i64(a[5]), w.v_head = as_i64(a[6]);
+  w.q_row = as_i64(a[7]), w.q_head = as_i64(a[8]);
+  w.q_out = as_ptr(a[9]), w.q_heads = as_i64(a[10]), w.cos_sin = as_ptr(a[11]), w.rot = as_i64(a[12]), w.positions = as_i64(a[13]);
+  w.type = (int32_t)as_i64(a[14]), w.neighbours = (int32_t)as_i64(a[15]), w.fill = (int32_t)as_i64(a[16]);
+  w.alpha_q = as_f32(a[17]), w.alpha_k = as_f32(a[18]), w.alpha_v = as_f32(a[19]);
+  void* st = as_ptr(a[20]);
+  if (PyErr_Occurred()) return NULL;
+  return PyLong_FromLong(ti_paged_kv_append_s8(&c, &b, &w, st));
+}
+
+/* paged_attn(..., q, q_row, q_head, q_heads, out, out_type, fill, alpha_qk, alpha_pv, ws, ws_bytes, stream) -> status */
+static PyObject* fc_paged_attn(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (n != PAGED_ARGS + 12) {
+    PyErr_SetString(PyExc_TypeError, "paged_attn expects 30 arguments");
+    return NULL;
+  }
+  TiPagedCache c;
+  TiPagedBatch b;
+  TiPagedAttn w;
+  paged_args(a, &c, &b);
+  a += PAGED_ARGS;
+  w.q = as_ptr(a[0]), w.q_row = as_i64(a[1]), w.q_head = as_i64(a[2]), w.q_heads = as_i64(a[3]);
+  w.out = as_ptr(a[4]), w.out_type = (int32_t)as_i64(a[5]), w.fill = (int32_t)as_i64(a[6]);
+  w.alpha_qk = as_f32(a[7]), w.alpha_pv = as_f32(a[8]);
+  void* ws = as_ptr(a[9]);
+  int64_t wsb = as_i64(a[10]);
+  void* st = as_ptr(a[11]);
+  if (PyErr_Occurred()) return NULL;
+  return PyLong_FromLong(ti_paged_attn_s8(&c, &b, &w, ws, wsb, st));
+}
+
 static PyObject* fc_last_error(PyObject* self, PyObject* noargs) {
   (void)self;
   (void)noargs;
@@ -320,6 +378,8 @@ static PyMethodDef methods[] = {
     {"decode_attn", (PyCFunction)(void (*)(void))fc_decode_attn, METH_FASTCALL, "forward to ti_decode_attn_s8"},
     {"opt_layer_decode", (PyCFunction)(void (*)(void))fc_opt_layer_decode, METH_FASTCALL, "forward to ti_opt_decoder_layer_decode_from"},
     {"opt_layer_prefill", (PyCFunction)(void (*)(void))fc_opt_layer_prefill, METH_FASTCALL, "forward to ti_opt_decoder_layer_prefill_chained"},
+    {"paged_append", (PyCFunction)(void (*)(void))fc_paged_append, METH_FASTCALL, "forward to ti_paged_kv_append_s8"},
+    {"paged_attn", (PyCFunction)(void (*)(void))fc_paged_attn, METH_FASTCALL, "forward to ti_paged_attn_s8"},
     {"plan_current", (PyCFunction)(void (*)(void))fc_plan_current, METH_FASTCALL, "tensors and hooks as a plan found them"},
     {"last_error", fc_last_error, METH_NOARGS, "ti_last_error()"},
     {NULL, NULL, 0, NULL}};

@@ -1,1 +1,1 @@
-from . import bmm, fused, quantization  # noqa: F401
+from . import bmm, fused, paged, quantization  # noqa: F401
