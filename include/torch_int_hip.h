@@ -642,14 +642,19 @@ int ti_paged_kv_append_s8(const TiPagedCache* cache, const TiPagedBatch* batch, 
  * that): a row's largest counts 2^8 to 2^15 in fp16, and where little else bounds the kernel they have 22 bits.
  * `workspace` (16-byte aligned, private to the stream, contents irrelevant) of ti_paged_attn_workspace_bytes lets long
  * sequences be cut into slices; with less, or NULL, each is read by one workgroup.  `capacity` there: pages_per_seq *
- * page_size. */
+ * page_size.  The slices meet in the same launch where `arrivals` gives ti_paged_attn_arrivals (same arguments) int32
+ * counters, zero before the first call and again after every one, that no call on another stream and no other recorded graph
+ * uses; without them a second launch joins the slices.  Same bits. */
 typedef struct {
   const int8_t* q;
   int64_t q_row, q_head, q_heads;
   void* out;
   int32_t out_type, fill;
   float alpha_qk, alpha_pv;
+  int32_t* arrivals;
+  int64_t arrivals_count;
 } TiPagedAttn;
+int64_t ti_paged_attn_arrivals(int64_t rows, int64_t seqs, int64_t q_heads, int64_t heads, int64_t head_dim, int64_t capacity);
 int64_t ti_paged_attn_workspace_bytes(int64_t rows, int64_t seqs, int64_t q_heads, int64_t heads, int64_t head_dim,
                                       int64_t capacity);
 int ti_paged_attn_s8(const TiPagedCache* cache, const TiPagedBatch* batch, const TiPagedAttn* what, void* workspace,

@@ -304,6 +304,36 @@ def test_the_same_inputs_give_the_same_bits_on_any_stream():
     assert all(torch.equal(x, first) for x in got)
 
 
+@pytest.mark.parametrize("hq,hk,d,lens,new", [(1, 1, 128, [70000], [1]), (8, 1, 64, [9000, 2, 700], [1, 1, 1]), (4, 2, 80, [3000, 2900], [9, 1]),
+                                              (32, 2, 128, [5000, 40, 6001], [1, 1, 2]), (12, 12, 64, [1025], [1])])
+def test_slices_that_meet_in_the_launch_or_behind_it(hq, hk, d, lens, new, monkeypatch):
+    # the same bits with the counters, without them (a second launch), again and again, and after calls whose tables hold
+    # nonsense: the counters are zero behind every call; against fp64 as well
+    P = _paged()
+    g = torch.Generator().manual_seed(41 + hq)
+    cu, lens, table, pages, rows = _batch(g, lens, new, 16)
+    k, v = (_s8(g, pages, hk, 16, d, spread=30).to(DEV) for _ in range(2))
+    q = _s8(g, rows, hq, d, spread=30)
+    a_qk = 2.0 / (900 * d ** 0.5)
+    first = _attend(("meet", hq, hk, d), q, k, v, table, lens, cu, a_qk, 0.02, FP16_WEIGHTS, out_dtype=torch.float16).to(DEV)
+    args = (q.to(DEV), k, v, table.to(DEV), lens.to(DEV), cu.to(DEV), a_qk, 0.02)
+    assert len(P._counters) > 0
+    for i in range(60):
+        got = P.paged_attn_s8(*args, out_dtype=torch.float16)
+        assert torch.equal(got, first), i
+    for bad in ([0] + [rows, 0] * len(lens), [-7, 2 ** 31 - 1] * len(lens)):
+        bad_cu = torch.tensor(bad[: len(lens) + 1], dtype=torch.int32, device=DEV)
+        P.paged_attn_s8(args[0], k, v, args[3], torch.full_like(args[4], 2 ** 31 - 1), bad_cu, a_qk, 0.02)
+        assert all(int(t.abs().max()) == 0 for t in P._counters.values())
+        assert torch.equal(P.paged_attn_s8(*args, out_dtype=torch.float16), first)
+    monkeypatch.setattr(P, "_arrivals", lambda *a: (None, 0))
+    assert torch.equal(P.paged_attn_s8(*args, out_dtype=torch.float16), first)
+    monkeypatch.setattr(P._CUDA, "_workspace", lambda *a: (None, 0, 0))     # nothing is cut
+    got = P.paged_attn_s8(*args, out_dtype=torch.float16).cpu()
+    want, size, most = orc.attention(q, k.cpu(), v.cpu(), table, lens, cu, a_qk, 0.02)
+    assert orc.attention_error(got, want, size, most, int(lens.max()), FP16_WEIGHTS) <= 1.0
+
+
 def test_recorded_steps_read_the_batch_when_they_replay():
     g = torch.Generator().manual_seed(37)
     seqs, per, page, hq, hk, d = 3, 100, 16, 8, 2, 128

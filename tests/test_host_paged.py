@@ -30,7 +30,7 @@ def test_pools_that_are_refused(field, value, word):
     P, lib = _lib()
     c, b = _good()
     setattr(c, field, value)
-    w = P._Attn(4096, 128, 64, 2, 4096, 3, 1, 1e-3, 1.0)
+    w = P._Attn(4096, 128, 64, 2, 4096, 3, 1, 1e-3, 1.0, None, 0)
     assert lib.ti_paged_attn_s8(c, b, w, None, 0, None) in (1, 2) and word in lib.ti_last_error()
     a = P._Append(4096, 4096, None, 128, 64, 128, 64, 0, 0, None, 0, None, 0, 0, 0, 0, 0, 1.0, 1.0, 1.0)
     assert lib.ti_paged_kv_append_s8(c, b, a, None) in (1, 2) and word in lib.ti_last_error()
@@ -43,7 +43,7 @@ def test_batches_that_are_refused(field, value, word):
     P, lib = _lib()
     c, b = _good()
     setattr(b, field, value)
-    w = P._Attn(4096, 128, 64, 2, 4096, 3, 1, 1e-3, 1.0)
+    w = P._Attn(4096, 128, 64, 2, 4096, 3, 1, 1e-3, 1.0, None, 0)
     assert lib.ti_paged_attn_s8(c, b, w, None, 0, None) in (1, 2) and word in lib.ti_last_error()
 
 
@@ -55,10 +55,10 @@ def test_batches_that_are_refused(field, value, word):
 def test_attention_that_is_refused(field, value, word):
     P, lib = _lib()
     c, b = _good()
-    w = P._Attn(4096, 128, 64, 2, 4096, 3, 1, 1e-3, 1.0)
+    w = P._Attn(4096, 128, 64, 2, 4096, 3, 1, 1e-3, 1.0, None, 0)
     setattr(w, field, value)
     assert lib.ti_paged_attn_s8(c, b, w, None, 0, None) in (1, 2) and word in lib.ti_last_error()
-    w = P._Attn(4096, 128, 64, 2, 4096, 3, 1, 1e-3, 1.0)
+    w = P._Attn(4096, 128, 64, 2, 4096, 3, 1, 1e-3, 1.0, None, 0)
     assert lib.ti_paged_attn_s8(c, b, w, 4100, 64, None) == 2 and lib.ti_paged_attn_s8(c, b, w, None, -1, None) == 1
     assert lib.ti_paged_attn_s8(None, b, w, None, 0, None) == 1 and lib.ti_paged_attn_s8(c, b, None, None, 0, None) == 1
 

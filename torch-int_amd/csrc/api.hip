@@ -1235,6 +1235,11 @@ int ti_paged_kv_append_s8(const TiPagedCache* cache, const TiPagedBatch* batch, 
   return launch_paged_kv_append_s8(w->type, a, c, b, static_cast<hipStream_t>(stream));
 }
 
+int64_t ti_paged_attn_arrivals(int64_t rows, int64_t seqs, int64_t q_heads, int64_t heads, int64_t head_dim, int64_t capacity) {
+  if (ti_paged_attn_workspace_bytes(rows, seqs, q_heads, heads, head_dim, capacity) == 0) return 0;
+  return paged_attn_arrivals(rows, seqs, q_heads, heads, capacity);
+}
+
 int64_t ti_paged_attn_workspace_bytes(int64_t rows, int64_t seqs, int64_t q_heads, int64_t heads, int64_t head_dim,
                                       int64_t capacity) {
   if (rows <= 0 || rows > (1 << 23) || seqs <= 0 || seqs > (1 << 20) || heads <= 0 || heads > 4096 || q_heads <= 0 ||
@@ -1264,9 +1269,14 @@ int ti_paged_attn_s8(const TiPagedCache* cache, const TiPagedBatch* batch, const
   if (int rc = check_rows(op, "q", w->q, w->q_row, w->q_head, 1)) return rc;
   if (int rc = check_ptr(op, "out", w->out, 16, true)) return rc;
   if (int rc = check_ptr(op, "workspace", workspace, 16, workspace != nullptr)) return rc;
+  if (int rc = check_ptr(op, "arrivals", w->arrivals, 4, w->arrivals != nullptr)) return rc;
+  if (b.rows * (w->q_heads / c.heads) > (1 << 30))
+    return fail(TI_ERR_INVALID_ARG, "%s: %d rows of %lld heads to a key head (at most 2^30 in all)", op, b.rows,
+                (long long)(w->q_heads / c.heads));
   PagedAttn a;
   a.q = w->q, a.q_row = w->q_row, a.q_head = w->q_head, a.q_heads = (int)w->q_heads, a.out = w->out;
   a.alpha_qk = w->alpha_qk, a.alpha_pv = w->alpha_pv, a.fill = w->fill != 0;
+  a.arrivals = w->arrivals, a.arrivals_count = w->arrivals_count;
   return launch_paged_attn_s8(w->out_type, a, c, b, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 

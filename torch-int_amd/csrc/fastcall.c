@@ -337,11 +337,12 @@ static PyObject* fc_paged_append(PyObject* self, PyObject* const* a, Py_ssize_t 
   return PyLong_FromLong(ti_paged_kv_append_s8(&c, &b, &w, st));
 }
 
-/* paged_attn(..., q, q_row, q_head, q_heads, out, out_type, fill, alpha_qk, alpha_pv, ws, ws_bytes, stream) -> status */
+/* paged_attn(..., q, q_row, q_head, q_heads, out, out_type, fill, alpha_qk, alpha_pv, arrivals, arrivals_count, ws, ws_bytes,
+ * stream) -> status */
 static PyObject* fc_paged_attn(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   (void)self;
-  if (n != PAGED_ARGS + 12) {
-    PyErr_SetString(PyExc_TypeError, "paged_attn expects 30 arguments");
+  if (n != PAGED_ARGS + 14) {
+    PyErr_SetString(PyExc_TypeError, "paged_attn expects 32 arguments");
     return NULL;
   }
   TiPagedCache c;
@@ -352,9 +353,10 @@ static PyObject* fc_paged_attn(PyObject* self, PyObject* const* a, Py_ssize_t n)
   w.q = as_ptr(a[0]), w.q_row = as_i64(a[1]), w.q_head = as_i64(a[2]), w.q_heads = as_i64(a[3]);
   w.out = as_ptr(a[4]), w.out_type = (int32_t)as_i64(a[5]), w.fill = (int32_t)as_i64(a[6]);
   w.alpha_qk = as_f32(a[7]), w.alpha_pv = as_f32(a[8]);
-  void* ws = as_ptr(a[9]);
-  int64_t wsb = as_i64(a[10]);
-  void* st = as_ptr(a[11]);
+  w.arrivals = as_ptr(a[9]), w.arrivals_count = as_i64(a[10]);
+  void* ws = as_ptr(a[11]);
+  int64_t wsb = as_i64(a[12]);
+  void* st = as_ptr(a[13]);
   if (PyErr_Occurred()) return NULL;
   return PyLong_FromLong(ti_paged_attn_s8(&c, &b, &w, ws, wsb, st));
 }

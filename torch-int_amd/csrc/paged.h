@@ -61,7 +61,10 @@ struct PagedAttn {
   void* out;  // [rows, q_heads, D] packed
   float alpha_qk, alpha_pv;
   bool fill;  // rows of no sequence become zeros
+  int* arrivals;  // zeros, kept for the stream, or null
+  long long arrivals_count;
 };
+long long paged_attn_arrivals(long long rows, long long seqs, long long q_heads, long long kv_heads, long long capacity);
 long long paged_attn_workspace_bytes(long long rows, long long seqs, long long q_heads, long long kv_heads, long long D,
                                      long long capacity);
 int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, const PagedBatch& b, void* workspace,

@@ -18,16 +18,23 @@ namespace ti {
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
-constexpr int PA_WAVES = 8;
+constexpr int PA_WAVES = 4;
 constexpr int PA_ROWS = 16;
-constexpr int PA_TARGET = 1024;    // work items that the keys are cut into, beyond one to each (sequence, key head, 16 rows)
-constexpr int PA_MIN_SLICE = 512;  // keys of a slice, at least
+#ifndef PA_TARGET_N
+#define PA_TARGET_N 1024
+#endif
+constexpr int PA_TARGET = PA_TARGET_N;    // work items that the keys are cut into, beyond one to each (sequence, key head, 16 rows)
+#ifndef PA_MIN_N
+#define PA_MIN_N 256
+#endif
+constexpr int PA_MIN_SLICE = PA_MIN_N;  // keys of a slice, at least
 constexpr float PA_EMPTY = 3.0e38f;  // offset of a row that has seen no key: 2^(-inf + PA_EMPTY) is 0
 
 struct PagedPlan {
   int group;      // query heads of a key head
-  int target;     // slices beyond which nothing is cut; 0: nothing is cut at all
+  int target;     // slices that the keys are cut into; 0: nothing is cut
   int slots;      // items the workspace holds
+  int* arrivals;  // [slots] zeros, or null: a second launch joins the slices
 };
 
 struct PagedItem {
@@ -38,10 +45,36 @@ struct PagedItem {
   bool found;
 };
 
-__device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v = v + __shfl_xor(v, off, 64);
-  return v;
+// Running sum over the lanes of a wave, in six steps through DPP: within rows of 16, then from row to row.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+// The sum of all lanes, in every lane.
+__device__ __forceinline__ float wave_add(float x) {
+  auto step = [&](auto ctrl, auto rows) {
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  step(std::integral_constant<int, 0x111>(), std::integral_constant<int, 0xf>());
+  step(std::integral_constant<int, 0x112>(), std::integral_constant<int, 0xf>());
+  step(std::integral_constant<int, 0x114>(), std::integral_constant<int, 0xf>());
+  step(std::integral_constant<int, 0x118>(), std::integral_constant<int, 0xf>());
+  step(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());
+  step(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
+// The largest of the four lanes n, n + 16, n + 32, n + 48, in all of them.
+__device__ __forceinline__ float rows_max(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __builtin_fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __builtin_fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 // Keys of a slice, the same in every workgroup: what cuts all keys of the batch into `target` equal parts.
@@ -77,14 +110,11 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
       s = paged_seq(b, page_shift, i0 + lane);
       tiles = (s.T * p.group + rows_per_tile - 1) / rows_per_tile;
       splits = s.len <= it.slice ? 1 : (s.len + it.slice - 1) / it.slice;
-      n = tiles * splits * heads;
+      // a cu_new that descends can count rows many times over: no sum of items passes the range of int
+      const long long all = (long long)tiles * splits * heads;
+      n = all > 0x800000 ? 0x800000 : (int)all;
     }
-    int upto = n;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(upto, off, 64);
-      if (lane >= off) upto += o;
-    }
+    const int upto = wave_scan(n);
     const unsigned long long past = __ballot(before + upto > index);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
@@ -102,11 +132,13 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
       it.tile = rest / heads;
       it.head = rest - it.tile * heads;
       it.first = first + rest;
-      // cu_new that does not ascend can count rows twice, and with them items past the range of int: no item then
-      it.found = first >= 0 && rel >= 0 && it.split < it.splits && it.tile < t;
+      // all slices have a slot and a workgroup, or (as a cu_new that descends can have it) the item is left out
+      it.found = it.split < it.splits && it.tile < t &&
+                 (it.splits == 1 || it.first + (long long)(it.splits - 1) * it.step < p.slots);
       return it;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
+    before = before > 0x20000000 ? 0x20000000 : before;
   }
   return it;
 }
@@ -148,9 +180,87 @@ __device__ __forceinline__ void store4(void* out, long long at, const float (&y)
   }
 }
 
-// Workspace: partial sums [slots][16][DP] fp32, then offsets [slots][16] and denominators [slots][16].
+// Two floats written, or read, past the caches of the XCD: partial results that another XCD's workgroup joins.
+__device__ __forceinline__ void put2(float* p, float x, float y) {
+  const unsigned long long w = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float* p) {
+  const unsigned long long w =
+      __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32)));
+}
+
+// A row's partial sums y relative to the offset `off`, with their denominator, and how two of them add up.
+struct PagedPart {
+  float off, den, y[4];
+  __device__ __forceinline__ void add(float o, float d, const float (&x)[4]) {
+    const float least = o < off ? o : off;
+    const float mine = __builtin_amdgcn_exp2f(least - off), theirs = __builtin_amdgcn_exp2f(least - o);
+    off = least;
+    den = den * mine + d * theirs;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = y[i] * mine + x[i] * theirs;
+  }
+};
+
+// The slices of one item, by the threads of one workgroup: a thread owns four columns of a row in every so many-th slice.
+constexpr int PA_THREADS = PA_WAVES * 64;
 template <int DP, int OUT>
-__global__ __launch_bounds__(PA_WAVES * 64) void paged_attn_rows_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p,
+__device__ __forceinline__ void join_slices(const PagedAttn& a, const PagedCache& c, const PagedPlan& p, const PagedItem& it,
+                                            const float* ws, float* meet) {
+  const int G = p.group;
+  int rows = it.s.T * G - it.tile * PA_ROWS;
+  rows = rows < PA_ROWS ? rows : PA_ROWS;
+  const int quads = c.D / 4, work = rows * quads;
+  const float* tail = ws + (long long)p.slots * PA_ROWS * DP;
+  const int lanes = work < PA_THREADS ? PA_THREADS / work : 1;  // threads that share a place
+  for (int e0 = 0; e0 < work; e0 += PA_THREADS) {
+    const int share = lanes > 1 ? (int)threadIdx.x / work : 0;
+    const int e = lanes > 1 ? (int)threadIdx.x - share * work : e0 + (int)threadIdx.x;
+    const bool live = share < lanes && e < work;
+    const int r = live ? e / quads : 0, d = live ? (e - r * quads) * 4 : 0;
+    PagedPart sum = {PA_EMPTY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+    if (live) {
+      for (int s0 = share; s0 < it.splits; s0 += 4 * lanes) {
+        float2 od[4], y0[4], y1[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {  // four slices on their way at once; those behind the last one read it again
+          const int s = s0 + u * lanes < it.splits ? s0 + u * lanes : it.splits - 1;
+          const long long row = (it.first + (long long)s * it.step) * PA_ROWS + r;
+          od[u] = get2(tail + row * 2);
+          y0[u] = get2(ws + row * DP + d);
+          y1[u] = get2(ws + row * DP + d + 2);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (s0 + u * lanes < it.splits) sum.add(od[u].x, od[u].y, {y0[u].x, y0[u].y, y1[u].x, y1[u].y});
+      }
+    }
+    if (lanes > 1) {
+      float* mine = meet + threadIdx.x * 8;
+      mine[0] = sum.off, mine[1] = sum.den;
+      *reinterpret_cast<v4f*>(mine + 4) = v4f{sum.y[0], sum.y[1], sum.y[2], sum.y[3]};
+      __syncthreads();
+      if (share != 0) return;
+      for (int o = 1; o < lanes; ++o) {
+        const float* at = meet + (threadIdx.x + o * work) * 8;
+        sum.add(at[0], at[1], {at[4], at[5], at[6], at[7]});
+      }
+    }
+    if (!live) continue;
+    const float f = sum.den > 0.0f ? a.alpha_pv * 1024.0f / sum.den : 0.0f;
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = sum.den > 0.0f ? sum.y[i] * f : 0.0f;
+    const int rr = it.tile * PA_ROWS + r, tt = rr / G;
+    store4<OUT>(a.out, ((long long)(it.s.row0 + tt) * a.q_heads + it.head * G + rr - tt * G) * c.D + d, y);
+  }
+}
+
+// Workspace: partial sums [slots][16][DP] fp32, then (offset, denominator) [slots][16].
+template <int DP, int OUT>
+__global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p,
                                                                         float* ws) {
   constexpr int NB = DP / 16;    // column blocks; lane n of 16 owns the columns NB n .. NB n + NB - 1
   constexpr int KC = DP / 64;    // 16-byte pieces of a key row that a lane holds
@@ -192,8 +302,10 @@ __global__ __launch_bounds__(PA_WAVES * 64) void paged_attn_rows_kernel(PagedAtt
   const float cl = a.alpha_qk * 1.44269504088896341f;
   const int8_t* kb = c.k + it.head * c.k_head;
   const int8_t* vb = c.v + it.head * c.v_head;
-  const int* table = b.table + (long long)it.seq * b.per_seq;
-  const int mask = (1 << c.page_shift) - 1, last_block = keys > 0 ? (keys - 1) >> 4 : 0;
+  // The table through the constant address space: nothing writes to it while the kernel runs, and scalar loads are counted
+  // apart from the keys and values in flight, which a vector load would have to wait for.
+  const auto table = (const __attribute__((address_space(4))) int*)(b.table + (long long)it.seq * b.per_seq);
+  const int mask = (1 << c.page_shift) - 1, last_block = hi > 0 ? (hi - 1) >> 4 : 0;
 
   float off = PA_EMPTY;
   v4f acc[NB], dsum = {0, 0, 0, 0};
@@ -208,36 +320,45 @@ __global__ __launch_bounds__(PA_WAVES * 64) void paged_attn_rows_kernel(PagedAtt
     unsigned v[8][VW];
     bool on[2];
   };
-  auto fetch = [&](Step& st, int s0) {
+  // pages of the two blocks of 16 keys from s0 on, asked for a step before the keys are; blocks behind the last key are
+  // masked, and read where there is memory
+  auto pages_of = [&](int (&pg)[2], int s0) {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
       int at = (s0 >> 4) + blk;
-      at = at < last_block ? at : last_block;  // blocks behind the last key: masked, read where there is memory
-      int page = table[(at << 4) >> c.page_shift];
+      at = at < last_block ? at : last_block;
+      pg[blk] = table[(at << 4) >> c.page_shift];
+    }
+  };
+  // Columns beyond the head size: the first ones are read instead, without a branch; Q is zero there, and what V makes of them
+  // is not stored.
+  unsigned kcol[KC];
+#pragma unroll
+  for (int i = 0; i < KC; ++i) kcol[i] = (unsigned)(n * c.k_token) + ((kg * KC + i) * 16 < c.D ? (unsigned)(kg * KC + i) * 16u : 0u);
+  const unsigned vcol = (unsigned)(kg * 4 * c.v_token) + (n * NB < c.D ? (unsigned)(n * NB) : 0u);
+  auto fetch = [&](Step& st, int s0, const int (&pg)[2]) {
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      int at = (s0 >> 4) + blk;
+      at = at < last_block ? at : last_block;
+      int page = pg[blk];
       st.on[blk] = page >= 0 && page < c.pages;
       page = st.on[blk] ? page : 0;
-      const int o = (at << 4) & mask;
-      const int8_t* kr = kb + (long long)page * c.k_page + (long long)(o + n) * c.k_token;
+      const long long o = (at << 4) & mask;
+      const int8_t* kr = kb + (long long)page * c.k_page + o * c.k_token;
 #pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const int d = (kg * KC + i) * 16;
-        st.k[blk][i] = v4i{0, 0, 0, 0};
-        if (d < c.D) st.k[blk][i] = *reinterpret_cast<const v4i*>(kr + d);
-      }
-      const int8_t* vr = vb + (long long)page * c.v_page + (long long)(o + kg * 4) * c.v_token + n * NB;
+      for (int i = 0; i < KC; ++i) st.k[blk][i] = *reinterpret_cast<const v4i*>(kr + kcol[i]);
+      const int8_t* vr = vb + (long long)page * c.v_page + o * c.v_token;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int w = 0; w < VW; ++w) st.v[blk * 4 + j][w] = 0;
-        if (n * NB < c.D) {
-          if constexpr (VW == 2) {
-            const uint2 x = *reinterpret_cast<const uint2*>(vr + (long long)j * c.v_token);
-            st.v[blk * 4 + j][0] = x.x;
-            st.v[blk * 4 + j][1] = x.y;
-          } else {
-            st.v[blk * 4 + j][0] = *reinterpret_cast<const unsigned*>(vr + (long long)j * c.v_token);
-          }
+        if constexpr (VW == 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(vr + vcol);
+          st.v[blk * 4 + j][0] = x.x;
+          st.v[blk * 4 + j][1] = x.y;
+        } else {
+          st.v[blk * 4 + j][0] = *reinterpret_cast<const unsigned*>(vr + vcol);
         }
+        vr += c.v_token;
       }
     }
   };
@@ -263,10 +384,7 @@ __global__ __launch_bounds__(PA_WAVES * 64) void paged_attn_rows_kernel(PagedAtt
     for (int i = 1; i < 8; ++i) top = x[i] > top ? x[i] : top;
     // a new reference only where a probability would pass 2^15: it starts at 2^8, fp16 ends at 2^16
     if (__ballot(__builtin_fmaf(top, cl, off) > 15.0f) != 0) {
-      float o = __shfl_xor(top, 16, 64);
-      top = o > top ? o : top;
-      o = __shfl_xor(top, 32, 64);
-      top = o > top ? o : top;
+      top = rows_max(top);
       if (__builtin_fmaf(top, cl, off) > 15.0f) {
         const float fresh = 8.0f - top * cl;
         const float scale = __builtin_amdgcn_exp2f(fresh - off);
@@ -311,18 +429,24 @@ __global__ __launch_bounds__(PA_WAVES * 64) void paged_attn_rows_kernel(PagedAtt
 
   int s0 = lo + wave * 32;
   if (s0 < hi) {
-    Step st;
-    fetch(st, s0);
-    for (;;) {
-      const int next = s0 + PA_WAVES * 32;
-      if (next >= hi) break;
-      Step after;
-      fetch(after, next);
-      work(st, s0);
-      st = after;
-      s0 = next;
+    constexpr int STRIDE = PA_WAVES * 32;
+    Step even, odd;
+    int pg[2];
+    pages_of(pg, s0);
+    fetch(even, s0, pg);
+    pages_of(pg, s0 + STRIDE);
+    for (;;) {  // a step's loads are issued without a branch around them, so that the waits can count them
+      fetch(odd, s0 + STRIDE, pg);
+      pages_of(pg, s0 + 2 * STRIDE);
+      work(even, s0);
+      s0 += STRIDE;
+      if (s0 >= hi) break;
+      fetch(even, s0 + STRIDE, pg);
+      pages_of(pg, s0 + 2 * STRIDE);
+      work(odd, s0);
+      s0 += STRIDE;
+      if (s0 >= hi) break;
     }
-    work(st, s0);
   }
 
   // the waves meet: lane (n, kg) holds of row n the columns NB (4 kg + r) + i in acc[i][r]
@@ -337,7 +461,7 @@ __global__ __launch_bounds__(PA_WAVES * 64) void paged_attn_rows_kernel(PagedAtt
   }
   __syncthreads();
   const int quads = c.D / 4;
-  for (int e = threadIdx.x; e < PA_ROWS * (DP / 4); e += PA_WAVES * 64) {
+  for (int e = threadIdx.x; e < PA_ROWS * (DP / 4); e += PA_THREADS) {
     const int r = e / (DP / 4), d = (e % (DP / 4)) * 4;
     const int rr = it.tile * PA_ROWS + r;
     if (rr >= live_rows || d >= quads * 4) continue;
@@ -355,13 +479,9 @@ __global__ __launch_bounds__(PA_WAVES * 64) void paged_attn_rows_kernel(PagedAtt
     }
     if (it.splits > 1) {
       const long long slot = it.first + (long long)it.split * it.step;
-      if (slot >= p.slots) continue;
-      *reinterpret_cast<v4f*>(ws + (slot * PA_ROWS + r) * DP + d) = v4f{y[0], y[1], y[2], y[3]};
-      if (d == 0) {
-        float* tail = ws + (long long)p.slots * PA_ROWS * DP;
-        tail[slot * PA_ROWS + r] = least;
-        tail[(long long)p.slots * PA_ROWS + slot * PA_ROWS + r] = l;
-      }
+      put2(ws + (slot * PA_ROWS + r) * DP + d, y[0], y[1]);
+      put2(ws + (slot * PA_ROWS + r) * DP + d + 2, y[2], y[3]);
+      if (d == 0) put2(ws + (long long)p.slots * PA_ROWS * DP + (slot * PA_ROWS + r) * 2, least, l);
     } else {
       const float f = l > 0.0f ? a.alpha_pv * 1024.0f / l : 0.0f;
 #pragma unroll
@@ -370,40 +490,29 @@ __global__ __launch_bounds__(PA_WAVES * 64) void paged_attn_rows_kernel(PagedAtt
       store4<OUT>(a.out, ((long long)(it.s.row0 + tt) * a.q_heads + it.head * G + rr - tt * G) * c.D + d, y);
     }
   }
+  if (it.splits == 1 || p.arrivals == nullptr) return;
+  // The workgroup that arrives last joins the slices, in their order: the bits do not depend on who that is.  Partial results
+  // and the counter go past the XCDs' caches (device-scope atomics), so no cache has to be written back or emptied: a
+  // thread's stores have arrived when its count of them is zero.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int* const seen = reinterpret_cast<int*>(&offs[0][0]);
+  if (threadIdx.x == 0) {
+    seen[0] = __hip_atomic_fetch_add(p.arrivals + it.first, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (seen[0] == it.splits - 1) __hip_atomic_store(p.arrivals + it.first, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (seen[0] != it.splits - 1) return;
+  join_slices<DP, OUT>(a, c, p, it, ws, &sum[0][0][0]);
 }
 
-// Joins the slices of the sequences that were cut: a workgroup to a (sequence, tile, head) item, found as above among the first slices.
+// Joins the slices of the sequences that were cut where they do not meet in the launch itself.
 template <int DP, int OUT>
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p, const float* ws) {
+__global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p, const float* ws) {
+  __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
   const PagedItem it = paged_item(b, c.page_shift, c.heads, PA_ROWS, p, blockIdx.x);
-  if (!it.found || it.split != 0 || it.splits == 1 || it.first + (long long)(it.splits - 1) * it.step >= p.slots) return;
-  const int G = p.group, live_rows = it.s.T * G;
-  const float* offs = ws + (long long)p.slots * PA_ROWS * DP;
-  const float* den = offs + (long long)p.slots * PA_ROWS;
-  for (int e = threadIdx.x; e < PA_ROWS * (DP / 4); e += 256) {
-    const int r = e / (DP / 4), d = (e % (DP / 4)) * 4;
-    const int rr = it.tile * PA_ROWS + r;
-    if (rr >= live_rows || d >= c.D) continue;
-    float least = PA_EMPTY;
-    for (int s = 0; s < it.splits; ++s) {
-      const float o = offs[(it.first + (long long)s * it.step) * PA_ROWS + r];
-      least = o < least ? o : least;
-    }
-    float y[4] = {0, 0, 0, 0}, l = 0;
-    for (int s = 0; s < it.splits; ++s) {
-      const long long slot = it.first + (long long)s * it.step;
-      const float scale = __builtin_amdgcn_exp2f(least - offs[slot * PA_ROWS + r]);
-      const v4f v = *reinterpret_cast<const v4f*>(ws + (slot * PA_ROWS + r) * DP + d);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] += v[i] * scale;
-      l += den[slot * PA_ROWS + r] * scale;
-    }
-    const float f = l > 0.0f ? a.alpha_pv * 1024.0f / l : 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = l > 0.0f ? y[i] * f : 0.0f;
-    const int tt = rr / G;
-    store4<OUT>(a.out, ((long long)(it.s.row0 + tt) * a.q_heads + it.head * G + rr - tt * G) * c.D + d, y);
-  }
+  if (!it.found || it.split != 0 || it.splits == 1) return;
+  join_slices<DP, OUT>(a, c, p, it, ws, meet);
 }
 
 // Items that a batch can make: one to each (sequence, key head, 16 rows), and the slices beyond that.
@@ -416,6 +525,10 @@ static long long paged_slots(long long rows, long long seqs, long long group, lo
 }
 static int paged_dp(long long D) { return D <= 64 ? 64 : 128; }
 
+long long paged_attn_arrivals(long long rows, long long seqs, long long q_heads, long long kv_heads, long long capacity) {
+  if (rows <= 0 || seqs <= 0 || kv_heads <= 0 || !paged_cuts(capacity)) return 0;
+  return paged_slots(rows, seqs, q_heads / kv_heads, kv_heads);
+}
 long long paged_attn_workspace_bytes(long long rows, long long seqs, long long q_heads, long long kv_heads, long long D,
                                      long long capacity) {
   if (rows <= 0 || seqs <= 0 || kv_heads <= 0 || !paged_cuts(capacity)) return 0;
@@ -425,9 +538,9 @@ long long paged_attn_workspace_bytes(long long rows, long long seqs, long long q
 template <int DP, int OUT>
 static void launch_rows(const PagedAttn& a, const PagedCache& c, const PagedBatch& b, const PagedPlan& p, float* ws, unsigned grid,
                         hipStream_t stream) {
-  hipLaunchKernelGGL((paged_attn_rows_kernel<DP, OUT>), dim3(grid), dim3(PA_WAVES * 64), 0, stream, a, c, b, p, ws);
-  if (p.target != 0)
-    hipLaunchKernelGGL((paged_attn_join_kernel<DP, OUT>), dim3(grid), dim3(256), 0, stream, a, c, b, p, ws);
+  hipLaunchKernelGGL((paged_attn_rows_kernel<DP, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, p, ws);
+  if (p.target != 0 && p.arrivals == nullptr)
+    hipLaunchKernelGGL((paged_attn_join_kernel<DP, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, p, ws);
 }
 
 int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, const PagedBatch& b, void* workspace,
@@ -440,6 +553,7 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
   const bool cut = need > 0 && workspace != nullptr && workspace_bytes >= need;
   p.target = cut ? PA_TARGET : 0;
   p.slots = cut ? (int)paged_slots(b.rows, b.seqs, p.group, c.heads) : 0;
+  p.arrivals = a.arrivals != nullptr && a.arrivals_count >= p.slots ? a.arrivals : nullptr;
   const long long grid = cut ? p.slots : paged_units(b.rows, b.seqs, p.group, c.heads, PA_ROWS);
   if (grid > 0x7fffff) return fail(TI_ERR_INVALID_ARG, "paged_attn_s8: %lld work items", grid);
   float* ws = static_cast<float*>(workspace);

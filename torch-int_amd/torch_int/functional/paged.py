@@ -48,13 +48,15 @@ class _Append(ctypes.Structure):
 class _Attn(ctypes.Structure):
     """``TiPagedAttn``."""
     _fields_ = [("q", _vp), ("q_row", _i64), ("q_head", _i64), ("q_heads", _i64), ("out", _vp), ("out_type", _i32), ("fill", _i32),
-                ("alpha_qk", _f32), ("alpha_pv", _f32)]
+                ("alpha_qk", _f32), ("alpha_pv", _f32), ("arrivals", _vp), ("arrivals_count", _i64)]
 
 
 _lib.ti_paged_kv_append_s8.argtypes = [ctypes.POINTER(_Cache), ctypes.POINTER(_Batch), ctypes.POINTER(_Append), _vp]
 _lib.ti_paged_kv_append_s8.restype = ctypes.c_int
 _lib.ti_paged_attn_workspace_bytes.argtypes = [_i64] * 6
 _lib.ti_paged_attn_workspace_bytes.restype = _i64
+_lib.ti_paged_attn_arrivals.argtypes = [_i64] * 6
+_lib.ti_paged_attn_arrivals.restype = _i64
 _lib.ti_paged_attn_s8.argtypes = [ctypes.POINTER(_Cache), ctypes.POINTER(_Batch), ctypes.POINTER(_Attn), _vp, _i64, _vp]
 _lib.ti_paged_attn_s8.restype = ctypes.c_int
 _fast_append = getattr(_CUDA._fast, "paged_append", None)
@@ -62,7 +64,22 @@ _fast_attn = getattr(_CUDA._fast, "paged_attn", None)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _I8, _I32, _F32 = torch.int8, torch.int32, torch.float32
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
-_ws_need = {}  # shape of a call -> bytes of workspace it can use
+_ws_need = {}  # shape of a call -> (bytes of workspace, counters) it can use
+_counters = {}  # (device index, stream) -> int32 zeros in which the slices of a call count themselves, zero again behind it
+
+
+def _arrivals(dev_index, stream, n):
+    """Counters for one stream, grown on demand; a recording gets its own, cleared by the recording itself."""
+    if n <= 0:
+        return None, 0
+    key = (dev_index, stream)
+    t = _counters.get(key)
+    capturing = torch.cuda.is_current_stream_capturing()
+    if capturing or t is None or t.numel() < n:
+        t = torch.zeros(int(n), dtype=_I32, device=torch.device("cuda", dev_index))
+        if not capturing:
+            _counters[key] = t
+    return t, t.data_ptr()
 
 
 def _fail(op, msg):
@@ -225,11 +242,13 @@ def paged_attn_s8(query, k_cache, v_cache, block_table, context_lens, cu_new, al
     if need is None:
         if len(_ws_need) >= 4096:
             _ws_need.clear()
-        need = _ws_need[key] = int(_lib.ti_paged_attn_workspace_bytes(*key))
+        need = _ws_need[key] = (int(_lib.ti_paged_attn_workspace_bytes(*key)), int(_lib.ti_paged_attn_arrivals(*key)))
     with _hip_ext._on(dev):
         stream = _raw_stream(dev.index)
-        ws, ws_ptr, ws_bytes = _CUDA._workspace(dev.index, stream, need)
-        tail = (query.data_ptr(), q_row, q_head, q_heads, out.data_ptr(), code, fill, float(alpha_qk), float(alpha_pv))
+        ws, ws_ptr, ws_bytes = _CUDA._workspace(dev.index, stream, need[0])
+        counters, counters_ptr = _arrivals(dev.index, stream, need[1])
+        tail = (query.data_ptr(), q_row, q_head, q_heads, out.data_ptr(), code, fill, float(alpha_qk), float(alpha_pv), counters_ptr,
+                need[1])
         if _fast_attn is not None:
             rc = _fast_attn(*args, *tail, ws_ptr, ws_bytes, stream)
         else:
