@@ -68,6 +68,16 @@ ATTENTION = [
     (4, 2, 128, 16, [5000], [1]),                        # cut into slices
     (2, 1, 64, 64, [2049, 9, 1030], [3, 1, 17]),
     (1, 1, 32, 256, [4097, 4096], [1, 40]),
+    # tiles of 128 rows: whole prompts, chunks, single tokens among them, rows and keys that end inside a tile
+    (1, 1, 128, 16, [128], [128]),
+    (8, 2, 128, 16, [700, 130, 64, 0], [300, 130, 1, 0]),
+    (12, 12, 64, 32, [257, 1], [257, 1]),
+    (3, 3, 80, 16, [200, 40], [150, 33]),
+    (5, 1, 48, 64, [65, 300], [64, 13]),
+    (16, 2, 112, 128, [500, 129, 17], [9, 129, 17]),
+    (4, 4, 96, 16, [20, 90], [60, 80]),                  # more new tokens than positions
+    (2, 1, 128, 16, [6000], [64]),                       # cut into slices
+    (24, 8, 64, 256, [3000, 2], [5, 2]),
 ]
 
 
@@ -136,6 +146,9 @@ def test_values_out_of_range_touch_nothing_else():
     table[0, 2], table[0, 12], table[1, 0], table[2, :] = -1, pages, 2 ** 31 - 1, -(2 ** 31)
     got = _attend("pages", q, k, v, table, lens, cu, 3e-4, 0.02, FP16_WEIGHTS, out_dtype=torch.float16)
     assert (got[3:] == 0).all()
+    q128, cu128, lens128 = _s8(g, 90, 8, 80, spread=30), torch.tensor([0, 60, 61, 90], dtype=torch.int32), lens + 60
+    got = _attend("pages, tiles", q128, k, v, table, lens128, cu128, 3e-4, 0.02, FP16_WEIGHTS, out_dtype=torch.float16)
+    assert (got[61:] == 0).all()
     for bad_lens in ([2 ** 31 - 1, -5, 64], [10 ** 6, 0, -(2 ** 31)]):
         _attend("lens", q, k, v, table, torch.tensor(bad_lens, dtype=torch.int32), cu, 3e-4, 0.02, FP16_WEIGHTS, out_dtype=torch.float16)
     for bad_cu in ([0, 2, 3, 10 ** 9], [0, 7, 3, 5], [-4, 2, -9, 2 ** 31 - 1], [5, 0, 7, 6]):
@@ -305,7 +318,8 @@ def test_the_same_inputs_give_the_same_bits_on_any_stream():
 
 
 @pytest.mark.parametrize("hq,hk,d,lens,new", [(1, 1, 128, [70000], [1]), (8, 1, 64, [9000, 2, 700], [1, 1, 1]), (4, 2, 80, [3000, 2900], [9, 1]),
-                                              (32, 2, 128, [5000, 40, 6001], [1, 1, 2]), (12, 12, 64, [1025], [1])])
+                                              (32, 2, 128, [5000, 40, 6001], [1, 1, 2]), (12, 12, 64, [1025], [1]),
+                                              (4, 2, 128, [4000, 70], [100, 1]), (1, 1, 64, [3000], [200]), (8, 8, 80, [1500], [33])])
 def test_slices_that_meet_in_the_launch_or_behind_it(hq, hk, d, lens, new, monkeypatch):
     # the same bits with the counters, without them (a second launch), again and again, and after calls whose tables hold
     # nonsense: the counters are zero behind every call; against fp64 as well

@@ -17,6 +17,8 @@ namespace ti {
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 
 constexpr int PA_WAVES = 4;
 constexpr int PA_ROWS = 16;
@@ -155,17 +157,19 @@ __device__ __forceinline__ void paged_fill(const PagedBatch& b, char* out, long 
   }
 }
 
-template <int OUT>
-__device__ __forceinline__ void store4(void* out, long long at, const float (&y)[4]) {
+// N neighbouring outputs (2 or 4)
+template <int N, int OUT>
+__device__ __forceinline__ void store_some(void* out, long long at, const float (&y)[N]) {
   if constexpr (OUT == PT_S8) {
-    int w = 0;
+    unsigned w = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w |= (rne_s8(y[i]) & 255) << (8 * i);
-    reinterpret_cast<int*>(static_cast<int8_t*>(out) + at)[0] = w;
+    for (int i = 0; i < N; ++i) w |= (unsigned)(rne_s8(y[i]) & 255) << (8 * i);
+    if constexpr (N == 4) reinterpret_cast<unsigned*>(static_cast<int8_t*>(out) + at)[0] = w;
+    else reinterpret_cast<unsigned short*>(static_cast<int8_t*>(out) + at)[0] = (unsigned short)w;
   } else {
-    unsigned short h[4];
+    unsigned short h[N];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < N; ++i) {
       if constexpr (OUT == PT_F16) {
         const _Float16 v = (_Float16)y[i];
         __builtin_memcpy(&h[i], &v, 2);
@@ -174,9 +178,11 @@ __device__ __forceinline__ void store4(void* out, long long at, const float (&y)
         __builtin_memcpy(&h[i], &v, 2);
       }
     }
-    int2 w;
-    __builtin_memcpy(&w, h, 8);
-    *reinterpret_cast<int2*>(static_cast<unsigned short*>(out) + at) = w;
+    unsigned w[N / 2];
+    __builtin_memcpy(w, h, 2 * N);
+    unsigned* to = reinterpret_cast<unsigned*>(static_cast<unsigned short*>(out) + at);
+    if constexpr (N == 4) *reinterpret_cast<v2u*>(to) = v2u{w[0], w[1]};
+    else to[0] = w[0];
   }
 }
 
@@ -206,14 +212,14 @@ struct PagedPart {
 
 // The slices of one item, by the threads of one workgroup: a thread owns four columns of a row in every so many-th slice.
 constexpr int PA_THREADS = PA_WAVES * 64;
-template <int DP, int OUT>
+template <int ROWS, int DP, int OUT>
 __device__ __forceinline__ void join_slices(const PagedAttn& a, const PagedCache& c, const PagedPlan& p, const PagedItem& it,
                                             const float* ws, float* meet) {
   const int G = p.group;
-  int rows = it.s.T * G - it.tile * PA_ROWS;
-  rows = rows < PA_ROWS ? rows : PA_ROWS;
+  int rows = it.s.T * G - it.tile * ROWS;
+  rows = rows < ROWS ? rows : ROWS;
   const int quads = c.D / 4, work = rows * quads;
-  const float* tail = ws + (long long)p.slots * PA_ROWS * DP;
+  const float* tail = ws + (long long)p.slots * ROWS * DP;
   const int lanes = work < PA_THREADS ? PA_THREADS / work : 1;  // threads that share a place
   for (int e0 = 0; e0 < work; e0 += PA_THREADS) {
     const int share = lanes > 1 ? (int)threadIdx.x / work : 0;
@@ -227,7 +233,7 @@ __device__ __forceinline__ void join_slices(const PagedAttn& a, const PagedCache
 #pragma unroll
         for (int u = 0; u < 4; ++u) {  // four slices on their way at once; those behind the last one read it again
           const int s = s0 + u * lanes < it.splits ? s0 + u * lanes : it.splits - 1;
-          const long long row = (it.first + (long long)s * it.step) * PA_ROWS + r;
+          const long long row = (it.first + (long long)s * it.step) * ROWS + r;
           od[u] = get2(tail + row * 2);
           y0[u] = get2(ws + row * DP + d);
           y1[u] = get2(ws + row * DP + d + 2);
@@ -253,9 +259,26 @@ __device__ __forceinline__ void join_slices(const PagedAttn& a, const PagedCache
     float y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = sum.den > 0.0f ? sum.y[i] * f : 0.0f;
-    const int rr = it.tile * PA_ROWS + r, tt = rr / G;
-    store4<OUT>(a.out, ((long long)(it.s.row0 + tt) * a.q_heads + it.head * G + rr - tt * G) * c.D + d, y);
+    const int rr = it.tile * ROWS + r, tt = rr / G;
+    store_some<4, OUT>(a.out, ((long long)(it.s.row0 + tt) * a.q_heads + it.head * G + rr - tt * G) * c.D + d, y);
   }
+}
+
+// The workgroup that arrives last joins the slices, in their order: the bits do not depend on who that is.  Partial results
+// and the counter go past the XCDs' caches (device-scope atomics), so no cache has to be written back or emptied: a
+// thread's stores have arrived when its count of them is zero.  `scratch`: LDS of the workgroup that nobody reads any more.
+template <int ROWS, int DP, int OUT>
+__device__ __forceinline__ void meet_and_join(const PagedAttn& a, const PagedCache& c, const PagedPlan& p, const PagedItem& it,
+                                              const float* ws, int* seen, float* scratch) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    seen[0] = __hip_atomic_fetch_add(p.arrivals + it.first, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (seen[0] == it.splits - 1) __hip_atomic_store(p.arrivals + it.first, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (seen[0] != it.splits - 1) return;
+  join_slices<ROWS, DP, OUT>(a, c, p, it, ws, scratch);
 }
 
 // Workspace: partial sums [slots][16][DP] fp32, then (offset, denominator) [slots][16].
@@ -295,7 +318,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAtt
 #pragma unroll
   for (int i = 0; i < KC; ++i) {
     qf[i] = v4i{0, 0, 0, 0};
-    const int d = (kg * KC + i) * 16;
+    const int d = (i * 4 + kg) * 16;
     if (real && d < c.D)
       qf[i] = *reinterpret_cast<const v4i*>(a.q + (long long)(it.s.row0 + t) * a.q_row + (long long)(it.head * G + g) * a.q_head + d);
   }
@@ -334,7 +357,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAtt
   // is not stored.
   unsigned kcol[KC];
 #pragma unroll
-  for (int i = 0; i < KC; ++i) kcol[i] = (unsigned)(n * c.k_token) + ((kg * KC + i) * 16 < c.D ? (unsigned)(kg * KC + i) * 16u : 0u);
+  for (int i = 0; i < KC; ++i) kcol[i] = (unsigned)(n * c.k_token) + ((i * 4 + kg) * 16 < c.D ? (unsigned)(i * 4 + kg) * 16u : 0u);
   const unsigned vcol = (unsigned)(kg * 4 * c.v_token) + (n * NB < c.D ? (unsigned)(n * NB) : 0u);
   auto fetch = [&](Step& st, int s0, const int (&pg)[2]) {
 #pragma unroll
@@ -352,9 +375,9 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAtt
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (VW == 2) {
-          const uint2 x = *reinterpret_cast<const uint2*>(vr + vcol);
-          st.v[blk * 4 + j][0] = x.x;
-          st.v[blk * 4 + j][1] = x.y;
+          const v2u x = *reinterpret_cast<const v2u*>(vr + vcol);
+          st.v[blk * 4 + j][0] = x[0];
+          st.v[blk * 4 + j][1] = x[1];
         } else {
           st.v[blk * 4 + j][0] = *reinterpret_cast<const unsigned*>(vr + vcol);
         }
@@ -487,41 +510,283 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAtt
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = l > 0.0f ? y[i] * f : 0.0f;
       const int tt = rr / G;
-      store4<OUT>(a.out, ((long long)(it.s.row0 + tt) * a.q_heads + it.head * G + rr - tt * G) * c.D + d, y);
+      store_some<4, OUT>(a.out, ((long long)(it.s.row0 + tt) * a.q_heads + it.head * G + rr - tt * G) * c.D + d, y);
     }
   }
   if (it.splits == 1 || p.arrivals == nullptr) return;
-  // The workgroup that arrives last joins the slices, in their order: the bits do not depend on who that is.  Partial results
-  // and the counter go past the XCDs' caches (device-scope atomics), so no cache has to be written back or emptied: a
-  // thread's stores have arrived when its count of them is zero.
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  int* const seen = reinterpret_cast<int*>(&offs[0][0]);
-  if (threadIdx.x == 0) {
-    seen[0] = __hip_atomic_fetch_add(p.arrivals + it.first, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (seen[0] == it.splits - 1) __hip_atomic_store(p.arrivals + it.first, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  meet_and_join<PA_ROWS, DP, OUT>(a, c, p, it, ws, reinterpret_cast<int*>(&offs[0][0]), &sum[0][0][0]);
+}
+
+// Many rows: 128 to a workgroup, 32 to each of its four waves, 64 keys to a step.  Each wave brings 16 of the keys: K as it is
+// into rows of the LDS (16-byte chunks exchanged by the row, so that 32 rows are read without conflicts), V as fp16 in the order in
+// which MFMA operands are read: of eight keys, chosen as S^T = K Q^T (32x32x32 int8) leaves them in a lane, one column in 16 bytes,
+// lane after lane.  One widening of V then serves 128 rows.  Column blocks are interleaved (block i holds the columns NDB m + i),
+// so a thread widens neighbouring columns and a lane of O^T ends up with neighbouring ones.
+// Scores start from 1.5 * 2^23 instead of 0: the int32 sum is then the fp32 number 12582912 + x, and the constant goes into the
+// row's offset, where one multiply-add removes it exactly.
+constexpr int PT_ROWS = 128, PT_KEYS = 64;
+template <int DP, int OUT>
+__global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p, float* ws) {
+  constexpr int NDB = DP / 32;   // column blocks of O^T, and steps of 32 along a key row
+  constexpr int KC = DP / 64;    // 16-byte pieces of K that a thread brings
+  constexpr int CH = DP / 16;    // 16-byte chunks of a key row
+  constexpr int KBYTES = PT_KEYS * DP, STAGE = 3 * KBYTES;
+  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+  __shared__ int seen;
+
+  if (a.fill) paged_fill(b, static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
+  const PagedItem it = paged_item(b, c.page_shift, c.heads, PT_ROWS, p, blockIdx.x);
+  if (!it.found) return;
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, h = lane >> 5;
+  const int G = p.group, live_rows = it.s.T * G;
+  const int base = it.s.len - it.s.T;
+  const int row0 = it.tile * PT_ROWS + wave * 32, row = row0 + n;
+  const int t = row / G, g = row - t * G;
+  const bool real = row < live_rows;
+  int limit = real ? base + t + 1 : 0x7fffffff;
+  limit = limit < 0 ? 0 : limit;
+  const int first_limit = base + row0 / G + 1;   // keys of the wave's first row
+  int keys = 0;                                  // keys of the wave's last row; none for a wave without rows
+  if (row0 < live_rows) {
+    const int last = row0 + 31 < live_rows ? row0 + 31 : live_rows - 1;
+    keys = base + last / G + 1;
+    keys = keys < 0 ? 0 : keys;
   }
-  __syncthreads();
-  if (seen[0] != it.splits - 1) return;
-  join_slices<DP, OUT>(a, c, p, it, ws, &sum[0][0][0]);
+  int most = it.tile * PT_ROWS + PT_ROWS - 1;    // keys of the workgroup's last row
+  most = base + (most < live_rows ? most : live_rows - 1) / G + 1;
+  most = most < 0 ? 0 : most;
+  const long long lo_ll = (long long)it.split * it.slice;
+  const int lo = lo_ll < most ? (int)lo_ll : most;
+  const int hi = lo_ll + it.slice < most ? (int)(lo_ll + it.slice) : most;
+  keys = keys < hi ? keys : hi;
+
+  v4i qf[NDB];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i) {
+    qf[i] = v4i{0, 0, 0, 0};
+    const int d = i * 32 + h * 16;
+    if (real && d < c.D)
+      qf[i] = *reinterpret_cast<const v4i*>(a.q + (long long)(it.s.row0 + t) * a.q_row + (long long)(it.head * G + g) * a.q_head + d);
+  }
+  const float cl = a.alpha_qk * 1.44269504088896341f;
+  const int8_t* kb = c.k + it.head * c.k_head;
+  const int8_t* vb = c.v + it.head * c.v_head;
+  const auto table = (const __attribute__((address_space(4))) int*)(b.table + (long long)it.seq * b.per_seq);
+  const int mask = (1 << c.page_shift) - 1, last_block = hi > 0 ? (hi - 1) >> 4 : 0;
+
+  // what this thread brings of a step: of the wave's 16 keys, KC chunks of K and the columns NDB n .. of eight rows of V
+  const int krow = lane / CH, kchunk = lane % CH;
+  const unsigned kcol = (unsigned)(krow * c.k_token) + (kchunk * 16 < c.D ? kchunk * 16u : 0u);
+  const unsigned vcol = (unsigned)(h * 4 * c.v_token) + (n * NDB < c.D ? (unsigned)(n * NDB) : 0u);
+  v4i kreg[KC];
+  unsigned vreg[8];
+  auto page_at = [&](int s0, int blk) {
+    int at = (s0 >> 4) + blk;
+    at = at < last_block ? at : last_block;
+    return table[(at << 4) >> c.page_shift];
+  };
+  auto fetch = [&](int s0, int page) {
+    int at = (s0 >> 4) + wave;
+    at = at < last_block ? at : last_block;
+    page = page >= 0 && page < c.pages ? page : 0;
+    const long long o = (at << 4) & mask;
+    const int8_t* kr = kb + (long long)page * c.k_page + o * c.k_token;
+#pragma unroll
+    for (int i = 0; i < KC; ++i) kreg[i] = *reinterpret_cast<const v4i*>(kr + (long long)(i * (64 / CH)) * c.k_token + kcol);
+    const int8_t* vr = vb + (long long)page * c.v_page + o * c.v_token;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int8_t* at_row = vr + (long long)((j & 3) + 8 * (j >> 2)) * c.v_token + vcol;
+      if constexpr (NDB == 4) vreg[j] = *reinterpret_cast<const unsigned*>(at_row);
+      else vreg[j] = *reinterpret_cast<const unsigned short*>(at_row);
+    }
+  };
+  auto swizzle = [](int r, int chunk) { return DP == 128 ? chunk ^ (r & 7) : chunk ^ ((r >> 2) & 3); };
+  auto put = [&](char* stage) {
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      const int r = wave * 16 + i * (64 / CH) + krow;
+      *reinterpret_cast<v4i*>(stage + r * DP + swizzle(r, kchunk) * 16) = kreg[i];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vreg[j] ^= 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < NDB; ++i) {
+      v8h x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned two = __builtin_amdgcn_perm(vreg[2 * j + 1], vreg[2 * j], 0x0c000c00u | (unsigned)(4 + i) << 16 | (unsigned)i);
+        v2h y;
+        __builtin_memcpy(&y, &two, 4);
+        y = __builtin_elementwise_fma(y, v2h{(_Float16)16384.0f, (_Float16)16384.0f}, v2h{(_Float16)-0.125f, (_Float16)-0.125f});
+        x[2 * j] = y[0];
+        x[2 * j + 1] = y[1];
+      }
+      *reinterpret_cast<v8h*>(stage + KBYTES + ((wave * NDB + i) * 64 + lane) * 16) = x;
+    }
+  };
+
+  float off = PA_EMPTY, den = 0.0f;
+  v16f acc[NDB];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
+  v16i start;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) start[r] = 0x4b400000;
+
+  // one step: the keys s0 .. s0 + 63 in `stage`; `lost`: bit i is set where the pool has no page for the i-th 16 of them
+  auto work = [&](const char* stage, int s0, int lost) {
+    if (s0 >= keys) return;   // the same for all lanes
+    v16f x[2];
+#pragma unroll
+    for (int kb2 = 0; kb2 < 2; ++kb2) {
+      v16i s = start;
+      const int r = kb2 * 32 + n;
+#pragma unroll
+      for (int i = 0; i < NDB; ++i)
+        s = __builtin_amdgcn_mfma_i32_32x32x32_i8(*reinterpret_cast<const v4i*>(stage + r * DP + swizzle(r, 2 * i + h) * 16), qf[i], s, 0, 0, 0);
+      __builtin_memcpy(&x[kb2], &s, sizeof(s));
+    }
+    if (s0 + PT_KEYS > hi || s0 + PT_KEYS > first_limit || lost != 0) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int r = i & 15;
+        const int key = s0 + (i >> 4) * 32 + (r & 3) + 8 * (r >> 2) + 4 * h;
+        if (key >= hi || key >= limit || (lost >> ((i >> 4) * 2 + (r >> 3)) & 1)) x[i >> 4][r] = -__builtin_inff();
+      }
+    }
+    float top = x[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) top = __builtin_fmaxf(top, x[i >> 4][i & 15]);
+    if (__ballot(__builtin_fmaf(top, cl, off) > 15.0f) != 0) {
+      auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = __builtin_fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
+      const bool moves = __builtin_fmaf(top, cl, off) > 15.0f;
+      const float fresh = moves ? __builtin_fmaf(-top, cl, 8.0f) : off;
+      const float scale = __builtin_amdgcn_exp2f(fresh - off);
+      off = fresh;
+      den *= scale;
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) acc[i] *= scale;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {  // 16 keys
+      v8h pr;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pr[j] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[q >> 1][(q & 1) * 8 + j], cl, off));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) den = __builtin_amdgcn_fdot2(v2h{pr[2 * j], pr[2 * j + 1]}, v2h{(_Float16)1.0f, (_Float16)1.0f}, den, false);
+#pragma unroll
+      for (int i = 0; i < NDB; ++i)
+        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const v8h*>(stage + KBYTES + ((q * NDB + i) * 64 + lane) * 16), pr,
+                                                        acc[i], 0, 0, 0);
+    }
+  };
+  auto lost_of = [&](const int (&pg)[4]) {
+    int lost = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lost |= (pg[i] >= 0 && pg[i] < c.pages ? 0 : 1) << i;
+    return lost;
+  };
+
+  if (lo < hi) {
+    int pg[4], lost, lost_next = 0;
+    auto pages_of = [&](int s0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pg[i] = page_at(s0, i);
+    };
+    auto mine = [&]() { return wave < 2 ? (wave == 0 ? pg[0] : pg[1]) : (wave == 2 ? pg[2] : pg[3]); };
+    pages_of(lo);
+    fetch(lo, mine());
+    lost = lost_of(pg);
+    put(lds);
+    pages_of(lo + PT_KEYS);
+    fetch(lo + PT_KEYS, mine());
+    lost_next = lost_of(pg);
+    pages_of(lo + 2 * PT_KEYS);
+    __syncthreads();
+    // While a step is worked on, the next one goes from registers into the other half of the LDS and the one after it is asked
+    // for.  One barrier a step: who passes it has read its half, which is written only behind it.
+    auto step = [&](const char* now, char* next, int s0) {
+      work(now, s0, lost);
+      lost = lost_next;
+      put(next);
+      fetch(s0 + 2 * PT_KEYS, mine());
+      lost_next = lost_of(pg);
+      pages_of(s0 + 3 * PT_KEYS);
+      __syncthreads();
+    };
+    for (int s0 = lo;;) {
+      step(lds, lds + STAGE, s0);
+      s0 += PT_KEYS;
+      if (s0 >= hi) break;
+      step(lds + STAGE, lds, s0);
+      s0 += PT_KEYS;
+      if (s0 >= hi) break;
+    }
+  }
+
+  // a lane has its row's columns NDB m + i, m = (r & 3) + 8 (r >> 2) + 4 h; the two halves of the wave add their denominators
+  {
+    auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(den), __float_as_uint(den), false, false);
+    den = __uint_as_float(o[0]) + __uint_as_float(o[1]);
+  }
+  if (it.splits == 1) {
+    const float f = den > 0.0f ? a.alpha_pv * 1024.0f / den : 0.0f;
+    if (real) {
+      const long long at = ((long long)(it.s.row0 + t) * a.q_heads + it.head * G + g) * c.D;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = NDB * ((r & 3) + 8 * (r >> 2) + 4 * h);
+        if (d < c.D) {
+          float y[NDB];
+#pragma unroll
+          for (int i = 0; i < NDB; ++i) y[i] = den > 0.0f ? acc[i][r] * f : 0.0f;
+          store_some<NDB, OUT>(a.out, at + d, y);
+        }
+      }
+    }
+    return;
+  }
+  const long long slot = it.first + (long long)it.split * it.step;
+  if (real) {
+    float* to = ws + (slot * PT_ROWS + wave * 32 + n) * DP;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int d = NDB * ((r & 3) + 8 * (r >> 2) + 4 * h);
+      if (d < c.D) {
+#pragma unroll
+        for (int i = 0; i < NDB; i += 2) put2(to + d + i, acc[i][r], acc[i + 1][r]);
+      }
+    }
+    if (h == 0) put2(ws + (long long)p.slots * PT_ROWS * DP + (slot * PT_ROWS + wave * 32 + n) * 2, off, den);
+  }
+  if (p.arrivals != nullptr) meet_and_join<PT_ROWS, DP, OUT>(a, c, p, it, ws, &seen, reinterpret_cast<float*>(lds));
 }
 
 // Joins the slices of the sequences that were cut where they do not meet in the launch itself.
-template <int DP, int OUT>
-__global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p, const float* ws) {
+template <int ROWS, int DP, int OUT>
+__global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p, float* ws) {
   __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
-  const PagedItem it = paged_item(b, c.page_shift, c.heads, PA_ROWS, p, blockIdx.x);
+  const PagedItem it = paged_item(b, c.page_shift, c.heads, ROWS, p, blockIdx.x);
   if (!it.found || it.split != 0 || it.splits == 1) return;
-  join_slices<DP, OUT>(a, c, p, it, ws, meet);
+  join_slices<ROWS, DP, OUT>(a, c, p, it, ws, meet);
 }
 
-// Items that a batch can make: one to each (sequence, key head, 16 rows), and the slices beyond that.
+// Rows to a work item.  Up to 16 rows to a sequence and key head on average, the kernel of few rows; beyond, tiles of 128, in
+// which few rows leave waves idle but keys are read once.
+static int paged_tile(long long rows, long long seqs, long long group) { return rows * group <= 16 * seqs ? PA_ROWS : PT_ROWS; }
+// Items that a batch can make: one to each (sequence, key head, tile of rows), and the slices beyond that.
 static long long paged_units(long long rows, long long seqs, long long group, long long kv_heads, int tile) {
   return kv_heads * (seqs + rows * group / tile);
 }
 static bool paged_cuts(long long capacity) { return capacity > PA_MIN_SLICE; }
 static long long paged_slots(long long rows, long long seqs, long long group, long long kv_heads) {
-  return paged_units(rows, seqs, group, kv_heads, PA_ROWS) + PA_TARGET + 8;
+  return paged_units(rows, seqs, group, kv_heads, paged_tile(rows, seqs, group)) + PA_TARGET + 8;
 }
 static int paged_dp(long long D) { return D <= 64 ? 64 : 128; }
 
@@ -532,15 +797,22 @@ long long paged_attn_arrivals(long long rows, long long seqs, long long q_heads,
 long long paged_attn_workspace_bytes(long long rows, long long seqs, long long q_heads, long long kv_heads, long long D,
                                      long long capacity) {
   if (rows <= 0 || seqs <= 0 || kv_heads <= 0 || !paged_cuts(capacity)) return 0;
-  return paged_slots(rows, seqs, q_heads / kv_heads, kv_heads) * PA_ROWS * (paged_dp(D) + 2) * 4;
+  const long long group = q_heads / kv_heads;
+  return paged_slots(rows, seqs, group, kv_heads) * paged_tile(rows, seqs, group) * (paged_dp(D) + 2) * 4;
 }
 
 template <int DP, int OUT>
-static void launch_rows(const PagedAttn& a, const PagedCache& c, const PagedBatch& b, const PagedPlan& p, float* ws, unsigned grid,
-                        hipStream_t stream) {
-  hipLaunchKernelGGL((paged_attn_rows_kernel<DP, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, p, ws);
-  if (p.target != 0 && p.arrivals == nullptr)
-    hipLaunchKernelGGL((paged_attn_join_kernel<DP, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, p, ws);
+static void launch_attn(int tile, const PagedAttn& a, const PagedCache& c, const PagedBatch& b, const PagedPlan& p, float* ws,
+                        unsigned grid, hipStream_t stream) {
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, p, ws); };
+  const bool join = p.target != 0 && p.arrivals == nullptr;
+  if (tile == PA_ROWS) {
+    launch(paged_attn_rows_kernel<DP, OUT>);
+    if (join) launch(paged_attn_join_kernel<PA_ROWS, DP, OUT>);
+  } else {
+    launch(paged_attn_tiles_kernel<DP, OUT>);
+    if (join) launch(paged_attn_join_kernel<PT_ROWS, DP, OUT>);
+  }
 }
 
 int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, const PagedBatch& b, void* workspace,
@@ -548,25 +820,25 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
   if (b.rows == 0 || a.q_heads == 0) return TI_OK;
   PagedPlan p;
   p.group = a.q_heads / c.heads;
+  const int tile = paged_tile(b.rows, b.seqs, p.group);
   const long long capacity = (long long)b.per_seq << c.page_shift;
   const long long need = paged_attn_workspace_bytes(b.rows, b.seqs, a.q_heads, c.heads, c.D, capacity);
   const bool cut = need > 0 && workspace != nullptr && workspace_bytes >= need;
   p.target = cut ? PA_TARGET : 0;
   p.slots = cut ? (int)paged_slots(b.rows, b.seqs, p.group, c.heads) : 0;
   p.arrivals = a.arrivals != nullptr && a.arrivals_count >= p.slots ? a.arrivals : nullptr;
-  const long long grid = cut ? p.slots : paged_units(b.rows, b.seqs, p.group, c.heads, PA_ROWS);
+  const long long grid = cut ? p.slots : paged_units(b.rows, b.seqs, p.group, c.heads, tile);
   if (grid > 0x7fffff) return fail(TI_ERR_INVALID_ARG, "paged_attn_s8: %lld work items", grid);
   float* ws = static_cast<float*>(workspace);
   const unsigned g = grid > 0 ? (unsigned)grid : 1u;
-  if (paged_dp(c.D) == 64) {
-    if (out_type == PT_S8) launch_rows<64, PT_S8>(a, c, b, p, ws, g, stream);
-    else if (out_type == PT_F16) launch_rows<64, PT_F16>(a, c, b, p, ws, g, stream);
-    else launch_rows<64, PT_BF16>(a, c, b, p, ws, g, stream);
-  } else {
-    if (out_type == PT_S8) launch_rows<128, PT_S8>(a, c, b, p, ws, g, stream);
-    else if (out_type == PT_F16) launch_rows<128, PT_F16>(a, c, b, p, ws, g, stream);
-    else launch_rows<128, PT_BF16>(a, c, b, p, ws, g, stream);
-  }
+  auto run = [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    if (out_type == PT_S8) launch_attn<DP, PT_S8>(tile, a, c, b, p, ws, g, stream);
+    else if (out_type == PT_F16) launch_attn<DP, PT_F16>(tile, a, c, b, p, ws, g, stream);
+    else launch_attn<DP, PT_BF16>(tile, a, c, b, p, ws, g, stream);
+  };
+  if (paged_dp(c.D) == 64) run(std::integral_constant<int, 64>());
+  else run(std::integral_constant<int, 128>());
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(TI_ERR_LAUNCH, "paged_attn_s8 launch: %s", hipGetErrorString(e));
   return TI_OK;
