@@ -22,14 +22,9 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 
 constexpr int PA_WAVES = 4;
 constexpr int PA_ROWS = 16;
-#ifndef PA_TARGET_N
-#define PA_TARGET_N 1024
-#endif
-constexpr int PA_TARGET = PA_TARGET_N;    // work items that the keys are cut into, beyond one to each (sequence, key head, 16 rows)
-#ifndef PA_MIN_N
-#define PA_MIN_N 256
-#endif
-constexpr int PA_MIN_SLICE = PA_MIN_N;  // keys of a slice, at least
+constexpr int PA_TARGET = 512;     // slices that the keys of a batch are cut into, beyond one to each item
+constexpr int PA_FULL = 512;       // items that fill the chip
+constexpr int PA_MIN_SLICE = 512;  // keys of a slice, at least
 constexpr float PA_EMPTY = 3.0e38f;  // offset of a row that has seen no key: 2^(-inf + PA_EMPTY) is 0
 
 struct PagedPlan {
@@ -79,21 +74,27 @@ __device__ __forceinline__ float rows_max(float x) {
   return __builtin_fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// Keys of a slice, the same in every workgroup: what cuts all keys of the batch into `target` equal parts.
+// Keys of a slice, the same in every workgroup: what cuts all keys of the batch into `target` equal parts.  Where the items
+// alone fill the chip, only sequences of more than twice the average are cut: a slice costs its partial sums and the join.
 __device__ __forceinline__ int paged_slice(const PagedBatch& b, int page_shift, int heads, int rows_per_tile, const PagedPlan& p) {
   if (p.target == 0) return 0x7fffffff;
   const int lane = threadIdx.x & 63;
-  float total = 0.0f;
+  float total = 0.0f, items = 0.0f;
   for (int i0 = 0; i0 < b.seqs; i0 += 64) {
-    float mine = 0.0f;
+    float tiles = 0.0f, len = 0.0f;
     if (i0 + lane < b.seqs) {
       const PagedSeq s = paged_seq(b, page_shift, i0 + lane);
-      mine = (float)((s.T * p.group + rows_per_tile - 1) / rows_per_tile) * (float)s.len;
+      tiles = (float)((s.T * p.group + rows_per_tile - 1) / rows_per_tile);
+      len = (float)s.len;
     }
-    total += wave_add(mine);
+    items += wave_add(tiles);
+    total += wave_add(tiles * len);
   }
-  const float want = total * (float)heads / (float)p.target;
-  int slice = want < 1.0e9f ? ((int)want + 64) & ~63 : 1 << 30;
+  items *= (float)heads;
+  total *= (float)heads;
+  float want = total / (float)p.target;
+  if (items >= (float)PA_FULL) want = __builtin_fmaxf(want, 2.0f * total / items);
+  const int slice = want < 1.0e9f ? ((int)want + 64) & ~63 : 1 << 30;
   return slice < PA_MIN_SLICE ? PA_MIN_SLICE : slice;
 }
 
@@ -210,14 +211,16 @@ struct PagedPart {
   }
 };
 
-// The slices of one item, by the threads of one workgroup: a thread owns four columns of a row in every so many-th slice.
+// The slices of one item, rows `first` to `first + rows - 1` of its ROWS, by the threads of one workgroup: a thread owns four
+// columns of a row in every so many-th slice.
 constexpr int PA_THREADS = PA_WAVES * 64;
 template <int ROWS, int DP, int OUT>
 __device__ __forceinline__ void join_slices(const PagedAttn& a, const PagedCache& c, const PagedPlan& p, const PagedItem& it,
-                                            const float* ws, float* meet) {
+                                            const float* ws, float* meet, int first, int rows) {
   const int G = p.group;
-  int rows = it.s.T * G - it.tile * ROWS;
-  rows = rows < ROWS ? rows : ROWS;
+  const int live_rows = it.s.T * G - it.tile * ROWS - first;
+  rows = rows < live_rows ? rows : live_rows;
+  if (rows <= 0) return;
   const int quads = c.D / 4, work = rows * quads;
   const float* tail = ws + (long long)p.slots * ROWS * DP;
   const int lanes = work < PA_THREADS ? PA_THREADS / work : 1;  // threads that share a place
@@ -225,7 +228,7 @@ __device__ __forceinline__ void join_slices(const PagedAttn& a, const PagedCache
     const int share = lanes > 1 ? (int)threadIdx.x / work : 0;
     const int e = lanes > 1 ? (int)threadIdx.x - share * work : e0 + (int)threadIdx.x;
     const bool live = share < lanes && e < work;
-    const int r = live ? e / quads : 0, d = live ? (e - r * quads) * 4 : 0;
+    const int r = first + (live ? e / quads : 0), d = live ? (e - (r - first) * quads) * 4 : 0;
     PagedPart sum = {PA_EMPTY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
     if (live) {
       for (int s0 = share; s0 < it.splits; s0 += 4 * lanes) {
@@ -278,7 +281,7 @@ __device__ __forceinline__ void meet_and_join(const PagedAttn& a, const PagedCac
   }
   __syncthreads();
   if (seen[0] != it.splits - 1) return;
-  join_slices<ROWS, DP, OUT>(a, c, p, it, ws, scratch);
+  join_slices<ROWS, DP, OUT>(a, c, p, it, ws, scratch, 0, ROWS);
 }
 
 // Workspace: partial sums [slots][16][DP] fp32, then (offset, denominator) [slots][16].
@@ -525,6 +528,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAtt
 // Scores start from 1.5 * 2^23 instead of 0: the int32 sum is then the fp32 number 12582912 + x, and the constant goes into the
 // row's offset, where one multiply-add removes it exactly.
 constexpr int PT_ROWS = 128, PT_KEYS = 64;
+constexpr int PT_MEET = 32;  // items from which on slices meet in the launch
 template <int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p, float* ws) {
   constexpr int NDB = DP / 32;   // column blocks of O^T, and steps of 32 along a key row
@@ -604,6 +608,9 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAt
     }
   };
   auto swizzle = [](int r, int chunk) { return DP == 128 ? chunk ^ (r & 7) : chunk ^ ((r >> 2) & 3); };
+  int kat[NDB];  // where this lane's operands of K begin, of the first 32 keys
+#pragma unroll
+  for (int i = 0; i < NDB; ++i) kat[i] = n * DP + swizzle(n, 2 * i + h) * 16;
   auto put = [&](char* stage) {
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
@@ -637,20 +644,31 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAt
   v16i start;
 #pragma unroll
   for (int r = 0; r < 16; ++r) start[r] = 0x4b400000;
+  asm("" : "+v"(start));   // kept in registers, not made anew at every step
 
   // one step: the keys s0 .. s0 + 63 in `stage`; `lost`: bit i is set where the pool has no page for the i-th 16 of them
   auto work = [&](const char* stage, int s0, int lost) {
     if (s0 >= keys) return;   // the same for all lanes
+    v4i kf[2][NDB];
+#pragma unroll
+    for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) kf[kb2][i] = *reinterpret_cast<const v4i*>(stage + kb2 * 32 * DP + kat[i]);
+    __builtin_amdgcn_sched_barrier(0);
     v16f x[2];
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2) {
       v16i s = start;
-      const int r = kb2 * 32 + n;
 #pragma unroll
-      for (int i = 0; i < NDB; ++i)
-        s = __builtin_amdgcn_mfma_i32_32x32x32_i8(*reinterpret_cast<const v4i*>(stage + r * DP + swizzle(r, 2 * i + h) * 16), qf[i], s, 0, 0, 0);
+      for (int i = 0; i < NDB; ++i) s = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[kb2][i], qf[i], s, 0, 0, 0);
       __builtin_memcpy(&x[kb2], &s, sizeof(s));
     }
+    v8h vf[2][NDB];
+    auto vload = [&](int q) {
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) vf[q & 1][i] = *reinterpret_cast<const v8h*>(stage + KBYTES + ((q * NDB + i) * 64 + lane) * 16);
+    };
+    vload(0);
     if (s0 + PT_KEYS > hi || s0 + PT_KEYS > first_limit || lost != 0) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
@@ -680,34 +698,32 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAt
       for (int j = 0; j < 8; ++j) pr[j] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[q >> 1][(q & 1) * 8 + j], cl, off));
 #pragma unroll
       for (int j = 0; j < 4; ++j) den = __builtin_amdgcn_fdot2(v2h{pr[2 * j], pr[2 * j + 1]}, v2h{(_Float16)1.0f, (_Float16)1.0f}, den, false);
+      if (q < 3) vload(q + 1);
 #pragma unroll
-      for (int i = 0; i < NDB; ++i)
-        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const v8h*>(stage + KBYTES + ((q * NDB + i) * 64 + lane) * 16), pr,
-                                                        acc[i], 0, 0, 0);
+      for (int i = 0; i < NDB; ++i) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[q & 1][i], pr, acc[i], 0, 0, 0);
     }
   };
-  auto lost_of = [&](const int (&pg)[4]) {
-    int lost = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) lost |= (pg[i] >= 0 && pg[i] < c.pages ? 0 : 1) << i;
-    return lost;
-  };
-
   if (lo < hi) {
-    int pg[4], lost, lost_next = 0;
-    auto pages_of = [&](int s0) {
+    // pages a step ahead of the keys: the wave's own, and which of the four blocks of 16 keys have none
+    int page, gone;
+    auto look = [&](int s0) {
+      page = page_at(s0, wave);
+      gone = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pg[i] = page_at(s0, i);
+      for (int i = 0; i < 4; ++i) {
+        const int pg = page_at(s0, i);
+        gone |= (pg >= 0 && pg < c.pages ? 0 : 1) << i;
+      }
     };
-    auto mine = [&]() { return wave < 2 ? (wave == 0 ? pg[0] : pg[1]) : (wave == 2 ? pg[2] : pg[3]); };
-    pages_of(lo);
-    fetch(lo, mine());
-    lost = lost_of(pg);
+    int lost, lost_next;
+    look(lo);
+    fetch(lo, page);
+    lost = gone;
     put(lds);
-    pages_of(lo + PT_KEYS);
-    fetch(lo + PT_KEYS, mine());
-    lost_next = lost_of(pg);
-    pages_of(lo + 2 * PT_KEYS);
+    look(lo + PT_KEYS);
+    fetch(lo + PT_KEYS, page);
+    lost_next = gone;
+    look(lo + 2 * PT_KEYS);
     __syncthreads();
     // While a step is worked on, the next one goes from registers into the other half of the LDS and the one after it is asked
     // for.  One barrier a step: who passes it has read its half, which is written only behind it.
@@ -715,9 +731,9 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAt
       work(now, s0, lost);
       lost = lost_next;
       put(next);
-      fetch(s0 + 2 * PT_KEYS, mine());
-      lost_next = lost_of(pg);
-      pages_of(s0 + 3 * PT_KEYS);
+      fetch(s0 + 2 * PT_KEYS, page);
+      lost_next = gone;
+      look(s0 + 3 * PT_KEYS);
       __syncthreads();
     };
     for (int s0 = lo;;) {
@@ -768,13 +784,13 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAt
   if (p.arrivals != nullptr) meet_and_join<PT_ROWS, DP, OUT>(a, c, p, it, ws, &seen, reinterpret_cast<float*>(lds));
 }
 
-// Joins the slices of the sequences that were cut where they do not meet in the launch itself.
+// Joins the slices of the sequences that were cut where they do not meet in the launch itself; 16 rows to blockIdx.y.
 template <int ROWS, int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p, float* ws) {
   __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
   const PagedItem it = paged_item(b, c.page_shift, c.heads, ROWS, p, blockIdx.x);
   if (!it.found || it.split != 0 || it.splits == 1) return;
-  join_slices<ROWS, DP, OUT>(a, c, p, it, ws, meet);
+  join_slices<ROWS, DP, OUT>(a, c, p, it, ws, meet, blockIdx.y * PA_ROWS, PA_ROWS);
 }
 
 // Rows to a work item.  Up to 16 rows to a sequence and key head on average, the kernel of few rows; beyond, tiles of 128, in
@@ -804,14 +820,16 @@ long long paged_attn_workspace_bytes(long long rows, long long seqs, long long q
 template <int DP, int OUT>
 static void launch_attn(int tile, const PagedAttn& a, const PagedCache& c, const PagedBatch& b, const PagedPlan& p, float* ws,
                         unsigned grid, hipStream_t stream) {
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, p, ws); };
+  auto launch = [&](auto kernel, unsigned groups) {
+    hipLaunchKernelGGL(kernel, dim3(grid, groups), dim3(PA_THREADS), 0, stream, a, c, b, p, ws);
+  };
   const bool join = p.target != 0 && p.arrivals == nullptr;
   if (tile == PA_ROWS) {
-    launch(paged_attn_rows_kernel<DP, OUT>);
-    if (join) launch(paged_attn_join_kernel<PA_ROWS, DP, OUT>);
+    launch(paged_attn_rows_kernel<DP, OUT>, 1);
+    if (join) launch(paged_attn_join_kernel<PA_ROWS, DP, OUT>, 1);
   } else {
-    launch(paged_attn_tiles_kernel<DP, OUT>);
-    if (join) launch(paged_attn_join_kernel<PT_ROWS, DP, OUT>);
+    launch(paged_attn_tiles_kernel<DP, OUT>, 1);
+    if (join) launch(paged_attn_join_kernel<PT_ROWS, DP, OUT>, PT_ROWS / PA_ROWS);
   }
 }
 
@@ -827,6 +845,8 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
   p.target = cut ? PA_TARGET : 0;
   p.slots = cut ? (int)paged_slots(b.rows, b.seqs, p.group, c.heads) : 0;
   p.arrivals = a.arrivals != nullptr && a.arrivals_count >= p.slots ? a.arrivals : nullptr;
+  // few items of 128 rows have many slices of 66 KB each, which one workgroup would be long in joining
+  if (tile == PT_ROWS && paged_units(b.rows, b.seqs, p.group, c.heads, tile) < PT_MEET) p.arrivals = nullptr;
   const long long grid = cut ? p.slots : paged_units(b.rows, b.seqs, p.group, c.heads, tile);
   if (grid > 0x7fffff) return fail(TI_ERR_INVALID_ARG, "paged_attn_s8: %lld work items", grid);
   float* ws = static_cast<float*>(workspace);
