@@ -534,8 +534,8 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAt
   constexpr int NDB = DP / 32;   // column blocks of O^T, and steps of 32 along a key row
   constexpr int KC = DP / 64;    // 16-byte pieces of K that a thread brings
   constexpr int CH = DP / 16;    // 16-byte chunks of a key row
-  constexpr int KBYTES = PT_KEYS * DP, STAGE = 3 * KBYTES;
-  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+  constexpr int KBYTES = PT_KEYS * DP, VBYTES = 2 * KBYTES;
+  __shared__ __attribute__((aligned(16))) char lds[3 * (KBYTES + VBYTES)];  // three steps of K, then of V
   __shared__ int seen;
 
   if (a.fill) paged_fill(b, static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
@@ -565,6 +565,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAt
   const int lo = lo_ll < most ? (int)lo_ll : most;
   const int hi = lo_ll + it.slice < most ? (int)(lo_ll + it.slice) : most;
   keys = keys < hi ? keys : hi;
+  const int whole = first_limit < hi ? first_limit : hi;  // up to here every row of the wave sees every key
 
   v4i qf[NDB];
 #pragma unroll
@@ -580,10 +581,14 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAt
   const auto table = (const __attribute__((address_space(4))) int*)(b.table + (long long)it.seq * b.per_seq);
   const int mask = (1 << c.page_shift) - 1, last_block = hi > 0 ? (hi - 1) >> 4 : 0;
 
-  // what this thread brings of a step: of the wave's 16 keys, KC chunks of K and the columns NDB n .. of eight rows of V
+  // What this thread brings of a step: of the wave's 16 keys, KC chunks of K and the columns NDB n .. of eight rows of V.
   const int krow = lane / CH, kchunk = lane % CH;
-  const unsigned kcol = (unsigned)(krow * c.k_token) + (kchunk * 16 < c.D ? kchunk * 16u : 0u);
-  const unsigned vcol = (unsigned)(h * 4 * c.v_token) + (n * NDB < c.D ? (unsigned)(n * NDB) : 0u);
+  unsigned kcol[KC], vcol[8];
+#pragma unroll
+  for (int i = 0; i < KC; ++i) kcol[i] = (unsigned)((i * (64 / CH) + krow) * c.k_token) + (kchunk * 16 < c.D ? kchunk * 16u : 0u);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    vcol[j] = (unsigned)((h * 4 + (j & 3) + 8 * (j >> 2)) * c.v_token) + (n * NDB < c.D ? (unsigned)(n * NDB) : 0u);
   v4i kreg[KC];
   unsigned vreg[8];
   auto page_at = [&](int s0, int blk) {
@@ -591,32 +596,41 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAt
     at = at < last_block ? at : last_block;
     return table[(at << 4) >> c.page_shift];
   };
-  auto fetch = [&](int s0, int page) {
+  auto have = [&](int page) { return page >= 0 && page < c.pages; };
+  auto place = [&](int s0) {  // where the wave's 16 keys begin in their page
     int at = (s0 >> 4) + wave;
     at = at < last_block ? at : last_block;
-    page = page >= 0 && page < c.pages ? page : 0;
-    const long long o = (at << 4) & mask;
-    const int8_t* kr = kb + (long long)page * c.k_page + o * c.k_token;
+    return (at << 4) & mask;
+  };
+  auto fetch_k = [&](int s0, int page) {
+    const int8_t* kr = kb + (long long)(have(page) ? page : 0) * c.k_page + place(s0) * c.k_token;
 #pragma unroll
-    for (int i = 0; i < KC; ++i) kreg[i] = *reinterpret_cast<const v4i*>(kr + (long long)(i * (64 / CH)) * c.k_token + kcol);
-    const int8_t* vr = vb + (long long)page * c.v_page + o * c.v_token;
+    for (int i = 0; i < KC; ++i) kreg[i] = *reinterpret_cast<const v4i*>(kr + kcol[i]);
+  };
+  auto fetch_v = [&](int s0, int page) {
+    const int8_t* vr = vb + (long long)(have(page) ? page : 0) * c.v_page + place(s0) * c.v_token;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int8_t* at_row = vr + (long long)((j & 3) + 8 * (j >> 2)) * c.v_token + vcol;
-      if constexpr (NDB == 4) vreg[j] = *reinterpret_cast<const unsigned*>(at_row);
-      else vreg[j] = *reinterpret_cast<const unsigned short*>(at_row);
+      if constexpr (NDB == 4) vreg[j] = *reinterpret_cast<const unsigned*>(vr + vcol[j]);
+      else vreg[j] = *reinterpret_cast<const unsigned short*>(vr + vcol[j]);
     }
   };
+  // whether the pool lacks any of the item's pages: looked at once, so that steps need not
+  bool holes = false;
+  for (int i = (lo >> c.page_shift) + lane; i <= (hi - 1) >> c.page_shift; i += 64) holes |= !have(table[i]);
+  holes = __ballot(holes) != 0;
   auto swizzle = [](int r, int chunk) { return DP == 128 ? chunk ^ (r & 7) : chunk ^ ((r >> 2) & 3); };
   int kat[NDB];  // where this lane's operands of K begin, of the first 32 keys
 #pragma unroll
   for (int i = 0; i < NDB; ++i) kat[i] = n * DP + swizzle(n, 2 * i + h) * 16;
-  auto put = [&](char* stage) {
+  auto put_k = [&](int slot) {
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
       const int r = wave * 16 + i * (64 / CH) + krow;
-      *reinterpret_cast<v4i*>(stage + r * DP + swizzle(r, kchunk) * 16) = kreg[i];
+      *reinterpret_cast<v4i*>(lds + slot * KBYTES + r * DP + swizzle(r, kchunk) * 16) = kreg[i];
     }
+  };
+  auto put_v = [&](int slot) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) vreg[j] ^= 0x80808080u;
 #pragma unroll
@@ -631,7 +645,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAt
         x[2 * j] = y[0];
         x[2 * j + 1] = y[1];
       }
-      *reinterpret_cast<v8h*>(stage + KBYTES + ((wave * NDB + i) * 64 + lane) * 16) = x;
+      *reinterpret_cast<v8h*>(lds + 3 * KBYTES + slot * VBYTES + ((wave * NDB + i) * 64 + lane) * 16) = x;
     }
   };
 
@@ -646,104 +660,170 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAt
   for (int r = 0; r < 16; ++r) start[r] = 0x4b400000;
   asm("" : "+v"(start));   // kept in registers, not made anew at every step
 
-  // one step: the keys s0 .. s0 + 63 in `stage`; `lost`: bit i is set where the pool has no page for the i-th 16 of them
-  auto work = [&](const char* stage, int s0, int lost) {
-    if (s0 >= keys) return;   // the same for all lanes
-    v4i kf[2][NDB];
+  // scores of 32 keys, whose rows of K begin at `at` in the LDS
+  auto scores = [&](int at) {
+    v4i kf[NDB];
 #pragma unroll
-    for (int kb2 = 0; kb2 < 2; ++kb2)
+    for (int i = 0; i < NDB; ++i) kf[i] = *reinterpret_cast<const v4i*>(lds + at + kat[i]);
+    v16i t = start;
 #pragma unroll
-      for (int i = 0; i < NDB; ++i) kf[kb2][i] = *reinterpret_cast<const v4i*>(stage + kb2 * 32 * DP + kat[i]);
-    __builtin_amdgcn_sched_barrier(0);
-    v16f x[2];
+    for (int i = 0; i < NDB; ++i) t = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[i], qf[i], t, 0, 0, 0);
+    v16f x;
+    __builtin_memcpy(&x, &t, sizeof(t));
+    return x;
+  };
+  // O^T += V^T P^T of 32 keys, whose operands begin at `at`
+  auto gather = [&](int at, const v8h (&pr)[2]) {
 #pragma unroll
-    for (int kb2 = 0; kb2 < 2; ++kb2) {
-      v16i s = start;
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
-      for (int i = 0; i < NDB; ++i) s = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[kb2][i], qf[i], s, 0, 0, 0);
-      __builtin_memcpy(&x[kb2], &s, sizeof(s));
-    }
-    v8h vf[2][NDB];
-    auto vload = [&](int q) {
+      for (int i = 0; i < NDB; ++i)
+        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const v8h*>(lds + at + ((q * NDB + i) * 64 + lane) * 16), pr[q],
+                                                        acc[i], 0, 0, 0);
+  };
+  // 32 keys from s0 on: the softmax of their scores x into `pr`, beside it the scores of the 32 keys behind them and the products
+  // of the 32 before them, whose probabilities are `before`
+  auto half = [&](v16f& x, v16f& next, v8h (&pr)[2], v8h (&before)[2], int s0, int lost, int k_at, int v_at) {
+    if (__builtin_expect(s0 + 32 > whole || lost != 0, 0)) {
 #pragma unroll
-      for (int i = 0; i < NDB; ++i) vf[q & 1][i] = *reinterpret_cast<const v8h*>(stage + KBYTES + ((q * NDB + i) * 64 + lane) * 16);
-    };
-    vload(0);
-    if (s0 + PT_KEYS > hi || s0 + PT_KEYS > first_limit || lost != 0) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const int r = i & 15;
-        const int key = s0 + (i >> 4) * 32 + (r & 3) + 8 * (r >> 2) + 4 * h;
-        if (key >= hi || key >= limit || (lost >> ((i >> 4) * 2 + (r >> 3)) & 1)) x[i >> 4][r] = -__builtin_inff();
+      for (int r = 0; r < 16; ++r) {
+        const int key = s0 + (r & 3) + 8 * (r >> 2) + 4 * h;
+        if (key >= hi || key >= limit || (lost >> (r >> 3) & 1)) x[r] = -__builtin_inff();
       }
     }
-    float top = x[0][0];
+    float top = x[0];
 #pragma unroll
-    for (int i = 1; i < 32; ++i) top = __builtin_fmaxf(top, x[i >> 4][i & 15]);
-    if (__ballot(__builtin_fmaf(top, cl, off) > 15.0f) != 0) {
+    for (int r = 1; r < 16; ++r) top = __builtin_fmaxf(top, x[r]);
+    if (__builtin_expect(__ballot(__builtin_fmaf(top, cl, off) > 15.0f) != 0, 0)) {
+      // A new reference.  It moves by a whole number, so that what is relative to the old one is scaled without rounding.
       auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
       top = __builtin_fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
-      const bool moves = __builtin_fmaf(top, cl, off) > 15.0f;
-      const float fresh = moves ? __builtin_fmaf(-top, cl, 8.0f) : off;
-      const float scale = __builtin_amdgcn_exp2f(fresh - off);
-      off = fresh;
+      const float above = __builtin_fmaf(top, cl, off) - 8.0f;
+      const bool moves = above > 7.0f, first = off == PA_EMPTY;
+      const float by = moves ? __builtin_ceilf(above) : 0.0f;
+      const float scale = first && moves ? 0.0f : __builtin_amdgcn_exp2f(-by);
+      off = !moves ? off : first ? __builtin_fmaf(-top, cl, 8.0f) : off - by;
       den *= scale;
+      const _Float16 scale_h = (_Float16)scale;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) before[q] *= scale_h;
 #pragma unroll
       for (int i = 0; i < NDB; ++i) acc[i] *= scale;
     }
+    v4i kf[NDB];
+    v8h vf[2][NDB];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {  // 16 keys
-      v8h pr;
+    for (int i = 0; i < NDB; ++i) kf[i] = *reinterpret_cast<const v4i*>(lds + k_at + kat[i]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) pr[j] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[q >> 1][(q & 1) * 8 + j], cl, off));
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) den = __builtin_amdgcn_fdot2(v2h{pr[2 * j], pr[2 * j + 1]}, v2h{(_Float16)1.0f, (_Float16)1.0f}, den, false);
-      if (q < 3) vload(q + 1);
-#pragma unroll
-      for (int i = 0; i < NDB; ++i) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[q & 1][i], pr, acc[i], 0, 0, 0);
-    }
-  };
-  if (lo < hi) {
-    // pages a step ahead of the keys: the wave's own, and which of the four blocks of 16 keys have none
-    int page, gone;
-    auto look = [&](int s0) {
-      page = page_at(s0, wave);
-      gone = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int pg = page_at(s0, i);
-        gone |= (pg >= 0 && pg < c.pages ? 0 : 1) << i;
+      for (int i = 0; i < NDB; ++i) vf[q][i] = *reinterpret_cast<const v8h*>(lds + v_at + ((q * NDB + i) * 64 + lane) * 16);
+    // Products and softmax in bundles that the compiler keeps in order: a matrix instruction, then the vector instructions that
+    // run beside it.  A pair of scores goes through its multiply-adds and exponentials in one bundle, is rounded in the next and
+    // added to the denominator in the one behind that, so nothing waits for the instruction before it.
+    v16i t = start;
+    float e[2][2];
+    v2h two[8];
+    auto softmax = [&](int m) {
+      if (m >= 2 && m - 2 < 8) den = __builtin_amdgcn_fdot2(two[m - 2], v2h{(_Float16)1.0f, (_Float16)1.0f}, den, false);
+      if (m >= 1 && m - 1 < 8) two[m - 1] = v2h{(_Float16)e[(m - 1) & 1][0], (_Float16)e[(m - 1) & 1][1]};
+      if (m < 8) {
+        e[m & 1][0] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * m], cl, off));
+        e[m & 1][1] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * m + 1], cl, off));
       }
     };
-    int lost, lost_next;
-    look(lo);
-    fetch(lo, page);
-    lost = gone;
-    put(lds);
-    look(lo + PT_KEYS);
-    fetch(lo + PT_KEYS, page);
-    lost_next = gone;
-    look(lo + 2 * PT_KEYS);
-    __syncthreads();
-    // While a step is worked on, the next one goes from registers into the other half of the LDS and the one after it is asked
-    // for.  One barrier a step: who passes it has read its half, which is written only behind it.
-    auto step = [&](const char* now, char* next, int s0) {
-      work(now, s0, lost);
-      lost = lost_next;
-      put(next);
-      fetch(s0 + 2 * PT_KEYS, page);
-      lost_next = gone;
-      look(s0 + 3 * PT_KEYS);
-      __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    softmax(0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < NDB; ++i) {
+      t = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[i], qf[i], t, 0, 0, 0);
+      softmax(2 * i + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0][i], before[0], acc[i], 0, 0, 0);
+      softmax(2 * i + 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < NDB; ++i) {
+      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[1][i], before[1], acc[i], 0, 0, 0);
+      softmax(2 * NDB + 1 + i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int m = 3 * NDB + 1; m < 10; ++m) softmax(m);
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        pr[q][2 * j] = two[q * 4 + j][0];
+        pr[q][2 * j + 1] = two[q * 4 + j][1];
+      }
+    __builtin_memcpy(&next, &t, sizeof(t));
+  };
+
+  if (lo < hi) {
+    auto lost = [&](int s0) {
+      int bits = 0;
+      if (__builtin_expect(holes, 0))
+        for (int i = 0; i < 4; ++i) bits |= (have(page_at(s0, i)) ? 0 : 1) << i;
+      return bits;
     };
-    for (int s0 = lo;;) {
-      step(lds, lds + STAGE, s0);
-      s0 += PT_KEYS;
-      if (s0 >= hi) break;
-      step(lds + STAGE, lds, s0);
+    // Pages are looked up a step ahead, by vector loads: these return in order, so that the wait for the keys and values in
+    // front of one is all the wait it needs (a scalar one would have to be over at every wait for the LDS).
+    int zero = 0;
+    asm("" : "+v"(zero));
+    auto ask = [&](int s0) {
+      int at = (s0 >> 4) + wave;
+      at = at < last_block ? at : last_block;
+      return b.table[(long long)it.seq * b.per_seq + ((at << 4) >> c.page_shift) + zero];
+    };
+    int page = page_at(lo, wave), page_v;
+    fetch_k(lo, page);
+    fetch_v(lo, page);
+    put_k(0);
+    put_v(0);
+    page = page_at(lo + PT_KEYS, wave);
+    fetch_k(lo + PT_KEYS, page);
+    fetch_v(lo + PT_KEYS, page);
+    put_k(1);
+    page_v = page_at(lo + 2 * PT_KEYS, wave);
+    fetch_k(lo + 2 * PT_KEYS, page_v);
+    int asked = ask(lo + 3 * PT_KEYS);
+    __syncthreads();
+    v16f even = scores(0), odd;
+    v8h pr_even[2], pr_odd[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pr_odd[q][j] = (_Float16)0.0f;
+    constexpr int V0 = 3 * KBYTES, K_HALF = 32 * DP, V_HALF = VBYTES / 2;
+    // slots of this step, of the next one and of the one behind it; V of the step before is in the third of them
+    int k0 = 0, k1 = 1, k2 = 2;
+    int v_before = V0 + V_HALF;   // (the first step takes its own V, times zero)
+    // A step is 64 keys.  What is read in it: the second half of its K and the first of the next one's, the second half of V
+    // before it and the first of its own; what is written: V of the next step and K of the one behind that, in places that the
+    // step before has read, which one barrier a step makes sure of.
+    int s0 = lo;
+    for (;;) {
+      const int gone = lost(s0);
+      const bool here = s0 < keys + 32;  // the same for all lanes: with the half behind its last keys a wave gathers those
+      if (__builtin_expect(here, 1)) half(even, odd, pr_even, pr_odd, s0, gone & 3, k0 * KBYTES + K_HALF, v_before);
+      put_v(k1);
+      fetch_v(s0 + 2 * PT_KEYS, page_v);
+      if (__builtin_expect(here, 1)) half(odd, even, pr_odd, pr_even, s0 + 32, gone >> 2, k1 * KBYTES, V0 + k0 * VBYTES);
+      put_k(k2);
+      page_v = __builtin_amdgcn_readfirstlane(asked);
+      fetch_k(s0 + 3 * PT_KEYS, page_v);
+      asked = ask(s0 + 4 * PT_KEYS);
+      __syncthreads();
+      v_before = V0 + k0 * VBYTES + V_HALF;
+      const int k = k0;
+      k0 = k1, k1 = k2, k2 = k;
       s0 += PT_KEYS;
       if (s0 >= hi) break;
     }
+    if (s0 < keys + 32) gather(v_before, pr_odd);  // nobody has done it: the wave's keys reach into the last half
   }
 
   // a lane has its row's columns NDB m + i, m = (r & 3) + 8 (r >> 2) + 4 h; the two halves of the wave add their denominators
