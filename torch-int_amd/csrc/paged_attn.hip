@@ -27,11 +27,18 @@ constexpr int PA_FULL = 512;       // items that fill the chip
 constexpr int PA_MIN_SLICE = 512;  // keys of a slice, at least
 constexpr float PA_EMPTY = 3.0e38f;  // offset of a row that has seen no key: 2^(-inf + PA_EMPTY) is 0
 
+// The sequences that one of the two kernels takes, by how many rows a key head has in them, and how their keys are cut.
 struct PagedPlan {
-  int group;      // query heads of a key head
-  int target;     // slices that the keys are cut into; 0: nothing is cut
-  int slots;      // items the workspace holds
-  int* arrivals;  // [slots] zeros, or null: a second launch joins the slices
+  int group;        // query heads of a key head
+  int least, most;  // rows of a sequence: more than `least`, up to `most`
+  int target;       // slices that the keys are cut into; 0: nothing is cut
+  int slots;        // work items at most: what the grid and the workspace hold
+  float* ws;        // partial sums [slots][rows of an item][DP] fp32, then (offset, denominator) [slots][rows]
+  int* arrivals;    // [slots] zeros, or null: a second launch joins the slices
+  __device__ __forceinline__ int tiles(const PagedSeq& s, int rows_per_tile) const {
+    const int rows = s.T * group;
+    return rows > least && rows <= most ? (rows + rows_per_tile - 1) / rows_per_tile : 0;
+  }
 };
 
 struct PagedItem {
@@ -84,7 +91,7 @@ __device__ __forceinline__ int paged_slice(const PagedBatch& b, int page_shift, 
     float tiles = 0.0f, len = 0.0f;
     if (i0 + lane < b.seqs) {
       const PagedSeq s = paged_seq(b, page_shift, i0 + lane);
-      tiles = (float)((s.T * p.group + rows_per_tile - 1) / rows_per_tile);
+      tiles = (float)p.tiles(s, rows_per_tile);
       len = (float)s.len;
     }
     items += wave_add(tiles);
@@ -111,7 +118,7 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
     int n = 0, tiles = 0, splits = 0;
     if (i0 + lane < b.seqs) {
       s = paged_seq(b, page_shift, i0 + lane);
-      tiles = (s.T * p.group + rows_per_tile - 1) / rows_per_tile;
+      tiles = p.tiles(s, rows_per_tile);
       splits = s.len <= it.slice ? 1 : (s.len + it.slice - 1) / it.slice;
       // a cu_new that descends can count rows many times over: no sum of items passes the range of int
       const long long all = (long long)tiles * splits * heads;
@@ -187,21 +194,21 @@ __device__ __forceinline__ void store_some(void* out, long long at, const float 
   }
 }
 
-// Two floats written, or read, past the caches of the XCD: partial results that another XCD's workgroup joins.
+// Partial sums are written past the cache of the XCD, for another XCD's workgroup to join.
+__device__ __forceinline__ void put4(float* p, float x, float y, float z, float w) {
+  const v4f v = {x, y, z, w};
+  asm volatile("global_store_dwordx4 %0, %1, off sc1" ::"v"(p), "v"(v) : "memory");
+}
 __device__ __forceinline__ void put2(float* p, float x, float y) {
   const unsigned long long w = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
   __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float2 get2(const float* p) {
-  const unsigned long long w =
-      __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return make_float2(__uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32)));
-}
 
 // A row's partial sums y relative to the offset `off`, with their denominator, and how two of them add up.
 struct PagedPart {
-  float off, den, y[4];
-  __device__ __forceinline__ void add(float o, float d, const float (&x)[4]) {
+  float off, den;
+  v4f y;
+  __device__ __forceinline__ void add(float o, float d, const v4f& x) {
     const float least = o < off ? o : off;
     const float mine = __builtin_amdgcn_exp2f(least - off), theirs = __builtin_amdgcn_exp2f(least - o);
     off = least;
@@ -211,68 +218,79 @@ struct PagedPart {
   }
 };
 
-// The slices of one item, rows `first` to `first + rows - 1` of its ROWS, by the threads of one workgroup: a thread owns four
-// columns of a row in every so many-th slice.
 constexpr int PA_THREADS = PA_WAVES * 64;
+// The slices of one item, rows `first` to `first + rows - 1` of its ROWS, by the threads of one workgroup.  A place is four
+// columns of a row; where there are fewer places than threads, several threads share one and meet in the LDS.
 template <int ROWS, int DP, int OUT>
 __device__ __forceinline__ void join_slices(const PagedAttn& a, const PagedCache& c, const PagedPlan& p, const PagedItem& it,
-                                            const float* ws, float* meet, int first, int rows) {
-  const int G = p.group;
+                                            float* meet, int first, int rows) {
+  const int G = p.group, tid = threadIdx.x;
   const int live_rows = it.s.T * G - it.tile * ROWS - first;
   rows = rows < live_rows ? rows : live_rows;
   if (rows <= 0) return;
   const int quads = c.D / 4, work = rows * quads;
-  const float* tail = ws + (long long)p.slots * ROWS * DP;
-  const int lanes = work < PA_THREADS ? PA_THREADS / work : 1;  // threads that share a place
-  for (int e0 = 0; e0 < work; e0 += PA_THREADS) {
-    const int share = lanes > 1 ? (int)threadIdx.x / work : 0;
-    const int e = lanes > 1 ? (int)threadIdx.x - share * work : e0 + (int)threadIdx.x;
-    const bool live = share < lanes && e < work;
-    const int r = first + (live ? e / quads : 0), d = live ? (e - (r - first) * quads) * 4 : 0;
-    PagedPart sum = {PA_EMPTY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
-    if (live) {
-      for (int s0 = share; s0 < it.splits; s0 += 4 * lanes) {
-        float2 od[4], y0[4], y1[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {  // four slices on their way at once; those behind the last one read it again
-          const int s = s0 + u * lanes < it.splits ? s0 + u * lanes : it.splits - 1;
-          const long long row = (it.first + (long long)s * it.step) * ROWS + r;
-          od[u] = get2(tail + row * 2);
-          y0[u] = get2(ws + row * DP + d);
-          y1[u] = get2(ws + row * DP + d + 2);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (s0 + u * lanes < it.splits) sum.add(od[u].x, od[u].y, {y0[u].x, y0[u].y, y1[u].x, y1[u].y});
-      }
-    }
-    if (lanes > 1) {
-      float* mine = meet + threadIdx.x * 8;
-      mine[0] = sum.off, mine[1] = sum.den;
-      *reinterpret_cast<v4f*>(mine + 4) = v4f{sum.y[0], sum.y[1], sum.y[2], sum.y[3]};
-      __syncthreads();
-      if (share != 0) return;
-      for (int o = 1; o < lanes; ++o) {
-        const float* at = meet + (threadIdx.x + o * work) * 8;
-        sum.add(at[0], at[1], {at[4], at[5], at[6], at[7]});
-      }
-    }
-    if (!live) continue;
+  const float* tail = p.ws + (long long)p.slots * ROWS * DP;
+  const PagedPart none = {PA_EMPTY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+  auto row_of = [&](int e) { return first + e / quads; };
+  auto take = [&](PagedPart& sum, int e, int s) {
+    const int r = row_of(e), d = (e - (r - first) * quads) * 4;
+    const long long row = (it.first + (long long)s * it.step) * ROWS + r;
+    const float2 od = *reinterpret_cast<const float2*>(tail + row * 2);
+    sum.add(od.x, od.y, *reinterpret_cast<const v4f*>(p.ws + row * DP + d));
+  };
+  auto give = [&](const PagedPart& sum, int e) {
+    const int r = row_of(e), d = (e - (r - first) * quads) * 4;
     const float f = sum.den > 0.0f ? a.alpha_pv * 1024.0f / sum.den : 0.0f;
     float y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = sum.den > 0.0f ? sum.y[i] * f : 0.0f;
     const int rr = it.tile * ROWS + r, tt = rr / G;
     store_some<4, OUT>(a.out, ((long long)(it.s.row0 + tt) * a.q_heads + it.head * G + rr - tt * G) * c.D + d, y);
+  };
+  if (work < PA_THREADS) {
+    const int lanes = PA_THREADS / work, share = tid / work, e = tid - share * work;  // (a few threads may be left over)
+    PagedPart sum = none;
+    if (share < lanes) {
+#pragma unroll 4
+      for (int s = share; s < it.splits; s += lanes) take(sum, e, s);
+    }
+    float* mine = meet + tid * 8;
+    mine[0] = sum.off, mine[1] = sum.den;
+    *reinterpret_cast<v4f*>(mine + 4) = sum.y;
+    __syncthreads();
+    if (share != 0) return;
+    for (int o = 1; o < lanes; ++o) {
+      const float* at = meet + (tid + o * work) * 8;
+      sum.add(at[0], at[1], *reinterpret_cast<const v4f*>(at + 4));
+    }
+    give(sum, e);
+    return;
+  }
+  constexpr int EACH = 4;  // places of a thread at once: their loads are under way together
+  for (int e0 = tid; e0 < work; e0 += EACH * PA_THREADS) {
+    PagedPart sum[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) sum[k] = none;
+#pragma unroll 2
+    for (int s = 0; s < it.splits; ++s)
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        const int e = e0 + k * PA_THREADS;
+        take(sum[k], e < work ? e : e0, s);
+      }
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+      if (e0 + k * PA_THREADS < work) give(sum[k], e0 + k * PA_THREADS);
   }
 }
 
-// The workgroup that arrives last joins the slices, in their order: the bits do not depend on who that is.  Partial results
-// and the counter go past the XCDs' caches (device-scope atomics), so no cache has to be written back or emptied: a
-// thread's stores have arrived when its count of them is zero.  `scratch`: LDS of the workgroup that nobody reads any more.
+// The workgroup that arrives last joins the slices, in their order: the bits do not depend on who that is.  Partial sums are
+// written through to memory and the counter is a device-scope atomic, so no cache has to be written back: a thread's stores have
+// arrived when its count of them is zero.  `scratch`: LDS of the workgroup that nobody reads any more.
 template <int ROWS, int DP, int OUT>
 __device__ __forceinline__ void meet_and_join(const PagedAttn& a, const PagedCache& c, const PagedPlan& p, const PagedItem& it,
-                                              const float* ws, int* seen, float* scratch) {
+                                              int* seen, float* scratch) {
+  if (p.arrivals == nullptr) return;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -281,21 +299,22 @@ __device__ __forceinline__ void meet_and_join(const PagedAttn& a, const PagedCac
   }
   __syncthreads();
   if (seen[0] != it.splits - 1) return;
-  join_slices<ROWS, DP, OUT>(a, c, p, it, ws, scratch, 0, ROWS);
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  join_slices<ROWS, DP, OUT>(a, c, p, it, scratch, 0, ROWS);
 }
 
-// Workspace: partial sums [slots][16][DP] fp32, then (offset, denominator) [slots][16].
+constexpr int rows_lds(int DP) { return PA_WAVES * PA_ROWS * (DP + 4 + 2) * 4; }
 template <int DP, int OUT>
-__global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p,
-                                                                        float* ws) {
+__device__ __forceinline__ void paged_rows(const PagedAttn& a, const PagedCache& c, const PagedBatch& b, const PagedPlan& p, int index,
+                                           char* lds) {
   constexpr int NB = DP / 16;    // column blocks; lane n of 16 owns the columns NB n .. NB n + NB - 1
   constexpr int KC = DP / 64;    // 16-byte pieces of a key row that a lane holds
   constexpr int VW = NB / 4;     // dwords of a value row that a lane holds
-  __shared__ __attribute__((aligned(16))) float sum[PA_WAVES][PA_ROWS][DP + 4];
-  __shared__ float offs[PA_WAVES][PA_ROWS], den[PA_WAVES][PA_ROWS];
+  const auto sum = reinterpret_cast<float(*)[PA_ROWS][DP + 4]>(lds);
+  const auto offs = reinterpret_cast<float(*)[PA_ROWS]>(lds + PA_WAVES * PA_ROWS * (DP + 4) * 4);
+  const auto den = offs + PA_WAVES;
 
-  if (a.fill) paged_fill(b, static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
-  const PagedItem it = paged_item(b, c.page_shift, c.heads, PA_ROWS, p, blockIdx.x);
+  const PagedItem it = paged_item(b, c.page_shift, c.heads, PA_ROWS, p, index);
   if (!it.found) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -505,9 +524,8 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAtt
     }
     if (it.splits > 1) {
       const long long slot = it.first + (long long)it.split * it.step;
-      put2(ws + (slot * PA_ROWS + r) * DP + d, y[0], y[1]);
-      put2(ws + (slot * PA_ROWS + r) * DP + d + 2, y[2], y[3]);
-      if (d == 0) put2(ws + (long long)p.slots * PA_ROWS * DP + (slot * PA_ROWS + r) * 2, least, l);
+      put4(p.ws + (slot * PA_ROWS + r) * DP + d, y[0], y[1], y[2], y[3]);
+      if (d == 0) put2(p.ws + (long long)p.slots * PA_ROWS * DP + (slot * PA_ROWS + r) * 2, least, l);
     } else {
       const float f = l > 0.0f ? a.alpha_pv * 1024.0f / l : 0.0f;
 #pragma unroll
@@ -516,8 +534,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAtt
       store_some<4, OUT>(a.out, ((long long)(it.s.row0 + tt) * a.q_heads + it.head * G + rr - tt * G) * c.D + d, y);
     }
   }
-  if (it.splits == 1 || p.arrivals == nullptr) return;
-  meet_and_join<PA_ROWS, DP, OUT>(a, c, p, it, ws, reinterpret_cast<int*>(&offs[0][0]), &sum[0][0][0]);
+  if (it.splits > 1) meet_and_join<PA_ROWS, DP, OUT>(a, c, p, it, reinterpret_cast<int*>(&offs[0][0]), &sum[0][0][0]);
 }
 
 // Many rows: 128 to a workgroup, 32 to each of its four waves, 64 keys to a step.  Each wave brings 16 of the keys: K as it is
@@ -528,18 +545,18 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAtt
 // Scores start from 1.5 * 2^23 instead of 0: the int32 sum is then the fp32 number 12582912 + x, and the constant goes into the
 // row's offset, where one multiply-add removes it exactly.
 constexpr int PT_ROWS = 128, PT_KEYS = 64;
-constexpr int PT_MEET = 32;  // items from which on slices meet in the launch
+constexpr int PT_MEET = 32;      // items from which on slices meet in the launch
+constexpr int PT_PLENTY = 2048;  // items from which on nothing is cut: four to each place on the chip
+constexpr int tiles_lds(int DP) { return 3 * 3 * PT_KEYS * DP + 16; }  // three steps of K, then of V as fp16; a word to meet by
 template <int DP, int OUT>
-__global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p, float* ws) {
+__device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache& c, const PagedBatch& b, const PagedPlan& p, int index,
+                                            char* lds) {
   constexpr int NDB = DP / 32;   // column blocks of O^T, and steps of 32 along a key row
   constexpr int KC = DP / 64;    // 16-byte pieces of K that a thread brings
   constexpr int CH = DP / 16;    // 16-byte chunks of a key row
   constexpr int KBYTES = PT_KEYS * DP, VBYTES = 2 * KBYTES;
-  __shared__ __attribute__((aligned(16))) char lds[3 * (KBYTES + VBYTES)];  // three steps of K, then of V
-  __shared__ int seen;
 
-  if (a.fill) paged_fill(b, static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
-  const PagedItem it = paged_item(b, c.page_shift, c.heads, PT_ROWS, p, blockIdx.x);
+  const PagedItem it = paged_item(b, c.page_shift, c.heads, PT_ROWS, p, index);
   if (!it.found) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -850,92 +867,137 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_tiles_kernel(PagedAt
   }
   const long long slot = it.first + (long long)it.split * it.step;
   if (real) {
-    float* to = ws + (slot * PT_ROWS + wave * 32 + n) * DP;
+    float* to = p.ws + (slot * PT_ROWS + wave * 32 + n) * DP;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int d = NDB * ((r & 3) + 8 * (r >> 2) + 4 * h);
       if (d < c.D) {
-#pragma unroll
-        for (int i = 0; i < NDB; i += 2) put2(to + d + i, acc[i][r], acc[i + 1][r]);
+        if constexpr (NDB == 4) put4(to + d, acc[0][r], acc[1][r], acc[2][r], acc[3][r]);
+        else put2(to + d, acc[0][r], acc[1][r]);
       }
     }
-    if (h == 0) put2(ws + (long long)p.slots * PT_ROWS * DP + (slot * PT_ROWS + wave * 32 + n) * 2, off, den);
+    if (h == 0) put2(p.ws + (long long)p.slots * PT_ROWS * DP + (slot * PT_ROWS + wave * 32 + n) * 2, off, den);
   }
-  if (p.arrivals != nullptr) meet_and_join<PT_ROWS, DP, OUT>(a, c, p, it, ws, &seen, reinterpret_cast<float*>(lds));
+  meet_and_join<PT_ROWS, DP, OUT>(a, c, p, it, reinterpret_cast<int*>(lds + tiles_lds(DP) - 16), reinterpret_cast<float*>(lds));
+}
+
+template <int DP, int OUT>
+__global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan rows) {
+  __shared__ __attribute__((aligned(16))) char lds[rows_lds(DP)];
+  if (a.fill) paged_fill(b, static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
+  paged_rows<DP, OUT>(a, c, b, rows, blockIdx.x, lds);
+}
+
+// Sequences of few rows and of many in one launch, an item of the one kind after one of the other as long as both last: those
+// with few rows wait for memory while the others compute.
+template <int DP, int OUT>
+__global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_both_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan rows,
+                                                                        PagedPlan tiles) {
+  __shared__ __attribute__((aligned(16))) char lds[tiles_lds(DP) > rows_lds(DP) ? tiles_lds(DP) : rows_lds(DP)];
+  if (a.fill) paged_fill(b, static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
+  const int i = blockIdx.x, both = 2 * (rows.slots < tiles.slots ? rows.slots : tiles.slots);
+  const bool many = i < both ? (i & 1) == 0 : tiles.slots > rows.slots;
+  const int index = i < both ? i >> 1 : i - both / 2;
+  if (many) paged_tiles<DP, OUT>(a, c, b, tiles, index, lds);
+  else paged_rows<DP, OUT>(a, c, b, rows, index, lds);
 }
 
 // Joins the slices of the sequences that were cut where they do not meet in the launch itself; 16 rows to blockIdx.y.
 template <int ROWS, int DP, int OUT>
-__global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p, float* ws) {
+__global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p) {
   __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
   const PagedItem it = paged_item(b, c.page_shift, c.heads, ROWS, p, blockIdx.x);
   if (!it.found || it.split != 0 || it.splits == 1) return;
-  join_slices<ROWS, DP, OUT>(a, c, p, it, ws, meet, blockIdx.y * PA_ROWS, PA_ROWS);
+  join_slices<ROWS, DP, OUT>(a, c, p, it, meet, blockIdx.y * PA_ROWS, PA_ROWS);
 }
 
-// Rows to a work item.  Up to 16 rows to a sequence and key head on average, the kernel of few rows; beyond, tiles of 128, in
-// which few rows leave waves idle but keys are read once.
-static int paged_tile(long long rows, long long seqs, long long group) { return rows * group <= 16 * seqs ? PA_ROWS : PT_ROWS; }
-// Items that a batch can make: one to each (sequence, key head, tile of rows), and the slices beyond that.
-static long long paged_units(long long rows, long long seqs, long long group, long long kv_heads, int tile) {
-  return kv_heads * (seqs + rows * group / tile);
-}
-static bool paged_cuts(long long capacity) { return capacity > PA_MIN_SLICE; }
-static long long paged_slots(long long rows, long long seqs, long long group, long long kv_heads) {
-  return paged_units(rows, seqs, group, kv_heads, paged_tile(rows, seqs, group)) + PA_TARGET + 8;
+// What a call of these sizes runs.  The lengths are on the device, so the grids and the workspace are bounds: one item to each
+// (sequence, key head, tile of rows) and the slices beyond that.
+struct PagedShape {
+  long long rows_slots, tiles_slots;  // items of either kind; 0: none
+  bool rows_cut, tiles_cut;
+};
+static PagedShape paged_shape(long long rows, long long seqs, long long group, long long heads, long long capacity) {
+  PagedShape s = {0, 0, false, false};
+  const bool cut = capacity > PA_MIN_SLICE;
+  if (rows * group <= PA_ROWS * seqs) {  // few rows to a sequence on average: all of them by that kernel
+    s.rows_slots = heads * (seqs + rows * group / PA_ROWS);
+    s.rows_cut = cut;
+    if (cut) s.rows_slots += PA_TARGET + 8;
+    return s;
+  }
+  // sequences with more than 16 rows are at most a 17th of all rows
+  const long long many = rows * group / (PA_ROWS + 1) < seqs ? rows * group / (PA_ROWS + 1) : seqs;
+  s.tiles_slots = heads * (many + rows * group / PT_ROWS);
+  s.tiles_cut = cut && s.tiles_slots < PT_PLENTY;
+  if (s.tiles_cut) s.tiles_slots += PA_TARGET + 8;
+  if (seqs > 1) {  // (a single one has more than 16)
+    s.rows_slots = heads * seqs;
+    s.rows_cut = cut;
+    if (cut) s.rows_slots += PA_TARGET + 8;
+  }
+  return s;
 }
 static int paged_dp(long long D) { return D <= 64 ? 64 : 128; }
+static long long paged_bytes(long long slots, int rows, long long D) { return slots * rows * (paged_dp(D) + 2) * 4; }
 
-long long paged_attn_arrivals(long long rows, long long seqs, long long q_heads, long long kv_heads, long long capacity) {
-  if (rows <= 0 || seqs <= 0 || kv_heads <= 0 || !paged_cuts(capacity)) return 0;
-  return paged_slots(rows, seqs, q_heads / kv_heads, kv_heads);
+long long paged_attn_arrivals(long long rows, long long seqs, long long q_heads, long long heads, long long capacity) {
+  const PagedShape s = paged_shape(rows, seqs, q_heads / heads, heads, capacity);
+  return (s.rows_cut ? s.rows_slots : 0) + (s.tiles_cut ? s.tiles_slots : 0);
 }
-long long paged_attn_workspace_bytes(long long rows, long long seqs, long long q_heads, long long kv_heads, long long D,
+long long paged_attn_workspace_bytes(long long rows, long long seqs, long long q_heads, long long heads, long long D,
                                      long long capacity) {
-  if (rows <= 0 || seqs <= 0 || kv_heads <= 0 || !paged_cuts(capacity)) return 0;
-  const long long group = q_heads / kv_heads;
-  return paged_slots(rows, seqs, group, kv_heads) * paged_tile(rows, seqs, group) * (paged_dp(D) + 2) * 4;
+  const PagedShape s = paged_shape(rows, seqs, q_heads / heads, heads, capacity);
+  return (s.rows_cut ? paged_bytes(s.rows_slots, PA_ROWS, D) : 0) + (s.tiles_cut ? paged_bytes(s.tiles_slots, PT_ROWS, D) : 0);
 }
 
 template <int DP, int OUT>
-static void launch_attn(int tile, const PagedAttn& a, const PagedCache& c, const PagedBatch& b, const PagedPlan& p, float* ws,
-                        unsigned grid, hipStream_t stream) {
-  auto launch = [&](auto kernel, unsigned groups) {
-    hipLaunchKernelGGL(kernel, dim3(grid, groups), dim3(PA_THREADS), 0, stream, a, c, b, p, ws);
-  };
-  const bool join = p.target != 0 && p.arrivals == nullptr;
-  if (tile == PA_ROWS) {
-    launch(paged_attn_rows_kernel<DP, OUT>, 1);
-    if (join) launch(paged_attn_join_kernel<PA_ROWS, DP, OUT>, 1);
-  } else {
-    launch(paged_attn_tiles_kernel<DP, OUT>, 1);
-    if (join) launch(paged_attn_join_kernel<PT_ROWS, DP, OUT>, PT_ROWS / PA_ROWS);
-  }
+static void launch_attn(const PagedAttn& a, const PagedCache& c, const PagedBatch& b, const PagedPlan& rows, const PagedPlan& tiles,
+                        hipStream_t stream) {
+  const unsigned grid = (unsigned)(rows.slots + tiles.slots > 0 ? rows.slots + tiles.slots : 1);
+  if (tiles.slots > 0)
+    hipLaunchKernelGGL((paged_attn_both_kernel<DP, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows, tiles);
+  else
+    hipLaunchKernelGGL((paged_attn_rows_kernel<DP, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows);
+  if (rows.target > 0 && rows.arrivals == nullptr)
+    hipLaunchKernelGGL((paged_attn_join_kernel<PA_ROWS, DP, OUT>), dim3(rows.slots), dim3(PA_THREADS), 0, stream, a, c, b, rows);
+  if (tiles.target > 0 && tiles.arrivals == nullptr)
+    hipLaunchKernelGGL((paged_attn_join_kernel<PT_ROWS, DP, OUT>), dim3(tiles.slots, PT_ROWS / PA_ROWS), dim3(PA_THREADS), 0, stream, a,
+                       c, b, tiles);
 }
 
 int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, const PagedBatch& b, void* workspace,
                          long long workspace_bytes, hipStream_t stream) {
   if (b.rows == 0 || a.q_heads == 0) return TI_OK;
-  PagedPlan p;
-  p.group = a.q_heads / c.heads;
-  const int tile = paged_tile(b.rows, b.seqs, p.group);
+  const int group = a.q_heads / c.heads;
   const long long capacity = (long long)b.per_seq << c.page_shift;
-  const long long need = paged_attn_workspace_bytes(b.rows, b.seqs, a.q_heads, c.heads, c.D, capacity);
-  const bool cut = need > 0 && workspace != nullptr && workspace_bytes >= need;
-  p.target = cut ? PA_TARGET : 0;
-  p.slots = cut ? (int)paged_slots(b.rows, b.seqs, p.group, c.heads) : 0;
-  p.arrivals = a.arrivals != nullptr && a.arrivals_count >= p.slots ? a.arrivals : nullptr;
+  PagedShape s = paged_shape(b.rows, b.seqs, group, c.heads, capacity);
+  if (workspace == nullptr || workspace_bytes < paged_attn_workspace_bytes(b.rows, b.seqs, a.q_heads, c.heads, c.D, capacity))
+    s.rows_cut = s.tiles_cut = false;
+  if (s.rows_slots + s.tiles_slots > 0x7fffff)
+    return fail(TI_ERR_INVALID_ARG, "paged_attn_s8: %lld work items", s.rows_slots + s.tiles_slots);
+  const bool meet = a.arrivals != nullptr && a.arrivals_count >= paged_attn_arrivals(b.rows, b.seqs, a.q_heads, c.heads, capacity);
+  char* ws = static_cast<char*>(workspace);
+  PagedPlan rows, tiles;
+  rows.group = tiles.group = group;
+  rows.least = 0;
+  rows.most = s.tiles_slots > 0 ? PA_ROWS : 0x7fffffff;
+  rows.slots = (int)s.rows_slots;
+  rows.target = s.rows_cut ? PA_TARGET : 0;
+  rows.ws = reinterpret_cast<float*>(ws);
+  rows.arrivals = meet && s.rows_cut ? a.arrivals : nullptr;
+  tiles.least = s.rows_slots > 0 ? PA_ROWS : 0;
+  tiles.most = 0x7fffffff;
+  tiles.slots = (int)s.tiles_slots;
+  tiles.target = s.tiles_cut ? PA_TARGET : 0;
+  tiles.ws = reinterpret_cast<float*>(ws + (s.rows_cut ? paged_bytes(s.rows_slots, PA_ROWS, c.D) : 0));
   // few items of 128 rows have many slices of 66 KB each, which one workgroup would be long in joining
-  if (tile == PT_ROWS && paged_units(b.rows, b.seqs, p.group, c.heads, tile) < PT_MEET) p.arrivals = nullptr;
-  const long long grid = cut ? p.slots : paged_units(b.rows, b.seqs, p.group, c.heads, tile);
-  if (grid > 0x7fffff) return fail(TI_ERR_INVALID_ARG, "paged_attn_s8: %lld work items", grid);
-  float* ws = static_cast<float*>(workspace);
-  const unsigned g = grid > 0 ? (unsigned)grid : 1u;
+  tiles.arrivals = meet && s.tiles_cut && s.tiles_slots - PA_TARGET - 8 >= PT_MEET ? a.arrivals + (s.rows_cut ? rows.slots : 0) : nullptr;
   auto run = [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
-    if (out_type == PT_S8) launch_attn<DP, PT_S8>(tile, a, c, b, p, ws, g, stream);
-    else if (out_type == PT_F16) launch_attn<DP, PT_F16>(tile, a, c, b, p, ws, g, stream);
-    else launch_attn<DP, PT_BF16>(tile, a, c, b, p, ws, g, stream);
+    if (out_type == PT_S8) launch_attn<DP, PT_S8>(a, c, b, rows, tiles, stream);
+    else if (out_type == PT_F16) launch_attn<DP, PT_F16>(a, c, b, rows, tiles, stream);
+    else launch_attn<DP, PT_BF16>(a, c, b, rows, tiles, stream);
   };
   if (paged_dp(c.D) == 64) run(std::integral_constant<int, 64>());
   else run(std::integral_constant<int, 128>());
