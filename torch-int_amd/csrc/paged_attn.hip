@@ -594,7 +594,7 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
   }
   const float cl = a.alpha_qk * 1.44269504088896341f;
   const int8_t* kb = c.k + it.head * c.k_head;
-  const int8_t* vb = c.v + it.head * c.v_head;
+  const int8_t* vb_ = c.v + it.head * c.v_head;
   const auto table = (const __attribute__((address_space(4))) int*)(b.table + (long long)it.seq * b.per_seq);
   const int mask = (1 << c.page_shift) - 1, last_block = hi > 0 ? (hi - 1) >> 4 : 0;
 
@@ -619,17 +619,17 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
     at = at < last_block ? at : last_block;
     return (at << 4) & mask;
   };
-  auto fetch_k = [&](int s0, int page) {
-    const int8_t* kr = kb + (long long)(have(page) ? page : 0) * c.k_page + place(s0) * c.k_token;
+  auto k_from = [&](int s0, int page) { return kb + (long long)(have(page) ? page : 0) * c.k_page + place(s0) * c.k_token; };
+  auto v_from = [&](int s0, int page) { return vb_ + (long long)(have(page) ? page : 0) * c.v_page + place(s0) * c.v_token; };
+  auto fetch_k = [&](const int8_t* from) {
 #pragma unroll
-    for (int i = 0; i < KC; ++i) kreg[i] = *reinterpret_cast<const v4i*>(kr + kcol[i]);
+    for (int i = 0; i < KC; ++i) kreg[i] = *reinterpret_cast<const v4i*>(from + kcol[i]);
   };
-  auto fetch_v = [&](int s0, int page) {
-    const int8_t* vr = vb + (long long)(have(page) ? page : 0) * c.v_page + place(s0) * c.v_token;
+  auto fetch_v = [&](const int8_t* from) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if constexpr (NDB == 4) vreg[j] = *reinterpret_cast<const unsigned*>(vr + vcol[j]);
-      else vreg[j] = *reinterpret_cast<const unsigned short*>(vr + vcol[j]);
+      if constexpr (NDB == 4) vreg[j] = *reinterpret_cast<const unsigned*>(from + vcol[j]);
+      else vreg[j] = *reinterpret_cast<const unsigned short*>(from + vcol[j]);
     }
   };
   // whether the pool lacks any of the item's pages: looked at once, so that steps need not
@@ -647,23 +647,22 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
       *reinterpret_cast<v4i*>(lds + slot * KBYTES + r * DP + swizzle(r, kchunk) * 16) = kreg[i];
     }
   };
-  auto put_v = [&](int slot) {
+  // V: bytes plus 128 (which are never negative) as the low bytes of fp16 numbers, (v + 128) 2^-24; times 2^14 less 2^-3 is
+  // v 2^-10, exactly
+  unsigned vplus[8];
+  auto lift = [&](int j) { vplus[j] = vreg[j] ^ 0x80808080u; };
+  auto put_v = [&](int slot, int i) {
+    v8h x;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) vreg[j] ^= 0x80808080u;
-#pragma unroll
-    for (int i = 0; i < NDB; ++i) {
-      v8h x;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned two = __builtin_amdgcn_perm(vreg[2 * j + 1], vreg[2 * j], 0x0c000c00u | (unsigned)(4 + i) << 16 | (unsigned)i);
-        v2h y;
-        __builtin_memcpy(&y, &two, 4);
-        y = __builtin_elementwise_fma(y, v2h{(_Float16)16384.0f, (_Float16)16384.0f}, v2h{(_Float16)-0.125f, (_Float16)-0.125f});
-        x[2 * j] = y[0];
-        x[2 * j + 1] = y[1];
-      }
-      *reinterpret_cast<v8h*>(lds + 3 * KBYTES + slot * VBYTES + ((wave * NDB + i) * 64 + lane) * 16) = x;
+    for (int j = 0; j < 4; ++j) {
+      const unsigned two = __builtin_amdgcn_perm(vplus[2 * j + 1], vplus[2 * j], 0x0c000c00u | (unsigned)(4 + i) << 16 | (unsigned)i);
+      v2h y;
+      __builtin_memcpy(&y, &two, 4);
+      y = __builtin_elementwise_fma(y, v2h{(_Float16)16384.0f, (_Float16)16384.0f}, v2h{(_Float16)-0.125f, (_Float16)-0.125f});
+      x[2 * j] = y[0];
+      x[2 * j + 1] = y[1];
     }
+    *reinterpret_cast<v8h*>(lds + 3 * KBYTES + slot * VBYTES + ((wave * NDB + i) * 64 + lane) * 16) = x;
   };
 
   float off = PA_EMPTY, den = 0.0f;
@@ -677,44 +676,38 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
   for (int r = 0; r < 16; ++r) start[r] = 0x4b400000;
   asm("" : "+v"(start));   // kept in registers, not made anew at every step
 
-  // scores of 32 keys, whose rows of K begin at `at` in the LDS
-  auto scores = [&](int at) {
-    v4i kf[NDB];
-#pragma unroll
-    for (int i = 0; i < NDB; ++i) kf[i] = *reinterpret_cast<const v4i*>(lds + at + kat[i]);
-    v16i t = start;
-#pragma unroll
-    for (int i = 0; i < NDB; ++i) t = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[i], qf[i], t, 0, 0, 0);
-    v16f x;
-    __builtin_memcpy(&x, &t, sizeof(t));
-    return x;
+  // The operands of 32 keys: of K for their scores, of V for their products, first 16 keys and second.
+  v4i kf[NDB];
+  v8h va[NDB], vb[NDB];
+  auto read_k = [&](int at, int i) { kf[i] = *reinterpret_cast<const v4i*>(lds + at + kat[i]); };
+  auto read_v = [&](v8h (&v)[NDB], int at, int q, int i) { v[i] = *reinterpret_cast<const v8h*>(lds + at + ((q * NDB + i) * 64 + lane) * 16); };
+  struct Half {
+    v16f x;         // scores of 32 keys
+    float top;      // the largest of them
+    v8h pr[2];      // their probabilities
   };
-  // O^T += V^T P^T of 32 keys, whose operands begin at `at`
-  auto gather = [&](int at, const v8h (&pr)[2]) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-#pragma unroll
-      for (int i = 0; i < NDB; ++i)
-        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const v8h*>(lds + at + ((q * NDB + i) * 64 + lane) * 16), pr[q],
-                                                        acc[i], 0, 0, 0);
-  };
-  // 32 keys from s0 on: the softmax of their scores x into `pr`, beside it the scores of the 32 keys behind them and the products
-  // of the 32 before them, whose probabilities are `before`
-  auto half = [&](v16f& x, v16f& next, v8h (&pr)[2], v8h (&before)[2], int s0, int lost, int k_at, int v_at) {
+  constexpr int BUNDLES = 3 * NDB;
+  // 32 keys from s0 on: the softmax of their scores into their probabilities, beside it the scores of the next 32 keys and the
+  // products of the 32 before, in bundles that the compiler keeps in order: a matrix instruction, then what runs beside
+  // it.  A pair of scores goes through its multiply-adds and exponentials in one bundle, is rounded in the next and added to
+  // the denominator in the one behind that, so nothing waits for the instruction before it; operands are read from the LDS
+  // bundles, or a half, before they are used: kf and va are here, vb comes from `v_at`, the next half's from `k_next` and
+  // `v_next`.  `beside(m)` is what else is to be done in bundle m.
+  auto half = [&](Half& now, Half& next, v8h (&before)[2], int s0, int lost, int v_at, int k_next, int v_next, auto beside) {
     if (__builtin_expect(s0 + 32 > whole || lost != 0, 0)) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int key = s0 + (r & 3) + 8 * (r >> 2) + 4 * h;
-        if (key >= hi || key >= limit || (lost >> (r >> 3) & 1)) x[r] = -__builtin_inff();
+        if (key >= hi || key >= limit || (lost >> (r >> 3) & 1)) now.x[r] = -__builtin_inff();
       }
-    }
-    float top = x[0];
+      now.top = now.x[0];
 #pragma unroll
-    for (int r = 1; r < 16; ++r) top = __builtin_fmaxf(top, x[r]);
-    if (__builtin_expect(__ballot(__builtin_fmaf(top, cl, off) > 15.0f) != 0, 0)) {
+      for (int r = 1; r < 16; ++r) now.top = __builtin_fmaxf(now.top, now.x[r]);
+    }
+    if (__builtin_expect(__ballot(__builtin_fmaf(now.top, cl, off) > 15.0f) != 0, 0)) {
       // A new reference.  It moves by a whole number, so that what is relative to the old one is scaled without rounding.
-      auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-      top = __builtin_fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
+      auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(now.top), __float_as_uint(now.top), false, false);
+      const float top = __builtin_fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
       const float above = __builtin_fmaf(top, cl, off) - 8.0f;
       const bool moves = above > 7.0f, first = off == PA_EMPTY;
       const float by = moves ? __builtin_ceilf(above) : 0.0f;
@@ -727,56 +720,57 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
 #pragma unroll
       for (int i = 0; i < NDB; ++i) acc[i] *= scale;
     }
-    v4i kf[NDB];
-    v8h vf[2][NDB];
-#pragma unroll
-    for (int i = 0; i < NDB; ++i) kf[i] = *reinterpret_cast<const v4i*>(lds + k_at + kat[i]);
-#pragma unroll
-    for (int q = 0; q < 2; ++q)
-#pragma unroll
-      for (int i = 0; i < NDB; ++i) vf[q][i] = *reinterpret_cast<const v8h*>(lds + v_at + ((q * NDB + i) * 64 + lane) * 16);
-    // Products and softmax in bundles that the compiler keeps in order: a matrix instruction, then the vector instructions that
-    // run beside it.  A pair of scores goes through its multiply-adds and exponentials in one bundle, is rounded in the next and
-    // added to the denominator in the one behind that, so nothing waits for the instruction before it.
     v16i t = start;
+    v16f tf;
     float e[2][2];
     v2h two[8];
     auto softmax = [&](int m) {
-      if (m >= 2 && m - 2 < 8) den = __builtin_amdgcn_fdot2(two[m - 2], v2h{(_Float16)1.0f, (_Float16)1.0f}, den, false);
-      if (m >= 1 && m - 1 < 8) two[m - 1] = v2h{(_Float16)e[(m - 1) & 1][0], (_Float16)e[(m - 1) & 1][1]};
+      if (m >= 2 && m < 10) den = __builtin_amdgcn_fdot2(two[m - 2], v2h{(_Float16)1.0f, (_Float16)1.0f}, den, false);
+      if (m >= 1 && m < 9) {
+        two[m - 1] = v2h{(_Float16)e[(m - 1) & 1][0], (_Float16)e[(m - 1) & 1][1]};
+        asm volatile("" : "+v"(two[m - 1]));  // computed here, not where the next half needs it
+      }
       if (m < 8) {
-        e[m & 1][0] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * m], cl, off));
-        e[m & 1][1] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * m + 1], cl, off));
+        e[m & 1][0] = __builtin_amdgcn_exp2f(__builtin_fmaf(now.x[2 * m], cl, off));
+        e[m & 1][1] = __builtin_amdgcn_exp2f(__builtin_fmaf(now.x[2 * m + 1], cl, off));
       }
     };
     __builtin_amdgcn_sched_barrier(0);
     softmax(0);
+#pragma unroll
+    for (int m = 0; m < BUNDLES; ++m) {
+      __builtin_amdgcn_sched_barrier(0);
+      const int i = m < 2 * NDB ? m >> 1 : m - 2 * NDB;
+      if (m < 2 * NDB && (m & 1) == 0) t = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[i], qf[i], t, 0, 0, 0);
+      else if (m < 2 * NDB) acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i], before[0], acc[i], 0, 0, 0);
+      else acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb[i], before[1], acc[i], 0, 0, 0);
+      softmax(m + 1);
+      if (m < NDB) read_v(vb, v_at, 1, m);
+      if (m >= 2 * NDB) {
+        read_k(k_next, i);
+        read_v(va, v_next, 0, i);
+      }
+      constexpr int PARTS = NDB == 4 ? 3 : 2;  // bundles at the end, in which the next scores are there
+      const int part = m - (BUNDLES - PARTS);
+      if (part == 0) __builtin_memcpy(&tf, &t, sizeof(t));
+      if (part >= 0) {
+#pragma unroll
+        for (int r = 16 * part / PARTS; r < 16 * (part + 1) / PARTS; ++r) next.top = r == 0 ? tf[0] : __builtin_fmaxf(next.top, tf[r]);
+      }
+      beside(m);
+    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < NDB; ++i) {
-      t = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[i], qf[i], t, 0, 0, 0);
-      softmax(2 * i + 1);
-      __builtin_amdgcn_sched_barrier(0);
-      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0][i], before[0], acc[i], 0, 0, 0);
-      softmax(2 * i + 2);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int i = 0; i < NDB; ++i) {
-      acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[1][i], before[1], acc[i], 0, 0, 0);
-      softmax(2 * NDB + 1 + i);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#pragma unroll
-    for (int m = 3 * NDB + 1; m < 10; ++m) softmax(m);
+    for (int m = BUNDLES + 1; m < 10; ++m) softmax(m);
+    asm volatile("" : "+v"(den), "+v"(next.top));
+    next.x = tf;
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        pr[q][2 * j] = two[q * 4 + j][0];
-        pr[q][2 * j + 1] = two[q * 4 + j][1];
+        now.pr[q][2 * j] = two[q * 4 + j][0];
+        now.pr[q][2 * j + 1] = two[q * 4 + j][1];
       }
-    __builtin_memcpy(&next, &t, sizeof(t));
   };
 
   if (lo < hi) {
@@ -796,51 +790,104 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
       return b.table[(long long)it.seq * b.per_seq + ((at << 4) >> c.page_shift) + zero];
     };
     int page = page_at(lo, wave), page_v;
-    fetch_k(lo, page);
-    fetch_v(lo, page);
+    fetch_k(k_from(lo, page));
+    fetch_v(v_from(lo, page));
     put_k(0);
-    put_v(0);
+    auto put_all = [&](int slot) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) lift(j);
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) put_v(slot, i);
+    };
+    put_all(0);
     page = page_at(lo + PT_KEYS, wave);
-    fetch_k(lo + PT_KEYS, page);
-    fetch_v(lo + PT_KEYS, page);
+    fetch_k(k_from(lo + PT_KEYS, page));
+    fetch_v(v_from(lo + PT_KEYS, page));
     put_k(1);
     page_v = page_at(lo + 2 * PT_KEYS, wave);
-    fetch_k(lo + 2 * PT_KEYS, page_v);
+    fetch_k(k_from(lo + 2 * PT_KEYS, page_v));
     int asked = ask(lo + 3 * PT_KEYS);
     __syncthreads();
-    v16f even = scores(0), odd;
-    v8h pr_even[2], pr_odd[2];
+    constexpr int V0 = 3 * KBYTES, K_HALF = 32 * DP, V_HALF = VBYTES / 2;
+    Half even, odd;
+    {
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) read_k(0, i);
+      v16i t = start;
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) t = __builtin_amdgcn_mfma_i32_32x32x32_i8(kf[i], qf[i], t, 0, 0, 0);
+      __builtin_memcpy(&even.x, &t, sizeof(t));
+      even.top = even.x[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) even.top = __builtin_fmaxf(even.top, even.x[r]);
+    }
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) pr_odd[q][j] = (_Float16)0.0f;
-    constexpr int V0 = 3 * KBYTES, K_HALF = 32 * DP, V_HALF = VBYTES / 2;
+      for (int j = 0; j < 8; ++j) odd.pr[q][j] = (_Float16)0.0f;
     // slots of this step, of the next one and of the one behind it; V of the step before is in the third of them
     int k0 = 0, k1 = 1, k2 = 2;
     int v_before = V0 + V_HALF;   // (the first step takes its own V, times zero)
+#pragma unroll
+    for (int i = 0; i < NDB; ++i) {
+      read_k(K_HALF, i);
+      read_v(va, v_before, 0, i);
+    }
     // A step is 64 keys.  What is read in it: the second half of its K and the first of the next one's, the second half of V
-    // before it and the first of its own; what is written: V of the next step and K of the one behind that, in places that the
-    // step before has read, which one barrier a step makes sure of.
+    // before it and the first of its own, and ahead of the next step K's second half of that and V's of this; what is written:
+    // V of the next step and K of the one behind that, in places that the step before has read, which one barrier a step
+    // makes sure of.
     int s0 = lo;
     for (;;) {
       const int gone = lost(s0);
       const bool here = s0 < keys + 32;  // the same for all lanes: with the half behind its last keys a wave gathers those
-      if (__builtin_expect(here, 1)) half(even, odd, pr_even, pr_odd, s0, gone & 3, k0 * KBYTES + K_HALF, v_before);
-      put_v(k1);
-      fetch_v(s0 + 2 * PT_KEYS, page_v);
-      if (__builtin_expect(here, 1)) half(odd, even, pr_odd, pr_even, s0 + 32, gone >> 2, k1 * KBYTES, V0 + k0 * VBYTES);
-      put_k(k2);
-      page_v = __builtin_amdgcn_readfirstlane(asked);
-      fetch_k(s0 + 3 * PT_KEYS, page_v);
-      asked = ask(s0 + 4 * PT_KEYS);
+      const int v_now = V0 + k0 * VBYTES;
+      const int8_t* from;
+      auto stage_v = [&](int m) {
+        if (m == 0) from = v_from(s0 + 2 * PT_KEYS, page_v);
+        if (m >= NDB && m < 2 * NDB) {
+#pragma unroll
+          for (int j = 0; j < 8 / NDB; ++j) lift((m - NDB) * (8 / NDB) + j);
+        }
+        if (m == 2 * NDB) fetch_v(from);
+        if (m >= 2 * NDB) put_v(k1, m - 2 * NDB);
+      };
+      auto stage_k = [&](int m) {
+        if (m == 0) {
+          page_v = __builtin_amdgcn_readfirstlane(asked);
+          from = k_from(s0 + 3 * PT_KEYS, page_v);
+        }
+        if (m == NDB) put_k(k2);
+        if (m == NDB + 1) {
+          fetch_k(from);
+          asked = ask(s0 + 4 * PT_KEYS);
+        }
+      };
+      if (__builtin_expect(here, 1)) {
+        half(even, odd, odd.pr, s0, gone & 3, v_before, k1 * KBYTES, v_now, stage_v);
+        half(odd, even, even.pr, s0 + 32, gone >> 2, v_now, k1 * KBYTES + K_HALF, v_now + V_HALF, stage_k);
+      } else {
+#pragma unroll
+        for (int m = 0; m < BUNDLES; ++m) stage_v(m);
+#pragma unroll
+        for (int m = 0; m < BUNDLES; ++m) stage_k(m);
+      }
       __syncthreads();
-      v_before = V0 + k0 * VBYTES + V_HALF;
+      v_before = v_now + V_HALF;
       const int k = k0;
       k0 = k1, k1 = k2, k2 = k;
       s0 += PT_KEYS;
       if (s0 >= hi) break;
     }
-    if (s0 < keys + 32) gather(v_before, pr_odd);  // nobody has done it: the wave's keys reach into the last half
+    if (s0 < keys + 32) {  // nobody has gathered them: the wave's keys reach into the last half
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) read_v(vb, v_before, 1, i);
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) {
+        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[i], odd.pr[0], acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vb[i], odd.pr[1], acc[i], 0, 0, 0);
+      }
+    }
   }
 
   // a lane has its row's columns NDB m + i, m = (r & 3) + 8 (r >> 2) + 4 h; the two halves of the wave add their denominators
