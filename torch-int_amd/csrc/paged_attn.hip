@@ -18,6 +18,7 @@ namespace ti {
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef unsigned v2u __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 constexpr int PA_WAVES = 4;
@@ -105,17 +106,19 @@ __device__ __forceinline__ int paged_slice(const PagedBatch& b, int page_shift, 
   return slice < PA_MIN_SLICE ? PA_MIN_SLICE : slice;
 }
 
-// The work item with number `index`, in the order sequence, slice, tile of rows, head.
+// The work item with number `index`, in the order sequence, slice, tile of rows, head.  CUT: the first slice of the `index`-th
+// item among those that are cut.
+template <bool CUT = false>
 __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_shift, int heads, int rows_per_tile, const PagedPlan& p,
                                                 int index) {
   PagedItem it;
   it.found = false;
   it.slice = paged_slice(b, page_shift, heads, rows_per_tile, p);
   const int lane = threadIdx.x & 63;
-  int before = 0;
+  int before = 0, before_cut = 0;
   for (int i0 = 0; i0 < b.seqs; i0 += 64) {
     PagedSeq s = {0, 0, 0};
-    int n = 0, tiles = 0, splits = 0;
+    int n = 0, cut = 0, tiles = 0, splits = 0;
     if (i0 + lane < b.seqs) {
       s = paged_seq(b, page_shift, i0 + lane);
       tiles = p.tiles(s, rows_per_tile);
@@ -123,13 +126,14 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
       // a cu_new that descends can count rows many times over: no sum of items passes the range of int
       const long long all = (long long)tiles * splits * heads;
       n = all > 0x800000 ? 0x800000 : (int)all;
+      cut = splits > 1 ? n / splits : 0;
     }
-    const int upto = wave_scan(n);
-    const unsigned long long past = __ballot(before + upto > index);
+    const int upto = wave_scan(n), upto_cut = CUT ? wave_scan(cut) : 0;
+    const unsigned long long past = __ballot(CUT ? before_cut + upto_cut > index : before + upto > index);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
       const int first = before + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at);
-      const int rel = index - first;
+      const int rel = CUT ? index - (before_cut + __builtin_amdgcn_readlane(upto_cut, at) - __builtin_amdgcn_readlane(cut, at)) : index - first;
       const int t = __builtin_amdgcn_readlane(tiles, at);
       it.s.row0 = __builtin_amdgcn_readlane(s.row0, at);
       it.s.T = __builtin_amdgcn_readlane(s.T, at);
@@ -149,6 +153,10 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
     }
     before += __builtin_amdgcn_readlane(upto, 63);
     before = before > 0x20000000 ? 0x20000000 : before;
+    if (CUT) {
+      before_cut += __builtin_amdgcn_readlane(upto_cut, 63);
+      before_cut = before_cut > 0x20000000 ? 0x20000000 : before_cut;
+    }
   }
   return it;
 }
@@ -164,6 +172,24 @@ __device__ __forceinline__ void paged_fill(const PagedBatch& b, char* out, long 
     for (long long j = threadIdx.x * 16ll; j < row_bytes; j += blockDim.x * 16ll) *reinterpret_cast<v4i*>(at + j) = v4i{0, 0, 0, 0};
   }
 }
+
+// Where the rows of a tile are in the output: row r of it is token (r0 + r) / group, head (r0 + r) % group.  The quotient comes
+// from a multiplication: r0 + r < 4096 + 128 is small enough for it to be exact.
+struct PagedRows {
+  long long out0;   // output row of the tile's first token and of the key head's first query head
+  int group, rest, step;
+  float inv;
+  __device__ __forceinline__ PagedRows(const PagedItem& it, const PagedAttn& a, int G, int rows_per_tile) : group(G), step(a.q_heads) {
+    const int first = it.tile * rows_per_tile, t0 = first / G;
+    rest = first - t0 * G;
+    out0 = (long long)(it.s.row0 + t0) * a.q_heads + it.head * G;
+    inv = 1.0f / (float)G;
+  }
+  __device__ __forceinline__ long long operator()(int r) const {
+    const int x = rest + r, t = (int)(((float)x + 0.5f) * inv);
+    return out0 + (long long)t * step + (x - t * group);
+  }
+};
 
 // N neighbouring outputs (2 or 4)
 template <int N, int OUT>
@@ -194,7 +220,7 @@ __device__ __forceinline__ void store_some(void* out, long long at, const float 
   }
 }
 
-// Partial sums are written past the cache of the XCD, for another XCD's workgroup to join.
+// Partial sums are written and read past the cache of the XCD: another XCD's workgroup may join them.
 __device__ __forceinline__ void put4(float* p, float x, float y, float z, float w) {
   const v4f v = {x, y, z, w};
   asm volatile("global_store_dwordx4 %0, %1, off sc1" ::"v"(p), "v"(v) : "memory");
@@ -202,6 +228,12 @@ __device__ __forceinline__ void put4(float* p, float x, float y, float z, float 
 __device__ __forceinline__ void put2(float* p, float x, float y) {
   const unsigned long long w = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
   __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ float2 get2(const float* p) {
+  const unsigned long long w =
+      __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((unsigned)w), __uint_as_float((unsigned)(w >> 32)));
 }
 
 // A row's partial sums y relative to the offset `off`, with their denominator, and how two of them add up.
@@ -219,74 +251,72 @@ struct PagedPart {
 };
 
 constexpr int PA_THREADS = PA_WAVES * 64;
-// The slices of one item, rows `first` to `first + rows - 1` of its ROWS, by the threads of one workgroup.  A place is four
-// columns of a row; where there are fewer places than threads, several threads share one and meet in the LDS.
-template <int ROWS, int DP, int OUT>
+// The slices of one item, COUNT of its ROWS rows from `first` on, by the threads of one workgroup.  A place is four
+// columns of a row.  Its slices add up in four chains, every fourth slice to one, by four threads that meet in the LDS where
+// places are few: the order, and the bits, are the same whoever joins.
+constexpr int CHAINS = 4;
+template <int ROWS, int COUNT, int DP, int OUT>
 __device__ __forceinline__ void join_slices(const PagedAttn& a, const PagedCache& c, const PagedPlan& p, const PagedItem& it,
-                                            float* meet, int first, int rows) {
+                                            float* meet, int first) {
   const int G = p.group, tid = threadIdx.x;
   const int live_rows = it.s.T * G - it.tile * ROWS - first;
-  rows = rows < live_rows ? rows : live_rows;
+  const int rows = COUNT < live_rows ? COUNT : live_rows;
   if (rows <= 0) return;
-  const int quads = c.D / 4, work = rows * quads;
+  constexpr int QUADS = DP / 4;  // places of a row; those beyond the head size are idle
+  const int work = rows * QUADS;
   const float* tail = p.ws + (long long)p.slots * ROWS * DP;
+  const PagedRows out_row(it, a, G, ROWS);
   const PagedPart none = {PA_EMPTY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
-  auto row_of = [&](int e) { return first + e / quads; };
   auto take = [&](PagedPart& sum, int e, int s) {
-    const int r = row_of(e), d = (e - (r - first) * quads) * 4;
-    const long long row = (it.first + (long long)s * it.step) * ROWS + r;
-    const float2 od = *reinterpret_cast<const float2*>(tail + row * 2);
-    sum.add(od.x, od.y, *reinterpret_cast<const v4f*>(p.ws + row * DP + d));
+    const long long row = (it.first + (long long)s * it.step) * ROWS + first + e / QUADS;
+    const float* from = p.ws + row * DP + e % QUADS * 4;
+    const float2 od = get2(tail + row * 2), y0 = get2(from), y1 = get2(from + 2);
+    sum.add(od.x, od.y, v4f{y0.x, y0.y, y1.x, y1.y});
   };
   auto give = [&](const PagedPart& sum, int e) {
-    const int r = row_of(e), d = (e - (r - first) * quads) * 4;
+    const int r = first + e / QUADS, d = e % QUADS * 4;
+    if (d >= c.D) return;
     const float f = sum.den > 0.0f ? a.alpha_pv * 1024.0f / sum.den : 0.0f;
     float y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = sum.den > 0.0f ? sum.y[i] * f : 0.0f;
-    const int rr = it.tile * ROWS + r, tt = rr / G;
-    store_some<4, OUT>(a.out, ((long long)(it.s.row0 + tt) * a.q_heads + it.head * G + rr - tt * G) * c.D + d, y);
+    store_some<4, OUT>(a.out, out_row(r) * c.D + d, y);
   };
-  if (work < PA_THREADS) {
-    const int lanes = PA_THREADS / work, share = tid / work, e = tid - share * work;  // (a few threads may be left over)
+  if (work * CHAINS <= PA_THREADS) {
+    const int share = tid / work, e = tid - share * work;
     PagedPart sum = none;
-    if (share < lanes) {
+    if (share < CHAINS) {
 #pragma unroll 4
-      for (int s = share; s < it.splits; s += lanes) take(sum, e, s);
+      for (int s = share; s < it.splits; s += CHAINS) take(sum, e, s);
     }
     float* mine = meet + tid * 8;
     mine[0] = sum.off, mine[1] = sum.den;
     *reinterpret_cast<v4f*>(mine + 4) = sum.y;
     __syncthreads();
     if (share != 0) return;
-    for (int o = 1; o < lanes; ++o) {
+#pragma unroll
+    for (int o = 1; o < CHAINS; ++o) {
       const float* at = meet + (tid + o * work) * 8;
       sum.add(at[0], at[1], *reinterpret_cast<const v4f*>(at + 4));
     }
     give(sum, e);
     return;
   }
-  constexpr int EACH = 4;  // places of a thread at once: their loads are under way together
-  for (int e0 = tid; e0 < work; e0 += EACH * PA_THREADS) {
-    PagedPart sum[EACH];
+  for (int e = tid; e < work; e += PA_THREADS) {
+    PagedPart sum[CHAINS] = {none, none, none, none};
+    for (int s = 0; s < it.splits; s += CHAINS)
 #pragma unroll
-    for (int k = 0; k < EACH; ++k) sum[k] = none;
-#pragma unroll 2
-    for (int s = 0; s < it.splits; ++s)
+      for (int o = 0; o < CHAINS; ++o)
+        if (s + o < it.splits) take(sum[o], e, s + o);
 #pragma unroll
-      for (int k = 0; k < EACH; ++k) {
-        const int e = e0 + k * PA_THREADS;
-        take(sum[k], e < work ? e : e0, s);
-      }
-#pragma unroll
-    for (int k = 0; k < EACH; ++k)
-      if (e0 + k * PA_THREADS < work) give(sum[k], e0 + k * PA_THREADS);
+    for (int o = 1; o < CHAINS; ++o) sum[0].add(sum[o].off, sum[o].den, sum[o].y);
+    give(sum[0], e);
   }
 }
 
 // The workgroup that arrives last joins the slices, in their order: the bits do not depend on who that is.  Partial sums are
-// written through to memory and the counter is a device-scope atomic, so no cache has to be written back: a thread's stores have
-// arrived when its count of them is zero.  `scratch`: LDS of the workgroup that nobody reads any more.
+// written through to memory and read from there, and the counter is a device-scope atomic, so no cache has to be written back
+// or emptied (which would take the other workgroups' keys with it): a thread's stores have arrived when its count of them is zero.  `scratch`: LDS of the workgroup that nobody reads any more.
 template <int ROWS, int DP, int OUT>
 __device__ __forceinline__ void meet_and_join(const PagedAttn& a, const PagedCache& c, const PagedPlan& p, const PagedItem& it,
                                               int* seen, float* scratch) {
@@ -299,8 +329,7 @@ __device__ __forceinline__ void meet_and_join(const PagedAttn& a, const PagedCac
   }
   __syncthreads();
   if (seen[0] != it.splits - 1) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  join_slices<ROWS, DP, OUT>(a, c, p, it, scratch, 0, ROWS);
+  join_slices<ROWS, ROWS, DP, OUT>(a, c, p, it, scratch, 0);
 }
 
 constexpr int rows_lds(int DP) { return PA_WAVES * PA_ROWS * (DP + 4 + 2) * 4; }
@@ -506,6 +535,7 @@ __device__ __forceinline__ void paged_rows(const PagedAttn& a, const PagedCache&
   }
   __syncthreads();
   const int quads = c.D / 4;
+  const PagedRows out_row(it, a, G, PA_ROWS);
   for (int e = threadIdx.x; e < PA_ROWS * (DP / 4); e += PA_THREADS) {
     const int r = e / (DP / 4), d = (e % (DP / 4)) * 4;
     const int rr = it.tile * PA_ROWS + r;
@@ -530,8 +560,7 @@ __device__ __forceinline__ void paged_rows(const PagedAttn& a, const PagedCache&
       const float f = l > 0.0f ? a.alpha_pv * 1024.0f / l : 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = l > 0.0f ? y[i] * f : 0.0f;
-      const int tt = rr / G;
-      store_some<4, OUT>(a.out, ((long long)(it.s.row0 + tt) * a.q_heads + it.head * G + rr - tt * G) * c.D + d, y);
+      store_some<4, OUT>(a.out, out_row(r) * c.D + d, y);
     }
   }
   if (it.splits > 1) meet_and_join<PA_ROWS, DP, OUT>(a, c, p, it, reinterpret_cast<int*>(&offs[0][0]), &sum[0][0][0]);
@@ -545,9 +574,8 @@ __device__ __forceinline__ void paged_rows(const PagedAttn& a, const PagedCache&
 // Scores start from 1.5 * 2^23 instead of 0: the int32 sum is then the fp32 number 12582912 + x, and the constant goes into the
 // row's offset, where one multiply-add removes it exactly.
 constexpr int PT_ROWS = 128, PT_KEYS = 64;
-constexpr int PT_MEET = 32;      // items from which on slices meet in the launch
 constexpr int PT_PLENTY = 2048;  // items from which on nothing is cut: four to each place on the chip
-constexpr int tiles_lds(int DP) { return 3 * 3 * PT_KEYS * DP + 16; }  // three steps of K, then of V as fp16; a word to meet by
+constexpr int tiles_lds(int DP) { return 3 * 3 * PT_KEYS * DP; }  // three steps of K, then of V as fp16
 template <int DP, int OUT>
 __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache& c, const PagedBatch& b, const PagedPlan& p, int index,
                                             char* lds) {
@@ -621,11 +649,11 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
   };
   auto k_from = [&](int s0, int page) { return kb + (long long)(have(page) ? page : 0) * c.k_page + place(s0) * c.k_token; };
   auto v_from = [&](int s0, int page) { return vb_ + (long long)(have(page) ? page : 0) * c.v_page + place(s0) * c.v_token; };
-  auto fetch_k = [&](const int8_t* from) {
+  auto fetch_k = [&](v4i (&kreg)[KC], const int8_t* from) {
 #pragma unroll
     for (int i = 0; i < KC; ++i) kreg[i] = *reinterpret_cast<const v4i*>(from + kcol[i]);
   };
-  auto fetch_v = [&](const int8_t* from) {
+  auto fetch_v = [&](unsigned (&vreg)[8], const int8_t* from) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if constexpr (NDB == 4) vreg[j] = *reinterpret_cast<const unsigned*>(from + vcol[j]);
@@ -640,7 +668,7 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
   int kat[NDB];  // where this lane's operands of K begin, of the first 32 keys
 #pragma unroll
   for (int i = 0; i < NDB; ++i) kat[i] = n * DP + swizzle(n, 2 * i + h) * 16;
-  auto put_k = [&](int slot) {
+  auto put_k = [&](const v4i (&kreg)[KC], int slot) {
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
       const int r = wave * 16 + i * (64 / CH) + krow;
@@ -789,24 +817,23 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
       at = at < last_block ? at : last_block;
       return b.table[(long long)it.seq * b.per_seq + ((at << 4) >> c.page_shift) + zero];
     };
-    int page = page_at(lo, wave), page_v;
-    fetch_k(k_from(lo, page));
-    fetch_v(v_from(lo, page));
-    put_k(0);
-    auto put_all = [&](int slot) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) lift(j);
-#pragma unroll
-      for (int i = 0; i < NDB; ++i) put_v(slot, i);
-    };
-    put_all(0);
-    page = page_at(lo + PT_KEYS, wave);
-    fetch_k(k_from(lo + PT_KEYS, page));
-    fetch_v(v_from(lo + PT_KEYS, page));
-    put_k(1);
-    page_v = page_at(lo + 2 * PT_KEYS, wave);
-    fetch_k(k_from(lo + 2 * PT_KEYS, page_v));
+    // the first three steps of K and two of V are asked for at once
+    const int page0 = page_at(lo, wave), page1 = page_at(lo + PT_KEYS, wave);
+    int page_v = page_at(lo + 2 * PT_KEYS, wave);
     int asked = ask(lo + 3 * PT_KEYS);
+    v4i k_0[KC], k_1[KC];
+    unsigned v_0[8];
+    fetch_k(k_0, k_from(lo, page0));
+    fetch_v(v_0, v_from(lo, page0));
+    fetch_k(k_1, k_from(lo + PT_KEYS, page1));
+    fetch_v(vreg, v_from(lo + PT_KEYS, page1));
+    fetch_k(kreg, k_from(lo + 2 * PT_KEYS, page_v));
+    put_k(k_0, 0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vplus[j] = v_0[j] ^ 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < NDB; ++i) put_v(0, i);
+    put_k(k_1, 1);
     __syncthreads();
     constexpr int V0 = 3 * KBYTES, K_HALF = 32 * DP, V_HALF = VBYTES / 2;
     Half even, odd;
@@ -849,7 +876,7 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
 #pragma unroll
           for (int j = 0; j < 8 / NDB; ++j) lift((m - NDB) * (8 / NDB) + j);
         }
-        if (m == 2 * NDB) fetch_v(from);
+        if (m == 2 * NDB) fetch_v(vreg, from);
         if (m >= 2 * NDB) put_v(k1, m - 2 * NDB);
       };
       auto stage_k = [&](int m) {
@@ -857,9 +884,9 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
           page_v = __builtin_amdgcn_readfirstlane(asked);
           from = k_from(s0 + 3 * PT_KEYS, page_v);
         }
-        if (m == NDB) put_k(k2);
+        if (m == NDB) put_k(kreg, k2);
         if (m == NDB + 1) {
-          fetch_k(from);
+          fetch_k(kreg, from);
           asked = ask(s0 + 4 * PT_KEYS);
         }
       };
@@ -895,37 +922,39 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
     auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(den), __float_as_uint(den), false, false);
     den = __uint_as_float(o[0]) + __uint_as_float(o[1]);
   }
-  if (it.splits == 1) {
-    const float f = den > 0.0f ? a.alpha_pv * 1024.0f / den : 0.0f;
-    if (real) {
-      const long long at = ((long long)(it.s.row0 + t) * a.q_heads + it.head * G + g) * c.D;
+  // Through the LDS, four columns at a place that the row moves, so that rows leave as whole lines.
+  __syncthreads();
+  float f = 1.0f;
+  if (it.splits == 1) f = den > 0.0f ? a.alpha_pv * 1024.0f / den : 0.0f;
+  constexpr int QUADS = DP / 4, PER = 64 / QUADS;  // rows that a wave stores at once
+  v4f* const own = reinterpret_cast<v4f*>(lds) + wave * 32 * QUADS;
+  auto spot = [](int r, int quad) { return r * QUADS + (quad ^ (r & (QUADS - 1))); };
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int d = NDB * ((r & 3) + 8 * (r >> 2) + 4 * h);
-        if (d < c.D) {
-          float y[NDB];
+  for (int r = 0; r < 16; ++r) {
+    const int m = (r & 3) + 8 * (r >> 2) + 4 * h;
+    float y[NDB];
 #pragma unroll
-          for (int i = 0; i < NDB; ++i) y[i] = den > 0.0f ? acc[i][r] * f : 0.0f;
-          store_some<NDB, OUT>(a.out, at + d, y);
-        }
-      }
-    }
-    return;
+    for (int i = 0; i < NDB; ++i) y[i] = f > 0.0f || f < 0.0f ? acc[i][r] * f : 0.0f;
+    if constexpr (NDB == 4) own[spot(n, m)] = v4f{y[0], y[1], y[2], y[3]};
+    else *(reinterpret_cast<v2f*>(&own[spot(n, m >> 1)]) + (m & 1)) = v2f{y[0], y[1]};
   }
+  __builtin_amdgcn_wave_barrier();
   const long long slot = it.first + (long long)it.split * it.step;
-  if (real) {
-    float* to = p.ws + (slot * PT_ROWS + wave * 32 + n) * DP;
+  const int quad = lane % QUADS;
+  const PagedRows out_row(it, a, G, PT_ROWS);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int d = NDB * ((r & 3) + 8 * (r >> 2) + 4 * h);
-      if (d < c.D) {
-        if constexpr (NDB == 4) put4(to + d, acc[0][r], acc[1][r], acc[2][r], acc[3][r]);
-        else put2(to + d, acc[0][r], acc[1][r]);
-      }
+  for (int i = 0; i < 32 / PER; ++i) {
+    const int r = i * PER + lane / QUADS, rr = row0 + r;
+    if (rr >= live_rows || quad * 4 >= c.D) continue;
+    const v4f y = own[spot(r, quad)];
+    if (it.splits == 1) {
+      store_some<4, OUT>(a.out, out_row(wave * 32 + r) * c.D + quad * 4, {y[0], y[1], y[2], y[3]});
+    } else {
+      put4(p.ws + (slot * PT_ROWS + wave * 32 + r) * DP + quad * 4, y[0], y[1], y[2], y[3]);
     }
-    if (h == 0) put2(p.ws + (long long)p.slots * PT_ROWS * DP + (slot * PT_ROWS + wave * 32 + n) * 2, off, den);
   }
-  meet_and_join<PT_ROWS, DP, OUT>(a, c, p, it, reinterpret_cast<int*>(lds + tiles_lds(DP) - 16), reinterpret_cast<float*>(lds));
+  if (it.splits > 1 && real && h == 0)
+    put2(p.ws + (long long)p.slots * PT_ROWS * DP + (slot * PT_ROWS + wave * 32 + n) * 2, off, den);
 }
 
 template <int DP, int OUT>
@@ -949,13 +978,13 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_both_kernel(PagedAtt
   else paged_rows<DP, OUT>(a, c, b, rows, index, lds);
 }
 
-// Joins the slices of the sequences that were cut where they do not meet in the launch itself; 16 rows to blockIdx.y.
-template <int ROWS, int DP, int OUT>
+// Joins slices that do not meet in the launch itself: an item that was cut to blockIdx.x, EACH of its rows to blockIdx.y.
+template <int ROWS, int EACH, int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p) {
   __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
-  const PagedItem it = paged_item(b, c.page_shift, c.heads, ROWS, p, blockIdx.x);
-  if (!it.found || it.split != 0 || it.splits == 1) return;
-  join_slices<ROWS, DP, OUT>(a, c, p, it, meet, blockIdx.y * PA_ROWS, PA_ROWS);
+  const PagedItem it = paged_item<true>(b, c.page_shift, c.heads, ROWS, p, blockIdx.x);
+  if (!it.found || it.split != 0) return;
+  join_slices<ROWS, EACH, DP, OUT>(a, c, p, it, meet, blockIdx.y * EACH);
 }
 
 // What a call of these sizes runs.  The lengths are on the device, so the grids and the workspace are bounds: one item to each
@@ -963,13 +992,18 @@ __global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a
 struct PagedShape {
   long long rows_slots, tiles_slots;  // items of either kind; 0: none
   bool rows_cut, tiles_cut;
+  bool rows_meet;  // slices of few rows meet in the launch
 };
 static PagedShape paged_shape(long long rows, long long seqs, long long group, long long heads, long long capacity) {
-  PagedShape s = {0, 0, false, false};
+  PagedShape s = {0, 0, false, false, true};
   const bool cut = capacity > PA_MIN_SLICE;
   if (rows * group <= PA_ROWS * seqs) {  // few rows to a sequence on average: all of them by that kernel
     s.rows_slots = heads * (seqs + rows * group / PA_ROWS);
     s.rows_cut = cut;
+    // where the slices of an item come to more than some 64 KB, one workgroup would be longer in joining them than another launch
+    // takes (2 x 100000 keys, 8 key heads of 8: 135 KB, REPLACE)
+    const long long each = rows * group / seqs + 1 < PA_ROWS ? rows * group / seqs + 1 : PA_ROWS;
+    s.rows_meet = PA_TARGET * each * 520 < 65536 * s.rows_slots;
     if (cut) s.rows_slots += PA_TARGET + 8;
     return s;
   }
@@ -990,7 +1024,7 @@ static long long paged_bytes(long long slots, int rows, long long D) { return sl
 
 long long paged_attn_arrivals(long long rows, long long seqs, long long q_heads, long long heads, long long capacity) {
   const PagedShape s = paged_shape(rows, seqs, q_heads / heads, heads, capacity);
-  return (s.rows_cut ? s.rows_slots : 0) + (s.tiles_cut ? s.tiles_slots : 0);
+  return s.rows_cut && s.rows_meet ? s.rows_slots : 0;
 }
 long long paged_attn_workspace_bytes(long long rows, long long seqs, long long q_heads, long long heads, long long D,
                                      long long capacity) {
@@ -1006,11 +1040,17 @@ static void launch_attn(const PagedAttn& a, const PagedCache& c, const PagedBatc
     hipLaunchKernelGGL((paged_attn_both_kernel<DP, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows, tiles);
   else
     hipLaunchKernelGGL((paged_attn_rows_kernel<DP, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows);
+  // an item that is cut has more than a PA_TARGET-th of all keys, so there are fewer than PA_TARGET of them
+  auto items = [](const PagedPlan& p) {
+    const int most = p.slots - PA_TARGET - 8;
+    return (unsigned)(most < PA_TARGET ? most : PA_TARGET);
+  };
   if (rows.target > 0 && rows.arrivals == nullptr)
-    hipLaunchKernelGGL((paged_attn_join_kernel<PA_ROWS, DP, OUT>), dim3(rows.slots), dim3(PA_THREADS), 0, stream, a, c, b, rows);
-  if (tiles.target > 0 && tiles.arrivals == nullptr)
-    hipLaunchKernelGGL((paged_attn_join_kernel<PT_ROWS, DP, OUT>), dim3(tiles.slots, PT_ROWS / PA_ROWS), dim3(PA_THREADS), 0, stream, a,
-                       c, b, tiles);
+    hipLaunchKernelGGL((paged_attn_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(items(rows), PA_ROWS / 2), dim3(PA_THREADS), 0, stream, a, c, b,
+                       rows);
+  if (tiles.target > 0)
+    hipLaunchKernelGGL((paged_attn_join_kernel<PT_ROWS, 16, DP, OUT>), dim3(items(tiles), PT_ROWS / 16), dim3(PA_THREADS), 0, stream, a, c, b,
+                       tiles);
 }
 
 int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, const PagedBatch& b, void* workspace,
@@ -1032,14 +1072,13 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
   rows.slots = (int)s.rows_slots;
   rows.target = s.rows_cut ? PA_TARGET : 0;
   rows.ws = reinterpret_cast<float*>(ws);
-  rows.arrivals = meet && s.rows_cut ? a.arrivals : nullptr;
+  rows.arrivals = meet && s.rows_cut && s.rows_meet ? a.arrivals : nullptr;
   tiles.least = s.rows_slots > 0 ? PA_ROWS : 0;
   tiles.most = 0x7fffffff;
   tiles.slots = (int)s.tiles_slots;
   tiles.target = s.tiles_cut ? PA_TARGET : 0;
   tiles.ws = reinterpret_cast<float*>(ws + (s.rows_cut ? paged_bytes(s.rows_slots, PA_ROWS, c.D) : 0));
-  // few items of 128 rows have many slices of 66 KB each, which one workgroup would be long in joining
-  tiles.arrivals = meet && s.tiles_cut && s.tiles_slots - PA_TARGET - 8 >= PT_MEET ? a.arrivals + (s.rows_cut ? rows.slots : 0) : nullptr;
+  tiles.arrivals = nullptr;  // slices of 66 KB: many workgroups join them, in a launch of their own
   auto run = [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
     if (out_type == PT_S8) launch_attn<DP, PT_S8>(a, c, b, rows, tiles, stream);
