@@ -70,8 +70,6 @@ _counters = {}  # (device index, stream) -> int32 zeros in which the slices of a
 
 def _arrivals(dev_index, stream, n):
     """Counters for one stream, grown on demand; a recording gets its own, cleared by the recording itself."""
-    if n <= 0:
-        return None, 0
     key = (dev_index, stream)
     t = _counters.get(key)
     capturing = torch.cuda.is_current_stream_capturing()
@@ -91,7 +89,23 @@ def _describe(t):
 
 
 def _cache_and_batch(op, k_cache, v_cache, block_table, context_lens, cu_new, rows):
-    """The arguments that both calls begin with, checked."""
+    """The arguments that both calls begin with, checked.  The usual call passes one expression; whatever does not is looked at
+    argument by argument, for the message."""
+    try:
+        dev = k_cache.get_device()
+        if (k_cache.is_cuda and k_cache.dtype is _I8 and v_cache.dtype is _I8 and v_cache.get_device() == dev
+                and block_table.dtype is _I32 and block_table.get_device() == dev and block_table.is_contiguous()
+                and context_lens.dtype is _I32 and context_lens.get_device() == dev and context_lens.is_contiguous()
+                and cu_new.dtype is _I32 and cu_new.get_device() == dev and cu_new.is_contiguous()):
+            shape = pages, heads, page_size, head_dim = k_cache.shape
+            kp, kh, kt, kd = k_cache.stride()
+            vp, vh, vt, vd = v_cache.stride()
+            seqs, per_seq = block_table.shape
+            if v_cache.shape == shape and kd == 1 and vd == 1 and context_lens.shape == (seqs,) and cu_new.shape == (seqs + 1,):
+                return (k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, heads, head_dim, kp, kh, kt, vp, vh, vt,
+                        block_table.data_ptr(), context_lens.data_ptr(), cu_new.data_ptr(), per_seq, seqs, rows)
+    except (AttributeError, TypeError, ValueError):
+        pass
     for name, t, dtype, ndim in (("k_cache", k_cache, _I8, 4), ("v_cache", v_cache, _I8, 4), ("block_table", block_table, _I32, 2),
                                  ("context_lens", context_lens, _I32, 1), ("cu_new", cu_new, _I32, 1)):
         if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != ndim:
@@ -103,39 +117,37 @@ def _cache_and_batch(op, k_cache, v_cache, block_table, context_lens, cu_new, ro
     shape = k_cache.shape
     if v_cache.shape != shape:
         _fail(op, f"k_cache is {tuple(shape)} but v_cache is {tuple(v_cache.shape)}")
-    pages, heads, page_size, head_dim = shape
-    kp, kh, kt, kd = k_cache.stride()
-    vp, vh, vt, vd = v_cache.stride()
-    if (kd != 1 or vd != 1) and head_dim > 1:
+    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
         _fail(op, "the last dimension of k_cache and v_cache must be contiguous")
     seqs = context_lens.shape[0]
     if cu_new.shape[0] != seqs + 1 or block_table.shape[0] != seqs:
         _fail(op, f"context_lens has {seqs} sequences, cu_new {cu_new.shape[0]} entries (one more is needed), block_table "
                   f"{block_table.shape[0]} rows")
-    if not (block_table.is_contiguous() and context_lens.is_contiguous() and cu_new.is_contiguous()):
-        _fail(op, "block_table, context_lens and cu_new must be contiguous")
-    return (k_cache.data_ptr(), v_cache.data_ptr(), pages, page_size, heads, head_dim, kp, kh, kt, vp, vh, vt,
-            block_table.data_ptr(), context_lens.data_ptr(), cu_new.data_ptr(), block_table.shape[1], seqs, rows)
+    _fail(op, "block_table, context_lens and cu_new must be contiguous")
 
 
-def _rows(op, name, t, dtype, shape, device):
-    """Row and head stride of a [rows, heads, head_dim] tensor whose last dimension is contiguous; ``shape`` -1: any number."""
+def _rows(op, name, t, dtype, shape, k_cache):
+    """Row and head stride of a tensor [rows, heads, head_dim] = ``shape`` whose last dimension is contiguous."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == k_cache.get_device():
+        row, head, last = t.stride()
+        if last == 1:
+            return row, head
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != 3:
         _fail(op, f"{name} must be a 3-D {dtype} tensor, got {_describe(t)}")
-    if t.device != device:
-        _fail(op, f"{name} is on {t.device}, expected {device}")
-    for have, want in zip(t.shape, shape):
-        if want not in (-1, have):
-            _fail(op, f"{name} is {tuple(t.shape)}, expected {tuple(shape)} (-1: any)")
-    row, head, last = t.stride()
-    if last != 1 and t.shape[2] > 1:
-        _fail(op, f"the last dimension of {name} must be contiguous")
-    return row, head
+    if t.device != k_cache.device:
+        _fail(op, f"{name} is on {t.device}, expected {k_cache.device}")
+    if t.shape != shape:
+        _fail(op, f"{name} is {tuple(t.shape)}, expected {tuple(shape)}")
+    _fail(op, f"the last dimension of {name} must be contiguous")
+
+
+def _on(dev):
+    """Context that makes device number ``dev`` current; free when it already is."""
+    return _hip_ext._NO_SWITCH if dev == _hip_ext._current_device() else torch.cuda.device(dev)
 
 
 def _status(op, rc):
-    if rc:
-        _fail(op, f"{_lib.ti_last_error().decode()} (status {rc})")
+    _fail(op, f"{_lib.ti_last_error().decode()} (status {rc})")
 
 
 def paged_kv_append_s8(key, value, k_cache, v_cache, block_table, context_lens, cu_new, alpha_k, alpha_v, query=None, alpha_q=1.0,
@@ -158,20 +170,24 @@ def paged_kv_append_s8(key, value, k_cache, v_cache, block_table, context_lens, 
         _fail(op, f"key must be a 3-D tensor of float32, float16, bfloat16 or int8, got {_describe(key)}")
     rows = key.shape[0]
     args = _cache_and_batch(op, k_cache, v_cache, block_table, context_lens, cu_new, rows)
-    dev = k_cache.device
+    dev = k_cache.get_device()
     heads, d = args[4], args[5]
-    k_row, k_head = _rows(op, "key", key, dtype, (rows, heads, d), dev)
-    v_row, v_head = _rows(op, "value", value, dtype, (rows, heads, d), dev)
+    shape = (rows, heads, d)
+    k_row, k_head = _rows(op, "key", key, dtype, shape, k_cache)
+    v_row, v_head = _rows(op, "value", value, dtype, shape, k_cache)
     q_ptr = q_row = q_head = q_heads = out_ptr = 0
     out = None
     if query is not None:
-        q_row, q_head = _rows(op, "query", query, dtype, (rows, -1, d), dev)
+        if not isinstance(query, torch.Tensor) or query.dim() != 3:
+            _fail(op, f"query must be a 3-D {dtype} tensor, got {_describe(query)}")
         q_heads, q_ptr = query.shape[1], query.data_ptr()
+        shape = (rows, q_heads, d)
+        q_row, q_head = _rows(op, "query", query, dtype, shape, k_cache)
         if query_out is None:
-            out = torch.empty((rows, q_heads, d), dtype=_I8, device=dev)
+            out = query.new_empty(shape, dtype=_I8)
         else:
             out = query_out
-            _rows(op, "query_out", out, _I8, (rows, q_heads, d), dev)
+            _rows(op, "query_out", out, _I8, shape, k_cache)
             if not out.is_contiguous():
                 _fail(op, "query_out must be contiguous")
         out_ptr = out.data_ptr()
@@ -181,8 +197,8 @@ def paged_kv_append_s8(key, value, k_cache, v_cache, block_table, context_lens, 
     if cos_sin is not None:
         if not isinstance(cos_sin, torch.Tensor) or cos_sin.dtype is not _F32 or cos_sin.dim() != 2:
             _fail(op, f"cos_sin must be a 2-D torch.float32 tensor, got {_describe(cos_sin)}")
-        if cos_sin.device != dev or not cos_sin.is_contiguous():
-            _fail(op, f"cos_sin must be contiguous and on {dev}")
+        if cos_sin.get_device() != dev or not cos_sin.is_contiguous():
+            _fail(op, f"cos_sin must be contiguous and on {k_cache.device}")
         positions, rot = cos_sin.shape
         cs_ptr = cos_sin.data_ptr()
         if rot < 16 or rot > d or rot % 16:
@@ -193,13 +209,14 @@ def paged_kv_append_s8(key, value, k_cache, v_cache, block_table, context_lens, 
         return out
     tail = (key.data_ptr(), value.data_ptr(), q_ptr, k_row, k_head, v_row, v_head, q_row, q_head, out_ptr, q_heads, cs_ptr, rot,
             positions, code, 1 if neighbours else 0, 1 if query_out is None else 0, float(alpha_q), float(alpha_k), float(alpha_v))
-    with _hip_ext._on(dev):
-        stream = _raw_stream(dev.index)
+    with _on(dev):
+        stream = _raw_stream(dev)
         if _fast_append is not None:
             rc = _fast_append(*args, *tail, stream)
         else:
             rc = _lib.ti_paged_kv_append_s8(_Cache(*args[:12]), _Batch(*args[12:]), _Append(*tail), stream or None)
-    _status(op, rc)
+    if rc:
+        _status(op, rc)
     return out
 
 
@@ -216,9 +233,10 @@ def paged_attn_s8(query, k_cache, v_cache, block_table, context_lens, cu_new, al
         _fail(op, f"query must be a 3-D torch.int8 tensor, got {_describe(query)}")
     rows, q_heads, _ = query.shape
     args = _cache_and_batch(op, k_cache, v_cache, block_table, context_lens, cu_new, rows)
-    dev = k_cache.device
+    dev = k_cache.get_device()
     heads, d, seqs = args[4], args[5], args[16]
-    q_row, q_head = _rows(op, "query", query, _I8, (-1, -1, d), dev)
+    shape = (rows, q_heads, d)
+    q_row, q_head = _rows(op, "query", query, _I8, shape, k_cache)
     if heads == 0 or q_heads == 0 or q_heads % heads:
         _fail(op, f"{q_heads} query heads are no multiple of {heads} key heads")
     if out is None:
@@ -226,13 +244,13 @@ def paged_attn_s8(query, k_cache, v_cache, block_table, context_lens, cu_new, al
         code = _TYPES.get(out_dtype)
         if code is None or code == 0:
             _fail(op, f"out_dtype must be torch.int8, torch.float16 or torch.bfloat16, got {out_dtype}")
-        out = torch.empty((rows, q_heads, d), dtype=out_dtype, device=dev)
+        out = query.new_empty(shape, dtype=out_dtype)
     else:
         fill = 0
         code = _TYPES.get(out.dtype) if isinstance(out, torch.Tensor) else None
         if code is None or code == 0:
             _fail(op, f"out must be a tensor of int8, float16 or bfloat16, got {_describe(out)}")
-        _rows(op, "out", out, out.dtype, (rows, q_heads, d), dev)
+        _rows(op, "out", out, out.dtype, shape, k_cache)
         if not out.is_contiguous():
             _fail(op, "out must be contiguous")
     if rows == 0:
@@ -243,15 +261,16 @@ def paged_attn_s8(query, k_cache, v_cache, block_table, context_lens, cu_new, al
         if len(_ws_need) >= 4096:
             _ws_need.clear()
         need = _ws_need[key] = (int(_lib.ti_paged_attn_workspace_bytes(*key)), int(_lib.ti_paged_attn_arrivals(*key)))
-    with _hip_ext._on(dev):
-        stream = _raw_stream(dev.index)
-        ws, ws_ptr, ws_bytes = _CUDA._workspace(dev.index, stream, need[0])
-        counters, counters_ptr = _arrivals(dev.index, stream, need[1])
+    with _on(dev):
+        stream = _raw_stream(dev)
+        ws, ws_ptr, ws_bytes = _CUDA._workspace(dev, stream, need[0])
+        counters, counters_ptr = _arrivals(dev, stream, need[1]) if need[1] > 0 else (None, 0)
         tail = (query.data_ptr(), q_row, q_head, q_heads, out.data_ptr(), code, fill, float(alpha_qk), float(alpha_pv), counters_ptr,
                 need[1])
         if _fast_attn is not None:
             rc = _fast_attn(*args, *tail, ws_ptr, ws_bytes, stream)
         else:
             rc = _lib.ti_paged_attn_s8(_Cache(*args[:12]), _Batch(*args[12:]), _Attn(*tail), ws_ptr or None, ws_bytes, stream or None)
-    _status(op, rc)
+    if rc:
+        _status(op, rc)
     return out
