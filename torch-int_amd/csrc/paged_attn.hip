@@ -91,9 +91,10 @@ __device__ __forceinline__ int paged_slice(float items, float total, int target)
   return slice < PA_MIN_SLICE ? PA_MIN_SLICE : slice;
 }
 
-// The work item with number `index`, in the order sequence, slice, tile of rows (the last, which has the most keys,
-// first), head.  CUT: the first slice of the `index`-th item among those that are cut.
-template <bool CUT = false>
+// The work item with number `index`, in the order part, sequence, slice, tile of rows, head.  A sequence's tiles come from the
+// last, which has the most keys, to the first, in PARTS parts, so that the long items of all sequences begin before the short
+// ones.  CUT: the first slice of the `index`-th item among those that are cut.
+template <int PARTS, bool CUT = false>
 __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_shift, int heads, int rows_per_tile, const PagedPlan& p,
                                                 int index) {
   PagedItem it;
@@ -120,20 +121,32 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
     it.slice = paged_slice(items * (float)heads, total * (float)heads, p.target);
   }
   int before = 0, before_cut = 0;
+  int splits = 1;
+  auto cut_up = [&] { splits = s.len <= it.slice ? 1 : (s.len + it.slice - 1) / it.slice; };
+  if (b.seqs <= 64) {
+    if (p.target == 0) look(0);
+    cut_up();
+    if (CUT && __ballot(splits > 1 && tiles > 0) == 0) return it;
+  }
+  for (int part = 0; part < PARTS; ++part)
   for (int i0 = 0; i0 < b.seqs; i0 += 64) {
-    if (i0 > 0 || p.target == 0) look(i0);
-    const int splits = s.len <= it.slice ? 1 : (s.len + it.slice - 1) / it.slice;
+    if (b.seqs > 64) {
+      look(i0);
+      cut_up();
+    }
+    const int behind = PARTS == 1 ? 0 : (int)((long long)tiles * part / PARTS);  // tiles of the parts before
+    const int here = PARTS == 1 ? tiles : (int)((long long)tiles * (part + 1) / PARTS) - behind;
     // a cu_new that descends can count rows many times over: no sum of items passes the range of int
-    const long long all = (long long)tiles * splits * heads;
+    const long long whole = (long long)here * heads, all = whole * splits;
     const int n = all > 0x800000 ? 0x800000 : (int)all;
-    const int cut = splits > 1 ? n / splits : 0;
+    const int cut = splits == 1 ? 0 : whole > 0x800000 ? 0x800000 : (int)whole;
     const int upto = wave_scan(n), upto_cut = CUT ? wave_scan(cut) : 0;
     const unsigned long long past = __ballot(CUT ? before_cut + upto_cut > index : before + upto > index);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
       const int first = before + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at);
       const int rel = CUT ? index - (before_cut + __builtin_amdgcn_readlane(upto_cut, at) - __builtin_amdgcn_readlane(cut, at)) : index - first;
-      const int t = __builtin_amdgcn_readlane(tiles, at);
+      const int t = __builtin_amdgcn_readlane(here, at), skip = __builtin_amdgcn_readlane(behind, at);
       it.s.row0 = __builtin_amdgcn_readlane(s.row0, at);
       it.s.T = __builtin_amdgcn_readlane(s.T, at);
       it.s.len = __builtin_amdgcn_readlane(s.len, at);
@@ -142,7 +155,7 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
       it.step = heads * t;
       it.split = rel / it.step;
       const int rest = rel - it.split * it.step, from_last = rest / heads;
-      it.tile = t - 1 - from_last;
+      it.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - skip - from_last;
       it.head = rest - from_last * heads;
       it.first = first + rest;
       // all slices have a slot and a workgroup, or (as a cu_new that descends can have it) the item is left out
@@ -349,7 +362,7 @@ __device__ __forceinline__ void paged_rows(const PagedAttn& a, const PagedCache&
   const auto offs = reinterpret_cast<float(*)[PA_ROWS]>(lds + PA_WAVES * PA_ROWS * (DP + 4) * 4);
   const auto den = offs + PA_WAVES;
 
-  const PagedItem it = paged_item(b, c.page_shift, c.heads, PA_ROWS, p, index);
+  const PagedItem it = paged_item<1>(b, c.page_shift, c.heads, PA_ROWS, p, index);
   if (!it.found) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -580,6 +593,9 @@ __device__ __forceinline__ void paged_rows(const PagedAttn& a, const PagedCache&
 // Scores start from 1.5 * 2^23 instead of 0: the int32 sum is then the fp32 number 12582912 + x, and the constant goes into the
 // row's offset, where one multiply-add removes it exactly.
 constexpr int PT_ROWS = 128, PT_KEYS = 64;
+// Parts in which the tiles come (paged_item): 4 x 512 rows of 40 heads, four tiles to each, 39.1 us in one part, 38.3 in two, 36.5
+// in four.
+constexpr int PT_PARTS = 4;
 constexpr int PT_JOIN = 32;      // rows that a workgroup joins
 constexpr int PT_PLENTY = 2048;  // items from which on nothing is cut: four to each place on the chip
 constexpr int tiles_lds(int DP) { return 3 * 3 * PT_KEYS * DP; }  // three steps of K, then of V as fp16
@@ -591,7 +607,7 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
   constexpr int CH = DP / 16;    // 16-byte chunks of a key row
   constexpr int KBYTES = PT_KEYS * DP, VBYTES = 2 * KBYTES;
 
-  const PagedItem it = paged_item(b, c.page_shift, c.heads, PT_ROWS, p, index);
+  const PagedItem it = paged_item<PT_PARTS>(b, c.page_shift, c.heads, PT_ROWS, p, index);
   if (!it.found) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -667,10 +683,6 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
       else vreg[j] = *reinterpret_cast<const unsigned short*>(from + vcol[j]);
     }
   };
-  // whether the pool lacks any of the item's pages: looked at once, so that steps need not
-  bool holes = false;
-  for (int i = (lo >> c.page_shift) + lane; i <= (hi - 1) >> c.page_shift; i += 64) holes |= !have(table[i]);
-  holes = __ballot(holes) != 0;
   auto swizzle = [](int r, int chunk) { return DP == 128 ? chunk ^ (r & 7) : chunk ^ ((r >> 2) & 3); };
   int kat[NDB];  // where this lane's operands of K begin, of the first 32 keys
 #pragma unroll
@@ -809,12 +821,6 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
   };
 
   if (lo < hi) {
-    auto lost = [&](int s0) {
-      int bits = 0;
-      if (__builtin_expect(holes, 0))
-        for (int i = 0; i < 4; ++i) bits |= (have(page_at(s0, i)) ? 0 : 1) << i;
-      return bits;
-    };
     // Pages are looked up a step ahead, by vector loads: these return in order, so that the wait for the keys and values in
     // front of one is all the wait it needs (a scalar one would have to be over at every wait for the LDS).
     int zero = 0;
@@ -835,6 +841,16 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
     fetch_k(k_1, k_from(lo + PT_KEYS, page1));
     fetch_v(vreg, v_from(lo + PT_KEYS, page1));
     fetch_k(kreg, k_from(lo + 2 * PT_KEYS, page_v));
+    // whether the pool lacks any of the item's pages: looked at once, while the first keys are on their way, so that steps need not
+    bool holes = false;
+    for (int i = (lo >> c.page_shift) + lane; i <= (hi - 1) >> c.page_shift; i += 64) holes |= !have(table[i]);
+    holes = __ballot(holes) != 0;
+    auto lost = [&](int s0) {
+      int bits = 0;
+      if (__builtin_expect(holes, 0))
+        for (int i = 0; i < 4; ++i) bits |= (have(page_at(s0, i)) ? 0 : 1) << i;
+      return bits;
+    };
     put_k(k_0, 0);
 #pragma unroll
     for (int j = 0; j < 8; ++j) vplus[j] = v_0[j] ^ 0x80808080u;
@@ -971,16 +987,20 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAtt
   paged_rows<DP, OUT>(a, c, b, rows, blockIdx.x, lds);
 }
 
-// Sequences of few rows and of many in one launch, an item of the one kind after one of the other as long as both last: those
-// with few rows wait for memory while the others compute.
+// Sequences of few rows and of many in one launch, 32 items of the one kind after 32 of the other as long as both last: those
+// with few rows wait for memory while the others compute.  Workgroups go to the eight XCDs and, within one, to its four shader
+// engines in turn, and the next waits until there is room at its own engine: one kind after the other in turns of 1 or 8 would
+// leave the long items, two to a CU, to half of the chip, with the other half idle behind them (4 x 512 rows of 40 heads 41.4
+// against 36.5 us, 512 rows over 2000 keys beside a sequence of one row 56.7 against 43.9).
+constexpr int TURN = 32;
 template <int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_both_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan rows,
                                                                         PagedPlan tiles) {
   __shared__ __attribute__((aligned(16))) char lds[tiles_lds(DP) > rows_lds(DP) ? tiles_lds(DP) : rows_lds(DP)];
   if (a.fill) paged_fill(b, static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
-  const int i = blockIdx.x, both = 2 * (rows.slots < tiles.slots ? rows.slots : tiles.slots);
-  const bool many = i < both ? (i & 1) == 0 : tiles.slots > rows.slots;
-  const int index = i < both ? i >> 1 : i - both / 2;
+  const int i = blockIdx.x, each = (rows.slots < tiles.slots ? rows.slots : tiles.slots) & -TURN, rest = i - 2 * each;
+  const bool many = rest < 0 ? (i & TURN) == 0 : rest < tiles.slots - each;
+  const int index = rest < 0 ? i / (2 * TURN) * TURN + i % TURN : each + rest - (many ? 0 : tiles.slots - each);
   if (many) paged_tiles<DP, OUT>(a, c, b, tiles, index, lds);
   else paged_rows<DP, OUT>(a, c, b, rows, index, lds);
 }
@@ -989,7 +1009,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_both_kernel(PagedAtt
 template <int ROWS, int EACH, int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p) {
   __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
-  const PagedItem it = paged_item<true>(b, c.page_shift, c.heads, ROWS, p, blockIdx.x);
+  const PagedItem it = paged_item<ROWS == PT_ROWS ? PT_PARTS : 1, true>(b, c.page_shift, c.heads, ROWS, p, blockIdx.x);
   if (!it.found || it.split != 0) return;
   join_slices<ROWS, EACH, DP, OUT, false>(a, c, p, it, meet, blockIdx.y * EACH);
 }
@@ -1047,10 +1067,10 @@ static void launch_attn(const PagedAttn& a, const PagedCache& c, const PagedBatc
     hipLaunchKernelGGL((paged_attn_both_kernel<DP, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows, tiles);
   else
     hipLaunchKernelGGL((paged_attn_rows_kernel<DP, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows);
-  // an item that is cut has more than a PA_TARGET-th of all keys, so there are fewer than PA_TARGET of them
+  // an item that is cut has more than a target-th of all keys, so there are fewer than `target` of them
   auto items = [](const PagedPlan& p) {
     const int most = p.slots - PA_TARGET - 8;
-    return (unsigned)(most < PA_TARGET ? most : PA_TARGET);
+    return (unsigned)(most < p.target ? most : p.target);
   };
   if (rows.target > 0 && rows.arrivals == nullptr)
     hipLaunchKernelGGL((paged_attn_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(items(rows), PA_ROWS / 2), dim3(PA_THREADS), 0, stream, a, c, b,
@@ -1072,18 +1092,21 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
     return fail(TI_ERR_INVALID_ARG, "paged_attn_s8: %lld work items", s.rows_slots + s.tiles_slots);
   const bool meet = a.arrivals != nullptr && a.arrivals_count >= paged_attn_arrivals(b.rows, b.seqs, a.q_heads, c.heads, capacity);
   char* ws = static_cast<char*>(workspace);
+  // where both kinds share the chip, half of it for each: 512 rows over 2000 keys beside 31 sequences of one row took 58.8 us
+  // with 512 slices of each, 50.4 with 256
+  const int target = s.rows_slots > 0 && s.tiles_slots > 0 ? PA_TARGET / 2 : PA_TARGET;
   PagedPlan rows, tiles;
   rows.group = tiles.group = group;
   rows.least = 0;
   rows.most = s.tiles_slots > 0 ? PA_ROWS : 0x7fffffff;
   rows.slots = (int)s.rows_slots;
-  rows.target = s.rows_cut ? PA_TARGET : 0;
+  rows.target = s.rows_cut ? target : 0;
   rows.ws = reinterpret_cast<float*>(ws);
   rows.arrivals = meet && s.rows_cut && s.rows_meet ? a.arrivals : nullptr;
   tiles.least = s.rows_slots > 0 ? PA_ROWS : 0;
   tiles.most = 0x7fffffff;
   tiles.slots = (int)s.tiles_slots;
-  tiles.target = s.tiles_cut ? PA_TARGET : 0;
+  tiles.target = s.tiles_cut ? target : 0;
   tiles.ws = reinterpret_cast<float*>(ws + (s.rows_cut ? paged_bytes(s.rows_slots, PA_ROWS, c.D) : 0));
   tiles.arrivals = nullptr;  // slices of 66 KB: many workgroups join them, in a launch of their own
   auto run = [&](auto dp) {
