@@ -133,3 +133,16 @@ def test_the_oracle_agrees_with_dense_attention():
     s = s.masked_fill(torch.ones(5, 40).triu(36).bool(), float("-inf"))
     want = 0.5 * torch.einsum("hts,shd->thd", torch.softmax(s, -1), vv)
     assert torch.allclose(got, want, rtol=1e-12, atol=1e-12) and (size >= got.abs() - 1e-12).all()
+
+
+def test_modules_keep_their_scales_as_buffers():
+    from torch_int.nn import PagedAttn_S8, PagedKVAppend_S8
+    append = PagedKVAppend_S8.from_scale(torch.tensor(0.25), 0.5, 0.125, neighbours=True)
+    assert {n: float(t) for n, t in append.state_dict().items()} == {"a_k": 4.0, "a_v": 2.0, "a_q": 8.0} and append.neighbours
+    attend = PagedAttn_S8.from_scale(0.125, torch.tensor(0.25), 0.5, softmax_scale=0.5)
+    assert {n: float(t) for n, t in attend.state_dict().items()} == {"a": 1 / 64, "b": 0.5} and attend.out_dtype is torch.float16
+    attend = PagedAttn_S8.from_scale(0.125, 0.25, 0.5, 0.25)
+    assert float(attend.b) == 2.0 and attend.out_dtype is torch.int8
+    other = PagedAttn_S8()
+    other.load_state_dict(attend.state_dict())
+    assert other._scalar("a") == 1 / 32 and other._scalar("b") == 2.0
