@@ -987,12 +987,12 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAtt
   paged_rows<DP, OUT>(a, c, b, rows, blockIdx.x, lds);
 }
 
-// Sequences of few rows and of many in one launch, 32 items of the one kind after 32 of the other as long as both last: those
-// with few rows wait for memory while the others compute.  Workgroups go to the eight XCDs and, within one, to its four shader
-// engines in turn, and the next waits until there is room at its own engine: one kind after the other in turns of 1 or 8 would
-// leave the long items, two to a CU, to half of the chip, with the other half idle behind them (4 x 512 rows of 40 heads 41.4
-// against 36.5 us, 512 rows over 2000 keys beside a sequence of one row 56.7 against 43.9).
-constexpr int TURN = 32;
+// Sequences of few rows and of many in one launch, 256 items of the one kind after 256 of the other as long as both last: those
+// with few rows wait for memory while the others compute.  Workgroups go in turn to the eight XCDs, within one to its four shader
+// engines, within one to its eight CUs, and the next waits until there is room at its own engine: so 256 leave one of each kind
+// to every CU, while turns of 1, 8 or 32 leave the long items, two to a CU, to half of the chip, with the other half idle
+// behind them (512 rows over 2000 keys beside a sequence of one row: 56.7 us by 8, 45.4 by 32, 39.5 by 256).
+constexpr int TURN = 256;
 template <int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_both_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan rows,
                                                                         PagedPlan tiles) {
