@@ -1005,13 +1005,14 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_both_kernel(PagedAtt
   else paged_rows<DP, OUT>(a, c, b, rows, index, lds);
 }
 
-// Joins slices that do not meet in the launch itself: an item that was cut to blockIdx.x, EACH of its rows to blockIdx.y.
+// Joins slices that do not meet in the launch itself: an item that was cut to blockIdx.y, EACH of its rows to blockIdx.x (so that
+// what there is to join comes first, and goes to all CUs).
 template <int ROWS, int EACH, int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p) {
   __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
-  const PagedItem it = paged_item<ROWS == PT_ROWS ? PT_PARTS : 1, true>(b, c.page_shift, c.heads, ROWS, p, blockIdx.x);
+  const PagedItem it = paged_item<ROWS == PT_ROWS ? PT_PARTS : 1, true>(b, c.page_shift, c.heads, ROWS, p, blockIdx.y);
   if (!it.found || it.split != 0) return;
-  join_slices<ROWS, EACH, DP, OUT, false>(a, c, p, it, meet, blockIdx.y * EACH);
+  join_slices<ROWS, EACH, DP, OUT, false>(a, c, p, it, meet, blockIdx.x * EACH);
 }
 
 // What a call of these sizes runs.  The lengths are on the device, so the grids and the workspace are bounds: one item to each
@@ -1073,10 +1074,10 @@ static void launch_attn(const PagedAttn& a, const PagedCache& c, const PagedBatc
     return (unsigned)(most < p.target ? most : p.target);
   };
   if (rows.target > 0 && rows.arrivals == nullptr)
-    hipLaunchKernelGGL((paged_attn_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(items(rows), PA_ROWS / 2), dim3(PA_THREADS), 0, stream, a, c, b,
+    hipLaunchKernelGGL((paged_attn_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(PA_ROWS / 2, items(rows)), dim3(PA_THREADS), 0, stream, a, c, b,
                        rows);
   if (tiles.target > 0)
-    hipLaunchKernelGGL((paged_attn_join_kernel<PT_ROWS, PT_JOIN, DP, OUT>), dim3(items(tiles), PT_ROWS / PT_JOIN), dim3(PA_THREADS), 0, stream, a, c, b,
+    hipLaunchKernelGGL((paged_attn_join_kernel<PT_ROWS, PT_JOIN, DP, OUT>), dim3(PT_ROWS / PT_JOIN, items(tiles)), dim3(PA_THREADS), 0, stream, a, c, b,
                        tiles);
 }
 
