@@ -638,13 +638,14 @@ int ti_paged_kv_append_s8(const TiPagedCache* cache, const TiPagedBatch* batch, 
  * q int8 [rows, q_heads, head_dim] with row and head strides in bytes, multiples of 16; q_heads a multiple of the cache's
  * heads, q head h reads key head h / (q_heads / heads).  out [rows, q_heads, head_dim] packed, of `out_type`: TI_TYPE_S8
  * (rint, clamp to [-128, 127]), TI_TYPE_F16 or TI_TYPE_BF16.  Rows of no sequence become zeros with `fill` and stay as they
- * are without.  alpha_qk in [1e-30, 0.25] (scores reach 2^21 alpha_qk).  Probabilities are not quantised to int8 (the whole-cache attentions above do
- * that): a row's largest counts 2^8 to 2^15 in fp16, and where little else bounds the kernel they have 22 bits.
+ * are without.  alpha_qk in [1e-30, 0.25] (scores reach 2^21 alpha_qk).  Probabilities are not quantised to int8 (the
+ * whole-cache attentions above do that): a row's largest counts 2^8 to 2^15 in fp16, and where little else bounds the kernel
+ * they have 22 bits.
  * `workspace` (16-byte aligned, private to the stream, contents irrelevant) of ti_paged_attn_workspace_bytes lets long
  * sequences be cut into slices; with less, or NULL, each is read by one workgroup.  `capacity` there: pages_per_seq *
- * page_size.  The slices meet in the same launch where `arrivals` gives ti_paged_attn_arrivals (same arguments) int32
+ * page_size.  Where ti_paged_attn_arrivals (same arguments) is not 0 and `arrivals` gives as many int32
  * counters, zero before the first call and again after every one, that no call on another stream and no other recorded graph
- * uses; without them a second launch joins the slices.  Same bits. */
+ * uses, slices of few rows meet in the same launch; all others are joined by a second one.  Same bits. */
 typedef struct {
   const int8_t* q;
   int64_t q_row, q_head, q_heads;

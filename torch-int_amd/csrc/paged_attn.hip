@@ -128,8 +128,7 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
     cut_up();
     if (CUT && __ballot(splits > 1 && tiles > 0) == 0) return it;
   }
-  for (int part = 0; part < PARTS; ++part)
-  for (int i0 = 0; i0 < b.seqs; i0 += 64) {
+  for (int part = 0, i0 = 0; part < PARTS; i0 + 64 < b.seqs ? i0 += 64 : (i0 = 0, ++part)) {
     if (b.seqs > 64) {
       look(i0);
       cut_up();
@@ -335,7 +334,8 @@ __device__ __forceinline__ void join_slices(const PagedAttn& a, const PagedCache
 
 // The workgroup that arrives last joins the slices, in their order: the bits do not depend on who that is.  Partial sums are
 // written through to memory and read from there, and the counter is a device-scope atomic, so no cache has to be written back
-// or emptied (which would take the other workgroups' keys with it): a thread's stores have arrived when its count of them is zero.  `scratch`: LDS of the workgroup that nobody reads any more.
+// or emptied (which would take the other workgroups' keys with it): a thread's stores have arrived when its count of them is zero.
+// `scratch`: LDS of the workgroup that nobody reads any more.
 template <int ROWS, int DP, int OUT>
 __device__ __forceinline__ void meet_and_join(const PagedAttn& a, const PagedCache& c, const PagedPlan& p, const PagedItem& it,
                                               int* seen, float* scratch) {
@@ -351,6 +351,10 @@ __device__ __forceinline__ void meet_and_join(const PagedAttn& a, const PagedCac
   join_slices<ROWS, ROWS, DP, OUT, true>(a, c, p, it, scratch, 0);
 }
 
+// Few rows: 16 to a workgroup, its four waves take 32 keys each in turn.  Bound by memory: 61 sequences of 40 to 4001 keys, 8 key
+// heads of four query heads, 252 MB, take 57 us (4.4 TB/s; a copy of as much runs at 5.2), 2 x 95000 keys 389 MB in 70 us (5.5).
+// A build that only loads takes as long; non-temporal loads, four waves to a SIMD instead of three and 64 keys a step did not help.
+// Short sequences are a chain of latencies: 500 keys, 12 heads take 6.8 us, some 2 us of them to the first key.
 constexpr int rows_lds(int DP) { return PA_WAVES * PA_ROWS * (DP + 4 + 2) * 4; }
 template <int DP, int OUT>
 __device__ __forceinline__ void paged_rows(const PagedAttn& a, const PagedCache& c, const PagedBatch& b, const PagedPlan& p, int index,
@@ -590,6 +594,10 @@ __device__ __forceinline__ void paged_rows(const PagedAttn& a, const PagedCache&
 // which MFMA operands are read: of eight keys, chosen as S^T = K Q^T (32x32x32 int8) leaves them in a lane, one column in 16 bytes,
 // lane after lane.  One widening of V then serves 128 rows.  Column blocks are interleaved (block i holds the columns NDB m + i),
 // so a thread widens neighbouring columns and a lane of O^T ends up with neighbouring ones.
+// Bound by what a wave can issue: a step of 64 keys takes a wave 1.6 us alone on its SIMD, the same with its keys in the nearest
+// cache, and two waves 2.0 us (matrix pipe 38 % busy, vector ALUs 49 %; 256 registers allow no third).  2048 rows over 16229 keys, 8
+// key heads of four: 470 to 500 us, 510 G operations, half of them int8, half fp16.  An item costs 4 us before its first step
+// (its place, its page, its keys) and some 2 behind the last: 4 x 512 rows of 40 heads are 640 items of 2 to 8 steps, 35 us.
 // Scores start from 1.5 * 2^23 instead of 0: the int32 sum is then the fp32 number 12582912 + x, and the constant goes into the
 // row's offset, where one multiply-add removes it exactly.
 constexpr int PT_ROWS = 128, PT_KEYS = 64;
