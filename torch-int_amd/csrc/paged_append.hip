@@ -40,49 +40,48 @@ __device__ __forceinline__ int s8_of(double y) {
   return y == y ? (int)y : 0;
 }
 
-// s8 of a whole number in fp32 (the conversion saturates, and makes 0 of NaN)
-__device__ __forceinline__ int s8_of_whole(float n) {
-  int i;
-  asm("v_cvt_i32_f32 %0, %1" : "=v"(i) : "v"(n));
-  return i < -128 ? -128 : i > 127 ? 127 : i;
-}
+// 1.5 * 2^23: a number added to it in one FMA is rounded, half to even, to a whole one, which the low bits then are.
+constexpr float WHOLE = 12582912.0f;
+// the low byte of what this returns is the s8 of n - WHOLE, for any n but NaN
+__device__ __forceinline__ int byte_of(float n) { return __float_as_int(__builtin_amdgcn_fmed3f(n, WHOLE - 128.0f, WHOLE + 127.0f)); }
 
-// s8(rint(x alpha)) with the product unrounded.  A border between two results is an fp32 number, and rounding to fp32 passes
-// none, so y = fl(x alpha) decides unless it is a border itself: then the remainder, which one FMA gives exactly, does.
+// s8(rint(x alpha)) in the low byte, the product unrounded; NaN becomes 0
 __device__ __forceinline__ int s8_of_product(float x, float alpha) {
-  const float y = x * alpha, n = __builtin_rintf(y), rest = __builtin_fmaf(x, alpha, -y);
-  const bool border = __builtin_fabsf(y - n) == 0.5f && rest != 0.0f;
-  return s8_of_whole(border ? y + __builtin_copysignf(0.5f, rest) : n);
+  const float n = __builtin_fmaf(x, alpha, WHOLE);
+  return n == n ? byte_of(n) : 0;
 }
 
-// s8(rint((p c + q s) alpha)) in fp32.  Three roundings and one of the bound's own are off by less than 2^-22 (|p c| + |q s|) alpha
-// together, the fp64 chain by 2^-51 of it; `far` keeps the bits of the largest |y - rint y| + twice that.  A result whose figure
-// stays below one half is the fp64 chain's; infinities and NaN have larger bits than any number.
+// s8(rint((p c + q s) alpha)) in the low byte, in fp32.  The two roundings, and the bound's own, are off by less than
+// 2^-22 (|p c| + |q s|) alpha together, the fp64 chain by 2^-51 of it; `far` keeps the bits of the largest |y - rint y| + twice
+// that.  A result whose figure stays below one half is the fp64 chain's; infinities and NaN have larger bits than any number, and
+// figures of numbers too large for WHOLE are above one half as well.
 __device__ __forceinline__ int s8_of_turned(float p, float c, float q, float s, float alpha, float bound, unsigned& far) {
   const float t = q * s, r = __builtin_fmaf(p, c, t), w = __builtin_fmaf(__builtin_fabsf(p), __builtin_fabsf(c), __builtin_fabsf(t));
-  const float y = r * alpha, n = __builtin_rintf(y);
-  const unsigned bits = __float_as_uint(__builtin_fabsf(__builtin_fmaf(w, bound, __builtin_fabsf(y - n))));
+  const float n = __builtin_fmaf(r, alpha, WHOLE), d = __builtin_fmaf(r, alpha, -(n - WHOLE));
+  const unsigned bits = __float_as_uint(__builtin_fabsf(__builtin_fmaf(w, bound, __builtin_fabsf(d))));
   far = far > bits ? far : bits;
-  return s8_of_whole(n);
+  return byte_of(n);
 }
 
+// the low bytes of eight
 __device__ __forceinline__ int2 pack8(const int (&o)[8]) {
-  int2 r;
-  r.x = (o[0] & 255) | (o[1] & 255) << 8 | (o[2] & 255) << 16 | o[3] << 24;
-  r.y = (o[4] & 255) | (o[5] & 255) << 8 | (o[6] & 255) << 16 | o[7] << 24;
-  return r;
+  auto four = [](int x, int y, int z, int w) {
+    return (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(w, z, 0x0c0c0400), __builtin_amdgcn_perm(y, x, 0x0c0c0400), 0x05040100);
+  };
+  return make_int2(four(o[0], o[1], o[2], o[3]), four(o[4], o[5], o[6], o[7]));
 }
 
 // One row to blockIdx.x; the threads of a block are the 16-element pieces of some heads, the keys', then the values', then the
 // queries'.  A piece is 16 neighbouring elements, or where pairs lie half apart 8 elements and their 8 partners.
-// Memory and vector ALUs are about level: 8192 rows of 32 + 2 x 8 heads of 128 fp16, 155 MB, take 37 us (4.2 TB/s; in fp64 alone 44),
-// 28 of them 350 instructions a wave, of which 130 look up rows and addresses; 2036 rows of 3 x 32 heads fp32, 125 MB, 27 us (4.6).
-// Several rows to a block, the next row's elements ahead of the present one's, needs 98 registers instead of 66 and took 36 us for the
-// second.
+// At the rate of a copy: 8192 rows of 32 + 2 x 8 heads of 128 fp16, 155 MB, take 29.6 us (5.2 TB/s), 2036 rows of 3 x 32 heads fp32,
+// 125 MB, 25.1 us (5.0).  That needs few instructions (280 a wave; in fp64 they took 44 us of the first) and the row's
+// elements on their way before its place is known, behind the one load that begins the search (33.9 us in front of it).  Several rows
+// to a block, the next row's elements ahead of the present one's, needs 98 registers instead of 66 and made the second 36 us.
 template <typename T>
-__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend a, PagedCache c, PagedBatch b, int pieces, int per_block) {
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend a, PagedCache c, PagedBatch b, int pieces, int per_piece,
+                                                            int per_block) {
   const int row = blockIdx.x;
-  const int unit = (int)(threadIdx.x * (65536u / (unsigned)pieces + 1u) >> 16);  // threadIdx.x / pieces, for 256 by up to 8
+  const int unit = (int)(threadIdx.x * (unsigned)per_piece >> 16);  // threadIdx.x / pieces
   const int piece = threadIdx.x - unit * pieces;
   const int head = blockIdx.y * per_block + unit;
   const int heads = 2 * c.heads + (a.query != nullptr ? a.q_heads : 0);
@@ -93,17 +92,22 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend a, PagedC
   const bool turned = piece * 16 < rot;
   const bool apart = turned && !a.neighbours;
   const int d0 = apart ? piece * 8 : piece * 16, d1 = apart ? rot / 2 + piece * 8 : piece * 16 + 8;
-  const T* src = which == 0   ? static_cast<const T*>(a.key) + row * a.k_row + h * a.k_head
-                 : which == 1 ? static_cast<const T*>(a.value) + row * a.v_row + h * a.v_head
-                              : static_cast<const T*>(a.query) + row * a.q_row + h * a.q_head;
-  Raw8<T> x0, x1;  // on their way while the row's place is looked up
+  // the row's sequence: how many of them end at or before it (all lanes of the wave take part); the first 64 ends are asked for in
+  // front of the row's elements, which are on their way while its place is looked up
+  const int lane = threadIdx.x & 63;
+  int end = b.cu[lane < b.seqs ? lane + 1 : b.seqs];
+  const T* const key = static_cast<const T*>(a.key) + row * a.k_row;
+  const T* const value = static_cast<const T*>(a.value) + row * a.v_row;
+  const T* const query = static_cast<const T*>(a.query) + row * a.q_row;
+  const T* src = (which == 0 ? key : which == 1 ? value : query) + h * (which == 0 ? a.k_head : which == 1 ? a.v_head : a.q_head);
+  Raw8<T> x0, x1;
   x0.load(src + d0);
   x1.load(src + d1);
-  // the row's sequence: how many of them end at or before it (all lanes of the wave take part)
   int seq = 0;
   for (int i0 = 0; i0 < b.seqs; i0 += 64) {
-    const int i = i0 + (threadIdx.x & 63);
-    const unsigned long long ended = __ballot(i < b.seqs && b.cu[i < b.seqs ? i + 1 : b.seqs] <= row);
+    const int i = i0 + lane;
+    if (i0 > 0) end = b.cu[i < b.seqs ? i + 1 : b.seqs];
+    const unsigned long long ended = __ballot(i < b.seqs && end <= row);
     seq += __popcll(ended);
     if (ended != ~0ull) break;
   }
@@ -190,7 +194,7 @@ int launch_paged_kv_append_s8(int type, const PagedAppend& a, const PagedCache& 
   const int most = 256 / pieces, even = (heads + blocks - 1) / blocks, per_block = even < most ? even : most;
   const int threads = (per_block * pieces + 63) & ~63;
   const dim3 grid((unsigned)b.rows, (unsigned)((heads + per_block - 1) / per_block));
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, a, c, b, pieces, per_block); };
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, a, c, b, pieces, 65536 / pieces + 1, per_block); };  // (exact for 256 threads by up to 8 pieces)
   switch (type) {
     case PT_F32: launch(paged_append_kernel<float>); break;
     case PT_F16: launch(paged_append_kernel<_Float16>); break;
