@@ -172,9 +172,9 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
   return it;
 }
 
-// Rows of no sequence (behind the last one; in front of the first, should it not begin at row 0) become zeros.
-__device__ __forceinline__ void paged_fill(const PagedBatch& b, char* out, long long row_bytes) {
-  int lo = b.cu[0], hi = b.cu[b.seqs];
+// Rows of no sequence (behind the last one; in front of the first, should it not begin at row 0) become zeros.  lo, hi: the first
+// and the last entry of cu.
+__device__ __forceinline__ void paged_fill(const PagedBatch& b, int lo, int hi, char* out, long long row_bytes) {
   lo = lo < 0 ? 0 : lo > b.rows ? b.rows : lo;
   hi = hi < lo ? lo : hi > b.rows ? b.rows : hi;
   const int rest = b.rows - (hi - lo);
@@ -991,8 +991,9 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
 template <int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan rows) {
   __shared__ __attribute__((aligned(16))) char lds[rows_lds(DP)];
-  if (a.fill) paged_fill(b, static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
+  const int lo = b.cu[0], hi = b.cu[b.seqs];  // (on their way beside what the item needs)
   paged_rows<DP, OUT>(a, c, b, rows, blockIdx.x, lds);
+  if (a.fill) paged_fill(b, lo, hi, static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
 }
 
 // Sequences of few rows and of many in one launch, 256 items of the one kind after 256 of the other as long as both last: those
@@ -1005,7 +1006,7 @@ template <int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_both_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan rows,
                                                                         PagedPlan tiles) {
   __shared__ __attribute__((aligned(16))) char lds[tiles_lds(DP) > rows_lds(DP) ? tiles_lds(DP) : rows_lds(DP)];
-  if (a.fill) paged_fill(b, static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
+  if (a.fill) paged_fill(b, b.cu[0], b.cu[b.seqs], static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
   const int i = blockIdx.x, each = (rows.slots < tiles.slots ? rows.slots : tiles.slots) & -TURN, rest = i - 2 * each;
   const bool many = rest < 0 ? (i & TURN) == 0 : rest < tiles.slots - each;
   const int index = rest < 0 ? i / (2 * TURN) * TURN + i % TURN : each + rest - (many ? 0 : tiles.slots - each);
@@ -1013,14 +1014,17 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_both_kernel(PagedAtt
   else paged_rows<DP, OUT>(a, c, b, rows, index, lds);
 }
 
-// Joins slices that do not meet in the launch itself: an item that was cut to blockIdx.y, EACH of its rows to blockIdx.x (so that
-// what there is to join comes first, and goes to all CUs).
+// Joins slices that do not meet in the launch itself: an item that was cut to ROWS / EACH workgroups, EACH of its rows to one.
+// Eight items take turns, so that what there is to join comes first and goes to all CUs, and that an item whose number leaves the
+// same rest by 8 as its slots' (as where key heads come in eights) is read by the XCD that has written it.
 template <int ROWS, int EACH, int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p) {
   __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
-  const PagedItem it = paged_item<ROWS == PT_ROWS ? PT_PARTS : 1, true>(b, c.page_shift, c.heads, ROWS, p, blockIdx.y);
+  constexpr int PIECES = ROWS / EACH;
+  const PagedItem it = paged_item<ROWS == PT_ROWS ? PT_PARTS : 1, true>(b, c.page_shift, c.heads, ROWS, p,
+                                                                                 blockIdx.x / (8 * PIECES) * 8 + blockIdx.x % 8);
   if (!it.found || it.split != 0) return;
-  join_slices<ROWS, EACH, DP, OUT, false>(a, c, p, it, meet, blockIdx.x * EACH);
+  join_slices<ROWS, EACH, DP, OUT, false>(a, c, p, it, meet, blockIdx.x / 8 % PIECES * EACH);
 }
 
 // What a call of these sizes runs.  The lengths are on the device, so the grids and the workspace are bounds: one item to each
@@ -1079,13 +1083,13 @@ static void launch_attn(const PagedAttn& a, const PagedCache& c, const PagedBatc
   // an item that is cut has more than a target-th of all keys, so there are fewer than `target` of them
   auto items = [](const PagedPlan& p) {
     const int most = p.slots - PA_TARGET - 8;
-    return (unsigned)(most < p.target ? most : p.target);
+    return (unsigned)((most < p.target ? most : p.target) + 7 & ~7);
   };
   if (rows.target > 0 && rows.arrivals == nullptr)
-    hipLaunchKernelGGL((paged_attn_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(PA_ROWS / 2, items(rows)), dim3(PA_THREADS), 0, stream, a, c, b,
+    hipLaunchKernelGGL((paged_attn_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(items(rows) * (PA_ROWS / 2)), dim3(PA_THREADS), 0, stream, a, c, b,
                        rows);
   if (tiles.target > 0)
-    hipLaunchKernelGGL((paged_attn_join_kernel<PT_ROWS, PT_JOIN, DP, OUT>), dim3(PT_ROWS / PT_JOIN, items(tiles)), dim3(PA_THREADS), 0, stream, a, c, b,
+    hipLaunchKernelGGL((paged_attn_join_kernel<PT_ROWS, PT_JOIN, DP, OUT>), dim3(items(tiles) * (PT_ROWS / PT_JOIN)), dim3(PA_THREADS), 0, stream, a, c, b,
                        tiles);
 }
 
@@ -1101,21 +1105,22 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
     return fail(TI_ERR_INVALID_ARG, "paged_attn_s8: %lld work items", s.rows_slots + s.tiles_slots);
   const bool meet = a.arrivals != nullptr && a.arrivals_count >= paged_attn_arrivals(b.rows, b.seqs, a.q_heads, c.heads, capacity);
   char* ws = static_cast<char*>(workspace);
-  // where both kinds share the chip, half of it for each: 512 rows over 2000 keys beside 31 sequences of one row took 58.8 us
-  // with 512 slices of each, 50.4 with 256
-  const int target = s.rows_slots > 0 && s.tiles_slots > 0 ? PA_TARGET / 2 : PA_TARGET;
+  // Where both kinds share the chip, a place on each CU for the tiles, and few cuts for the others, which have the time: 512 rows over
+  // 600 to 2007 keys beside 31 sequences of one row took 58.8 us with 512 slices of each kind, 48.3 with 256 of each, 44.4 with
+  // 256 of tiles and 128 of the others.
+  const bool both = s.rows_slots > 0 && s.tiles_slots > 0;
   PagedPlan rows, tiles;
   rows.group = tiles.group = group;
   rows.least = 0;
   rows.most = s.tiles_slots > 0 ? PA_ROWS : 0x7fffffff;
   rows.slots = (int)s.rows_slots;
-  rows.target = s.rows_cut ? target : 0;
+  rows.target = !s.rows_cut ? 0 : both ? PA_TARGET / 4 : PA_TARGET;
   rows.ws = reinterpret_cast<float*>(ws);
   rows.arrivals = meet && s.rows_cut && s.rows_meet ? a.arrivals : nullptr;
   tiles.least = s.rows_slots > 0 ? PA_ROWS : 0;
   tiles.most = 0x7fffffff;
   tiles.slots = (int)s.tiles_slots;
-  tiles.target = s.tiles_cut ? target : 0;
+  tiles.target = !s.tiles_cut ? 0 : both ? PA_TARGET / 2 : PA_TARGET;
   tiles.ws = reinterpret_cast<float*>(ws + (s.rows_cut ? paged_bytes(s.rows_slots, PA_ROWS, c.D) : 0));
   tiles.arrivals = nullptr;  // slices of 66 KB: many workgroups join them, in a launch of their own
   auto run = [&](auto dp) {
