@@ -636,9 +636,9 @@ int ti_paged_kv_append_s8(const TiPagedCache* cache, const TiPagedBatch* batch, 
 /* Attention of the new tokens over their sequences' pages, each token over the positions up to its own:
  *   out[row, h] = alpha_pv * sum_j w_j v_j,  w = softmax(alpha_qk * q . k_j),  0 where there is no position.
  * q int8 [rows, q_heads, head_dim] with row and head strides in bytes, multiples of 16; q_heads a multiple of the cache's
- * heads, q head h reads key head h / (q_heads / heads).  out [rows, q_heads, head_dim] packed, of `out_type`: TI_TYPE_S8
- * (rint, clamp to [-128, 127]), TI_TYPE_F16 or TI_TYPE_BF16.  Rows of no sequence become zeros with `fill` and stay as they
- * are without.  alpha_qk in [1e-30, 0.25] (scores reach 2^21 alpha_qk).  Probabilities are not quantised to int8 (the
+ * heads, q head h reads key head h / (q_heads / heads).  out [rows, q_heads, head_dim] packed, apart from the inputs, of
+ * `out_type`: TI_TYPE_S8 (rint, clamp to [-128, 127]), TI_TYPE_F16 or TI_TYPE_BF16.  Rows of no sequence become zeros with
+ * `fill` and stay as they are without.  alpha_qk in [1e-30, 0.25] (scores reach 2^21 alpha_qk).  Probabilities are not quantised to int8 (the
  * whole-cache attentions above do that): a row's largest counts 2^8 to 2^15 in fp16, and where little else bounds the kernel
  * they have 22 bits.
  * `workspace` (16-byte aligned, private to the stream, contents irrelevant) of ti_paged_attn_workspace_bytes lets long

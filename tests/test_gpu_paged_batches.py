@@ -99,3 +99,17 @@ def test_modules_do_what_the_functions_do(out):
     assert append(kn, vn, *a, *batch) is None
     into = torch.empty_like(got)
     assert attend(qs, *b, *batch, out=into) is into and torch.equal(into, want)
+
+
+def test_the_query_is_refused_as_output_and_taken_as_quantised_query():
+    g = torch.Generator().manual_seed(29)
+    cu, lens, table, pages, rows = _batch(g, [40, 3], [5, 3], 16)
+    q, kn, vn = (_s8(g, rows, h, 64, spread=30).to(DEV) for h in (4, 2, 2))
+    pools = [_s8(g, pages, 2, 16, 64, spread=30).to(DEV) for _ in range(2)]
+    batch = (table.to(DEV), lens.to(DEV), cu.to(DEV))
+    with pytest.raises(RuntimeError, match="must not be the query"):
+        _paged().paged_attn_s8(q, *pools, *batch, 1e-3, 1.0, out=q)
+    kw = dict(alpha_q=0.7, cos_sin=_angles(64, 32).to(DEV))
+    want = _paged().paged_kv_append_s8(kn, vn, *[p.clone() for p in pools], *batch, 0.5, 0.5, query=q, **kw)
+    assert _paged().paged_kv_append_s8(kn, vn, *pools, *batch, 0.5, 0.5, query=q, query_out=q, **kw) is q
+    assert torch.equal(q, want)

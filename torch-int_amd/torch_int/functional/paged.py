@@ -227,7 +227,7 @@ def paged_attn_s8(query, k_cache, v_cache, block_table, context_lens, cu_new, al
     ``h // (q_heads // heads)``).  Every token sees the positions up to its own, which have to be in the cache already
     (:func:`paged_kv_append_s8`).  The result [rows, q_heads, head_dim] is fp16, bf16 or int8 (``sat_s8(round(...))``, for a W8A8
     layer behind it).  A token that sees nothing gets zeros; rows of no sequence are zeros too, or left as they are in an
-    ``out`` that is handed in.  ``alpha_qk`` is positive and at most 0.25."""
+    ``out`` that is handed in, which must not share memory with the inputs.  ``alpha_qk`` is positive and at most 0.25."""
     op = "paged_attn_s8"
     if not isinstance(query, torch.Tensor) or query.dim() != 3:
         _fail(op, f"query must be a 3-D torch.int8 tensor, got {_describe(query)}")
@@ -253,6 +253,8 @@ def paged_attn_s8(query, k_cache, v_cache, block_table, context_lens, cu_new, al
         _rows(op, "out", out, out.dtype, shape, k_cache)
         if not out.is_contiguous():
             _fail(op, "out must be contiguous")
+        if rows > 0 and out.data_ptr() == query.data_ptr():
+            _fail(op, "out must not be the query: other workgroups read it while its rows are written")
     if rows == 0:
         return out
     key = (rows, seqs, q_heads, heads, d, args[15] * args[3])
