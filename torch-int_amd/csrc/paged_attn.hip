@@ -898,7 +898,8 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
     int s0 = lo;
     for (;;) {
       const int gone = lost(s0);
-      const bool here = s0 < keys + 32;  // the same for all lanes: with the half behind its last keys a wave gathers those
+      // the same for all lanes: with the half behind its last keys a wave gathers those
+      const bool here = __builtin_amdgcn_readfirstlane(s0 < keys + 32) != 0;
       const int v_now = V0 + k0 * VBYTES;
       const int8_t* from;
       auto stage_v = [&](int m) {
@@ -929,6 +930,8 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
         for (int m = 0; m < BUNDLES; ++m) stage_v(m);
 #pragma unroll
         for (int m = 0; m < BUNDLES; ++m) stage_k(m);
+        // nothing is left on its way into registers that the other path uses for something else: it would wait for all its loads
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
       }
       __syncthreads();
       v_before = v_now + V_HALF;
