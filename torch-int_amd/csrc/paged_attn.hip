@@ -595,8 +595,9 @@ __device__ __forceinline__ void paged_rows(const PagedAttn& a, const PagedCache&
 // lane after lane.  One widening of V then serves 128 rows.  Column blocks are interleaved (block i holds the columns NDB m + i),
 // so a thread widens neighbouring columns and a lane of O^T ends up with neighbouring ones.
 // Bound by what a wave can issue: a step of 64 keys takes a wave 1.6 us alone on its SIMD, the same with its keys in the nearest
-// cache, and two waves 2.0 us (matrix pipe 38 % busy, vector ALUs 49 %; 256 registers allow no third).  2048 rows over 16229 keys, 8
-// key heads of four: 470 to 500 us, 510 G operations, half of them int8, half fp16.  An item costs 4 us before its first step
+// cache, and two waves 2.0 us (matrix pipe 38 % busy, vector ALUs 49 %; its 241 registers allow no third,
+// but those of head sizes up to 64 do).  2048 rows over 16229 keys, 8 key heads of four: 445 to 480 us, 510 G operations, half of them
+// int8, half fp16.  An item costs 4 us before its first step
 // (its place, its page, its keys) and some 2 behind the last: 4 x 512 rows of 40 heads are 640 items of 2 to 8 steps, 35 us.
 // Scores start from 1.5 * 2^23 instead of 0: the int32 sum is then the fp32 number 12582912 + x, and the constant goes into the
 // row's offset, where one multiply-add removes it exactly.
@@ -680,15 +681,20 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
   };
   auto k_from = [&](int s0, int page) { return kb + (long long)(have(page) ? page : 0) * c.k_page + place(s0) * c.k_token; };
   auto v_from = [&](int s0, int page) { return vb_ + (long long)(have(page) ? page : 0) * c.v_page + place(s0) * c.v_token; };
+  // by buffer instructions: a column is one register beside the page's place in scalar ones, not two (241 registers instead of 255,
+  // for head sizes up to 64 164 instead of 178, which makes room for a third workgroup: 16 x 512 rows of 32 heads 62.4 to 50.7 us)
+  auto pool = [](const int8_t* from) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(from), 0, -1, 0x00020000); };
   auto fetch_k = [&](v4i (&kreg)[KC], const int8_t* from) {
+    const auto r = pool(from);
 #pragma unroll
-    for (int i = 0; i < KC; ++i) kreg[i] = *reinterpret_cast<const v4i*>(from + kcol[i]);
+    for (int i = 0; i < KC; ++i) kreg[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, kcol[i], 0, 0));
   };
   auto fetch_v = [&](unsigned (&vreg)[8], const int8_t* from) {
+    const auto r = pool(from);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if constexpr (NDB == 4) vreg[j] = *reinterpret_cast<const unsigned*>(from + vcol[j]);
-      else vreg[j] = *reinterpret_cast<const unsigned short*>(from + vcol[j]);
+      if constexpr (NDB == 4) vreg[j] = __builtin_amdgcn_raw_buffer_load_b32(r, vcol[j], 0, 0);
+      else vreg[j] = __builtin_amdgcn_raw_buffer_load_b16(r, vcol[j], 0, 0);
     }
   };
   auto swizzle = [](int r, int chunk) { return DP == 128 ? chunk ^ (r & 7) : chunk ^ ((r >> 2) & 3); };
@@ -1006,7 +1012,7 @@ __global__ __launch_bounds__(PA_THREADS, 3) void paged_attn_rows_kernel(PagedAtt
 // behind them (512 rows over 2000 keys beside a sequence of one row: 56.7 us by 8, 45.4 by 32, 39.5 by 256).
 constexpr int TURN = 256;
 template <int DP, int OUT>
-__global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_both_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan rows,
+__global__ __launch_bounds__(PA_THREADS, DP == 64 ? 3 : 2) void paged_attn_both_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan rows,
                                                                         PagedPlan tiles) {
   __shared__ __attribute__((aligned(16))) char lds[tiles_lds(DP) > rows_lds(DP) ? tiles_lds(DP) : rows_lds(DP)];
   if (a.fill) paged_fill(b, b.cu[0], b.cu[b.seqs], static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
