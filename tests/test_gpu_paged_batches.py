@@ -113,3 +113,31 @@ def test_the_query_is_refused_as_output_and_taken_as_quantised_query():
     want = _paged().paged_kv_append_s8(kn, vn, *[p.clone() for p in pools], *batch, 0.5, 0.5, query=q, **kw)
     assert _paged().paged_kv_append_s8(kn, vn, *pools, *batch, 0.5, 0.5, query=q, query_out=q, **kw) is q
     assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_pool_without_pages(new):
+    g = torch.Generator().manual_seed(31)
+    lens, cu = torch.tensor([100, 100], dtype=torch.int32), torch.tensor([0, new, 2 * new], dtype=torch.int32)
+    table = torch.zeros(2, 7, dtype=torch.int32)
+    q, kn, vn = (_s8(g, 2 * new, h, 64, spread=30) for h in (4, 2, 2))
+    empty = torch.empty(0, 2, 16, 64, dtype=torch.int8)
+    batch = (table.to(DEV), lens.to(DEV), cu.to(DEV))
+    pools = (empty.to(DEV), empty.to(DEV))
+    got = _paged().paged_kv_append_s8(kn.to(DEV), vn.to(DEV), *pools, *batch, 1.0, 1.0, query=q.to(DEV), alpha_q=0.5)
+    assert torch.equal(got.cpu(), orc.append(kn, vn, empty, empty, table, lens, cu, 1.0, 1.0, q, 0.5)[2])
+    out = _paged().paged_attn_s8(got, *pools, *batch, 1e-3, 1.0, out_dtype=torch.float16)
+    assert out.shape == q.shape and not out.any()
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_rows_without_a_sequence(rows):
+    g = torch.Generator().manual_seed(33)
+    q, kn, vn = (_s8(g, rows, h, 64, spread=30).to(DEV) for h in (4, 2, 2))
+    pools = [_s8(g, 3, 2, 16, 64, spread=30).to(DEV) for _ in range(2)]
+    before = [p.clone() for p in pools]
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    batch = (none.view(0, 1).expand(0, 100).contiguous(), none, torch.zeros(1, dtype=torch.int32, device=DEV))
+    got = _paged().paged_kv_append_s8(kn, vn, *pools, *batch, 1.0, 1.0, query=q)
+    assert not got.any() and torch.equal(pools[0], before[0]) and torch.equal(pools[1], before[1])
+    assert not _paged().paged_attn_s8(q, *pools, *batch, 1e-3, 1.0, out_dtype=torch.float16).any()

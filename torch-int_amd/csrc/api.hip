@@ -1273,6 +1273,7 @@ int ti_paged_attn_s8(const TiPagedCache* cache, const TiPagedBatch* batch, const
   if (b.rows * (w->q_heads / c.heads) > (1 << 30))
     return fail(TI_ERR_INVALID_ARG, "%s: %d rows of %lld heads to a key head (at most 2^30 in all)", op, b.rows,
                 (long long)(w->q_heads / c.heads));
+  if (c.pages == 0) b.per_seq = 0;  // no page to read, not even in the place of one that is missing: no sequence has a key
   PagedAttn a;
   a.q = w->q, a.q_row = w->q_row, a.q_head = w->q_head, a.q_heads = (int)w->q_heads, a.out = w->out;
   a.alpha_qk = w->alpha_qk, a.alpha_pv = w->alpha_pv, a.fill = w->fill != 0;

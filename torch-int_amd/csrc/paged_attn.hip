@@ -99,6 +99,7 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
                                                 int index) {
   PagedItem it;
   it.found = false;
+  if (b.seqs == 0) return it;
   const int lane = threadIdx.x & 63;
   PagedSeq s;
   int tiles;
