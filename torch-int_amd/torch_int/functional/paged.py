@@ -63,6 +63,7 @@ _fast_append = getattr(_CUDA._fast, "paged_append", None)
 _fast_attn = getattr(_CUDA._fast, "paged_attn", None)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _I8, _I32, _F32 = torch.int8, torch.int32, torch.float32
+_empty_like, _PACKED = torch.empty_like, torch.contiguous_format
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}
 _ws_need = {}  # shape of a call -> (bytes of workspace, counters) it can use
 _counters = {}  # (device index, stream) -> int32 zeros in which the slices of a call count themselves, zero again behind it
@@ -126,16 +127,16 @@ def _cache_and_batch(op, k_cache, v_cache, block_table, context_lens, cu_new, ro
     _fail(op, "block_table, context_lens and cu_new must be contiguous")
 
 
-def _rows(op, name, t, dtype, shape, k_cache):
-    """Row and head stride of a tensor [rows, heads, head_dim] = ``shape`` whose last dimension is contiguous."""
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == k_cache.get_device():
+def _rows(op, name, t, dtype, shape, dev):
+    """Row and head stride of a tensor [rows, heads, head_dim] = ``shape`` on device number ``dev`` whose last dimension is contiguous."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == dev:
         row, head, last = t.stride()
         if last == 1:
             return row, head
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != 3:
         _fail(op, f"{name} must be a 3-D {dtype} tensor, got {_describe(t)}")
-    if t.device != k_cache.device:
-        _fail(op, f"{name} is on {t.device}, expected {k_cache.device}")
+    if t.get_device() != dev:
+        _fail(op, f"{name} is on {t.device}, expected cuda:{dev}")
     if t.shape != shape:
         _fail(op, f"{name} is {tuple(t.shape)}, expected {tuple(shape)}")
     _fail(op, f"the last dimension of {name} must be contiguous")
@@ -173,8 +174,8 @@ def paged_kv_append_s8(key, value, k_cache, v_cache, block_table, context_lens, 
     dev = k_cache.get_device()
     heads, d = args[4], args[5]
     shape = (rows, heads, d)
-    k_row, k_head = _rows(op, "key", key, dtype, shape, k_cache)
-    v_row, v_head = _rows(op, "value", value, dtype, shape, k_cache)
+    k_row, k_head = _rows(op, "key", key, dtype, shape, dev)
+    v_row, v_head = _rows(op, "value", value, dtype, shape, dev)
     q_ptr = q_row = q_head = q_heads = out_ptr = 0
     out = None
     if query is not None:
@@ -182,12 +183,12 @@ def paged_kv_append_s8(key, value, k_cache, v_cache, block_table, context_lens, 
             _fail(op, f"query must be a 3-D {dtype} tensor, got {_describe(query)}")
         q_heads, q_ptr = query.shape[1], query.data_ptr()
         shape = (rows, q_heads, d)
-        q_row, q_head = _rows(op, "query", query, dtype, shape, k_cache)
+        q_row, q_head = _rows(op, "query", query, dtype, shape, dev)
         if query_out is None:
-            out = query.new_empty(shape, dtype=_I8)
+            out = _empty_like(query, dtype=_I8, memory_format=_PACKED)
         else:
             out = query_out
-            _rows(op, "query_out", out, _I8, shape, k_cache)
+            _rows(op, "query_out", out, _I8, shape, dev)
             if not out.is_contiguous():
                 _fail(op, "query_out must be contiguous")
         out_ptr = out.data_ptr()
@@ -236,7 +237,7 @@ def paged_attn_s8(query, k_cache, v_cache, block_table, context_lens, cu_new, al
     dev = k_cache.get_device()
     heads, d, seqs = args[4], args[5], args[16]
     shape = (rows, q_heads, d)
-    q_row, q_head = _rows(op, "query", query, _I8, shape, k_cache)
+    q_row, q_head = _rows(op, "query", query, _I8, shape, dev)
     if heads == 0 or q_heads == 0 or q_heads % heads:
         _fail(op, f"{q_heads} query heads are no multiple of {heads} key heads")
     if out is None:
@@ -244,13 +245,13 @@ def paged_attn_s8(query, k_cache, v_cache, block_table, context_lens, cu_new, al
         code = _TYPES.get(out_dtype)
         if code is None or code == 0:
             _fail(op, f"out_dtype must be torch.int8, torch.float16 or torch.bfloat16, got {out_dtype}")
-        out = query.new_empty(shape, dtype=out_dtype)
+        out = _empty_like(query, dtype=out_dtype, memory_format=_PACKED)
     else:
         fill = 0
         code = _TYPES.get(out.dtype) if isinstance(out, torch.Tensor) else None
         if code is None or code == 0:
             _fail(op, f"out must be a tensor of int8, float16 or bfloat16, got {_describe(out)}")
-        _rows(op, "out", out, out.dtype, shape, k_cache)
+        _rows(op, "out", out, out.dtype, shape, dev)
         if not out.is_contiguous():
             _fail(op, "out must be contiguous")
         if rows > 0 and out.data_ptr() == query.data_ptr():
