@@ -194,7 +194,9 @@ int launch_paged_kv_append_s8(int type, const PagedAppend& a, const PagedCache& 
   const int most = 256 / pieces, even = (heads + blocks - 1) / blocks, per_block = even < most ? even : most;
   const int threads = (per_block * pieces + 63) & ~63;
   const dim3 grid((unsigned)b.rows, (unsigned)((heads + per_block - 1) / per_block));
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, a, c, b, pieces, 65536 / pieces + 1, per_block); };  // (exact for 256 threads by up to 8 pieces)
+  auto launch = [&](auto kernel) {  // (65536 / pieces + 1 is exact for 256 threads by up to 8 pieces)
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, stream, a, c, b, pieces, 65536 / pieces + 1, per_block);
+  };
   switch (type) {
     case PT_F32: launch(paged_append_kernel<float>); break;
     case PT_F16: launch(paged_append_kernel<_Float16>); break;

@@ -1040,33 +1040,44 @@ __global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a
 // What a call of these sizes runs.  The lengths are on the device, so the grids and the workspace are bounds: one item to each
 // (sequence, key head, tile of rows) and the slices beyond that.
 struct PagedShape {
-  long long rows_slots, tiles_slots;  // items of either kind; 0: none
-  bool rows_cut, tiles_cut;
-  bool rows_meet;  // slices of few rows meet in the launch
+  long long rows_slots, tiles_slots;  // items of either kind, slices included; 0: none
+  int rows_target, tiles_target;      // slices that the keys are cut into; 0: nothing is cut
+  bool rows_meet;                     // slices of few rows meet in the launch
+  void cut_rows(int target, long long each) {
+    rows_target = target;
+    // where the slices of an item come to more than 65 KB, one workgroup would be longer in joining them than another launch
+    // takes (2 x 100000 keys, 8 key heads of 8: 135 KB, 87 us in all against 71.6 + 5.5 us)
+    rows_meet = target * each * 520 <= 66560 * rows_slots;
+    rows_slots += target + 8;
+  }
+  void cut_tiles(int target) {
+    tiles_target = target;
+    tiles_slots += target + 8;
+  }
 };
 static PagedShape paged_shape(long long rows, long long seqs, long long group, long long heads, long long capacity) {
-  PagedShape s = {0, 0, false, false, true};
+  PagedShape s = {0, 0, 0, 0, false};
   const bool cut = capacity > PA_MIN_SLICE;
   if (rows * group <= PA_ROWS * seqs) {  // few rows to a sequence on average: all of them by that kernel
     s.rows_slots = heads * (seqs + rows * group / PA_ROWS);
-    s.rows_cut = cut;
-    // where the slices of an item come to more than some 64 KB, one workgroup would be longer in joining them than another launch
-    // takes (2 x 100000 keys, 8 key heads of 8: 135 KB, 87 us in all against 71.6 + 5.5 us)
     const long long each = rows * group / seqs + 1 < PA_ROWS ? rows * group / seqs + 1 : PA_ROWS;
-    s.rows_meet = PA_TARGET * each * 520 < 65536 * s.rows_slots;
-    if (cut) s.rows_slots += PA_TARGET + 8;
+    if (cut) s.cut_rows(PA_TARGET, each);
     return s;
   }
   // sequences with more than 16 rows are at most a 17th of all rows
   const long long many = rows * group / (PA_ROWS + 1) < seqs ? rows * group / (PA_ROWS + 1) : seqs;
   s.tiles_slots = heads * (many + rows * group / PT_ROWS);
-  s.tiles_cut = cut && s.tiles_slots < PT_PLENTY;
-  if (s.tiles_cut) s.tiles_slots += PA_TARGET + 8;
-  if (seqs > 1) {  // (a single one has more than 16)
-    s.rows_slots = heads * seqs;
-    s.rows_cut = cut;
-    if (cut) s.rows_slots += PA_TARGET + 8;
+  const bool cut_tiles = cut && s.tiles_slots < PT_PLENTY;
+  if (seqs == 1) {  // it has more than 16
+    if (cut_tiles) s.cut_tiles(PA_TARGET);
+    return s;
   }
+  // Where both kinds share the chip, a place on each CU for the tiles, and few cuts for the others, which have the time: 512 rows over
+  // 600 to 2007 keys beside 31 sequences of one row took 58.8 us with 512 slices of each kind, 48.3 with 256 of each, 44.4 with
+  // 256 of tiles and 128 of the others.
+  s.rows_slots = heads * seqs;
+  if (cut_tiles) s.cut_tiles(PA_TARGET / 2);
+  if (cut) s.cut_rows(PA_TARGET / 4, PA_ROWS);
   return s;
 }
 static int paged_dp(long long D) { return D <= 64 ? 64 : 128; }
@@ -1074,12 +1085,12 @@ static long long paged_bytes(long long slots, int rows, long long D) { return sl
 
 long long paged_attn_arrivals(long long rows, long long seqs, long long q_heads, long long heads, long long capacity) {
   const PagedShape s = paged_shape(rows, seqs, q_heads / heads, heads, capacity);
-  return s.rows_cut && s.rows_meet ? s.rows_slots : 0;
+  return s.rows_meet ? s.rows_slots : 0;
 }
 long long paged_attn_workspace_bytes(long long rows, long long seqs, long long q_heads, long long heads, long long D,
                                      long long capacity) {
   const PagedShape s = paged_shape(rows, seqs, q_heads / heads, heads, capacity);
-  return (s.rows_cut ? paged_bytes(s.rows_slots, PA_ROWS, D) : 0) + (s.tiles_cut ? paged_bytes(s.tiles_slots, PT_ROWS, D) : 0);
+  return (s.rows_target ? paged_bytes(s.rows_slots, PA_ROWS, D) : 0) + (s.tiles_target ? paged_bytes(s.tiles_slots, PT_ROWS, D) : 0);
 }
 
 template <int DP, int OUT>
@@ -1092,15 +1103,15 @@ static void launch_attn(const PagedAttn& a, const PagedCache& c, const PagedBatc
     hipLaunchKernelGGL((paged_attn_rows_kernel<DP, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows);
   // an item that is cut has more than a target-th of all keys, so there are fewer than `target` of them
   auto items = [](const PagedPlan& p) {
-    const int most = p.slots - PA_TARGET - 8;
+    const int most = p.slots - p.target - 8;
     return (unsigned)((most < p.target ? most : p.target) + 7 & ~7);
   };
   if (rows.target > 0 && rows.arrivals == nullptr)
-    hipLaunchKernelGGL((paged_attn_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(items(rows) * (PA_ROWS / 2)), dim3(PA_THREADS), 0, stream, a, c, b,
-                       rows);
+    hipLaunchKernelGGL((paged_attn_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(items(rows) * (PA_ROWS / 2)), dim3(PA_THREADS), 0,
+                       stream, a, c, b, rows);
   if (tiles.target > 0)
-    hipLaunchKernelGGL((paged_attn_join_kernel<PT_ROWS, PT_JOIN, DP, OUT>), dim3(items(tiles) * (PT_ROWS / PT_JOIN)), dim3(PA_THREADS), 0, stream, a, c, b,
-                       tiles);
+    hipLaunchKernelGGL((paged_attn_join_kernel<PT_ROWS, PT_JOIN, DP, OUT>), dim3(items(tiles) * (PT_ROWS / PT_JOIN)), dim3(PA_THREADS),
+                       0, stream, a, c, b, tiles);
 }
 
 int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, const PagedBatch& b, void* workspace,
@@ -1110,28 +1121,24 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
   const long long capacity = (long long)b.per_seq << c.page_shift;
   PagedShape s = paged_shape(b.rows, b.seqs, group, c.heads, capacity);
   if (workspace == nullptr || workspace_bytes < paged_attn_workspace_bytes(b.rows, b.seqs, a.q_heads, c.heads, c.D, capacity))
-    s.rows_cut = s.tiles_cut = false;
+    s.rows_target = s.tiles_target = 0, s.rows_meet = false;
   if (s.rows_slots + s.tiles_slots > 0x7fffff)
     return fail(TI_ERR_INVALID_ARG, "paged_attn_s8: %lld work items", s.rows_slots + s.tiles_slots);
   const bool meet = a.arrivals != nullptr && a.arrivals_count >= paged_attn_arrivals(b.rows, b.seqs, a.q_heads, c.heads, capacity);
   char* ws = static_cast<char*>(workspace);
-  // Where both kinds share the chip, a place on each CU for the tiles, and few cuts for the others, which have the time: 512 rows over
-  // 600 to 2007 keys beside 31 sequences of one row took 58.8 us with 512 slices of each kind, 48.3 with 256 of each, 44.4 with
-  // 256 of tiles and 128 of the others.
-  const bool both = s.rows_slots > 0 && s.tiles_slots > 0;
   PagedPlan rows, tiles;
   rows.group = tiles.group = group;
   rows.least = 0;
   rows.most = s.tiles_slots > 0 ? PA_ROWS : 0x7fffffff;
   rows.slots = (int)s.rows_slots;
-  rows.target = !s.rows_cut ? 0 : both ? PA_TARGET / 4 : PA_TARGET;
+  rows.target = s.rows_target;
   rows.ws = reinterpret_cast<float*>(ws);
-  rows.arrivals = meet && s.rows_cut && s.rows_meet ? a.arrivals : nullptr;
+  rows.arrivals = meet && s.rows_meet ? a.arrivals : nullptr;
   tiles.least = s.rows_slots > 0 ? PA_ROWS : 0;
   tiles.most = 0x7fffffff;
   tiles.slots = (int)s.tiles_slots;
-  tiles.target = !s.tiles_cut ? 0 : both ? PA_TARGET / 2 : PA_TARGET;
-  tiles.ws = reinterpret_cast<float*>(ws + (s.rows_cut ? paged_bytes(s.rows_slots, PA_ROWS, c.D) : 0));
+  tiles.target = s.tiles_target;
+  tiles.ws = reinterpret_cast<float*>(ws + (s.rows_target ? paged_bytes(s.rows_slots, PA_ROWS, c.D) : 0));
   tiles.arrivals = nullptr;  // slices of 66 KB: many workgroups join them, in a launch of their own
   auto run = [&](auto dp) {
     constexpr int DP = decltype(dp)::value;

@@ -128,7 +128,7 @@ def _cache_and_batch(op, k_cache, v_cache, block_table, context_lens, cu_new, ro
 
 
 def _rows(op, name, t, dtype, shape, dev):
-    """Row and head stride of a tensor [rows, heads, head_dim] = ``shape`` on device number ``dev`` whose last dimension is contiguous."""
+    """Row and head stride of a tensor of ``shape`` [rows, heads, head_dim] on device number ``dev``, the last dimension contiguous."""
     if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == dev:
         row, head, last = t.stride()
         if last == 1:
