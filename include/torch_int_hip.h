@@ -599,9 +599,11 @@ typedef struct {
  * tokens begin among the `rows` rows (ascending, from 0; the last entry is their end, rows behind it belong to nobody),
  * `context_lens` [seqs] how many positions each sequence has, its new tokens counted, and `block_table` [seqs,
  * pages_per_seq] its pages, of which only those that hold a position are read.  New token i of T is at position
- * context_len - T + i.  Whatever the arrays hold, nothing outside the tensors is accessed: lengths are cut off at
- * pages_per_seq * page_size, rows at `rows`; nothing is written to a page that the pool does not have, its keys take no
- * part in an attention, and a new token at a negative position is not appended and sees no key. */
+ * context_len - T + i.  Whatever the arrays hold, nothing outside the tensors is accessed: rows are cut off at `rows`; nothing
+ * is written to a page that the pool does not have, its keys take no part in an attention, and a new token at a negative
+ * position is not appended and sees no key.  A new token whose position the sequence's pages do not reach (pages_per_seq *
+ * page_size and beyond) is not appended; an attention cuts the length off there, so that the last new token of such a sequence
+ * sees all that its pages hold, and those before it one position less each. */
 typedef struct {
   const int32_t *block_table, *context_lens, *cu_new;
   int64_t pages_per_seq, seqs, rows;
@@ -618,8 +620,8 @@ typedef struct {
  * bytes.  With `cos_sin` fp32 [positions, rot] (rot a multiple of 16 up to head_dim; cosines, then sines) the first rot
  * elements of a key are rotated by their position: pairs (j, j + rot/2), or with `neighbours` (2j, 2j + 1), become
  * (x1 c - x2 s, x2 c + x1 s).  A token whose position the table does not reach is not appended.  `query` [rows,
- * q_heads, head_dim], if given, is rotated and quantised the same way into `q_out`, packed; its rows that are not appended
- * become zeros, rows of no sequence only with `fill`.  Two tokens of a batch that share a slot of the pool leave one of the
+ * q_heads, head_dim], if given, is rotated and quantised the same way into `q_out`, packed; its rows at a position that is
+ * negative or beyond the sequence's pages or the angles become zeros, rows of no sequence only with `fill`.  Two tokens of a batch that share a slot of the pool leave one of the
  * two, in pieces, in it. */
 typedef struct {
   const void *key, *value, *query;

@@ -1,0 +1,49 @@
+"""The paged INT8 KV cache at its limits: contexts that are longer than their pages."""
+import pytest
+import torch
+
+from tests import _paged_oracle as orc
+from tests.test_gpu_paged import DEV, _angles, _batch, _paged, _s8
+
+pytestmark = pytest.mark.gpu
+
+
+def _one_by_one(cu, lens, table, rows, capacity):
+    """The batch with every row a sequence of its own, as long as the row's position makes it, so that no length passes the pages: a
+    row whose position does gets no position, as a row at a negative position or of no sequence."""
+    own = torch.zeros(rows, dtype=torch.int32)
+    whose = torch.zeros(rows, dtype=torch.long)
+    for b, n in enumerate(lens.tolist()):
+        lo, hi = int(cu[b]), int(cu[b + 1])
+        for i in range(lo, hi):
+            p = n - (hi - i)
+            whose[i], own[i] = b, p + 1 if 0 <= p < capacity else 0
+    return torch.arange(rows + 1, dtype=torch.int32), own, table[whose].contiguous()
+
+
+# query heads, key heads, head size, page, pages of a sequence, context lengths, new tokens
+BEYOND = [
+    (4, 2, 64, 16, 2, [34, 32, 33, 5], [4, 1, 1, 2]),        # the second page ends in the middle of the new tokens
+    (2, 1, 128, 16, 3, [2 ** 31 - 1, 48, 10 ** 9], [3, 2, 1]),
+    (4, 1, 80, 16, 6, [130, 96, 7], [60, 40, 7]),
+    (1, 1, 128, 64, 5, [321, 2 ** 31 - 1], [200, 150]),
+]
+
+
+@pytest.mark.parametrize("rot", [0, 16])
+@pytest.mark.parametrize("i", range(len(BEYOND)))
+def test_tokens_beyond_the_pages_are_not_appended(i, rot):
+    hq, hk, d, page, per, lens, new = BEYOND[i]
+    print("beyond", BEYOND[i], flush=True)
+    g = torch.Generator().manual_seed(50 + i)
+    cu, _, table, pages, rows = _batch(g, [per * page] * len(lens), new, page, pad=2)
+    lens = torch.tensor(lens, dtype=torch.int32)
+    k, v = _s8(g, pages, hk, page, d), _s8(g, pages, hk, page, d)
+    q, kn, vn = (torch.randn(rows, h, d, generator=g) for h in (hq, hk, hk))
+    cs = _angles(2 * per * page, rot) if rot else None
+    cu1, lens1, table1 = _one_by_one(cu, lens, table, rows, per * page)
+    want = orc.append(kn, vn, k, v, table1, lens1, cu1, 30.0, 31.0, q, 29.0, cs)
+    kd, vd = k.to(DEV), v.to(DEV)
+    got = _paged().paged_kv_append_s8(kn.to(DEV), vn.to(DEV), kd, vd, table.to(DEV), lens.to(DEV), cu.to(DEV), 30.0, 31.0,
+                                      query=q.to(DEV), alpha_q=29.0, cos_sin=None if cs is None else cs.to(DEV))
+    assert torch.equal(kd.cpu(), want[0]) and torch.equal(vd.cpu(), want[1]) and torch.equal(got.cpu(), want[2])

@@ -21,9 +21,11 @@ struct PagedBatch {
 };
 
 // One sequence of a batch.  The three arrays are device memory that the host never sees, so whatever they hold is brought
-// into range here: no row, position or table entry outside the tensors is ever formed.
+// into range here: no row, position or table entry outside the tensors is ever formed from row0, T and len.  `end` is the
+// length before it is cut off (up to 2^30, which is beyond all the 2^28 positions that there can be pages for): appending keeps to
+// it, since a new token that moved down with the cut would be written over a position that is somebody else's.
 struct PagedSeq {
-  int row0, T, len;  // first row, new tokens, cached positions
+  int row0, T, len, end;  // first row, new tokens, cached positions that there are pages for, all positions
 };
 __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int page_shift, int i) {
   PagedSeq s;
@@ -31,10 +33,11 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int page_shif
   int lo = b.cu[i], hi = b.cu[i + 1];
   lo = lo < 0 ? 0 : lo > b.rows ? b.rows : lo;
   hi = hi < lo ? lo : hi > b.rows ? b.rows : hi;
-  int len = b.lens[i];
+  const int len = b.lens[i];
   s.row0 = lo;
   s.T = hi - lo;
-  s.len = len < 0 ? 0 : len > cap ? cap : len;
+  s.end = len < 0 ? 0 : len < (1 << 30) ? len : 1 << 30;
+  s.len = s.end > cap ? cap : s.end;
   return s;
 }
 

@@ -118,13 +118,14 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend a, PagedC
   if (seq < b.seqs) {
     const PagedSeq s = paged_seq(b, c.page_shift, seq);
     mine = row >= s.row0 && row < s.row0 + s.T;
-    if (mine) position = s.len - s.T + (row - s.row0);
+    if (mine) position = s.end - s.T + (row - s.row0);
+    if (position >= s.len) position = -1;  // no page for it
   }
   const bool live = position >= 0 && (a.cos_sin == nullptr || position < a.positions);
   int8_t* dst = nullptr;
   if (which == 2) {
     dst = a.q_out + ((long long)row * a.q_heads + h) * c.D;
-    if (!live) {  // a row of no sequence, or one whose position is before the first or beyond the table
+    if (!live) {  // a row of no sequence, or one whose position is before the first, beyond the pages or beyond the angles
       if (a.fill || mine) {
         *reinterpret_cast<int2*>(dst + d0) = make_int2(0, 0);
         *reinterpret_cast<int2*>(dst + d1) = make_int2(0, 0);

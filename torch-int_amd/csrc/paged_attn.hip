@@ -104,7 +104,7 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
   PagedSeq s;
   int tiles;
   auto look = [&](int i0) {  // at sequence i0 + lane; behind the last one there is none
-    s = PagedSeq{0, 0, 0};
+    s = PagedSeq{0, 0, 0, 0};
     tiles = 0;
     if (i0 + lane < b.seqs) {
       s = paged_seq(b, page_shift, i0 + lane);

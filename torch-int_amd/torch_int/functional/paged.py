@@ -159,8 +159,9 @@ def paged_kv_append_s8(key, value, k_cache, v_cache, block_table, context_lens, 
     ``key``, ``value`` [rows, heads, head_dim] (and ``query`` [rows, q_heads, head_dim]) share one dtype of fp32, fp16, bf16
     and int8; ``alpha_*`` is one over the step of the result (for int8 inputs, their step over it).  ``cos_sin`` fp32 [positions,
     rot], the cosines and then the sines, rotates the first ``rot`` elements of keys and queries, pairs ``(j, j + rot / 2)`` or
-    with ``neighbours`` ``(2j, 2j + 1)``; values are not rotated.  A token beyond its table is not appended.  The rounding is
-    half to even, of the fp64 result; NaN becomes 0.
+    with ``neighbours`` ``(2j, 2j + 1)``; values are not rotated.  A token whose position is
+    beyond that table, or beyond its sequence's pages in ``block_table``, is not appended, and its query becomes zeros.  The
+    rounding is half to even, of the fp64 result; NaN becomes 0.
 
     Returns the int8 queries [rows, q_heads, head_dim], or None without ``query``.  Rows of no sequence are zeros in them, or
     left as they are in a ``query_out`` that is handed in."""
