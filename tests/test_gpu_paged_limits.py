@@ -1,4 +1,4 @@
-"""The paged INT8 KV cache at its limits: contexts that are longer than their pages."""
+"""The paged INT8 KV cache at its limits: contexts that are longer than their pages, batches without a sequence."""
 import pytest
 import torch
 
@@ -47,3 +47,26 @@ def test_tokens_beyond_the_pages_are_not_appended(i, rot):
     got = _paged().paged_kv_append_s8(kn.to(DEV), vn.to(DEV), kd, vd, table.to(DEV), lens.to(DEV), cu.to(DEV), 30.0, 31.0,
                                       query=q.to(DEV), alpha_q=29.0, cos_sin=None if cs is None else cs.to(DEV))
     assert torch.equal(kd.cpu(), want[0]) and torch.equal(vd.cpu(), want[1]) and torch.equal(got.cpu(), want[2])
+
+
+@pytest.mark.parametrize("out_type,size", [(1, 2), (3, 1)])
+@pytest.mark.parametrize("rows", [5, 300])
+def test_no_sequence_beside_a_workspace(rows, out_type, size):
+    # through the C entry point, which takes a workspace that nothing needs: rows of nobody become zeros, or stay
+    P = _paged()
+    g = torch.Generator().manual_seed(rows)
+    k, v = (_s8(g, 3, 2, 16, 64).to(DEV) for _ in range(2))
+    q = _s8(g, rows, 4, 64).to(DEV)
+    cu = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ws = torch.empty(1 << 25, dtype=torch.int8, device=DEV)
+    counters = torch.zeros(1 << 12, dtype=torch.int32, device=DEV)
+    strides = (2 * 16 * 64, 16 * 64, 64)
+    cache = P._Cache(k.data_ptr(), v.data_ptr(), 3, 16, 2, 64, *strides, *strides)
+    batch = P._Batch(None, None, cu.data_ptr(), 100, 0, rows)
+    for fill in (1, 0):
+        out = torch.full((rows * 4 * 64 * size,), 7, dtype=torch.int8, device=DEV)
+        what = P._Attn(q.data_ptr(), 4 * 64, 64, 4, out.data_ptr(), out_type, fill, 1e-3, 1.0, counters.data_ptr(), counters.numel())
+        rc = P._lib.ti_paged_attn_s8(cache, batch, what, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream or None)
+        assert rc == 0, P._lib.ti_last_error()
+        torch.cuda.synchronize()
+        assert bool((out == (0 if fill else 7)).all()) and not counters.any()

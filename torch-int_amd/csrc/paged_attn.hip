@@ -1057,7 +1057,7 @@ struct PagedShape {
 };
 static PagedShape paged_shape(long long rows, long long seqs, long long group, long long heads, long long capacity) {
   PagedShape s = {0, 0, 0, 0, false};
-  const bool cut = capacity > PA_MIN_SLICE;
+  const bool cut = seqs > 0 && capacity > PA_MIN_SLICE;
   if (rows * group <= PA_ROWS * seqs) {  // few rows to a sequence on average: all of them by that kernel
     s.rows_slots = heads * (seqs + rows * group / PA_ROWS);
     const long long each = rows * group / seqs + 1 < PA_ROWS ? rows * group / seqs + 1 : PA_ROWS;
