@@ -70,3 +70,12 @@ def test_no_sequence_beside_a_workspace(rows, out_type, size):
         assert rc == 0, P._lib.ti_last_error()
         torch.cuda.synchronize()
         assert bool((out == (0 if fill else 7)).all()) and not counters.any()
+
+
+def test_a_module_as_it_is_constructed():
+    from torch_int.nn import PagedAttn_S8
+    g = torch.Generator().manual_seed(3)
+    cu, lens, table, pages, rows = _batch(g, [40, 3], [5, 3], 16)
+    k, v = (_s8(g, pages, 2, 16, 64, spread=30).to(DEV) for _ in range(2))
+    args = (_s8(g, rows, 4, 64, spread=30).to(DEV), k, v, table.to(DEV), lens.to(DEV), cu.to(DEV))
+    assert torch.equal(PagedAttn_S8().to(DEV)(*args), _paged().paged_attn_s8(*args, 0.25, 1.0))

@@ -35,9 +35,10 @@ class PagedKVAppend_S8(ScalarCacheMixin, torch.nn.Module):
 
 
 class PagedAttn_S8(ScalarCacheMixin, torch.nn.Module):
-    """Causal attention of new tokens over their pages, ``b * softmax(a * q . K) . V`` in ``out_dtype``."""
+    """Causal attention of new tokens over their pages, ``b * softmax(a * q . K) . V`` in ``out_dtype``.  ``a`` is at most 0.25, which
+    a module keeps until its scales are set or loaded."""
 
-    def __init__(self, alpha_qk=1.0, alpha_pv=1.0, out_dtype=torch.int8):
+    def __init__(self, alpha_qk=0.25, alpha_pv=1.0, out_dtype=torch.int8):
         super().__init__()
         self.out_dtype = out_dtype
         self.register_buffer("a", torch.tensor(float(alpha_qk)))
