@@ -1,9 +1,10 @@
-"""The paged INT8 KV cache at its limits: contexts that are longer than their pages, batches without a sequence."""
+"""The paged INT8 KV cache at its limits: contexts that are longer than their pages, batches without a sequence,
+many sequences of which some are cut."""
 import pytest
 import torch
 
 from tests import _paged_oracle as orc
-from tests.test_gpu_paged import DEV, _angles, _batch, _paged, _s8
+from tests.test_gpu_paged import DEV, FP16_WEIGHTS, _angles, _attend, _batch, _paged, _s8
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +80,54 @@ def test_a_module_as_it_is_constructed():
     k, v = (_s8(g, pages, 2, 16, 64, spread=30).to(DEV) for _ in range(2))
     args = (_s8(g, rows, 4, 64, spread=30).to(DEV), k, v, table.to(DEV), lens.to(DEV), cu.to(DEV))
     assert torch.equal(PagedAttn_S8().to(DEV)(*args), _paged().paged_attn_s8(*args, 0.25, 1.0))
+
+
+# query heads, key heads, head size, sequences, context lengths of some of them, new tokens of some of them
+SOME_CUT = [
+    (8, 8, 16, 60, dict.fromkeys(range(60), 2000), {}),                                  # as many slices as there are places for
+    (4, 4, 64, 300, {5: 4000, 70: 3000, 131: 900, 299: 3500}, {}),                       # over several looks of 64 sequences
+    (2, 1, 128, 129, {0: 2500, 64: 2600, 128: 2700}, {64: 5}),
+    (8, 1, 32, 70, {3: 3000, 66: 2500}, {3: 100, 66: 100}),                              # tiles that are cut
+    (16, 2, 128, 66, {0: 1500, 1: 40, 30: 1800, 65: 1700}, {0: 40, 1: 20, 30: 64}),      # tiles and few rows, both cut
+]
+
+
+@pytest.mark.parametrize("i", range(len(SOME_CUT)))
+def test_slices_of_some_sequences_among_many(i, monkeypatch):
+    # the places of the slices are counted apart from the items: right, the same again and again and whoever joins them
+    P = _paged()
+    hq, hk, d, seqs, longs, news = SOME_CUT[i]
+    print("some cut", hq, hk, d, seqs, flush=True)
+    g = torch.Generator().manual_seed(70 + i)
+    new = [news.get(b, 1) for b in range(seqs)]
+    lens = [longs.get(b, 0) or new[b] + int(torch.randint(0, 60, (1,), generator=g)) for b in range(seqs)]
+    cu, lens, table, pages, rows = _batch(g, lens, new, 16, pad=1)
+    k, v = (_s8(g, pages, hk, 16, d, spread=30).to(DEV) for _ in range(2))
+    q = _s8(g, rows, hq, d, spread=30)
+    a_qk = 2.0 / (900 * d ** 0.5)
+    first = _attend(SOME_CUT[i][:4], q, k, v, table, lens, cu, a_qk, 0.02, FP16_WEIGHTS, out_dtype=torch.float16).to(DEV)
+    args = (q.to(DEV), k, v, table.to(DEV), lens.to(DEV), cu.to(DEV), a_qk, 0.02)
+    for _ in range(5):
+        assert torch.equal(P.paged_attn_s8(*args, out_dtype=torch.float16), first)
+    assert all(int(t.abs().max()) == 0 for t in P._counters.values())
+    monkeypatch.setattr(P, "_arrivals", lambda *a: (None, 0))
+    assert torch.equal(P.paged_attn_s8(*args, out_dtype=torch.float16), first)
+
+
+def test_bounds_that_descend_leave_places_and_counters_alone():
+    # cu_new counts its rows many times over: more items and slices than there are workgroups or places for
+    P = _paged()
+    g = torch.Generator().manual_seed(81)
+    for seqs, rows, hq, hk in ((200, 100, 8, 8), (66, 300, 8, 1)):
+        cu, lens, table, pages, _ = _batch(g, [3000] + [20] * (seqs - 1), [1] * seqs, 16)
+        table[:] = table[0]
+        k, v = (_s8(g, pages, hk, 16, 64, spread=30).to(DEV) for _ in range(2))
+        q = _s8(g, rows, hq, 64, spread=30).to(DEV)
+        cu = torch.tensor([0, rows] * (seqs // 2) + [rows], dtype=torch.int32, device=DEV)
+        lens = torch.where(torch.arange(seqs) % 20 == 0, 3000, rows + 20).int().to(DEV)
+        out = torch.zeros(rows + 2, hq, 64, dtype=torch.float16, device=DEV)
+        out[rows:] = 7
+        print("descending", seqs, rows, flush=True)
+        P.paged_attn_s8(q, k, v, table.to(DEV), lens, cu, 3e-4, 0.02, out=out[:rows])
+        assert torch.isfinite(out).all() and (out[rows:] == 7).all()
+        assert all(int(t.abs().max()) == 0 for t in P._counters.values())

@@ -11,3 +11,17 @@ def test_the_default_scales_are_taken():
     w = P._Attn(None, 0, 0, 2, None, 3, 1, attend._scalar("a"), attend._scalar("b"))
     assert lib.ti_paged_attn_s8(c, b, w, None, 0, None) == 0, lib.ti_last_error()
     assert [append._scalar(n) for n in ("a_k", "a_v", "a_q")] == [1.0, 1.0, 1.0]
+
+
+def test_the_workspace_does_not_grow_with_the_batch():
+    # slices of what is cut: at most 1032 of 16 rows, or 520 of 128 rows and 264 of 16, or 1032 of 128 rows
+    _, lib = _lib()
+    need, counters = lib.ti_paged_attn_workspace_bytes, lib.ti_paged_attn_arrivals
+    for seqs in (64, 512, 1024, 4096):
+        assert need(seqs, seqs, 32, 32, 128, 4096) == 1032 * 16 * 130 * 4
+        assert counters(seqs, seqs, 32, 32, 128, 4096) == 1032
+        assert need(seqs, seqs, 64, 64, 128, 1 << 20) == 1032 * 16 * 130 * 4
+    for rows, seqs, q_heads, heads in ((600, 64, 8, 2), (4000, 1000, 32, 8), (5000, 4096, 64, 8), (2048, 1, 32, 8), (1 << 20, 4000, 8, 1),
+                                       (100000, 1, 4, 1)):
+        assert need(rows, seqs, q_heads, heads, 128, 1 << 16) <= 1032 * 128 * 130 * 4
+        assert counters(rows, seqs, q_heads, heads, 128, 1 << 16) <= 1032

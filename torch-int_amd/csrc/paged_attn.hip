@@ -33,9 +33,10 @@ struct PagedPlan {
   int group;        // query heads of a key head
   int least, most;  // rows of a sequence: more than `least`, up to `most`
   int target;       // slices that the keys are cut into; 0: nothing is cut
-  int slots;        // work items at most: what the grid and the workspace hold
-  float* ws;        // partial sums [slots][rows of an item][DP] fp32, then (offset, denominator) [slots][rows]
-  int* arrivals;    // [slots] zeros, or null: a second launch joins the slices
+  int slots;        // work items at most, slices included: what the grid holds
+  int places;       // slices of items that are cut, at most: what the workspace holds
+  float* ws;        // partial sums [places][rows of an item][DP] fp32, then (offset, denominator) [places][rows]
+  int* arrivals;    // [places] zeros, or null: a second launch joins the slices
   __device__ __forceinline__ int tiles(const PagedSeq& s, int rows_per_tile) const {
     const int rows = s.T * group;
     return rows > least && rows <= most ? (rows + rows_per_tile - 1) / rows_per_tile : 0;
@@ -44,9 +45,10 @@ struct PagedPlan {
 
 struct PagedItem {
   PagedSeq s;
-  int seq, head, tile, split, splits, first;  // `first`: slot of the item's slice 0 (its slices are kv_heads * tiles apart)
-  int step;                                   // slots from one slice to the next
-  int slice;                                  // keys of a slice
+  int seq, head, tile, split, splits;
+  int place;  // of the slice 0 of an item that is cut, among all such slices (its others are `step` apart)
+  int step;   // from one slice to the next: kv_heads * tiles
+  int slice;  // keys of a slice
   bool found;
 };
 
@@ -121,7 +123,7 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
     }
     it.slice = paged_slice(items * (float)heads, total * (float)heads, p.target);
   }
-  int before = 0, before_cut = 0;
+  int before = 0, before_cut = 0, before_sliced = 0;
   int splits = 1;
   auto cut_up = [&] { splits = s.len <= it.slice ? 1 : (s.len + it.slice - 1) / it.slice; };
   if (b.seqs <= 64) {
@@ -140,7 +142,8 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
     const long long whole = (long long)here * heads, all = whole * splits;
     const int n = all > 0x800000 ? 0x800000 : (int)all;
     const int cut = splits == 1 ? 0 : whole > 0x800000 ? 0x800000 : (int)whole;
-    const int upto = wave_scan(n), upto_cut = CUT ? wave_scan(cut) : 0;
+    const int sliced = splits == 1 ? 0 : n;
+    const int upto = wave_scan(n), upto_cut = CUT ? wave_scan(cut) : 0, upto_sliced = p.target != 0 ? wave_scan(sliced) : 0;
     const unsigned long long past = __ballot(CUT ? before_cut + upto_cut > index : before + upto > index);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
@@ -157,14 +160,17 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
       const int rest = rel - it.split * it.step, from_last = rest / heads;
       it.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - skip - from_last;
       it.head = rest - from_last * heads;
-      it.first = first + rest;
-      // all slices have a slot and a workgroup, or (as a cu_new that descends can have it) the item is left out
+      it.place = before_sliced + __builtin_amdgcn_readlane(upto_sliced, at) - __builtin_amdgcn_readlane(sliced, at) + rest;
+      // all slices have a workgroup and a place, or (as a cu_new that descends can have it) the item is left out
+      const long long behind_first = (long long)(it.splits - 1) * it.step;
       it.found = it.split < it.splits && it.tile >= 0 &&
-                 (it.splits == 1 || it.first + (long long)(it.splits - 1) * it.step < p.slots);
+                 (it.splits == 1 || (first + rest + behind_first < p.slots && it.place + behind_first < p.places));
       return it;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
     before = before > 0x20000000 ? 0x20000000 : before;
+    before_sliced += __builtin_amdgcn_readlane(upto_sliced, 63);
+    before_sliced = before_sliced > 0x20000000 ? 0x20000000 : before_sliced;
     if (CUT) {
       before_cut += __builtin_amdgcn_readlane(upto_cut, 63);
       before_cut = before_cut > 0x20000000 ? 0x20000000 : before_cut;
@@ -278,11 +284,11 @@ __device__ __forceinline__ void join_slices(const PagedAttn& a, const PagedCache
   if (rows <= 0) return;
   constexpr int QUADS = DP / 4;  // places of a row; those beyond the head size are idle
   const int work = rows * QUADS;
-  const float* tail = p.ws + (long long)p.slots * ROWS * DP;
+  const float* tail = p.ws + (long long)p.places * ROWS * DP;
   const PagedRows out_row(it, a, G, ROWS);
   const PagedPart none = {PA_EMPTY, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
   auto take = [&](PagedPart& sum, int e, int s) {
-    const long long row = (it.first + (long long)s * it.step) * ROWS + first + e / QUADS;
+    const long long row = (it.place + (long long)s * it.step) * ROWS + first + e / QUADS;
     const float* from = p.ws + row * DP + e % QUADS * 4;
     const float2 od = get2<THROUGH>(tail + row * 2);
     if constexpr (THROUGH) {
@@ -344,8 +350,8 @@ __device__ __forceinline__ void meet_and_join(const PagedAttn& a, const PagedCac
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) {
-    seen[0] = __hip_atomic_fetch_add(p.arrivals + it.first, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (seen[0] == it.splits - 1) __hip_atomic_store(p.arrivals + it.first, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    seen[0] = __hip_atomic_fetch_add(p.arrivals + it.place, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (seen[0] == it.splits - 1) __hip_atomic_store(p.arrivals + it.place, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (seen[0] != it.splits - 1) return;
@@ -577,9 +583,9 @@ __device__ __forceinline__ void paged_rows(const PagedAttn& a, const PagedCache&
       l += den[w][r] * scale;
     }
     if (it.splits > 1) {
-      const long long slot = it.first + (long long)it.split * it.step;
+      const long long slot = it.place + (long long)it.split * it.step;
       put4(p.ws + (slot * PA_ROWS + r) * DP + d, y[0], y[1], y[2], y[3]);
-      if (d == 0) put2(p.ws + (long long)p.slots * PA_ROWS * DP + (slot * PA_ROWS + r) * 2, least, l);
+      if (d == 0) put2(p.ws + (long long)p.places * PA_ROWS * DP + (slot * PA_ROWS + r) * 2, least, l);
     } else {
       const float f = l > 0.0f ? a.alpha_pv * 1024.0f / l : 0.0f;
 #pragma unroll
@@ -980,7 +986,7 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
     else *(reinterpret_cast<v2f*>(&own[spot(n, m >> 1)]) + (m & 1)) = v2f{y[0], y[1]};
   }
   __builtin_amdgcn_wave_barrier();
-  const long long slot = it.first + (long long)it.split * it.step;
+  const long long slot = it.place + (long long)it.split * it.step;
   const int quad = lane % QUADS;
   const PagedRows out_row(it, a, G, PT_ROWS);
 #pragma unroll
@@ -995,7 +1001,7 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
     }
   }
   if (it.splits > 1 && real && h == 0)
-    *reinterpret_cast<v2f*>(p.ws + (long long)p.slots * PT_ROWS * DP + (slot * PT_ROWS + wave * 32 + n) * 2) = v2f{off, den};
+    *reinterpret_cast<v2f*>(p.ws + (long long)p.places * PT_ROWS * DP + (slot * PT_ROWS + wave * 32 + n) * 2) = v2f{off, den};
 }
 
 template <int DP, int OUT>
@@ -1026,7 +1032,7 @@ __global__ __launch_bounds__(PA_THREADS, DP == 64 ? 3 : 2) void paged_attn_both_
 
 // Joins slices that do not meet in the launch itself: an item that was cut to ROWS / EACH workgroups, EACH of its rows to one.
 // Eight items take turns, so that what there is to join comes first and goes to all CUs, and that an item whose number leaves the
-// same rest by 8 as its slots' (as where key heads come in eights) is read by the XCD that has written it.
+// same rest by 8 as its slices' (as where key heads come in eights) is read by the XCD that has written it.
 template <int ROWS, int EACH, int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p) {
   __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
@@ -1037,26 +1043,32 @@ __global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a
   join_slices<ROWS, EACH, DP, OUT, false>(a, c, p, it, meet, blockIdx.x / 8 % PIECES * EACH);
 }
 
-// What a call of these sizes runs.  The lengths are on the device, so the grids and the workspace are bounds: one item to each
-// (sequence, key head, tile of rows) and the slices beyond that.
+// What a call of these sizes runs.  The lengths are on the device, so the grids and the workspace are bounds.  The grid: one item to
+// each (sequence, key head, tile of rows) and the slices beyond that.  The workspace: an item that is cut is longer than a slice,
+// a slice at least the target-th part of all keys, so there are fewer than `target` such items, and of their slices fewer than
+// `target` whole ones and one more to each.
 struct PagedShape {
-  long long rows_slots, tiles_slots;  // items of either kind, slices included; 0: none
-  int rows_target, tiles_target;      // slices that the keys are cut into; 0: nothing is cut
-  bool rows_meet;                     // slices of few rows meet in the launch
+  long long rows_slots, tiles_slots;    // items of either kind, slices included; 0: none
+  long long rows_places, tiles_places;  // slices of those that are cut
+  int rows_target, tiles_target;        // slices that the keys are cut into; 0: nothing is cut
+  bool rows_meet;                       // slices of few rows meet in the launch
+  static long long places(long long slots, int target) { return slots < 2 * target + 8 ? slots : 2 * target + 8; }
   void cut_rows(int target, long long each) {
     rows_target = target;
     // where the slices of an item come to more than 65 KB, one workgroup would be longer in joining them than another launch
     // takes (2 x 100000 keys, 8 key heads of 8: 135 KB, 87 us in all against 71.6 + 5.5 us)
     rows_meet = target * each * 520 <= 66560 * rows_slots;
     rows_slots += target + 8;
+    rows_places = places(rows_slots, target);
   }
   void cut_tiles(int target) {
     tiles_target = target;
     tiles_slots += target + 8;
+    tiles_places = places(tiles_slots, target);
   }
 };
 static PagedShape paged_shape(long long rows, long long seqs, long long group, long long heads, long long capacity) {
-  PagedShape s = {0, 0, 0, 0, false};
+  PagedShape s = {0, 0, 0, 0, 0, 0, false};
   const bool cut = seqs > 0 && capacity > PA_MIN_SLICE;
   if (rows * group <= PA_ROWS * seqs) {  // few rows to a sequence on average: all of them by that kernel
     s.rows_slots = heads * (seqs + rows * group / PA_ROWS);
@@ -1081,16 +1093,16 @@ static PagedShape paged_shape(long long rows, long long seqs, long long group, l
   return s;
 }
 static int paged_dp(long long D) { return D <= 64 ? 64 : 128; }
-static long long paged_bytes(long long slots, int rows, long long D) { return slots * rows * (paged_dp(D) + 2) * 4; }
+static long long paged_bytes(long long places, int rows, long long D) { return places * rows * (paged_dp(D) + 2) * 4; }
 
 long long paged_attn_arrivals(long long rows, long long seqs, long long q_heads, long long heads, long long capacity) {
   const PagedShape s = paged_shape(rows, seqs, q_heads / heads, heads, capacity);
-  return s.rows_meet ? s.rows_slots : 0;
+  return s.rows_meet ? s.rows_places : 0;
 }
 long long paged_attn_workspace_bytes(long long rows, long long seqs, long long q_heads, long long heads, long long D,
                                      long long capacity) {
   const PagedShape s = paged_shape(rows, seqs, q_heads / heads, heads, capacity);
-  return (s.rows_target ? paged_bytes(s.rows_slots, PA_ROWS, D) : 0) + (s.tiles_target ? paged_bytes(s.tiles_slots, PT_ROWS, D) : 0);
+  return (s.rows_target ? paged_bytes(s.rows_places, PA_ROWS, D) : 0) + (s.tiles_target ? paged_bytes(s.tiles_places, PT_ROWS, D) : 0);
 }
 
 template <int DP, int OUT>
@@ -1131,14 +1143,16 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
   rows.least = 0;
   rows.most = s.tiles_slots > 0 ? PA_ROWS : 0x7fffffff;
   rows.slots = (int)s.rows_slots;
+  rows.places = (int)s.rows_places;
   rows.target = s.rows_target;
   rows.ws = reinterpret_cast<float*>(ws);
   rows.arrivals = meet && s.rows_meet ? a.arrivals : nullptr;
   tiles.least = s.rows_slots > 0 ? PA_ROWS : 0;
   tiles.most = 0x7fffffff;
   tiles.slots = (int)s.tiles_slots;
+  tiles.places = (int)s.tiles_places;
   tiles.target = s.tiles_target;
-  tiles.ws = reinterpret_cast<float*>(ws + (s.rows_target ? paged_bytes(s.rows_slots, PA_ROWS, c.D) : 0));
+  tiles.ws = reinterpret_cast<float*>(ws + (s.rows_target ? paged_bytes(s.rows_places, PA_ROWS, c.D) : 0));
   tiles.arrivals = nullptr;  // slices of 66 KB: many workgroups join them, in a launch of their own
   auto run = [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
