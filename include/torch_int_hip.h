@@ -645,7 +645,7 @@ int ti_paged_kv_append_s8(const TiPagedCache* cache, const TiPagedBatch* batch, 
  * they have 22 bits.
  * `workspace` (16-byte aligned, private to the stream, contents irrelevant) of ti_paged_attn_workspace_bytes lets long
  * sequences be cut into slices; with less, or NULL, each is read by one workgroup.  `capacity` there: pages_per_seq *
- * page_size.  Where ti_paged_attn_arrivals (same arguments) is not 0 and `arrivals` gives as many int32
+ * page_size.  It is at most 69 MB, and 8.6 MB for single tokens, whatever the number of sequences.  Where ti_paged_attn_arrivals (same arguments) is not 0 and `arrivals` gives as many int32
  * counters, zero before the first call and again after every one, that no call on another stream and no other recorded graph
  * uses, slices of few rows meet in the same launch; all others are joined by a second one.  Same bits. */
 typedef struct {

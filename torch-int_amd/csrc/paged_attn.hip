@@ -125,11 +125,15 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
   }
   int before = 0, before_cut = 0, before_sliced = 0;
   int splits = 1;
-  auto cut_up = [&] { splits = s.len <= it.slice ? 1 : (s.len + it.slice - 1) / it.slice; };
+  unsigned long long cuts = 0;  // which of the 64 sequences looked at are cut
+  auto cut_up = [&] {
+    splits = s.len <= it.slice ? 1 : (s.len + it.slice - 1) / it.slice;
+    cuts = __ballot(splits > 1 && tiles > 0);
+  };
   if (b.seqs <= 64) {
     if (p.target == 0) look(0);
     cut_up();
-    if (CUT && __ballot(splits > 1 && tiles > 0) == 0) return it;
+    if (CUT && cuts == 0) return it;
   }
   for (int part = 0, i0 = 0; part < PARTS; i0 + 64 < b.seqs ? i0 += 64 : (i0 = 0, ++part)) {
     if (b.seqs > 64) {
@@ -142,8 +146,13 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
     const long long whole = (long long)here * heads, all = whole * splits;
     const int n = all > 0x800000 ? 0x800000 : (int)all;
     const int cut = splits == 1 ? 0 : whole > 0x800000 ? 0x800000 : (int)whole;
-    const int sliced = splits == 1 ? 0 : n;
-    const int upto = wave_scan(n), upto_cut = CUT ? wave_scan(cut) : 0, upto_sliced = p.target != 0 ? wave_scan(sliced) : 0;
+    const int upto = wave_scan(n), upto_cut = CUT ? wave_scan(cut) : 0;
+    // what those of some lanes that are cut have of n, whose sum `all` is; mostly all of them are, or none
+    auto sliced = [&](unsigned long long lanes, int all) {
+      if ((cuts & lanes) == 0) return 0;
+      if ((__ballot(n > 0) & lanes & ~cuts) == 0) return all;
+      return __builtin_amdgcn_readlane(wave_scan((cuts & lanes) >> lane & 1 ? n : 0), 63);
+    };
     const unsigned long long past = __ballot(CUT ? before_cut + upto_cut > index : before + upto > index);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
@@ -160,17 +169,20 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
       const int rest = rel - it.split * it.step, from_last = rest / heads;
       it.tile = __builtin_amdgcn_readlane(tiles, at) - 1 - skip - from_last;
       it.head = rest - from_last * heads;
-      it.place = before_sliced + __builtin_amdgcn_readlane(upto_sliced, at) - __builtin_amdgcn_readlane(sliced, at) + rest;
-      // all slices have a workgroup and a place, or (as a cu_new that descends can have it) the item is left out
-      const long long behind_first = (long long)(it.splits - 1) * it.step;
-      it.found = it.split < it.splits && it.tile >= 0 &&
-                 (it.splits == 1 || (first + rest + behind_first < p.slots && it.place + behind_first < p.places));
+      it.found = it.split < it.splits && it.tile >= 0;
+      if (it.splits > 1) {
+        it.place = before_sliced + sliced((1ull << at) - 1, first - before) + rest;
+        // all slices have a workgroup and a place, or (as a cu_new that descends can have it) the item is left out
+        const long long behind_first = (long long)(it.splits - 1) * it.step;
+        it.found = it.found && first + rest + behind_first < p.slots && it.place + behind_first < p.places;
+      }
       return it;
     }
-    before += __builtin_amdgcn_readlane(upto, 63);
-    before = before > 0x20000000 ? 0x20000000 : before;
-    before_sliced += __builtin_amdgcn_readlane(upto_sliced, 63);
+    const int sum = __builtin_amdgcn_readlane(upto, 63);
+    before_sliced += sliced(~0ull, sum);
     before_sliced = before_sliced > 0x20000000 ? 0x20000000 : before_sliced;
+    before += sum;
+    before = before > 0x20000000 ? 0x20000000 : before;
     if (CUT) {
       before_cut += __builtin_amdgcn_readlane(upto_cut, 63);
       before_cut = before_cut > 0x20000000 ? 0x20000000 : before_cut;
