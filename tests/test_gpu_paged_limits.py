@@ -3,8 +3,9 @@ many sequences of which some are cut."""
 import pytest
 import torch
 
+from tests import _paged_cancelling as data
 from tests import _paged_oracle as orc
-from tests.test_gpu_paged import DEV, FP16_WEIGHTS, _angles, _attend, _batch, _paged, _s8
+from tests.test_gpu_paged import DEV, EXACT_WEIGHTS, FP16_WEIGHTS, _angles, _attend, _batch, _paged, _s8
 
 pytestmark = pytest.mark.gpu
 
@@ -131,3 +132,31 @@ def test_bounds_that_descend_leave_places_and_counters_alone():
         P.paged_attn_s8(q, k, v, table.to(DEV), lens, cu, 3e-4, 0.02, out=out[:rows])
         assert torch.isfinite(out).all() and (out[rows:] == 7).all()
         assert all(int(t.abs().max()) == 0 for t in P._counters.values())
+
+
+@pytest.mark.parametrize("hk", [1, data.HEADS])
+@pytest.mark.parametrize("lens,heavy,chunk", [([64], 64, 0), ([160, 64, 31], 64, 0), ([3000], 80, 0), ([3000, 700, 5000], 80, 0),
+                                              ([3000, 64], 64, 40)])
+def test_single_tokens_have_weights_of_22_bits(lens, heavy, chunk, hk, monkeypatch):
+    # whole, in slices that meet in the launch or behind it, beside a chunk that goes by tiles
+    P = _paged()
+    g = torch.Generator().manual_seed(sum(lens) + heavy)
+    hq, d = data.HEADS, data.D
+    new = [1] * len(lens) + [chunk] * (chunk > 0)
+    cu, lens_t, table, pages, rows = _batch(g, lens + [chunk] * (chunk > 0), new, 16)
+    k, v, q = (_s8(g, *shape, spread=30) for shape in ((pages, hk, 16, d), (pages, hk, 16, d), (rows, hq, d)))
+    wants = []
+    for b, n in enumerate(lens):
+        q[b], kk, vv, at = data.sequence(g, n // 2 * 2, min(heavy, n // 2 * 2))
+        pos = torch.arange(n // 2 * 2)
+        lens_t[b] = len(pos)
+        k[table[b].long()[pos // 16], :, pos % 16], v[table[b].long()[pos // 16], :, pos % 16] = kk[:, None], vv[:, None]
+        wants.append((data.wanted(q[b], kk, vv, at), len(at)))
+    args = (q.to(DEV), k.to(DEV), v.to(DEV), table.to(DEV), lens_t.to(DEV), cu.to(DEV), data.ALPHA, 1.0)
+    for where in ("in the launch", "behind it"):
+        got = P.paged_attn_s8(*args, out_dtype=torch.float16).cpu()
+        for b, ((want, size, most), keys) in enumerate(wants):
+            worst = orc.attention_error(got[b], want, size, most, keys, EXACT_WEIGHTS)
+            print("22 bits", lens[b], hk, where, "error over its bound", worst, flush=True)
+            assert worst <= 1.0
+        monkeypatch.setattr(P, "_arrivals", lambda *a: (None, 0))

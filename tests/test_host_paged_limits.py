@@ -1,4 +1,9 @@
 """The paged cache's defaults and bounds, on the host: nothing is launched here."""
+import pytest
+import torch
+
+from tests import _paged_cancelling as data
+from tests import _paged_oracle as orc
 from tests.test_host_paged import _good, _lib
 
 
@@ -25,3 +30,19 @@ def test_the_workspace_does_not_grow_with_the_batch():
                                        (100000, 1, 4, 1)):
         assert need(rows, seqs, q_heads, heads, 128, 1 << 16) <= 1032 * 128 * 130 * 4
         assert counters(rows, seqs, q_heads, heads, 128, 1 << 16) <= 1032
+
+
+@pytest.mark.parametrize("keys", [64, 160])
+def test_the_bound_tells_weights_of_11_bits_from_weights_of_22(keys):
+    # the kernels' way of holding a weight, on the CPU: the largest is 2^8, in one fp16 number or in the sum of two
+    g = torch.Generator().manual_seed(keys)
+    q, k, v, at = data.sequence(g, keys, keys)
+    want, size, most = data.wanted(q, k, v, at)
+    x = (q.double() @ k.double().T).float()
+    c = torch.tensor(data.ALPHA, dtype=torch.float32) * torch.tensor(1.44269504088896341, dtype=torch.float32)
+    e = torch.exp2((x.double() * c.double() + (8 - x.amax(1, keepdim=True) * c).double()).float().double()).float()
+    one = e.half().double()
+    two = one + (e.double() - one).half().double()
+    off = [orc.attention_error(((w @ v.double()) / w.sum(1, keepdim=True)).half(), want, size, most, keys, 2.0 ** -22) for w in (one, two)]
+    print("error over its bound, 11 bits and 22", off)
+    assert off[0] > 2.0 and off[1] <= 1.0
