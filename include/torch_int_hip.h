@@ -641,13 +641,16 @@ int ti_paged_kv_append_s8(const TiPagedCache* cache, const TiPagedBatch* batch, 
  * heads, q head h reads key head h / (q_heads / heads).  out [rows, q_heads, head_dim] packed, apart from the inputs, of
  * `out_type`: TI_TYPE_S8 (rint, clamp to [-128, 127]), TI_TYPE_F16 or TI_TYPE_BF16.  Rows of no sequence become zeros with
  * `fill` and stay as they are without.  alpha_qk in [1e-30, 0.25] (scores reach 2^21 alpha_qk).  Probabilities are not quantised to int8 (the
- * whole-cache attentions above do that): a row's largest counts 2^8 to 2^15 in fp16, and where little else bounds the kernel
- * they have 22 bits.
+ * whole-cache attentions above do that): a row's largest counts 2^8 to 2^15 in fp16.  They have 22 bits in a sequence of up to 16
+ * rows (new tokens times query heads of a key head), and in longer ones as long as the batch has no more than 16 on average; 11
+ * bits, the fp16 number's, in longer sequences of all other batches.  How the keys are cut into slices depends on the batch as
+ * well, so the last bits of a token's context can differ with the sequences beside it.
  * `workspace` (16-byte aligned, private to the stream, contents irrelevant) of ti_paged_attn_workspace_bytes lets long
  * sequences be cut into slices; with less, or NULL, each is read by one workgroup.  `capacity` there: pages_per_seq *
  * page_size.  It is at most 69 MB, and 8.6 MB for single tokens, whatever the number of sequences.  Where ti_paged_attn_arrivals (same arguments) is not 0 and `arrivals` gives as many int32
  * counters, zero before the first call and again after every one, that no call on another stream and no other recorded graph
- * uses, slices of few rows meet in the same launch; all others are joined by a second one.  Same bits. */
+ * uses, slices of few rows meet in the same launch; all others are joined by a second one: same bits either way.  Whether
+ * there is a workspace changes them, since nothing is cut without one. */
 typedef struct {
   const int8_t* q;
   int64_t q_row, q_head, q_heads;

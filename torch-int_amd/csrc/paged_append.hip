@@ -73,8 +73,8 @@ __device__ __forceinline__ int2 pack8(const int (&o)[8]) {
 
 // One row to blockIdx.x; the threads of a block are the 16-element pieces of some heads, the keys', then the values', then the
 // queries'.  A piece is 16 neighbouring elements, or where pairs lie half apart 8 elements and their 8 partners.
-// At the rate of a copy: 8192 rows of 32 + 2 x 8 heads of 128 fp16, 155 MB, take 29.6 us (5.2 TB/s), 2036 rows of 3 x 32 heads fp32,
-// 125 MB, 25.1 us (5.0).  That needs few instructions (280 a wave; in fp64 they took 44 us of the first) and the row's
+// At the rate of a copy: 8192 rows of 32 + 2 x 8 heads of 128 fp16, 155 MB, take 29.4 us (5.3 TB/s), 2036 rows of 3 x 32 heads fp32,
+// 125 MB, 23.9 us (5.2).  That needs few instructions (280 a wave; in fp64 they took 44 us of the first) and the row's
 // elements on their way before its place is known, behind the one load that begins the search (33.9 us in front of it).  Several rows
 // to a block, the next row's elements ahead of the present one's, needs 98 registers instead of 66 and made the second 36 us.
 template <typename T>

@@ -371,7 +371,7 @@ __device__ __forceinline__ void meet_and_join(const PagedAttn& a, const PagedCac
 }
 
 // Few rows: 16 to a workgroup, its four waves take 32 keys each in turn.  Bound by memory: 61 sequences of 40 to 4001 keys, 8 key
-// heads of four query heads, 252 MB, take 57 us (4.4 TB/s; a copy of as much runs at 5.2), 2 x 95000 keys 389 MB in 70 us (5.5).
+// heads of four query heads, 252 MB, take 57 us (4.4 TB/s; a copy of as much runs at 5.25), 2 x 95000 keys 389 MB in 70 us (5.6).
 // A build that only loads takes as long; non-temporal loads, four waves to a SIMD instead of three and 64 keys a step did not help.
 // Short sequences are a chain of latencies: 500 keys, 12 heads take 6.8 us, some 2 us of them to the first key.
 constexpr int rows_lds(int DP) { return PA_WAVES * PA_ROWS * (DP + 4 + 2) * 4; }
@@ -615,9 +615,14 @@ __device__ __forceinline__ void paged_rows(const PagedAttn& a, const PagedCache&
 // so a thread widens neighbouring columns and a lane of O^T ends up with neighbouring ones.
 // Bound by what a wave can issue: a step of 64 keys takes a wave 1.6 us alone on its SIMD, the same with its keys in the nearest
 // cache, and two waves 2.0 us (matrix pipe 38 % busy, vector ALUs 49 %; its 241 registers allow no third,
-// but those of head sizes up to 64 do).  2048 rows over 16229 keys, 8 key heads of four: 445 to 480 us, 510 G operations, half of them
-// int8, half fp16.  An item costs 4 us before its first step
+// but those of head sizes up to 64 do).  2048 rows over 16229 keys, 8 key heads of four: 442 to 452 us a pass, 510 G operations, half
+// of them int8, half fp16.  An item costs 4 us before its first step
 // (its place, its page, its keys) and some 2 behind the last: 4 x 512 rows of 40 heads are 640 items of 2 to 8 steps, 35 us.
+// A probability is one fp16 number here, 11 bits: there is no time to spare that a second one could go into, as it does where few
+// rows wait for memory.  With two (the sum of them in numerator and denominator, 255 registers) 2048 rows over 16229 keys take 657 us
+// instead of 445, 512 rows beside 31 single tokens 47.6 instead of 41.0, 4 x 512 rows of 40 heads 38.4 instead of 34.3.  What that
+// would gain, root mean square of the error over that of the contexts: 2.5e-4 to 2.1e-4 where contexts are fp16, whose own rounding
+// is the 2.1e-4, and nothing to speak of in bf16 (1.7e-3).
 // Scores start from 1.5 * 2^23 instead of 0: the int32 sum is then the fp32 number 12582912 + x, and the constant goes into the
 // row's offset, where one multiply-add removes it exactly.
 constexpr int PT_ROWS = 128, PT_KEYS = 64;
@@ -701,7 +706,7 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
   auto k_from = [&](int s0, int page) { return kb + (long long)(have(page) ? page : 0) * c.k_page + place(s0) * c.k_token; };
   auto v_from = [&](int s0, int page) { return vb_ + (long long)(have(page) ? page : 0) * c.v_page + place(s0) * c.v_token; };
   // by buffer instructions: a column is one register beside the page's place in scalar ones, not two (241 registers instead of 255,
-  // for head sizes up to 64 164 instead of 178, which makes room for a third workgroup: 16 x 512 rows of 32 heads 62.4 to 50.7 us)
+  // for head sizes up to 64 165 instead of 178, which makes room for a third workgroup: 16 x 512 rows of 32 heads 62.4 to 50.7 us)
   auto pool = [](const int8_t* from) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(from), 0, -1, 0x00020000); };
   auto fetch_k = [&](v4i (&kreg)[KC], const int8_t* from) {
     const auto r = pool(from);

@@ -229,7 +229,11 @@ def paged_attn_s8(query, k_cache, v_cache, block_table, context_lens, cu_new, al
     ``h // (q_heads // heads)``).  Every token sees the positions up to its own, which have to be in the cache already
     (:func:`paged_kv_append_s8`).  The result [rows, q_heads, head_dim] is fp16, bf16 or int8 (``sat_s8(round(...))``, for a W8A8
     layer behind it).  A token that sees nothing gets zeros; rows of no sequence are zeros too, or left as they are in an
-    ``out`` that is handed in, which must not share memory with the inputs.  ``alpha_qk`` is positive and at most 0.25."""
+    ``out`` that is handed in, which must not share memory with the inputs.  ``alpha_qk`` is positive and at most 0.25.
+
+    Weights have 22 bits in sequences of up to 16 rows (new tokens times ``q_heads // heads``) and, as long as a batch has no more
+    than 16 on average, in all; longer sequences of other batches have weights of 11 bits.  The same batch gives the same bits on any
+    stream and in a recorded graph; beside other sequences the last bits of a token's context can differ."""
     op = "paged_attn_s8"
     if not isinstance(query, torch.Tensor) or query.dim() != 3:
         _fail(op, f"query must be a 3-D torch.int8 tensor, got {_describe(query)}")
