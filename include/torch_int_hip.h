@@ -621,8 +621,8 @@ typedef struct {
  * elements of a key are rotated by their position: pairs (j, j + rot/2), or with `neighbours` (2j, 2j + 1), become
  * (x1 c - x2 s, x2 c + x1 s).  A token whose position the table does not reach is not appended.  `query` [rows,
  * q_heads, head_dim], if given, is rotated and quantised the same way into `q_out`, packed; its rows at a position that is
- * negative or beyond the sequence's pages or the angles become zeros, rows of no sequence only with `fill`.  Two tokens of a batch that share a slot of the pool leave one of the
- * two, in pieces, in it. */
+ * negative or beyond the sequence's pages or the angles become zeros, rows of no sequence only with `fill`.  Two tokens of a
+ * batch that share a slot of the pool leave one of the two, in pieces, in it. */
 typedef struct {
   const void *key, *value, *query;
   int64_t k_row, k_head, v_row, v_head, q_row, q_head;
@@ -647,10 +647,11 @@ int ti_paged_kv_append_s8(const TiPagedCache* cache, const TiPagedBatch* batch, 
  * well, so the last bits of a token's context can differ with the sequences beside it.
  * `workspace` (16-byte aligned, private to the stream, contents irrelevant) of ti_paged_attn_workspace_bytes lets long
  * sequences be cut into slices; with less, or NULL, each is read by one workgroup.  `capacity` there: pages_per_seq *
- * page_size.  It is at most 69 MB, and 8.6 MB for single tokens, whatever the number of sequences.  Where ti_paged_attn_arrivals (same arguments) is not 0 and `arrivals` gives as many int32
- * counters, zero before the first call and again after every one, that no call on another stream and no other recorded graph
- * uses, slices of few rows meet in the same launch; all others are joined by a second one: same bits either way.  Whether
- * there is a workspace changes them, since nothing is cut without one. */
+ * page_size.  It is at most 69 MB, and 8.6 MB for single tokens, whatever the number of sequences.  Where
+ * ti_paged_attn_arrivals (same arguments) is not 0 and `arrivals` gives as many int32 counters, zero before the first call and
+ * again after every one, that no call on another stream and no other recorded graph uses, slices of few rows meet in the same
+ * launch; all others are joined by a second one: same bits either way.  Whether there is a workspace changes them, since
+ * nothing is cut without one. */
 typedef struct {
   const int8_t* q;
   int64_t q_row, q_head, q_heads;

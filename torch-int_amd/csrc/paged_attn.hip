@@ -101,6 +101,7 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
                                                 int index) {
   PagedItem it;
   it.found = false;
+  it.place = 0;
   if (b.seqs == 0) return it;
   const int lane = threadIdx.x & 63;
   PagedSeq s;
@@ -615,7 +616,7 @@ __device__ __forceinline__ void paged_rows(const PagedAttn& a, const PagedCache&
 // so a thread widens neighbouring columns and a lane of O^T ends up with neighbouring ones.
 // Bound by what a wave can issue: a step of 64 keys takes a wave 1.6 us alone on its SIMD, the same with its keys in the nearest
 // cache, and two waves 2.0 us (matrix pipe 38 % busy, vector ALUs 49 %; its 241 registers allow no third,
-// but those of head sizes up to 64 do).  2048 rows over 16229 keys, 8 key heads of four: 442 to 452 us a pass, 510 G operations, half
+// but those of head sizes up to 64 do).  2048 rows over 16229 keys, 8 key heads of four: 442 to 456 us a pass, 510 G operations, half
 // of them int8, half fp16.  An item costs 4 us before its first step
 // (its place, its page, its keys) and some 2 behind the last: 4 x 512 rows of 40 heads are 640 items of 2 to 8 steps, 35 us.
 // A probability is one fp16 number here, 11 bits: there is no time to spare that a second one could go into, as it does where few
