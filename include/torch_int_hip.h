@@ -667,6 +667,76 @@ int64_t ti_paged_attn_workspace_bytes(int64_t rows, int64_t seqs, int64_t q_head
 int ti_paged_attn_s8(const TiPagedCache* cache, const TiPagedBatch* batch, const TiPagedAttn* what, void* workspace,
                      int64_t workspace_bytes, void* stream);
 
+/* ---- The same cache in 4 bits, whose steps are found as it is written. ----
+ * A position's row of a head has head_dim (a multiple of 16 from 32 to 128) values s (u - z): u a code of 4 bits; s and z, of
+ * `groups` groups, one for the whole head or one for each half of its columns.  Byte j of k and v (0 <= j < head_dim / 2) holds
+ * the code of column j in its low four bits and that of column head_dim / 2 + j in the others.  A group's 16-bit word holds s in
+ * its bits 4 to 14, where an fp16 number has them (its other bits 0: 7 significant bits, multiples of 2^-20), and z, 0 to 15, in
+ * the low four.  Codes: strides in bytes, multiples of 8 that do not overlap, any order of pages, heads and positions.  Words:
+ * [pages, heads, page_size, groups], the last two dimensions packed, the other strides in bytes, multiples of 16.  All four
+ * pointers are 16-byte aligned. */
+typedef struct {
+  uint8_t *k, *v;
+  uint16_t *k_scale, *v_scale;
+  int64_t pages, page_size, heads, head_dim, groups;
+  int64_t k_page, k_head, k_token;
+  int64_t v_page, v_head, v_token;
+  int64_t k_scale_page, k_scale_head, v_scale_page, v_scale_head;
+} TiPagedCacheS4;
+
+/* Appends the new tokens' keys and values as ti_paged_kv_append_s8 does (batch, types, strides, rotation and what is left out are the
+ * same), in 4 bits: y = fp32(alpha x) or fp32(alpha times the rotation) of the fp64 result, NaN -> 0, cut off at +-57344; of a group's
+ * values a = min(0, y), b = max(0, y); s the smallest step of the format with 15 s >= b - a, z = rint(-a / s),
+ * u = clamp(rint(y / s) + z, 0, 15), roundings half to even, s = z = u = 0 where all are 0.  No value is further than s / 2 from
+ * its own.  `query` is rotated into `q_out` of `q_type`: TI_TYPE_S8 as there, or TI_TYPE_F16 / TI_TYPE_BF16 of fp32(alpha_q y). */
+typedef struct {
+  const void *key, *value, *query;
+  int64_t k_row, k_head, v_row, v_head, q_row, q_head;
+  void* q_out;
+  int64_t q_heads;
+  const float* cos_sin;
+  int64_t rot, positions;
+  int32_t type, q_type, neighbours, fill;
+  float alpha_q, alpha_k, alpha_v;
+} TiPagedAppendS4;
+int ti_paged_kv_append_s4(const TiPagedCacheS4* cache, const TiPagedBatch* batch, const TiPagedAppendS4* what, void* stream);
+
+/* Reads positions back: row cu_new[i] + t of key and value [rows, heads, head_dim], packed, of `type`, is that of position
+ * context_len - T + t of sequence i (the T last ones; all with T = context_len), alpha s (u - z) rounded to fp32 and to the type
+ * (TI_TYPE_S8: rint of the exact product, clamp to [-128, 127]).  Rows of a sequence whose position is negative, or that has no page,
+ * are zeros; rows of no sequence with `fill`, and stay as they are without. */
+typedef struct {
+  void *key, *value;
+  int32_t type, fill;
+  float alpha_k, alpha_v;
+} TiPagedReadS4;
+int ti_paged_kv_read_s4(const TiPagedCacheS4* cache, const TiPagedBatch* batch, const TiPagedReadS4* what, void* stream);
+
+/* Attention of the new tokens over their sequences' pages (ti_paged_attn_s8's, and what is said there of batches, rows, workspace and
+ * arrivals holds):
+ *   out[row, h] = alpha_pv * sum_j w_j v_j,  w = softmax(alpha_qk * q . k_j) over the positions j <= p that the token at p sees:
+ * all of them with window = 0, otherwise those with p - j < window and those with j < sinks.  Pages and words of positions that no
+ * token of a call sees may hold anything, and their entries of the block table may be anything.
+ * q of `q_type` (TI_TYPE_S8, TI_TYPE_F16, TI_TYPE_BF16; bf16 is computed with as fp16: beyond 65504 it is infinite, below 2^-14 its bits
+ * get fewer), strides in elements, multiples of 16 bytes; alpha_qk in [1e-30, 1e4].  Scores, alpha_qk * q . k, are meant to stay below
+ * 2^24, beyond which fp32 no longer tells them apart; a row whose query holds an infinity or a NaN has NaN.  Products are exact
+ * or fp32's, probabilities have 22 bits. */
+typedef struct {
+  const void* q;
+  int64_t q_row, q_head, q_heads;
+  void* out;
+  int32_t q_type, out_type, fill;
+  float alpha_qk, alpha_pv;
+  int64_t window, sinks;
+  int32_t* arrivals;
+  int64_t arrivals_count;
+} TiPagedAttnS4;
+int64_t ti_paged_attn_s4_arrivals(int64_t rows, int64_t seqs, int64_t q_heads, int64_t heads, int64_t head_dim, int64_t capacity);
+int64_t ti_paged_attn_s4_workspace_bytes(int64_t rows, int64_t seqs, int64_t q_heads, int64_t heads, int64_t head_dim,
+                                         int64_t capacity);
+int ti_paged_attn_s4(const TiPagedCacheS4* cache, const TiPagedBatch* batch, const TiPagedAttnS4* what, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1132,15 +1132,19 @@ int ti_opt_decoder_layer_prefill_chained(const TiOptDecodeLayer* L, void* hidden
 
 // ---------------------------------------------------------------- a KV cache in pages
 namespace {
-// One of the two pools: 16-byte aligned, strides that step over whole positions without overlapping.
-int check_pool(const char* op, const char* name, const void* p, const TiPagedCache& c, int64_t page, int64_t head, int64_t token) {
+// What a pool's strides step over: `row` bytes to each of page_size positions of each head of each page, all multiples of `unit`.
+struct PoolShape {
+  int64_t pages, heads, page_size, row, unit;
+};
+// One of the pools: 16-byte aligned, strides that step over whole positions without overlapping.
+int check_pool(const char* op, const char* name, const void* p, const PoolShape& c, int64_t page, int64_t head, int64_t token) {
   if (int rc = check_ptr(op, name, p, 16, c.pages > 0)) return rc;
   int64_t stride[3] = {page, head, token}, size[3] = {c.pages, c.heads, c.page_size};
   for (int i = 0; i < 3; ++i) {
     if (size[i] <= 1) continue;
-    if (stride[i] < c.head_dim || stride[i] % 16 || stride[i] > (INT64_C(1) << 40))
-      return fail(TI_ERR_INVALID_ARG, "%s: %s strides (%lld, %lld, %lld bytes) must be multiples of 16 that step over a position's "
-                  "%lld bytes", op, name, (long long)page, (long long)head, (long long)token, (long long)c.head_dim);
+    if (stride[i] < c.row || stride[i] % c.unit || stride[i] > (INT64_C(1) << 40))
+      return fail(TI_ERR_INVALID_ARG, "%s: %s strides (%lld, %lld, %lld bytes) must be multiples of %lld that step over a position's "
+                  "%lld bytes", op, name, (long long)page, (long long)head, (long long)token, (long long)c.unit, (long long)c.row);
   }
   for (int i = 0; i < 2; ++i)
     for (int j = 0; j < 2 - i; ++j)
@@ -1149,7 +1153,7 @@ int check_pool(const char* op, const char* name, const void* p, const TiPagedCac
         stride[j] = stride[j + 1], size[j] = size[j + 1];
         stride[j + 1] = a, size[j + 1] = b;
       }
-  int64_t extent = c.head_dim;  // bytes from the first to the last of what the smaller strides reach
+  int64_t extent = c.row;  // bytes from the first to the last of what the smaller strides reach
   for (int i = 2; i >= 0; --i) {
     if (size[i] <= 1) continue;
     if (stride[i] < extent)
@@ -1162,33 +1166,76 @@ int check_pool(const char* op, const char* name, const void* p, const TiPagedCac
   return TI_OK;
 }
 
-int paged_args(const char* op, const TiPagedCache* c, const TiPagedBatch* b, ti::PagedCache* cache, ti::PagedBatch* batch) {
-  if (c == nullptr || b == nullptr) return fail(TI_ERR_INVALID_ARG, "%s: cache and batch must be given", op);
-  const int64_t lim = 0x7fffffffLL;
-  if (c->page_size < 16 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)))
-    return fail(TI_ERR_INVALID_ARG, "%s: a page of %lld positions (a power of two from 16 to 65536 is needed)", op,
-                (long long)c->page_size);
-  if (c->head_dim < 16 || c->head_dim > 128 || c->head_dim % 16)
-    return fail(TI_ERR_INVALID_ARG, "%s: head size %lld (a multiple of 16 up to 128 is needed)", op, (long long)c->head_dim);
-  if (c->heads < 1 || c->heads > 4096 || c->pages < 0 || c->pages > lim)
-    return fail(TI_ERR_INVALID_ARG, "%s: %lld heads in %lld pages (1 to 4096 heads, fewer than 2^31 pages)", op, (long long)c->heads,
-                (long long)c->pages);
+int check_pages(const char* op, int64_t page_size, int64_t heads, int64_t pages) {
+  if (page_size < 16 || page_size > 65536 || (page_size & (page_size - 1)))
+    return fail(TI_ERR_INVALID_ARG, "%s: a page of %lld positions (a power of two from 16 to 65536 is needed)", op, (long long)page_size);
+  if (heads < 1 || heads > 4096 || pages < 0 || pages > 0x7fffffffLL)
+    return fail(TI_ERR_INVALID_ARG, "%s: %lld heads in %lld pages (1 to 4096 heads, fewer than 2^31 pages)", op, (long long)heads,
+                (long long)pages);
+  return TI_OK;
+}
+
+int check_batch(const char* op, const TiPagedBatch* b, int64_t page_size) {
   if (b->rows < 0 || b->rows > (1 << 23) || b->seqs < 0 || b->seqs > (1 << 20) || b->pages_per_seq < 0)
     return fail(TI_ERR_INVALID_ARG, "%s: %lld rows of %lld sequences of %lld pages (at most 2^23 rows and 2^20 sequences)", op,
                 (long long)b->rows, (long long)b->seqs, (long long)b->pages_per_seq);
-  if (b->pages_per_seq > (1 << 28) || b->pages_per_seq * c->page_size > (1 << 28))
+  if (b->pages_per_seq > (1 << 28) || b->pages_per_seq * page_size > (1 << 28))
     return fail(TI_ERR_INVALID_ARG, "%s: sequences of up to %lld pages of %lld positions (at most 2^28 positions)", op,
-                (long long)b->pages_per_seq, (long long)c->page_size);
-  if (int rc = check_pool(op, "k_cache", c->k, *c, c->k_page, c->k_head, c->k_token)) return rc;
-  if (int rc = check_pool(op, "v_cache", c->v, *c, c->v_page, c->v_head, c->v_token)) return rc;
+                (long long)b->pages_per_seq, (long long)page_size);
+  return TI_OK;
+}
+
+int check_batch_ptrs(const char* op, const TiPagedBatch* b) {
   if (int rc = check_ptr(op, "block_table", b->block_table, 4, b->seqs > 0 && b->pages_per_seq > 0)) return rc;
   if (int rc = check_ptr(op, "context_lens", b->context_lens, 4, b->seqs > 0)) return rc;
-  if (int rc = check_ptr(op, "cu_new", b->cu_new, 4, b->rows > 0)) return rc;
+  return check_ptr(op, "cu_new", b->cu_new, 4, b->rows > 0);
+}
+
+int page_shift_of(int64_t page_size) {
   int shift = 4;
-  while ((1 << shift) < c->page_size) ++shift;
+  while ((1 << shift) < page_size) ++shift;
+  return shift;
+}
+
+ti::PagedBatch batch_of(const TiPagedBatch* b) {
+  return ti::PagedBatch{b->block_table, b->context_lens, b->cu_new, (int)b->pages_per_seq, (int)b->seqs, (int)b->rows};
+}
+
+int paged_args(const char* op, const TiPagedCache* c, const TiPagedBatch* b, ti::PagedCache* cache, ti::PagedBatch* batch) {
+  if (c == nullptr || b == nullptr) return fail(TI_ERR_INVALID_ARG, "%s: cache and batch must be given", op);
+  if (c->head_dim < 16 || c->head_dim > 128 || c->head_dim % 16)
+    return fail(TI_ERR_INVALID_ARG, "%s: head size %lld (a multiple of 16 up to 128 is needed)", op, (long long)c->head_dim);
+  if (int rc = check_pages(op, c->page_size, c->heads, c->pages)) return rc;
+  if (int rc = check_batch(op, b, c->page_size)) return rc;
+  const PoolShape pool = {c->pages, c->heads, c->page_size, c->head_dim, 16};
+  if (int rc = check_pool(op, "k_cache", c->k, pool, c->k_page, c->k_head, c->k_token)) return rc;
+  if (int rc = check_pool(op, "v_cache", c->v, pool, c->v_page, c->v_head, c->v_token)) return rc;
+  if (int rc = check_batch_ptrs(op, b)) return rc;
   *cache = ti::PagedCache{c->k, c->v, c->k_page, c->k_head, c->v_page, c->v_head, (int)c->k_token, (int)c->v_token, (int)c->pages,
-                          shift, (int)c->heads, (int)c->head_dim};
-  *batch = ti::PagedBatch{b->block_table, b->context_lens, b->cu_new, (int)b->pages_per_seq, (int)b->seqs, (int)b->rows};
+                          page_shift_of(c->page_size), (int)c->heads, (int)c->head_dim};
+  *batch = batch_of(b);
+  return TI_OK;
+}
+
+int paged_s4_args(const char* op, const TiPagedCacheS4* c, const TiPagedBatch* b, ti::PagedCache4* cache, ti::PagedBatch* batch) {
+  if (c == nullptr || b == nullptr) return fail(TI_ERR_INVALID_ARG, "%s: cache and batch must be given", op);
+  if (c->head_dim < 32 || c->head_dim > 128 || c->head_dim % 16)
+    return fail(TI_ERR_INVALID_ARG, "%s: head size %lld (a multiple of 16 from 32 to 128 is needed)", op, (long long)c->head_dim);
+  if (c->groups != 1 && c->groups != 2)
+    return fail(TI_ERR_INVALID_ARG, "%s: %lld groups to a head (1 or 2)", op, (long long)c->groups);
+  if (int rc = check_pages(op, c->page_size, c->heads, c->pages)) return rc;
+  if (int rc = check_batch(op, b, c->page_size)) return rc;
+  const PoolShape codes = {c->pages, c->heads, c->page_size, c->head_dim / 2, 8};
+  if (int rc = check_pool(op, "k_cache", c->k, codes, c->k_page, c->k_head, c->k_token)) return rc;
+  if (int rc = check_pool(op, "v_cache", c->v, codes, c->v_page, c->v_head, c->v_token)) return rc;
+  const PoolShape words = {c->pages, c->heads, 1, c->page_size * c->groups * 2, 16};
+  if (int rc = check_pool(op, "k_scale", c->k_scale, words, c->k_scale_page, c->k_scale_head, 0)) return rc;
+  if (int rc = check_pool(op, "v_scale", c->v_scale, words, c->v_scale_page, c->v_scale_head, 0)) return rc;
+  if (int rc = check_batch_ptrs(op, b)) return rc;
+  *cache = ti::PagedCache4{c->k, c->v, c->k_scale, c->v_scale, c->k_page, c->k_head, c->v_page, c->v_head, c->k_scale_page,
+                           c->k_scale_head, c->v_scale_page, c->v_scale_head, (int)c->k_token, (int)c->v_token, (int)c->pages,
+                           page_shift_of(c->page_size), (int)c->heads, (int)c->head_dim, (int)c->groups};
+  *batch = batch_of(b);
   return TI_OK;
 }
 
@@ -1279,6 +1326,107 @@ int ti_paged_attn_s8(const TiPagedCache* cache, const TiPagedBatch* batch, const
   a.alpha_qk = w->alpha_qk, a.alpha_pv = w->alpha_pv, a.fill = w->fill != 0;
   a.arrivals = w->arrivals, a.arrivals_count = w->arrivals_count;
   return launch_paged_attn_s8(w->out_type, a, c, b, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+int ti_paged_kv_append_s4(const TiPagedCacheS4* cache, const TiPagedBatch* batch, const TiPagedAppendS4* w, void* stream) {
+  g_err[0] = 0;
+  const char* op = "paged_kv_append_s4";
+  PagedCache4 c;
+  PagedBatch b;
+  if (int rc = paged_s4_args(op, cache, batch, &c, &b)) return rc;
+  if (w == nullptr) return fail(TI_ERR_INVALID_ARG, "%s: what to append must be given", op);
+  if (w->type < TI_TYPE_F32 || w->type > TI_TYPE_S8) return fail(TI_ERR_INVALID_ARG, "%s: type %d", op, (int)w->type);
+  const bool query = w->query != nullptr;
+  if (query && (w->q_heads < 1 || w->q_heads > 4096))
+    return fail(TI_ERR_INVALID_ARG, "%s: %lld query heads (1 to 4096)", op, (long long)w->q_heads);
+  if (query && w->q_type != TI_TYPE_S8 && w->q_type != TI_TYPE_F16 && w->q_type != TI_TYPE_BF16)
+    return fail(TI_ERR_INVALID_ARG, "%s: query type %d (int8, fp16 and bf16 are there)", op, (int)w->q_type);
+  if (w->cos_sin != nullptr && (w->rot < 16 || w->rot > c.D || w->rot % 16 || w->positions < 0 || w->positions > 0x7fffffffLL))
+    return fail(TI_ERR_INVALID_ARG, "%s: %lld of %d elements rotated (a multiple of 16 up to the head size), %lld positions", op,
+                (long long)w->rot, c.D, (long long)w->positions);
+  if (b.rows == 0) return TI_OK;
+  const int64_t size = w->type == TI_TYPE_F32 ? 4 : w->type == TI_TYPE_S8 ? 1 : 2;
+  if (int rc = check_rows(op, "key", w->key, w->k_row, w->k_head, size)) return rc;
+  if (int rc = check_rows(op, "value", w->value, w->v_row, w->v_head, size)) return rc;
+  if (query) {
+    if (int rc = check_rows(op, "query", w->query, w->q_row, w->q_head, size)) return rc;
+    if (int rc = check_ptr(op, "q_out", w->q_out, 16, true)) return rc;
+  }
+  if (int rc = check_ptr(op, "cos_sin", w->cos_sin, 16, w->cos_sin != nullptr)) return rc;
+  PagedAppend4 a;
+  a.key = w->key, a.value = w->value, a.query = w->query;
+  a.k_row = w->k_row, a.k_head = w->k_head, a.v_row = w->v_row, a.v_head = w->v_head, a.q_row = w->q_row, a.q_head = w->q_head;
+  a.q_out = w->q_out, a.q_heads = query ? (int)w->q_heads : 0, a.q_type = w->q_type;
+  a.cos_sin = w->cos_sin, a.rot = (int)w->rot, a.positions = (int)w->positions;
+  a.neighbours = w->neighbours != 0, a.fill = w->fill != 0;
+  a.alpha_q = w->alpha_q, a.alpha_k = w->alpha_k, a.alpha_v = w->alpha_v;
+  return launch_paged_kv_append_s4(w->type, a, c, b, static_cast<hipStream_t>(stream));
+}
+
+int ti_paged_kv_read_s4(const TiPagedCacheS4* cache, const TiPagedBatch* batch, const TiPagedReadS4* w, void* stream) {
+  g_err[0] = 0;
+  const char* op = "paged_kv_read_s4";
+  PagedCache4 c;
+  PagedBatch b;
+  if (int rc = paged_s4_args(op, cache, batch, &c, &b)) return rc;
+  if (w == nullptr) return fail(TI_ERR_INVALID_ARG, "%s: the outputs must be given", op);
+  if (w->type < TI_TYPE_F32 || w->type > TI_TYPE_S8) return fail(TI_ERR_INVALID_ARG, "%s: type %d", op, (int)w->type);
+  if (b.rows == 0) return TI_OK;
+  if (int rc = check_ptr(op, "key", w->key, 16, true)) return rc;
+  if (int rc = check_ptr(op, "value", w->value, 16, true)) return rc;
+  return launch_paged_kv_read_s4(w->type, PagedRead4{w->key, w->value, w->fill != 0, w->alpha_k, w->alpha_v}, c, b,
+                                 static_cast<hipStream_t>(stream));
+}
+
+int64_t ti_paged_attn_s4_workspace_bytes(int64_t rows, int64_t seqs, int64_t q_heads, int64_t heads, int64_t head_dim,
+                                         int64_t capacity) {
+  if (rows <= 0 || rows > (1 << 23) || seqs <= 0 || seqs > (1 << 20) || heads <= 0 || heads > 4096 || q_heads <= 0 ||
+      q_heads > 4096 || q_heads % heads || head_dim <= 0 || head_dim > 128 || capacity <= 0)
+    return 0;
+  return paged_attn_s4_workspace_bytes(rows, seqs, q_heads, heads, head_dim, capacity);
+}
+
+int64_t ti_paged_attn_s4_arrivals(int64_t rows, int64_t seqs, int64_t q_heads, int64_t heads, int64_t head_dim, int64_t capacity) {
+  if (ti_paged_attn_s4_workspace_bytes(rows, seqs, q_heads, heads, head_dim, capacity) == 0) return 0;
+  return paged_attn_s4_arrivals(rows, seqs, q_heads, heads, capacity);
+}
+
+int ti_paged_attn_s4(const TiPagedCacheS4* cache, const TiPagedBatch* batch, const TiPagedAttnS4* w, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  const char* op = "paged_attn_s4";
+  PagedCache4 c;
+  PagedBatch b;
+  if (int rc = paged_s4_args(op, cache, batch, &c, &b)) return rc;
+  if (w == nullptr) return fail(TI_ERR_INVALID_ARG, "%s: query and output must be given", op);
+  if (w->q_type != TI_TYPE_S8 && w->q_type != TI_TYPE_F16 && w->q_type != TI_TYPE_BF16)
+    return fail(TI_ERR_INVALID_ARG, "%s: query type %d (int8, fp16 and bf16 are there)", op, (int)w->q_type);
+  if (w->out_type != TI_TYPE_S8 && w->out_type != TI_TYPE_F16 && w->out_type != TI_TYPE_BF16)
+    return fail(TI_ERR_INVALID_ARG, "%s: output type %d (int8, fp16 and bf16 are there)", op, (int)w->out_type);
+  if (w->q_heads < 1 || w->q_heads > 4096 || w->q_heads % c.heads)
+    return fail(TI_ERR_INVALID_ARG, "%s: %lld query heads over %d key heads (a multiple up to 4096 is needed)", op,
+                (long long)w->q_heads, c.heads);
+  if (!(w->alpha_qk >= 1e-30f && w->alpha_qk <= 1e4f))
+    return fail(TI_ERR_INVALID_ARG, "%s: alpha_qk = %g (1e-30 to 1e4 is taken)", op, (double)w->alpha_qk);
+  if (w->window < 0 || w->window > (1 << 28) || w->sinks < 0 || w->sinks > (1 << 28) || (w->sinks > 0 && w->window == 0))
+    return fail(TI_ERR_INVALID_ARG, "%s: a window of %lld keys (0 for all, at most 2^28) beside %lld first ones (0 without a window)",
+                op, (long long)w->window, (long long)w->sinks);
+  if (workspace_bytes < 0) return fail(TI_ERR_INVALID_ARG, "%s: negative workspace size", op);
+  if (b.rows == 0) return TI_OK;
+  if (int rc = check_rows(op, "q", w->q, w->q_row, w->q_head, w->q_type == TI_TYPE_S8 ? 1 : 2)) return rc;
+  if (int rc = check_ptr(op, "out", w->out, 16, true)) return rc;
+  if (int rc = check_ptr(op, "workspace", workspace, 16, workspace != nullptr)) return rc;
+  if (int rc = check_ptr(op, "arrivals", w->arrivals, 4, w->arrivals != nullptr)) return rc;
+  if (b.rows * (w->q_heads / c.heads) > (1 << 30))
+    return fail(TI_ERR_INVALID_ARG, "%s: %d rows of %lld heads to a key head (at most 2^30 in all)", op, b.rows,
+                (long long)(w->q_heads / c.heads));
+  if (c.pages == 0) b.per_seq = 0;  // no page to read, not even in the place of one that is missing: no sequence has a key
+  PagedAttn4 a;
+  a.q = w->q, a.q_row = w->q_row, a.q_head = w->q_head, a.q_heads = (int)w->q_heads, a.q_type = w->q_type, a.out = w->out;
+  a.alpha_qk = w->alpha_qk, a.alpha_pv = w->alpha_pv, a.fill = w->fill != 0;
+  a.window = (int)w->window, a.sinks = (int)w->sinks;
+  a.arrivals = w->arrivals, a.arrivals_count = w->arrivals_count;
+  return launch_paged_attn_s4(w->out_type, a, c, b, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -361,6 +361,87 @@ static PyObject* fc_paged_attn(PyObject* self, PyObject* const* a, Py_ssize_t n)
   return PyLong_FromLong(ti_paged_attn_s8(&c, &b, &w, ws, wsb, st));
 }
 
+/* The 4-bit cache and the batch: k, v, k_scale, v_scale, pages, page_size, heads, head_dim, groups, k strides (page, head, token),
+ * v strides, k_scale strides (page, head), v_scale strides, then the batch as above */
+enum { PAGED_S4_ARGS = 25 };
+static void paged_s4_args(PyObject* const* a, TiPagedCacheS4* c, TiPagedBatch* b) {
+  c->k = as_ptr(a[0]), c->v = as_ptr(a[1]), c->k_scale = as_ptr(a[2]), c->v_scale = as_ptr(a[3]);
+  c->pages = as_i64(a[4]), c->page_size = as_i64(a[5]), c->heads = as_i64(a[6]), c->head_dim = as_i64(a[7]), c->groups = as_i64(a[8]);
+  c->k_page = as_i64(a[9]), c->k_head = as_i64(a[10]), c->k_token = as_i64(a[11]);
+  c->v_page = as_i64(a[12]), c->v_head = as_i64(a[13]), c->v_token = as_i64(a[14]);
+  c->k_scale_page = as_i64(a[15]), c->k_scale_head = as_i64(a[16]), c->v_scale_page = as_i64(a[17]), c->v_scale_head = as_i64(a[18]);
+  b->block_table = as_ptr(a[19]), b->context_lens = as_ptr(a[20]), b->cu_new = as_ptr(a[21]);
+  b->pages_per_seq = as_i64(a[22]), b->seqs = as_i64(a[23]), b->rows = as_i64(a[24]);
+}
+
+/* paged_append_s4(..., key, value, query, k_row, k_head, v_row, v_head, q_row, q_head, q_out, q_heads, cos_sin, rot, positions, type,
+ * q_type, neighbours, fill, alpha_q, alpha_k, alpha_v, stream) -> status */
+static PyObject* fc_paged_append_s4(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (n != PAGED_S4_ARGS + 22) {
+    PyErr_SetString(PyExc_TypeError, "paged_append_s4 expects 47 arguments");
+    return NULL;
+  }
+  TiPagedCacheS4 c;
+  TiPagedBatch b;
+  TiPagedAppendS4 w;
+  paged_s4_args(a, &c, &b);
+  a += PAGED_S4_ARGS;
+  w.key = as_ptr(a[0]), w.value = as_ptr(a[1]), w.query = as_ptr(a[2]);
+  w.k_row = as_i64(a[3]), w.k_head = as_i64(a[4]), w.v_row = as_i64(a[5]), w.v_head = as_i64(a[6]);
+  w.q_row = as_i64(a[7]), w.q_head = as_i64(a[8]);
+  w.q_out = as_ptr(a[9]), w.q_heads = as_i64(a[10]), w.cos_sin = as_ptr(a[11]), w.rot = as_i64(a[12]), w.positions = as_i64(a[13]);
+  w.type = (int32_t)as_i64(a[14]), w.q_type = (int32_t)as_i64(a[15]);
+  w.neighbours = (int32_t)as_i64(a[16]), w.fill = (int32_t)as_i64(a[17]);
+  w.alpha_q = as_f32(a[18]), w.alpha_k = as_f32(a[19]), w.alpha_v = as_f32(a[20]);
+  void* st = as_ptr(a[21]);
+  if (PyErr_Occurred()) return NULL;
+  return PyLong_FromLong(ti_paged_kv_append_s4(&c, &b, &w, st));
+}
+
+/* paged_read_s4(..., key, value, type, fill, alpha_k, alpha_v, stream) -> status */
+static PyObject* fc_paged_read_s4(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (n != PAGED_S4_ARGS + 7) {
+    PyErr_SetString(PyExc_TypeError, "paged_read_s4 expects 32 arguments");
+    return NULL;
+  }
+  TiPagedCacheS4 c;
+  TiPagedBatch b;
+  TiPagedReadS4 w;
+  paged_s4_args(a, &c, &b);
+  a += PAGED_S4_ARGS;
+  w.key = as_ptr(a[0]), w.value = as_ptr(a[1]), w.type = (int32_t)as_i64(a[2]), w.fill = (int32_t)as_i64(a[3]);
+  w.alpha_k = as_f32(a[4]), w.alpha_v = as_f32(a[5]);
+  void* st = as_ptr(a[6]);
+  if (PyErr_Occurred()) return NULL;
+  return PyLong_FromLong(ti_paged_kv_read_s4(&c, &b, &w, st));
+}
+
+/* paged_attn_s4(..., q, q_row, q_head, q_heads, out, q_type, out_type, fill, alpha_qk, alpha_pv, window, sinks, arrivals,
+ * arrivals_count, ws, ws_bytes, stream) -> status */
+static PyObject* fc_paged_attn_s4(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (n != PAGED_S4_ARGS + 17) {
+    PyErr_SetString(PyExc_TypeError, "paged_attn_s4 expects 42 arguments");
+    return NULL;
+  }
+  TiPagedCacheS4 c;
+  TiPagedBatch b;
+  TiPagedAttnS4 w;
+  paged_s4_args(a, &c, &b);
+  a += PAGED_S4_ARGS;
+  w.q = as_ptr(a[0]), w.q_row = as_i64(a[1]), w.q_head = as_i64(a[2]), w.q_heads = as_i64(a[3]);
+  w.out = as_ptr(a[4]), w.q_type = (int32_t)as_i64(a[5]), w.out_type = (int32_t)as_i64(a[6]), w.fill = (int32_t)as_i64(a[7]);
+  w.alpha_qk = as_f32(a[8]), w.alpha_pv = as_f32(a[9]), w.window = as_i64(a[10]), w.sinks = as_i64(a[11]);
+  w.arrivals = as_ptr(a[12]), w.arrivals_count = as_i64(a[13]);
+  void* ws = as_ptr(a[14]);
+  int64_t wsb = as_i64(a[15]);
+  void* st = as_ptr(a[16]);
+  if (PyErr_Occurred()) return NULL;
+  return PyLong_FromLong(ti_paged_attn_s4(&c, &b, &w, ws, wsb, st));
+}
+
 static PyObject* fc_last_error(PyObject* self, PyObject* noargs) {
   (void)self;
   (void)noargs;
@@ -382,6 +463,9 @@ static PyMethodDef methods[] = {
     {"opt_layer_prefill", (PyCFunction)(void (*)(void))fc_opt_layer_prefill, METH_FASTCALL, "forward to ti_opt_decoder_layer_prefill_chained"},
     {"paged_append", (PyCFunction)(void (*)(void))fc_paged_append, METH_FASTCALL, "forward to ti_paged_kv_append_s8"},
     {"paged_attn", (PyCFunction)(void (*)(void))fc_paged_attn, METH_FASTCALL, "forward to ti_paged_attn_s8"},
+    {"paged_append_s4", (PyCFunction)(void (*)(void))fc_paged_append_s4, METH_FASTCALL, "forward to ti_paged_kv_append_s4"},
+    {"paged_read_s4", (PyCFunction)(void (*)(void))fc_paged_read_s4, METH_FASTCALL, "forward to ti_paged_kv_read_s4"},
+    {"paged_attn_s4", (PyCFunction)(void (*)(void))fc_paged_attn_s4, METH_FASTCALL, "forward to ti_paged_attn_s4"},
     {"plan_current", (PyCFunction)(void (*)(void))fc_plan_current, METH_FASTCALL, "tensors and hooks as a plan found them"},
     {"last_error", fc_last_error, METH_NOARGS, "ti_last_error()"},
     {NULL, NULL, 0, NULL}};

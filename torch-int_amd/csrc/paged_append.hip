@@ -5,51 +5,9 @@
 // The bytes are those of a plain fp64 chain of the formula (products of two fp32 values are exact there, so they depend on no
 // order of operations), but the work is fp32, at twice the rate and without conversions: a result that lies too near a border
 // between two bytes to be told from fp32 is done again in fp64 (of normal keys at scales of 1/32 about one piece in 500).
-#include <hip/hip_fp16.h>
-#include "paged.h"
+#include "paged_io.h"
 
 namespace ti {
-
-template <typename T>
-__device__ __forceinline__ float as_float(T x) { return (float)x; }
-struct bf16_bits { unsigned short u; };
-template <>
-__device__ __forceinline__ float as_float<bf16_bits>(bf16_bits x) { return __uint_as_float((unsigned)x.u << 16); }
-
-// Eight neighbouring elements as they lie in memory, and their values.
-template <typename T>
-struct Raw8 {
-  T x[8];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (sizeof(T) == 4) {
-      reinterpret_cast<v4i*>(x)[0] = reinterpret_cast<const v4i*>(p)[0];
-      reinterpret_cast<v4i*>(x)[1] = reinterpret_cast<const v4i*>(p)[1];
-    } else if constexpr (sizeof(T) == 2) {
-      reinterpret_cast<v4i*>(x)[0] = reinterpret_cast<const v4i*>(p)[0];
-    } else {
-      reinterpret_cast<int2*>(x)[0] = reinterpret_cast<const int2*>(p)[0];
-    }
-  }
-  __device__ __forceinline__ float operator[](int i) const { return as_float(x[i]); }
-};
-
-// s8 of a value in fp64: NaN becomes 0
-__device__ __forceinline__ int s8_of(double y) {
-  y = __builtin_rint(y);
-  y = y < -128.0 ? -128.0 : y > 127.0 ? 127.0 : y;
-  return y == y ? (int)y : 0;
-}
-
-// 1.5 * 2^23: a number added to it in one FMA is rounded, half to even, to a whole one, which the low bits then are.
-constexpr float WHOLE = 12582912.0f;
-// the low byte of what this returns is the s8 of n - WHOLE, for any n but NaN
-__device__ __forceinline__ int byte_of(float n) { return __float_as_int(__builtin_amdgcn_fmed3f(n, WHOLE - 128.0f, WHOLE + 127.0f)); }
-
-// s8(rint(x alpha)) in the low byte, the product unrounded; NaN becomes 0
-__device__ __forceinline__ int s8_of_product(float x, float alpha) {
-  const float n = __builtin_fmaf(x, alpha, WHOLE);
-  return n == n ? byte_of(n) : 0;
-}
 
 // s8(rint((p c + q s) alpha)) in the low byte, in fp32.  The two roundings, and the bound's own, are off by less than
 // 2^-22 (|p c| + |q s|) alpha together, the fp64 chain by 2^-51 of it; `far` keeps the bits of the largest |y - rint y| + twice
@@ -61,14 +19,6 @@ __device__ __forceinline__ int s8_of_turned(float p, float c, float q, float s, 
   const unsigned bits = __float_as_uint(__builtin_fabsf(__builtin_fmaf(w, bound, __builtin_fabsf(d))));
   far = far > bits ? far : bits;
   return byte_of(n);
-}
-
-// the low bytes of eight
-__device__ __forceinline__ int2 pack8(const int (&o)[8]) {
-  auto four = [](int x, int y, int z, int w) {
-    return (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(w, z, 0x0c0c0400), __builtin_amdgcn_perm(y, x, 0x0c0c0400), 0x05040100);
-  };
-  return make_int2(four(o[0], o[1], o[2], o[3]), four(o[4], o[5], o[6], o[7]));
 }
 
 // One row to blockIdx.x; the threads of a block are the 16-element pieces of some heads, the keys', then the values', then the
@@ -94,8 +44,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend a, PagedC
   const int d0 = apart ? piece * 8 : piece * 16, d1 = apart ? rot / 2 + piece * 8 : piece * 16 + 8;
   // the row's sequence: how many of them end at or before it (all lanes of the wave take part); the first 64 ends are asked for in
   // front of the row's elements, which are on their way while its place is looked up
-  const int lane = threadIdx.x & 63;
-  int end = b.cu[lane < b.seqs ? lane + 1 : b.seqs];
+  const int end = paged_ends(b);
   const T* const key = static_cast<const T*>(a.key) + row * a.k_row;
   const T* const value = static_cast<const T*>(a.value) + row * a.v_row;
   const T* const query = static_cast<const T*>(a.query) + row * a.q_row;
@@ -103,24 +52,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend a, PagedC
   Raw8<T> x0, x1;
   x0.load(src + d0);
   x1.load(src + d1);
-  int seq = 0;
-  for (int i0 = 0; i0 < b.seqs; i0 += 64) {
-    const int i = i0 + lane;
-    if (i0 > 0) end = b.cu[i < b.seqs ? i + 1 : b.seqs];
-    const unsigned long long ended = __ballot(i < b.seqs && end <= row);
-    seq += __popcll(ended);
-    if (ended != ~0ull) break;
-  }
-  seq = __builtin_amdgcn_readfirstlane(seq);
+  const int seq = paged_seq_of(b, row, end);
   if (!real) return;
-  int position = -1;
-  bool mine = false;
-  if (seq < b.seqs) {
-    const PagedSeq s = paged_seq(b, c.page_shift, seq);
-    mine = row >= s.row0 && row < s.row0 + s.T;
-    if (mine) position = s.end - s.T + (row - s.row0);
-    if (position >= s.len) position = -1;  // no page for it
-  }
+  const PagedPlace place = paged_place(b, c.page_shift, row, seq);
+  const int position = place.position;
+  const bool mine = place.mine;
   const bool live = position >= 0 && (a.cos_sin == nullptr || position < a.positions);
   int8_t* dst = nullptr;
   if (which == 2) {

@@ -1,1 +1,1 @@
-from . import bmm, fused, paged, quantization  # noqa: F401
+from . import bmm, fused, paged, paged_s4, quantization  # noqa: F401

@@ -5,3 +5,4 @@ from .linear import (W8A8B8O8Linear, W8A8B8O8LinearReLU, W8A8B32O32Linear,  # no
                      W8A8B32O32LinearWithoutScaling, W8A8BFP32OFP32Linear)
 from .linear import W8A16Linear, W8FakeA8Linear  # noqa: F401  (upstream torch_int/nn/__init__.py exports these two)
 from .paged import PagedAttn_S8, PagedKVAppend_S8  # noqa: F401
+from .paged import PagedAttn_S4, PagedKVAppend_S4, PagedKVRead_S4  # noqa: F401
