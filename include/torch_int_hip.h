@@ -672,16 +672,15 @@ int ti_paged_attn_s8(const TiPagedCache* cache, const TiPagedBatch* batch, const
  * `groups` groups, one for the whole head or one for each half of its columns.  Byte j of k and v (0 <= j < head_dim / 2) holds
  * the code of column j in its low four bits and that of column head_dim / 2 + j in the others.  A group's 16-bit word holds s in
  * its bits 4 to 14, where an fp16 number has them (its other bits 0: 7 significant bits, multiples of 2^-20), and z, 0 to 15, in
- * the low four.  Codes: strides in bytes, multiples of 8 that do not overlap, any order of pages, heads and positions.  Words:
- * [pages, heads, page_size, groups], the last two dimensions packed, the other strides in bytes, multiples of 16.  All four
- * pointers are 16-byte aligned. */
+ * the low four.  Codes: strides in bytes, the same for k and v, multiples of 8 that do not overlap, any order of pages, heads and
+ * positions.  Words: [pages, heads, page_size, groups], the last two dimensions packed, the other strides in bytes, the same for
+ * both, multiples of 16.  All four pointers are 16-byte aligned. */
 typedef struct {
   uint8_t *k, *v;
   uint16_t *k_scale, *v_scale;
   int64_t pages, page_size, heads, head_dim, groups;
-  int64_t k_page, k_head, k_token;
-  int64_t v_page, v_head, v_token;
-  int64_t k_scale_page, k_scale_head, v_scale_page, v_scale_head;
+  int64_t page, head, token;        /* of k and of v */
+  int64_t scale_page, scale_head;   /* of k_scale and of v_scale */
 } TiPagedCacheS4;
 
 /* Appends the new tokens' keys and values as ti_paged_kv_append_s8 does (batch, types, strides, rotation and what is left out are the

@@ -14,7 +14,7 @@ def _lib():
 def _good():
     """C structures that are right but for their pointers, which nothing reads: there are no rows to work on."""
     P, _ = _lib()
-    c = P._Cache(4096, 8192, 16384, 32768, 8, 16, 2, 64, 2, 2 * 16 * 32, 16 * 32, 32, 2 * 16 * 32, 16 * 32, 32, 128, 64, 128, 64)
+    c = P._Cache(4096, 8192, 16384, 32768, 8, 16, 2, 64, 2, 2 * 16 * 32, 16 * 32, 32, 128, 64)
     b = P._Batch(4096, 4096, 4096, 4, 2, 2)
     return c, b
 
@@ -44,10 +44,10 @@ def _refused(c, b, word):
     ("head_dim", 72, b"head size 72"), ("head_dim", 144, b"head size 144"), ("head_dim", 16, b"head size 16"), ("groups", 0, b"0 groups"),
     ("groups", 4, b"4 groups"), ("heads", 0, b"0 heads"), ("heads", 5000, b"5000 heads"), ("pages", -1, b"pages"),
     ("k", 4097, b"k_cache is not aligned"), ("k", None, b"k_cache is NULL"), ("v", 8, b"v_cache is not aligned"),
-    ("k_scale", None, b"k_scale is NULL"), ("v_scale", 4104, b"v_scale is not aligned"), ("k_token", 16, b"step over"),
-    ("k_token", 36, b"multiples of 8"), ("v_head", 0, b"step over"), ("v_head", 64, b"overlap"), ("k_page", 512, b"overlap"),
-    ("v_page", -2048, b"step over"), ("k_scale_head", 32, b"step over"), ("k_scale_page", 64, b"overlap"),
-    ("v_scale_head", 72, b"multiples of 16"), ("v_scale_page", 0, b"step over")])
+    ("k_scale", None, b"k_scale is NULL"), ("v_scale", 4104, b"v_scale is not aligned"), ("token", 16, b"step over"),
+    ("token", 36, b"multiples of 8"), ("head", 0, b"step over"), ("head", 64, b"overlap"), ("page", 512, b"overlap"),
+    ("page", -2048, b"step over"), ("scale_head", 32, b"step over"), ("scale_page", 64, b"overlap"),
+    ("scale_head", 72, b"multiples of 16"), ("scale_page", 0, b"step over")])
 def test_pools_that_are_refused(field, value, word):
     c, b = _good()
     setattr(c, field, value)
@@ -117,7 +117,7 @@ def test_workspace_is_for_sequences_that_are_cut_and_does_not_grow_with_the_batc
     assert need(0, 0, 12, 12, 64, 4096) == 0 and need(4, 4, 12, 5, 64, 4096) == 0
     assert 0 < need(1, 1, 12, 12, 64, 4096) < need(64, 64, 32, 32, 128, 4096) < 2 ** 28
     for rows, seqs, q_heads, heads in ((64, 64, 32, 32), (4096, 4096, 64, 8), (600, 64, 8, 2), (1 << 20, 4000, 8, 1), (100000, 1, 4, 1)):
-        assert need(rows, seqs, q_heads, heads, 128, 1 << 16) <= 1032 * 128 * 130 * 4 and counters(rows, seqs, q_heads, heads, 128, 1 << 16) <= 1032
+        assert need(rows, seqs, q_heads, heads, 128, 1 << 16) <= 2 ** 27 and counters(rows, seqs, q_heads, heads, 128, 1 << 16) <= 2048
 
 
 def test_python_refuses_before_any_launch():
@@ -134,9 +134,13 @@ def test_python_refuses_before_any_launch():
                             ("block_table", t[:, ::2], "contiguous"), ("k_cache", k.transpose(2, 3), "v_cache is|contiguous"),
                             ("context_lens", n[0], "1-D"), ("k_cache", None, "NoneType"), ("k_cache", k.view(torch.int8), "4-D torch.uint8"),
                             ("k_scale", ks.view(torch.float16), "4-D torch.int16"), ("k_scale", ks[:, :, :8], "beside caches"),
-                            ("v_scale", vs[..., :1], "beside caches"), ("v_scale", vs.transpose(2, 3).contiguous().transpose(2, 3), "packed")):
+                            ("v_scale", vs[..., :1], "beside caches"), ("v_scale", vs.transpose(2, 3).contiguous().transpose(2, 3), "the same"),
+                            ("v_cache", v.transpose(1, 2).contiguous().transpose(1, 2), "the same")):
         with pytest.raises(RuntimeError, match=word):
             P._cache_and_batch("x", rows=1, **{m: _Fake(x) if x is not None else None for m, x in {**f, name: bad}.items()})
+    apart = [x.transpose(2, 3).contiguous().transpose(2, 3) for x in (ks, vs)]
+    with pytest.raises(RuntimeError, match="packed"):
+        P._cache_and_batch("x", rows=1, **{m: _Fake(x) for m, x in {**f, "k_scale": apart[0], "v_scale": apart[1]}.items()})
     with pytest.raises(RuntimeError, match="query must be a 3-D"):
         P.paged_attn_s4(q[0], k, v, ks, vs, t, n, cu, 1e-3)
     with pytest.raises(RuntimeError, match="query must be a 3-D"):

@@ -1226,15 +1226,14 @@ int paged_s4_args(const char* op, const TiPagedCacheS4* c, const TiPagedBatch* b
   if (int rc = check_pages(op, c->page_size, c->heads, c->pages)) return rc;
   if (int rc = check_batch(op, b, c->page_size)) return rc;
   const PoolShape codes = {c->pages, c->heads, c->page_size, c->head_dim / 2, 8};
-  if (int rc = check_pool(op, "k_cache", c->k, codes, c->k_page, c->k_head, c->k_token)) return rc;
-  if (int rc = check_pool(op, "v_cache", c->v, codes, c->v_page, c->v_head, c->v_token)) return rc;
+  if (int rc = check_pool(op, "k_cache", c->k, codes, c->page, c->head, c->token)) return rc;
+  if (int rc = check_ptr(op, "v_cache", c->v, 16, c->pages > 0)) return rc;
   const PoolShape words = {c->pages, c->heads, 1, c->page_size * c->groups * 2, 16};
-  if (int rc = check_pool(op, "k_scale", c->k_scale, words, c->k_scale_page, c->k_scale_head, 0)) return rc;
-  if (int rc = check_pool(op, "v_scale", c->v_scale, words, c->v_scale_page, c->v_scale_head, 0)) return rc;
+  if (int rc = check_pool(op, "k_scale", c->k_scale, words, c->scale_page, c->scale_head, 0)) return rc;
+  if (int rc = check_ptr(op, "v_scale", c->v_scale, 16, c->pages > 0)) return rc;
   if (int rc = check_batch_ptrs(op, b)) return rc;
-  *cache = ti::PagedCache4{c->k, c->v, c->k_scale, c->v_scale, c->k_page, c->k_head, c->v_page, c->v_head, c->k_scale_page,
-                           c->k_scale_head, c->v_scale_page, c->v_scale_head, (int)c->k_token, (int)c->v_token, (int)c->pages,
-                           page_shift_of(c->page_size), (int)c->heads, (int)c->head_dim, (int)c->groups};
+  *cache = ti::PagedCache4{c->k, c->v, c->k_scale, c->v_scale, c->page, c->head, c->scale_page, c->scale_head, (int)c->token,
+                           (int)c->pages, page_shift_of(c->page_size), (int)c->heads, (int)c->head_dim, (int)c->groups};
   *batch = batch_of(b);
   return TI_OK;
 }

@@ -361,17 +361,16 @@ static PyObject* fc_paged_attn(PyObject* self, PyObject* const* a, Py_ssize_t n)
   return PyLong_FromLong(ti_paged_attn_s8(&c, &b, &w, ws, wsb, st));
 }
 
-/* The 4-bit cache and the batch: k, v, k_scale, v_scale, pages, page_size, heads, head_dim, groups, k strides (page, head, token),
- * v strides, k_scale strides (page, head), v_scale strides, then the batch as above */
-enum { PAGED_S4_ARGS = 25 };
+/* The 4-bit cache and the batch: k, v, k_scale, v_scale, pages, page_size, heads, head_dim, groups, strides of the codes (page, head,
+ * token) and of the words (page, head), then the batch as above */
+enum { PAGED_S4_ARGS = 20 };
 static void paged_s4_args(PyObject* const* a, TiPagedCacheS4* c, TiPagedBatch* b) {
   c->k = as_ptr(a[0]), c->v = as_ptr(a[1]), c->k_scale = as_ptr(a[2]), c->v_scale = as_ptr(a[3]);
   c->pages = as_i64(a[4]), c->page_size = as_i64(a[5]), c->heads = as_i64(a[6]), c->head_dim = as_i64(a[7]), c->groups = as_i64(a[8]);
-  c->k_page = as_i64(a[9]), c->k_head = as_i64(a[10]), c->k_token = as_i64(a[11]);
-  c->v_page = as_i64(a[12]), c->v_head = as_i64(a[13]), c->v_token = as_i64(a[14]);
-  c->k_scale_page = as_i64(a[15]), c->k_scale_head = as_i64(a[16]), c->v_scale_page = as_i64(a[17]), c->v_scale_head = as_i64(a[18]);
-  b->block_table = as_ptr(a[19]), b->context_lens = as_ptr(a[20]), b->cu_new = as_ptr(a[21]);
-  b->pages_per_seq = as_i64(a[22]), b->seqs = as_i64(a[23]), b->rows = as_i64(a[24]);
+  c->page = as_i64(a[9]), c->head = as_i64(a[10]), c->token = as_i64(a[11]);
+  c->scale_page = as_i64(a[12]), c->scale_head = as_i64(a[13]);
+  b->block_table = as_ptr(a[14]), b->context_lens = as_ptr(a[15]), b->cu_new = as_ptr(a[16]);
+  b->pages_per_seq = as_i64(a[17]), b->seqs = as_i64(a[18]), b->rows = as_i64(a[19]);
 }
 
 /* paged_append_s4(..., key, value, query, k_row, k_head, v_row, v_head, q_row, q_head, q_out, q_heads, cos_sin, rot, positions, type,
@@ -379,7 +378,7 @@ static void paged_s4_args(PyObject* const* a, TiPagedCacheS4* c, TiPagedBatch* b
 static PyObject* fc_paged_append_s4(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   (void)self;
   if (n != PAGED_S4_ARGS + 22) {
-    PyErr_SetString(PyExc_TypeError, "paged_append_s4 expects 47 arguments");
+    PyErr_SetString(PyExc_TypeError, "paged_append_s4 expects 42 arguments");
     return NULL;
   }
   TiPagedCacheS4 c;
@@ -403,7 +402,7 @@ static PyObject* fc_paged_append_s4(PyObject* self, PyObject* const* a, Py_ssize
 static PyObject* fc_paged_read_s4(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   (void)self;
   if (n != PAGED_S4_ARGS + 7) {
-    PyErr_SetString(PyExc_TypeError, "paged_read_s4 expects 32 arguments");
+    PyErr_SetString(PyExc_TypeError, "paged_read_s4 expects 27 arguments");
     return NULL;
   }
   TiPagedCacheS4 c;
@@ -423,7 +422,7 @@ static PyObject* fc_paged_read_s4(PyObject* self, PyObject* const* a, Py_ssize_t
 static PyObject* fc_paged_attn_s4(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   (void)self;
   if (n != PAGED_S4_ARGS + 17) {
-    PyErr_SetString(PyExc_TypeError, "paged_attn_s4 expects 42 arguments");
+    PyErr_SetString(PyExc_TypeError, "paged_attn_s4 expects 37 arguments");
     return NULL;
   }
   TiPagedCacheS4 c;

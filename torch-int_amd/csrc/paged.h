@@ -80,9 +80,8 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
 struct PagedCache4 {
   uint8_t *k, *v;
   uint16_t *k_scale, *v_scale;               // [pages, heads, page, groups], the last two packed
-  long long k_page, k_head, v_page, v_head;  // bytes from page to page and from head to head
-  long long ks_page, ks_head, vs_page, vs_head;
-  int k_token, v_token;   // bytes from position to position inside a page
+  long long page, head, scale_page, scale_head;  // bytes from page to page and from head to head, of codes and of words
+  int token;              // bytes from position to position inside a page
   int pages, page_shift;  // pages in the pool; log2 of the positions of a page (4 or more)
   int heads, D, groups;   // key/value heads, head size (a multiple of 16 from 32 to 128), words of a row (1 or 2)
 };

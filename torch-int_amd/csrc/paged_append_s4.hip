@@ -186,12 +186,10 @@ __global__ __launch_bounds__(256) void paged_append_s4_kernel(PagedAppend4 a, Pa
   int w[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = first.code(y[0][i]) | second.code(y[1][i]) << 4;
-  uint8_t* const dst = which == 0 ? c.k + (long long)page * c.k_page + h * c.k_head + (long long)off * c.k_token
-                                  : c.v + (long long)page * c.v_page + h * c.v_head + (long long)off * c.v_token;
+  uint8_t* const dst = (which == 0 ? c.k : c.v) + (long long)page * c.page + h * c.head + (long long)off * c.token;
   *reinterpret_cast<int2*>(dst + at) = pack8(w);
   if (lane == 0) {
-    char* const scale = which == 0 ? reinterpret_cast<char*>(c.k_scale) + (long long)page * c.ks_page + h * c.ks_head
-                                   : reinterpret_cast<char*>(c.v_scale) + (long long)page * c.vs_page + h * c.vs_head;
+    char* const scale = reinterpret_cast<char*>(which == 0 ? c.k_scale : c.v_scale) + (long long)page * c.scale_page + h * c.scale_head;
     if (c.groups == 1) reinterpret_cast<uint16_t*>(scale)[off] = (uint16_t)first.word;
     else reinterpret_cast<unsigned*>(scale)[off] = (unsigned)(first.word | second.word << 16);
   }
@@ -212,10 +210,8 @@ __global__ __launch_bounds__(256) void paged_read_s4_kernel(PagedRead4 a, PagedC
   float y[2][8] = {};
   if (page >= 0 && page < c.pages) {
     const int off = place.position & ((1 << c.page_shift) - 1);
-    const uint8_t* src = keys ? c.k + (long long)page * c.k_page + h * c.k_head + (long long)off * c.k_token
-                              : c.v + (long long)page * c.v_page + h * c.v_head + (long long)off * c.v_token;
-    const char* scale = keys ? reinterpret_cast<const char*>(c.k_scale) + (long long)page * c.ks_page + h * c.ks_head
-                             : reinterpret_cast<const char*>(c.v_scale) + (long long)page * c.vs_page + h * c.vs_head;
+    const uint8_t* src = (keys ? c.k : c.v) + (long long)page * c.page + h * c.head + (long long)off * c.token;
+    const char* scale = reinterpret_cast<const char*>(keys ? c.k_scale : c.v_scale) + (long long)page * c.scale_page + h * c.scale_head;
     const int2 codes = *reinterpret_cast<const int2*>(src + at);
     const unsigned words = c.groups == 1 ? reinterpret_cast<const uint16_t*>(scale)[off] * 0x10001u : reinterpret_cast<const unsigned*>(scale)[off];
 #pragma unroll

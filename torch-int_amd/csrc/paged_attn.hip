@@ -809,6 +809,8 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
   PagedPlan rows, tiles;
   rows.group = tiles.group = group;
   rows.span = tiles.span = 0x7fffffff;
+  rows.full = tiles.full = PA_FULL;
+  rows.even = tiles.even = false;
   rows.least = 0;
   rows.most = s.tiles_slots > 0 ? PA_ROWS : 0x7fffffff;
   rows.slots = (int)s.rows_slots;

@@ -10,23 +10,29 @@
 
 namespace ti {
 
-typedef int v4i_8 __attribute__((ext_vector_type(4), aligned(8)));  // 16 bytes at a multiple of 8
-
 // A nibble in the low bits of a 16-bit half, or in the next four, is a number of fp16 with one bit operation: 0x6400 + u is 1024 + u,
 // 0x5400 + 16 u is 64 + u.  Less the same with z, times the step: exact.  `c` has two bytes in each half (of two columns, or of two
 // keys); the four results are the low byte's nibbles, then the high byte's.
+struct S4Bits {
+  unsigned low_mask, high_mask, low_one, high_one;
+  // masks in scalar registers, exponents in vector ones: one v_and_or_b32, which takes no constants of 32 bits, is enough then
+  __device__ __forceinline__ S4Bits() : low_mask(0x000f000fu), high_mask(0x00f000f0u), low_one(0x64006400u), high_one(0x54005400u) {
+    asm("" : "+s"(low_mask), "+s"(high_mask), "+v"(low_one), "+v"(high_one));
+  }
+  __device__ __forceinline__ unsigned low(unsigned c) const { return (c & low_mask) | low_one; }
+  __device__ __forceinline__ unsigned high(unsigned c) const { return (c & high_mask) | high_one; }
+};
 struct S4Two {
   v2h step[2], base[2];  // of low nibbles and of high ones: the step, and 1024 + z or 64 + z
-  __device__ __forceinline__ void set(int nibble, unsigned word) {  // `word`: a word in each half
-    const unsigned s = word & 0x7ff07ff0u, z = (word & 0x000f000fu) | 0x64006400u;
+  __device__ __forceinline__ void set(const S4Bits& b, int nibble, unsigned word) {  // `word`: a word in each half
+    const unsigned s = word & 0x7ff07ff0u, z = b.low(word);
     step[nibble] = __builtin_bit_cast(v2h, s);
     base[nibble] = __builtin_bit_cast(v2h, z);
     if (nibble) base[nibble] -= v2h{(_Float16)960.0f, (_Float16)960.0f};
   }
-  __device__ __forceinline__ void values(unsigned c, v2h (&y)[4]) const {
+  __device__ __forceinline__ void values(const S4Bits& b, unsigned c, v2h (&y)[4]) const {
     const unsigned d = c >> 8;
-    const unsigned w[4] = {(c & 0x000f000fu) | 0x64006400u, (c & 0x00f000f0u) | 0x54005400u, (d & 0x000f000fu) | 0x64006400u,
-                           (d & 0x00f000f0u) | 0x54005400u};
+    const unsigned w[4] = {b.low(c), b.high(c), b.low(d), b.high(d)};
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = (__builtin_bit_cast(v2h, w[i]) - base[i & 1]) * step[i & 1];
   }
@@ -36,11 +42,30 @@ __device__ __forceinline__ v8h join8(v2h a, v2h b, v2h c, v2h d) {
   return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// One element of a query as fp16.
-__device__ __forceinline__ _Float16 query_at(const void* q, int type, long long i) {
-  if (type == PT_S8) return (_Float16)(float)static_cast<const int8_t*>(q)[i];
-  if (type == PT_F16) return static_cast<const _Float16*>(q)[i];
-  return (_Float16)__uint_as_float((unsigned)static_cast<const uint16_t*>(q)[i] << 16);
+// Eight neighbouring elements of a query as fp16, in the order 0 2 1 3 4 6 5 7 in which the nibbles of two dwords come apart.
+__device__ __forceinline__ v8h query8(const void* q, int type, long long at) {
+  unsigned w[4];
+  if (type == PT_S8) {
+    const int2 x = *reinterpret_cast<const int2*>(static_cast<const int8_t*>(q) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // bytes plus 128 are the low bits of 1024 + them
+      const unsigned u = ((unsigned)(i < 2 ? x.x : x.y) ^ 0x80808080u) >> (8 * (i & 1)) & 0x00ff00ffu;
+      const v2h y = __builtin_bit_cast(v2h, u | 0x64006400u) - v2h{(_Float16)1152.0f, (_Float16)1152.0f};
+      w[i] = __builtin_bit_cast(unsigned, y);
+    }
+  } else {
+    const v4i x = *reinterpret_cast<const v4i*>(static_cast<const uint16_t*>(q) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(x[i | 1], x[i & 2], i & 1 ? 0x07060302u : 0x05040100u);
+    if (type == PT_BF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const v2f y = {__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)};
+        w[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(y, v2h));
+      }
+    }
+  }
+  return join8(__builtin_bit_cast(v2h, w[0]), __builtin_bit_cast(v2h, w[1]), __builtin_bit_cast(v2h, w[2]), __builtin_bit_cast(v2h, w[3]));
 }
 
 // The keys that an item reads, as one run of places: `shift` keys are left out behind the first `head`.
@@ -72,7 +97,7 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
   const auto offs = reinterpret_cast<float(*)[PA_ROWS]>(lds + PA_WAVES * PA_ROWS * (DP + 4) * 4);
   const auto den = offs + PA_WAVES;
 
-  const PagedItem it = paged_item<1>(b, c.page_shift, c.heads, PA_ROWS, p, index);
+  const PagedItem it = paged_item<4, false, true>(b, c.page_shift, c.heads, PA_ROWS, p, index);
   if (!it.found) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -97,31 +122,30 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
   const int hi = lo_ll + it.slice < places ? (int)(lo_ll + it.slice) : places;
 
   // A lane has the bytes KW * 4 * kg .. of a key row, and what the row's end has no such bytes for, the last ones before it, where Q is zero.
-  // Q in the order in which a dword's nibbles come apart: bytes 0, 2, 1, 3.
   const int kbyte = kg * KW * 4 <= half - KW * 4 ? kg * KW * 4 : half - KW * 4;
   v8h qf[KW];  // of low nibbles, then of high ones
   {
     const long long from_q = (long long)(it.s.row0 + t) * a.q_row + (long long)(it.head * G + g) * a.q_head;
 #pragma unroll
-    for (int i = 0; i < KW; ++i)
+    for (int i = 0; i < KW; ++i) {
+      const int byte = kbyte + i % (KW / 2) * 8;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int in = (i % (KW / 2)) * 8 + (j & 4) + ((j & 1) << 1 | (j & 2) >> 1), byte = kbyte + in;
-        const bool there = real && byte >= kg * KW * 4 && byte < half;
-        qf[i][j] = there ? query_at(a.q, a.q_type, from_q + byte + (i < KW / 2 ? 0 : half)) : (_Float16)0.0f;
-      }
+      for (int j = 0; j < 8; ++j) qf[i][j] = (_Float16)0.0f;
+      if (real && byte >= kg * KW * 4 && byte < half) qf[i] = query8(a.q, a.q_type, from_q + byte + (i < KW / 2 ? 0 : half));
+    }
   }
   const float cl = a.alpha_qk * 1.44269504088896341f;
-  const uint8_t* kb = c.k + it.head * c.k_head;
-  const uint8_t* vb = c.v + it.head * c.v_head;
-  const char* ksb = reinterpret_cast<const char*>(c.k_scale) + it.head * c.ks_head;
-  const char* vsb = reinterpret_cast<const char*>(c.v_scale) + it.head * c.vs_head;
+  const uint8_t* kb = c.k + it.head * c.head;
+  const uint8_t* vb = c.v + it.head * c.head;
+  const char* ksb = reinterpret_cast<const char*>(c.k_scale) + it.head * c.scale_head;
+  const char* vsb = reinterpret_cast<const char*>(c.v_scale) + it.head * c.scale_head;
   // The table through the constant address space: nothing writes to it while the kernel runs, and scalar loads are counted
   // apart from the keys and values in flight, which a vector load would have to wait for.
   const auto table = (const __attribute__((address_space(4))) int*)(b.table + (long long)it.seq * b.per_seq);
   const int mask = (1 << c.page_shift) - 1, last_block = hi > 0 ? (hi - 1) >> 4 : 0;
   const int head_blocks = span.head >> 4, shift_blocks = span.shift >> 4;
 
+  const S4Bits bits;
   float off = PA_EMPTY;
   v4f acc[NB], dsum = {0, 0, 0, 0};
 #pragma unroll
@@ -130,93 +154,105 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (_Float16)1.0f;
 
-  struct Step {
-    int k[2][KW];
-    unsigned v[8], ks[2], vs[2][2 * GROUPS];
-    bool on[2];
+  // Two blocks of 16 keys: their first keys, their pages; where these are, and what a lane has of them.
+  struct Blocks {
+    int key[2], page[2];
   };
-  auto block_of = [&](int s0, int blk) {  // blocks behind the last key are masked, and read where there is memory
-    int at = (s0 >> 4) + blk;
-    at = at < last_block ? at : last_block;
-    return at < head_blocks ? at : at + shift_blocks;
-  };
-  auto pages_of = [&](int (&pg)[2], int s0) {
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk) pg[blk] = table[(block_of(s0, blk) << 4) >> c.page_shift];
-  };
-  const unsigned kcol = (unsigned)(n * c.k_token) + (unsigned)kbyte;
-  const int vbyte = (n * NB / 2) & ~3;
-  const unsigned vcol = (unsigned)(kg * 4 * c.v_token) + (vbyte < half ? (unsigned)vbyte : 0u);
-  auto fetch = [&](Step& st, int s0, const int (&pg)[2]) {
+  auto blocks_at = [&](int s0) {  // asks for the pages; blocks behind the last key are masked, and read where there is memory
+    Blocks w;
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      int page = pg[blk];
-      st.on[blk] = page >= 0 && page < c.pages;
-      page = st.on[blk] ? page : 0;
-      const int o = (block_of(s0, blk) << 4) & mask;
-      const uint8_t* kr = kb + (long long)page * c.k_page + (long long)o * c.k_token + kcol;
+      int at = (s0 >> 4) + blk;
+      at = at < last_block ? at : last_block;
+      at = at < head_blocks ? at : at + shift_blocks;
+      w.key[blk] = at << 4;
+      w.page[blk] = table[w.key[blk] >> c.page_shift];
+    }
+    return w;
+  };
+  auto have = [&](int page) { return (unsigned)page < (unsigned)c.pages; };
+  // by buffer instructions: what a lane adds is one register, the block's place in scalar ones
+  auto pool = [](const void* from) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(from), 0, -1, 0x00020000); };
+  auto code_place = [&](const Blocks& w, int blk) {
+    return (have(w.page[blk]) ? (unsigned)w.page[blk] : 0u) * c.page + (unsigned)((w.key[blk] & mask) * c.token);
+  };
+  auto word_place = [&](const Blocks& w, int blk) {
+    return (have(w.page[blk]) ? (unsigned)w.page[blk] : 0u) * c.scale_page + (unsigned)((w.key[blk] & mask) * (2 * GROUPS));
+  };
+  const unsigned kcol = (unsigned)(n * c.token) + (unsigned)kbyte;
+  const int vbyte = (n * NB / 2) & ~3;
+  const unsigned vcol = (unsigned)(kg * 4 * c.token) + (vbyte < half ? (unsigned)vbyte : 0u);
+  int k[2][KW];
+  unsigned v[8], ks[2], vs[2][2 * GROUPS];
+  auto fetch_k = [&](const Blocks& w) {
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      const auto r = pool(kb + code_place(w, blk)), rw = pool(ksb + word_place(w, blk));
       if constexpr (KW == 4) {
-        const v4i x = *reinterpret_cast<const v4i_8*>(kr);
+        const v4i x = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, kcol, 0, 0));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) st.k[blk][i] = x[i];
+        for (int i = 0; i < 4; ++i) k[blk][i] = x[i];
       } else {
-        const int2 x = *reinterpret_cast<const int2*>(kr);
-        st.k[blk][0] = x.x, st.k[blk][1] = x.y;
+        const int2 x = __builtin_bit_cast(int2, __builtin_amdgcn_raw_buffer_load_b64(r, kcol, 0, 0));
+        k[blk][0] = x.x, k[blk][1] = x.y;
       }
-      const char* kw = ksb + (long long)page * c.ks_page + (long long)(o + n) * (2 * GROUPS);
-      st.ks[blk] = GROUPS == 2 ? *reinterpret_cast<const unsigned*>(kw) : *reinterpret_cast<const uint16_t*>(kw) * 0x10001u;
-      const uint8_t* vr = vb + (long long)page * c.v_page + (long long)o * c.v_token + vcol;
+      if constexpr (GROUPS == 2) ks[blk] = __builtin_amdgcn_raw_buffer_load_b32(rw, n * 4, 0, 0);
+      else ks[blk] = __builtin_amdgcn_raw_buffer_load_b16(rw, n * 2, 0, 0);
+    }
+  };
+  auto fetch_v = [&](const Blocks& w) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        st.v[blk * 4 + j] = *reinterpret_cast<const unsigned*>(vr);
-        vr += c.v_token;
-      }
-      const char* vw = vsb + (long long)page * c.vs_page + (long long)(o + kg * 4) * (2 * GROUPS);
+    for (int blk = 0; blk < 2; ++blk) {
+      const auto r = pool(vb + code_place(w, blk)), rw = pool(vsb + word_place(w, blk));
       if constexpr (GROUPS == 2) {
-        const v4i x = *reinterpret_cast<const v4i*>(vw);
+        const v4i x = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, kg * 16, 0, 0));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) st.vs[blk][i] = (unsigned)x[i];
+        for (int i = 0; i < 4; ++i) vs[blk][i] = (unsigned)x[i];
       } else {
-        const int2 x = *reinterpret_cast<const int2*>(vw);
-        st.vs[blk][0] = (unsigned)x.x, st.vs[blk][1] = (unsigned)x.y;
+        const int2 x = __builtin_bit_cast(int2, __builtin_amdgcn_raw_buffer_load_b64(rw, kg * 8, 0, 0));
+        vs[blk][0] = (unsigned)x.x, vs[blk][1] = (unsigned)x.y;
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[blk * 4 + j] = __builtin_amdgcn_raw_buffer_load_b32(r, vcol, j * c.token, 0);
     }
   };
   const unsigned vpick = DP == 128 || (n & 1) == 0 ? 0x05040100u : 0x07060302u;  // the half of a dword of V that this lane has
-  auto work = [&](Step& st, int s0) {
-    float x[8];
+  auto scores = [&](float (&x)[8]) {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      S4Two k;
-      k.set(0, __builtin_amdgcn_perm(st.ks[blk], st.ks[blk], 0x01000100u));
-      k.set(1, __builtin_amdgcn_perm(st.ks[blk], st.ks[blk], 0x03020302u));
+      S4Two two;
+      two.set(bits, 0, __builtin_amdgcn_perm(ks[blk], ks[blk], 0x01000100u));
+      two.set(bits, 1, __builtin_amdgcn_perm(ks[blk], ks[blk], GROUPS == 2 ? 0x03020302u : 0x01000100u));
       v4f s = {0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < KW / 2; ++i) {
         v2h u[4], w[4];
-        k.values((unsigned)st.k[blk][2 * i], u);
-        k.values((unsigned)st.k[blk][2 * i + 1], w);
+        two.values(bits, (unsigned)k[blk][2 * i], u);
+        two.values(bits, (unsigned)k[blk][2 * i + 1], w);
         s = __builtin_amdgcn_mfma_f32_16x16x32_f16(join8(u[0], u[2], w[0], w[2]), qf[i], s, 0, 0, 0);
         s = __builtin_amdgcn_mfma_f32_16x16x32_f16(join8(u[1], u[3], w[1], w[3]), qf[KW / 2 + i], s, 0, 0, 0);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[blk * 4 + r] = s[r];
     }
-    const int key0 = block_of(s0, 0) << 4, key1 = block_of(s0, 1) << 4;
-    if (s0 + 32 > hi || key1 + 16 > p0 + 1 || key0 < all_from || !st.on[0] || !st.on[1]) {
+  };
+  auto work = [&](float (&x)[8], int s0, const Blocks& at) {
+    const int key0 = at.key[0], key1 = at.key[1];
+    const bool on[2] = {have(at.page[0]), have(at.page[1])};
+    if (s0 + 32 > hi || key1 + 16 > p0 + 1 || key0 < all_from || !on[0] || !on[1]) {
       // What no row sees is not there: its values' steps, which may be anything, become zeros.
       auto dead = [&](int i) {
         const int key = (i >> 2 ? key1 : key0) + kg * 4 + (i & 3);
-        return s0 + (i >> 2) * 16 + kg * 4 + (i & 3) >= hi || !st.on[i >> 2] || (key < any_from && key >= a.sinks);
+        return s0 + (i >> 2) * 16 + kg * 4 + (i & 3) >= hi || !on[i >> 2] || (key < any_from && key >= a.sinks);
       };
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int key = (i >> 2 ? key1 : key0) + kg * 4 + (i & 3);
         if (dead(i) || key >= limit || (key < from && key >= a.sinks)) x[i] = -__builtin_inff();
         if (GROUPS == 2) {
-          if (dead(i)) st.vs[i >> 2][i & 3] = 0;
+          if (dead(i)) vs[i >> 2][i & 3] = 0;
         } else if (dead(i)) {
-          st.vs[i >> 2][(i & 3) >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+          vs[i >> 2][(i & 3) >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
         }
       }
     }
@@ -235,33 +271,35 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
         dsum *= scale;
       }
     }
-    v8h hi_p, lo_p;
+    v2h hi2[4], lo2[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], cl, off));
-      hi_p[i] = (_Float16)e;
-      lo_p[i] = (_Float16)(e - (float)hi_p[i]);
+    for (int i = 0; i < 4; ++i) {
+      const v2f e = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], cl, off)), __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], cl, off))};
+      hi2[i] = __builtin_convertvector(e, v2h);
+      const v2f rest = {__builtin_fmaf((float)hi2[i][0], -1.0f, e[0]), __builtin_fmaf((float)hi2[i][1], -1.0f, e[1])};
+      lo2[i] = __builtin_convertvector(rest, v2h);
     }
+    const v8h hi_p = join8(hi2[0], hi2[1], hi2[2], hi2[3]), lo_p = join8(lo2[0], lo2[1], lo2[2], lo2[3]);
     dsum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, hi_p, dsum, 0, 0, 0);
     dsum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, lo_p, dsum, 0, 0, 0);
-    S4Two v[4];  // of the keys' pairs
+    S4Two two[4];  // of the keys' pairs
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const unsigned* const w = st.vs[j >> 1];
+      const unsigned* const w = vs[j >> 1];
       if constexpr (GROUPS == 2) {
         const unsigned first = w[2 * (j & 1)], second = w[2 * (j & 1) + 1];
-        v[j].set(0, __builtin_amdgcn_perm(second, first, 0x05040100u));
-        v[j].set(1, __builtin_amdgcn_perm(second, first, 0x07060302u));
+        two[j].set(bits, 0, __builtin_amdgcn_perm(second, first, 0x05040100u));
+        two[j].set(bits, 1, __builtin_amdgcn_perm(second, first, 0x07060302u));
       } else {
-        v[j].set(0, w[j & 1]);
-        v[j].set(1, w[j & 1]);
+        two[j].set(bits, 0, w[j & 1]);
+        two[j].set(bits, 1, w[j & 1]);
       }
     }
 #pragma unroll
     for (int h = 0; h < NB / 4; ++h) {
       v2h y[4][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j].values(__builtin_amdgcn_perm(st.v[2 * j + 1], st.v[2 * j], h ? 0x07060302u : vpick), y[j]);
+      for (int j = 0; j < 4; ++j) two[j].values(bits, __builtin_amdgcn_perm(v[2 * j + 1], v[2 * j], h ? 0x07060302u : vpick), y[j]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const v8h vf = join8(y[0][i], y[1][i], y[2][i], y[3][i]);
@@ -271,23 +309,22 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
     }
   };
 
+  // A step's keys are asked for as soon as those of the step before have become numbers, its values when those have.
   int s0 = lo + wave * 32;
   if (s0 < hi) {
     constexpr int STRIDE = PA_WAVES * 32;
-    Step even, odd;
-    int pg[2];
-    pages_of(pg, s0);
-    fetch(even, s0, pg);
-    pages_of(pg, s0 + STRIDE);
-    for (;;) {  // a step's loads are issued without a branch around them, so that the waits can count them
-      fetch(odd, s0 + STRIDE, pg);
-      pages_of(pg, s0 + 2 * STRIDE);
-      work(even, s0);
-      s0 += STRIDE;
-      if (s0 >= hi) break;
-      fetch(even, s0 + STRIDE, pg);
-      pages_of(pg, s0 + 2 * STRIDE);
-      work(odd, s0);
+    Blocks here = blocks_at(s0);
+    fetch_k(here);
+    fetch_v(here);
+    Blocks next = blocks_at(s0 + STRIDE);
+    for (;;) {  // (loads are issued without a branch around them, so that the waits can count them)
+      float x[8];
+      scores(x);
+      fetch_k(next);
+      const Blocks after = blocks_at(s0 + 2 * STRIDE);
+      work(x, s0, here);
+      fetch_v(next);
+      here = next, next = after;
       s0 += STRIDE;
       if (s0 >= hi) break;
     }
@@ -341,7 +378,7 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
 }
 
 template <int DP, int GROUPS, int OUT>
-__global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_s4_rows_kernel(PagedAttn4 a, PagedCache4 c, PagedBatch b, PagedPlan rows) {
+__global__ __launch_bounds__(PA_THREADS, 4) void paged_attn_s4_rows_kernel(PagedAttn4 a, PagedCache4 c, PagedBatch b, PagedPlan rows) {
   __shared__ __attribute__((aligned(16))) char lds[s4_rows_lds(DP)];
   const int lo = b.cu[0], hi = b.cu[b.seqs];  // (on their way beside what the item needs)
   s4_rows<DP, GROUPS, OUT>(a, c, b, rows, blockIdx.x, lds);
@@ -353,25 +390,36 @@ template <int ROWS, int EACH, int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS) void paged_attn_s4_join_kernel(PagedAttn4 a, PagedCache4 c, PagedBatch b, PagedPlan p) {
   __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
   constexpr int PIECES = ROWS / EACH;
-  const PagedItem it = paged_item<1, true>(b, c.page_shift, c.heads, ROWS, p, blockIdx.x / (8 * PIECES) * 8 + blockIdx.x % 8);
+  const PagedItem it = paged_item<4, true, true>(b, c.page_shift, c.heads, ROWS, p, blockIdx.x / (8 * PIECES) * 8 + blockIdx.x % 8);
   if (!it.found || it.split != 0) return;
   join_slices<ROWS, EACH, DP, OUT, false, true>(PagedOut{a.out, a.q_heads, c.D, a.alpha_pv}, p, it, meet, blockIdx.x / 8 % PIECES * EACH);
 }
 
+// Slices that the keys of a batch are cut into, about: three to a CU.  An item is cut where it has one and a half times as many keys or
+// more, into even parts, and longer slices come first.  75 tokens over 50 to 7003 keys, 8 key heads of four, take 105 us with 512
+// slices of one length each and a rest, none where 512 items fill the chip (the int8 cache's rule, whose kernel waits for memory
+// longer), 83 without that exception, 75 with even ones, long ones first; 512, 768 and 1024 slices of them 80, 75 and 75, 20 x 4 tokens
+// in windows of 1024 keys 29, 29 and 34 (where 768 leave 640 items whole).
+constexpr int S4_TARGET = 768;
+
 // What a call of these sizes runs: bounds, since the lengths are on the device (see the int8 cache's).
 struct S4Shape {
-  long long slots;   // items, slices included
+  long long items;   // at most
+  long long slots;   // the same, slices included
   long long places;  // slices of those that are cut
   int target;        // slices that the keys are cut into; 0: nothing is cut
   bool meet;         // slices meet in the launch
 };
 static S4Shape s4_shape(long long rows, long long seqs, long long group, long long heads, long long capacity) {
-  S4Shape s = {heads * (seqs + rows * group / PA_ROWS), 0, 0, false};
-  if (seqs > 0 && capacity > PA_MIN_SLICE) {
-    s.target = PA_TARGET;
+  S4Shape s = {heads * (seqs + rows * group / PA_ROWS), 0, 0, 0, false};
+  s.slots = s.items;
+  if (seqs > 0 && capacity >= PA_MIN_SLICE + PA_MIN_SLICE / 2) {
+    s.target = S4_TARGET;
+    // slices of one item, and how many there are beyond one to each: those of the shortest length, or `target` in all
+    const long long of_one = capacity / PA_MIN_SLICE + 1, shared = s.target / s.items + 1, most = s.items * (of_one - 1);
     const long long each = rows * group / seqs + 1 < PA_ROWS ? rows * group / seqs + 1 : PA_ROWS;
-    s.meet = s.target * each * 520 <= 66560 * s.slots;
-    s.slots += s.target + 8;
+    s.meet = (of_one < shared ? of_one : shared) * each * 520 <= 66560;
+    s.slots += most < s.target + 8 ? most : s.target + 8;
     s.places = s.slots < 2 * s.target + 8 ? s.slots : 2 * s.target + 8;
   }
   return s;
@@ -388,13 +436,13 @@ long long paged_attn_s4_workspace_bytes(long long rows, long long seqs, long lon
 }
 
 template <int DP, int GROUPS, int OUT>
-static void launch_s4(const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, const PagedPlan& rows, hipStream_t stream) {
+static void launch_s4(const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, const PagedPlan& rows, long long items,
+                      hipStream_t stream) {
   const unsigned grid = (unsigned)(rows.slots > 0 ? rows.slots : 1);
   hipLaunchKernelGGL((paged_attn_s4_rows_kernel<DP, GROUPS, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows);
   if (rows.target > 0 && rows.arrivals == nullptr) {
-    const int most = rows.slots - rows.target - 8;
-    const unsigned items = (unsigned)((most < rows.target ? most : rows.target) + 7 & ~7);
-    hipLaunchKernelGGL((paged_attn_s4_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(items * (PA_ROWS / 2)), dim3(PA_THREADS), 0, stream, a,
+    const unsigned cut = (unsigned)((items < rows.target ? (int)items : rows.target) + 7 & ~7);
+    hipLaunchKernelGGL((paged_attn_s4_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(cut * (PA_ROWS / 2)), dim3(PA_THREADS), 0, stream, a,
                        c, b, rows);
   }
 }
@@ -413,6 +461,8 @@ int launch_paged_attn_s4(int out_type, const PagedAttn4& a, const PagedCache4& c
   rows.least = 0;
   rows.most = 0x7fffffff;
   rows.target = s.target;
+  rows.even = true;
+  rows.full = 0x7fffffff;
   // with a window an item reads its own keys, the first ones, and what its tokens' windows are apart
   const long long span = a.window > 0 ? (long long)a.window + ((a.sinks + 15) & ~15) + 16 + (PA_ROWS + group - 1) / group + 1 : 0x7fffffff;
   rows.span = span < 0x7fffffff ? (int)span : 0x7fffffff;
@@ -423,9 +473,9 @@ int launch_paged_attn_s4(int out_type, const PagedAttn4& a, const PagedCache4& c
   rows.arrivals = meet && s.meet ? a.arrivals : nullptr;
   auto run = [&](auto dp, auto groups) {
     constexpr int DP = decltype(dp)::value, GROUPS = decltype(groups)::value;
-    if (out_type == PT_S8) launch_s4<DP, GROUPS, PT_S8>(a, c, b, rows, stream);
-    else if (out_type == PT_F16) launch_s4<DP, GROUPS, PT_F16>(a, c, b, rows, stream);
-    else launch_s4<DP, GROUPS, PT_BF16>(a, c, b, rows, stream);
+    if (out_type == PT_S8) launch_s4<DP, GROUPS, PT_S8>(a, c, b, rows, s.items, stream);
+    else if (out_type == PT_F16) launch_s4<DP, GROUPS, PT_F16>(a, c, b, rows, s.items, stream);
+    else launch_s4<DP, GROUPS, PT_BF16>(a, c, b, rows, s.items, stream);
   };
   using std::integral_constant;
   if (s4_dp(c.D) == 64) {

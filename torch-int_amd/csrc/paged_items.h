@@ -23,6 +23,8 @@ struct PagedPlan {
   int group;        // query heads of a key head
   int least, most;  // rows of a sequence: more than `least`, up to `most`
   int target;       // slices that the keys are cut into; 0: nothing is cut
+  int full;         // items that fill the chip
+  bool even;        // slices of an item are of one length, up to half as long again, instead of the last one being what is left
   int span;         // keys that an item reads, at most
   int slots;        // work items at most, slices included: what the grid holds
   int places;       // slices of items that are cut, at most: what the workspace holds
@@ -84,17 +86,18 @@ __device__ __forceinline__ float rows_max(float x) {
 
 // Keys of a slice, the same in every workgroup: what cuts all keys of the batch into `target` equal parts.  Where the items
 // alone fill the chip, only sequences of more than twice the average are cut: a slice costs its partial sums and the join.
-__device__ __forceinline__ int paged_slice(float items, float total, int target) {
+__device__ __forceinline__ int paged_slice(float items, float total, int target, int full) {
   float want = total / (float)target;
-  if (items >= (float)PA_FULL) want = __builtin_fmaxf(want, 2.0f * total / items);
+  if (items >= (float)full) want = __builtin_fmaxf(want, 2.0f * total / items);
   const int slice = want < 1.0e9f ? ((int)want + 64) & ~63 : 1 << 30;
   return slice < PA_MIN_SLICE ? PA_MIN_SLICE : slice;
 }
 
 // The work item with number `index`, in the order part, sequence, slice, tile of rows, head.  A sequence's tiles come from the
 // last, which has the most keys, to the first, in PARTS parts, so that the long items of all sequences begin before the short
-// ones.  CUT: the first slice of the `index`-th item among those that are cut.
-template <int PARTS, bool CUT = false>
+// ones.  SORTED: instead, in PARTS classes of sequences, those of long slices first.  CUT: the first slice of the `index`-th item
+// among those that are cut.
+template <int PARTS, bool CUT = false, bool SORTED = false>
 __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_shift, int heads, int rows_per_tile, const PagedPlan& p,
                                                 int index) {
   PagedItem it;
@@ -120,14 +123,15 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
       items += wave_add((float)tiles);
       total += wave_add((float)tiles * (float)(s.len < p.span ? s.len : p.span));
     }
-    it.slice = paged_slice(items * (float)heads, total * (float)heads, p.target);
+    it.slice = paged_slice(items * (float)heads, total * (float)heads, p.target, p.full);
   }
   int before = 0, before_cut = 0, before_sliced = 0;
   int splits = 1;
   unsigned long long cuts = 0;  // which of the 64 sequences looked at are cut
   auto cut_up = [&] {
     const int keys = s.len < p.span ? s.len : p.span;
-    splits = keys <= it.slice ? 1 : (keys + it.slice - 1) / it.slice;
+    const int over = p.even ? it.slice >> 1 : it.slice - 1;
+    splits = keys <= it.slice ? 1 : (keys + over) / it.slice;
     cuts = __ballot(splits > 1 && tiles > 0);
   };
   if (b.seqs <= 64) {
@@ -140,8 +144,13 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
       look(i0);
       cut_up();
     }
-    const int behind = PARTS == 1 ? 0 : (int)((long long)tiles * part / PARTS);  // tiles of the parts before
-    const int here = PARTS == 1 ? tiles : (int)((long long)tiles * (part + 1) / PARTS) - behind;
+    const int behind = PARTS == 1 || SORTED ? 0 : (int)((long long)tiles * part / PARTS);  // tiles of the parts before
+    int here = PARTS == 1 || SORTED ? tiles : (int)((long long)tiles * (part + 1) / PARTS) - behind;
+    if (SORTED) {  // (four classes)
+      const int keys = (s.len < p.span ? s.len : p.span) / splits, want = it.slice;
+      const int mine = keys > want ? 0 : keys > (want >> 1) + (want >> 2) ? 1 : keys > want >> 1 ? 2 : 3;
+      here = mine == part ? tiles : 0;
+    }
     // a cu_new that descends can count rows many times over: no sum of items passes the range of int
     const long long whole = (long long)here * heads, all = whole * splits;
     const int n = all > 0x800000 ? 0x800000 : (int)all;
@@ -163,6 +172,10 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
       it.s.T = __builtin_amdgcn_readlane(s.T, at);
       it.s.len = __builtin_amdgcn_readlane(s.len, at);
       it.splits = __builtin_amdgcn_readlane(splits, at);
+      if (p.even) {
+        const int keys = it.s.len < p.span ? it.s.len : p.span;
+        it.slice = it.splits > 1 ? ((keys + it.splits - 1) / it.splits + 63) & ~63 : 0x7fffffff;
+      }
       it.seq = i0 + at;
       it.step = heads * t;
       it.split = rel / it.step;

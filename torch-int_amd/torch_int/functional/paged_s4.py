@@ -5,11 +5,11 @@ half the bytes, and no steps to be calibrated, since every token's are found as 
 (:func:`paged_cache_s4` makes them):
 
 * ``k_cache``, ``v_cache``: uint8 [pages, heads, page_size, head_dim / 2].  Byte j of a row holds the code of column j in its low four
-  bits, that of column head_dim / 2 + j in the others.  Any strides that keep the last dimension contiguous and are multiples
-  of 8 bytes; ``head_dim`` is a multiple of 16 from 32 to 128, ``page_size`` a power of two from 16;
+  bits, that of column head_dim / 2 + j in the others.  Any strides that keep the last dimension contiguous, are multiples of
+  8 bytes and are the same for both; ``head_dim`` is a multiple of 16 from 32 to 128, ``page_size`` a power of two from 16;
 * ``k_scale``, ``v_scale``: int16 [pages, heads, page_size, groups], a word for the whole head (``groups`` 1) or for each half of its
   columns (2).  Bits 4 to 14 are those of an fp16 number, the step; bits 0 to 3 are z, and a value is ``step * (code - z)``.
-  The last two dimensions are packed, the other strides multiples of 16 bytes.
+  The last two dimensions are packed, the other strides multiples of 16 bytes, the same for both.
 
 What the batch's tensors hold cannot be checked on the host; values out of range touch no memory outside the tensors
 (``include/torch_int_hip.h`` says what they do instead).
@@ -30,8 +30,8 @@ _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.
 class _Cache(ctypes.Structure):
     """``TiPagedCacheS4`` of include/torch_int_hip.h."""
     _fields_ = ([(n, _vp) for n in ("k", "v", "k_scale", "v_scale")]
-                + [(n, _i64) for n in ("pages", "page_size", "heads", "head_dim", "groups", "k_page", "k_head", "k_token", "v_page",
-                                       "v_head", "v_token", "k_scale_page", "k_scale_head", "v_scale_page", "v_scale_head")])
+                + [(n, _i64) for n in ("pages", "page_size", "heads", "head_dim", "groups", "page", "head", "token", "scale_page",
+                                       "scale_head")])
 
 
 class _Append(ctypes.Structure):
@@ -107,17 +107,16 @@ def _cache_and_batch(op, k_cache, v_cache, k_scale, v_scale, block_table, contex
             shape = pages, heads, page_size, half = k_cache.shape
             words = k_scale.shape
             groups = words[3]
-            kp, kh, kt, kd = k_cache.stride()
-            vp, vh, vt, vd = v_cache.stride()
-            ksp, ksh, kst, ksd = k_scale.stride()
-            vsp, vsh, vst, vsd = v_scale.stride()
+            strides = page, head, token, last = k_cache.stride()
+            word_strides = scale_page, scale_head, scale_token, scale_last = k_scale.stride()
             seqs, per_seq = block_table.shape
-            if (v_cache.shape == shape and kd == 1 and vd == 1 and words == (pages, heads, page_size, groups) and v_scale.shape == words
-                    and kst == groups and vst == groups and (groups == 1 or ksd == 1 and vsd == 1)
+            if (v_cache.shape == shape and v_cache.stride() == strides and last == 1 and words == (pages, heads, page_size, groups)
+                    and v_scale.shape == words and v_scale.stride() == word_strides and scale_token == groups
+                    and (groups == 1 or scale_last == 1)
                     and context_lens.shape == (seqs,) and cu_new.shape == (seqs + 1,)):
                 return (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, page_size, heads, 2 * half,
-                        groups, kp, kh, kt, vp, vh, vt, 2 * ksp, 2 * ksh, 2 * vsp, 2 * vsh, block_table.data_ptr(),
-                        context_lens.data_ptr(), cu_new.data_ptr(), per_seq, seqs, rows)
+                        groups, page, head, token, 2 * scale_page, 2 * scale_head, block_table.data_ptr(), context_lens.data_ptr(),
+                        cu_new.data_ptr(), per_seq, seqs, rows)
     except (AttributeError, TypeError, ValueError, IndexError):
         pass
     for name, t, dtype, ndim in (("k_cache", k_cache, _U8, 4), ("v_cache", v_cache, _U8, 4), ("k_scale", k_scale, _I16, 4),
@@ -133,6 +132,9 @@ def _cache_and_batch(op, k_cache, v_cache, k_scale, v_scale, block_table, contex
         _fail(op, f"k_cache is {tuple(k_cache.shape)} but v_cache is {tuple(v_cache.shape)}")
     if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
         _fail(op, "the last dimension of k_cache and v_cache must be contiguous")
+    for a, b, name in ((k_cache, v_cache, "k_cache and v_cache"), (k_scale, v_scale, "k_scale and v_scale")):
+        if a.shape == b.shape and a.stride() != b.stride():
+            _fail(op, f"{name} have strides of {a.stride()} and {b.stride()}, which must be the same")
     if k_scale.shape[:3] != k_cache.shape[:3] or v_scale.shape != k_scale.shape:
         _fail(op, f"k_scale is {tuple(k_scale.shape)} and v_scale {tuple(v_scale.shape)} beside caches of {tuple(k_cache.shape)}")
     for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
@@ -224,7 +226,7 @@ def paged_kv_append_s4(key, value, k_cache, v_cache, k_scale, v_scale, block_tab
         if _fast_append is not None:
             rc = _fast_append(*args, *tail, stream)
         else:
-            rc = _lib.ti_paged_kv_append_s4(_Cache(*args[:19]), _Batch(*args[19:]), _Append(*tail), stream or None)
+            rc = _lib.ti_paged_kv_append_s4(_Cache(*args[:14]), _Batch(*args[14:]), _Append(*tail), stream or None)
     if rc:
         _status(op, rc)
     return out
@@ -252,7 +254,7 @@ def paged_attn_s4(query, k_cache, v_cache, k_scale, v_scale, block_table, contex
     rows, q_heads, _ = query.shape
     args = _cache_and_batch(op, k_cache, v_cache, k_scale, v_scale, block_table, context_lens, cu_new, rows)
     dev = k_cache.get_device()
-    heads, d, seqs = args[6], args[7], args[23]
+    heads, d, seqs = args[6], args[7], args[18]
     shape = (rows, q_heads, d)
     q_row, q_head = _rows(op, "query", query, query.dtype, shape, dev)
     if heads == 0 or q_heads == 0 or q_heads % heads:
@@ -275,7 +277,7 @@ def paged_attn_s4(query, k_cache, v_cache, k_scale, v_scale, block_table, contex
             _fail(op, "out must not be the query: other workgroups read it while its rows are written")
     if rows == 0:
         return out
-    key = (rows, seqs, q_heads, heads, d, args[22] * args[5])
+    key = (rows, seqs, q_heads, heads, d, args[17] * args[5])
     need = _ws_need.get(key)
     if need is None:
         if len(_ws_need) >= 4096:
@@ -290,7 +292,7 @@ def paged_attn_s4(query, k_cache, v_cache, k_scale, v_scale, block_table, contex
         if _fast_attn is not None:
             rc = _fast_attn(*args, *tail, ws_ptr, ws_bytes, stream)
         else:
-            rc = _lib.ti_paged_attn_s4(_Cache(*args[:19]), _Batch(*args[19:]), _Attn(*tail), ws_ptr or None, ws_bytes, stream or None)
+            rc = _lib.ti_paged_attn_s4(_Cache(*args[:14]), _Batch(*args[14:]), _Attn(*tail), ws_ptr or None, ws_bytes, stream or None)
     if rc:
         _status(op, rc)
     return out
@@ -335,7 +337,7 @@ def paged_kv_read_s4(k_cache, v_cache, k_scale, v_scale, block_table, context_le
         if _fast_read is not None:
             rc = _fast_read(*args, *tail, stream)
         else:
-            rc = _lib.ti_paged_kv_read_s4(_Cache(*args[:19]), _Batch(*args[19:]), _Read(*tail), stream or None)
+            rc = _lib.ti_paged_kv_read_s4(_Cache(*args[:14]), _Batch(*args[14:]), _Read(*tail), stream or None)
     if rc:
         _status(op, rc)
     return key_out, value_out
