@@ -377,6 +377,325 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
   if (it.splits > 1) meet_and_join<PA_ROWS, DP, OUT, true>(to, p, it, reinterpret_cast<int*>(&offs[0][0]), &sum[0][0][0]);
 }
 
+// Many rows: 128 to a workgroup, 32 to each of its four waves, 64 keys to a step.  Each wave brings 16 of a step's keys from memory, a
+// step ahead of their becoming numbers, and writes them to the LDS as fp16: keys as rows, 16-byte chunks (eight bytes' low
+// nibbles, or high ones) exchanged by the row; values in the order in which MFMA operands are read, of eight keys, chosen as
+// S^T = K Q^T leaves them in a lane, one column in 16 bytes, lane after lane.  One unpacking then serves 128 rows.
+// Column block i of V holds, of lane m's NDB / 2 bytes of a row, byte i / 2's low nibble or high one.
+constexpr int ST_ROWS = 128, ST_KEYS = 64;
+constexpr int ST_PARTS = 4;
+constexpr int ST_JOIN = 32;      // rows that a workgroup joins
+constexpr int ST_PLENTY = 2048;  // items from which on nothing is cut
+constexpr int s4_tiles_lds(int DP) { return 2 * 2 * ST_KEYS * DP * 2; }  // two steps of K, then of V
+template <int DP, int GROUPS, int OUT>
+__device__ __forceinline__ void s4_tiles(const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, const PagedPlan& p, int index,
+                                         char* lds) {
+  constexpr int NDB = DP / 32;  // column blocks of O^T
+  constexpr int KS = DP / 16;   // steps of 16 along a key row
+  constexpr int KW = DP / 32;   // dwords of a key row that a thread brings
+  constexpr int BYTES = ST_KEYS * DP * 2;  // of a step of K, or of V
+
+  const PagedItem it = paged_item<ST_PARTS>(b, c.page_shift, c.heads, ST_ROWS, p, index);
+  if (!it.found) return;
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, h = lane >> 5;
+  const int G = p.group, live_rows = it.s.T * G, half = c.D / 2;
+  const int base = it.s.len - it.s.T;
+  const int row0 = it.tile * ST_ROWS + wave * 32, row = row0 + n;
+  const int t = row / G, g = row - t * G;
+  const bool real = row < live_rows;
+  const int limit = real ? base + t + 1 : 0x7fffffff;
+  const int from = real && a.window > 0 ? limit - a.window : -0x7fffffff;
+  // positions of the workgroup's first and last rows, and of the wave's (one without rows: behind everything, it sees no key)
+  const int last_row = it.tile * ST_ROWS + ST_ROWS - 1 < live_rows - 1 ? it.tile * ST_ROWS + ST_ROWS - 1 : live_rows - 1;
+  const int p0 = base + it.tile * ST_ROWS / G, p1 = base + last_row / G;
+  const int w0 = base + row0 / G, w1 = row0 < live_rows ? base + (row0 + 31 < live_rows ? row0 + 31 : live_rows - 1) / G : -1;
+  const S4Span span(a, p0, p1);
+  const int places = span.places();
+  const int any_from = a.window > 0 ? p0 + 1 - a.window : -0x7fffffff;       // before it no row sees keys, but for first ones
+  const int wave_from = a.window > 0 ? w0 + 1 - a.window : -0x7fffffff;      // nor before this one of the wave
+  const int wave_all_from = a.window > 0 ? w1 + 1 - a.window : -0x7fffffff;  // from here on all of its rows do
+  const long long lo_ll = (long long)it.split * it.slice;
+  const int lo = lo_ll < places ? (int)lo_ll : places;
+  const int hi = lo_ll + it.slice < places ? (int)(lo_ll + it.slice) : places;
+
+  v8h qf[KS];
+#pragma unroll
+  for (int i = 0; i < KS; ++i) {
+    const int chunk = 2 * i + h, byte = chunk % (DP / 16) * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) qf[i][j] = (_Float16)0.0f;
+    if (real && byte < half)
+      qf[i] = query8(a.q, a.q_type, (long long)(it.s.row0 + t) * a.q_row + (long long)(it.head * G + g) * a.q_head + byte +
+                                        (chunk < DP / 16 ? 0 : half));
+  }
+  const float cl = a.alpha_qk * 1.44269504088896341f;
+  const uint8_t* kb = c.k + it.head * c.head;
+  const uint8_t* vb = c.v + it.head * c.head;
+  const char* ksb = reinterpret_cast<const char*>(c.k_scale) + it.head * c.scale_head;
+  const char* vsb = reinterpret_cast<const char*>(c.v_scale) + it.head * c.scale_head;
+  const auto table = (const __attribute__((address_space(4))) int*)(b.table + (long long)it.seq * b.per_seq);
+  const int mask = (1 << c.page_shift) - 1, last_block = hi > 0 ? (hi - 1) >> 4 : 0;
+  const int head_blocks = span.head >> 4, shift_blocks = span.shift >> 4;
+  const S4Bits bits;
+
+  // the first key of a block of 16 places; blocks behind the last key are masked, and read where there is memory
+  auto key_of = [&](int block) {
+    int at = block < last_block ? block : last_block;
+    at = at < head_blocks ? at : at + shift_blocks;
+    return at << 4;
+  };
+  auto have = [&](int page) { return (unsigned)page < (unsigned)c.pages; };
+  auto pool = [](const void* from) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(from), 0, -1, 0x00020000); };
+
+  // What this thread brings of a step: of the wave's 16 keys, KW dwords of K and the NDB / 2 bytes n NDB / 2 .. of eight rows of V.
+  const int krow = lane >> 2;
+  const int kbyte = (lane & 3) * KW * 4 <= half - KW * 4 ? (lane & 3) * KW * 4 : half - KW * 4;
+  const unsigned kcol = (unsigned)(krow * c.token + kbyte);
+  const int vbyte = n * (NDB / 2);
+  const unsigned vcol = (unsigned)(h * 4 * c.token) + (vbyte < half ? (unsigned)vbyte : 0u);
+  int kreg[KW];
+  unsigned vreg[8], ks, vs[2][2 * GROUPS];
+  bool dead = false;  // the step on its way has keys that no row sees
+  int dead_key = 0;   // its first key
+  int dead_at = 0;    // and place
+  bool dead_page = false;
+  auto fetch = [&](int s0, int page) {
+    const int block = (s0 >> 4) + wave, key = key_of(block);
+    const bool on = have(page);
+    const unsigned long long at = on ? (unsigned)page : 0u;
+    const auto code = at * c.page + (unsigned)((key & mask) * c.token), word = at * c.scale_page + (unsigned)((key & mask) * (2 * GROUPS));
+    const auto rk = pool(kb + code), rv = pool(vb + code), rks = pool(ksb + word), rvs = pool(vsb + word);
+    if constexpr (KW == 4) {
+      const v4i x = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rk, kcol, 0, 0));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kreg[i] = x[i];
+    } else {
+      const int2 x = __builtin_bit_cast(int2, __builtin_amdgcn_raw_buffer_load_b64(rk, kcol, 0, 0));
+      kreg[0] = x.x, kreg[1] = x.y;
+    }
+    if constexpr (GROUPS == 2) ks = __builtin_amdgcn_raw_buffer_load_b32(rks, krow * 4, 0, 0);
+    else ks = __builtin_amdgcn_raw_buffer_load_b16(rks, krow * 2, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if constexpr (GROUPS == 2) {
+        const v4i x = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rvs, h * 16, 32 * i, 0));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vs[i][j] = (unsigned)x[j];
+      } else {
+        const int2 x = __builtin_bit_cast(int2, __builtin_amdgcn_raw_buffer_load_b64(rvs, h * 8, 16 * i, 0));
+        vs[i][0] = (unsigned)x.x, vs[i][1] = (unsigned)x.y;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (NDB == 4) vreg[i * 4 + j] = __builtin_amdgcn_raw_buffer_load_b16(rv, vcol, (8 * i + j) * c.token, 0);
+        else vreg[i * 4 + j] = __builtin_amdgcn_raw_buffer_load_b8(rv, vcol, (8 * i + j) * c.token, 0);
+      }
+    }
+    dead_at = block << 4, dead_key = key, dead_page = !on;
+    dead = !on || dead_at + 16 > hi || (key < any_from && key + 16 > a.sinks);
+  };
+  auto swizzle = [](int r, int chunk) { return chunk ^ (r & 7); };
+  auto put_k = [&](int slot) {
+    S4Two two;
+    two.set(bits, 0, __builtin_amdgcn_perm(ks, ks, 0x01000100u));
+    two.set(bits, 1, __builtin_amdgcn_perm(ks, ks, GROUPS == 2 ? 0x03020302u : 0x01000100u));
+    const int r = wave * 16 + krow;
+    char* const to = lds + slot * BYTES + r * (DP * 2);
+#pragma unroll
+    for (int i = 0; i < KW / 2; ++i) {
+      v2h u[4], w[4];
+      two.values(bits, (unsigned)kreg[2 * i], u);
+      two.values(bits, (unsigned)kreg[2 * i + 1], w);
+      const int chunk = (kbyte >> 3) + i;
+      *reinterpret_cast<v8h*>(to + swizzle(r, chunk) * 16) = join8(u[0], u[2], w[0], w[2]);
+      *reinterpret_cast<v8h*>(to + swizzle(r, chunk + DP / 16) * 16) = join8(u[1], u[3], w[1], w[3]);
+    }
+  };
+  auto put_v = [&](int slot) {
+    if (__builtin_expect(dead, 0)) {  // what no row sees is not there: steps, which may be anything, become zeros
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = (i >> 2) * 8 + h * 4 + (i & 3), key = dead_key + at;
+        if (dead_page || dead_at + at >= hi || (key < any_from && key >= a.sinks)) {
+          if (GROUPS == 2) vs[i >> 2][i & 3] = 0;
+          else vs[i >> 2][(i & 3) >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+        }
+      }
+    }
+    v2h y[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned* const w = vs[j >> 1];
+      S4Two two;
+      if constexpr (GROUPS == 2) {
+        const unsigned first = w[2 * (j & 1)], second = w[2 * (j & 1) + 1];
+        two.set(bits, 0, __builtin_amdgcn_perm(second, first, 0x05040100u));
+        two.set(bits, 1, __builtin_amdgcn_perm(second, first, 0x07060302u));
+      } else {
+        two.set(bits, 0, w[j & 1]);
+        two.set(bits, 1, w[j & 1]);
+      }
+      two.values(bits, vreg[2 * j] | vreg[2 * j + 1] << 16, y[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < NDB; ++i)
+      *reinterpret_cast<v8h*>(lds + 2 * BYTES + slot * BYTES + ((wave * NDB + i) * 64 + lane) * 16) = join8(y[0][i], y[1][i], y[2][i], y[3][i]);
+  };
+
+  float off = PA_EMPTY, den = 0.0f;
+  v16f acc[NDB];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
+
+  if (lo < hi) {
+    // whether the pool lacks any of the item's pages: looked at once, so that steps need not
+    bool holes = false;
+    for (int i = (lo >> 4) + lane; i <= last_block; i += 64) holes |= !have(table[key_of(i) >> c.page_shift]);
+    holes = __ballot(holes) != 0;
+    auto page_at = [&](int s0) { return table[key_of((s0 >> 4) + wave) >> c.page_shift]; };
+    fetch(lo, page_at(lo));
+    int page = page_at(lo + ST_KEYS);
+    if (c.D < DP) {  // chunks behind the head size are never written: zeros, as Q is there
+      for (int i = threadIdx.x * 16; i < 2 * BYTES; i += PA_THREADS * 16) *reinterpret_cast<v4i*>(lds + i) = v4i{0, 0, 0, 0};
+      __syncthreads();
+    }
+    put_k(0);
+    put_v(0);
+    fetch(lo + ST_KEYS, page);
+    page = page_at(lo + 2 * ST_KEYS);
+    __syncthreads();
+    int slot = 0;
+    for (int s0 = lo; s0 < hi; s0 += ST_KEYS) {
+      const char* const kl = lds + slot * BYTES;
+      const char* const vl = lds + 2 * BYTES + slot * BYTES;
+      // the places of the four blocks of 16 keys, and whether the wave's rows see all of them, or none
+      int key[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) key[i] = key_of((s0 >> 4) + i);
+      v16f x[2];
+      bool any[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        any[q] = s0 + 32 * q < hi && key[2 * q] <= w1 && (key[2 * q + 1] + 16 > wave_from || key[2 * q] < a.sinks);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[q][r] = 0.0f;
+        if (any[q]) {
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            const v8h kf = *reinterpret_cast<const v8h*>(kl + (32 * q + n) * (DP * 2) + swizzle(n, 2 * i + h) * 16);
+            x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[i], x[q], 0, 0, 0);
+          }
+        }
+      }
+      // the next step's keys and values, which have arrived, become numbers
+      put_k(slot ^ 1);
+      put_v(slot ^ 1);
+      fetch(s0 + 2 * ST_KEYS, page);
+      page = page_at(s0 + 3 * ST_KEYS);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if (!any[q]) continue;
+        if (__builtin_expect(s0 + 32 * q + 32 > hi || key[2 * q + 1] + 15 > w0 || key[2 * q] < wave_all_from || holes, 0)) {
+          bool on[2] = {true, true};
+          if (holes) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) on[i] = have(table[key[2 * q + i] >> c.page_shift]);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int at = (r & 3) + 8 * ((r >> 2) & 1) + 4 * h, mine = key[2 * q + (r >> 3)] + at;
+            if (s0 + 32 * q + 16 * (r >> 3) + at >= hi || mine >= limit || !on[r >> 3] || (mine < from && mine >= a.sinks))
+              x[q][r] = -__builtin_inff();
+          }
+        }
+        float top = x[q][0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = __builtin_fmaxf(top, x[q][r]);
+        if (__builtin_expect(__ballot(__builtin_fmaf(top, cl, off) > 15.0f) != 0, 0)) {
+          auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+          top = __builtin_fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
+          if (__builtin_fmaf(top, cl, off) > 15.0f) {
+            const float fresh = 8.0f - top * cl;
+            const float scale = __builtin_amdgcn_exp2f(fresh - off);
+            off = fresh;
+            den *= scale;
+#pragma unroll
+            for (int i = 0; i < NDB; ++i) acc[i] *= scale;
+          }
+        }
+        v8h pr[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          v2h two[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const v2f e = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[q][8 * i + 2 * j], cl, off)),
+                           __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][8 * i + 2 * j + 1], cl, off))};
+            two[j] = __builtin_convertvector(e, v2h);
+            den = __builtin_amdgcn_fdot2(two[j], v2h{(_Float16)1.0f, (_Float16)1.0f}, den, false);
+          }
+          pr[i] = join8(two[0], two[1], two[2], two[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < NDB; ++j) {
+            const v8h vf = *reinterpret_cast<const v8h*>(vl + (((2 * q + i) * NDB + j) * 64 + lane) * 16);
+            acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pr[i], acc[j], 0, 0, 0);
+          }
+      }
+      __syncthreads();
+      slot ^= 1;
+    }
+  }
+
+  // the two halves of the wave add their denominators
+  {
+    auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(den), __float_as_uint(den), false, false);
+    den = __uint_as_float(o[0]) + __uint_as_float(o[1]);
+  }
+  // Through the LDS, four places at a spot that the row moves, so that rows leave as whole lines.
+  __syncthreads();
+  const float f = it.splits > 1 ? 1.0f : den != 0.0f ? a.alpha_pv / den : 0.0f;
+  constexpr int QUADS = DP / 4, PER = 64 / QUADS;  // rows that a wave stores at once
+  v4f* const own = reinterpret_cast<v4f*>(lds) + wave * 32 * QUADS;
+  auto spot = [](int r, int quad) { return r * QUADS + (quad ^ (r & (QUADS - 1))); };
+#pragma unroll
+  for (int nib = 0; nib < 2; ++nib)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float y[NDB / 2][4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < NDB / 2; ++j) {
+          const int at = r * (NDB / 2) + j;
+          y[at >> 2][at & 3] = den != 0.0f ? acc[2 * j + nib][4 * i + r] * f : 0.0f;
+        }
+#pragma unroll
+      for (int j = 0; j < NDB / 2; ++j)
+        own[spot(n, nib * (QUADS / 2) + (2 * i + h) * (NDB / 2) + j)] = v4f{y[j][0], y[j][1], y[j][2], y[j][3]};
+    }
+  __builtin_amdgcn_wave_barrier();
+  const long long place = it.place + (long long)it.split * it.step;
+  const int quad = lane % QUADS, column = paged_column<DP>(quad * 4, c.D);
+  const PagedRows out_row(it, a.q_heads, G, ST_ROWS);
+#pragma unroll
+  for (int i = 0; i < 32 / PER; ++i) {
+    const int r = i * PER + lane / QUADS, rr = row0 + r;
+    if (rr >= live_rows || column >= c.D) continue;
+    const v4f y = own[spot(r, quad)];
+    if (it.splits == 1) store_some<4, OUT>(a.out, out_row(wave * 32 + r) * c.D + column, {y[0], y[1], y[2], y[3]});
+    else *reinterpret_cast<v4f*>(p.ws + (place * ST_ROWS + wave * 32 + r) * DP + quad * 4) = y;
+  }
+  if (it.splits > 1 && real && h == 0)
+    *reinterpret_cast<v2f*>(p.ws + (long long)p.places * ST_ROWS * DP + (place * ST_ROWS + wave * 32 + n) * 2) = v2f{off, den};
+}
+
 template <int DP, int GROUPS, int OUT>
 __global__ __launch_bounds__(PA_THREADS, 4) void paged_attn_s4_rows_kernel(PagedAttn4 a, PagedCache4 c, PagedBatch b, PagedPlan rows) {
   __shared__ __attribute__((aligned(16))) char lds[s4_rows_lds(DP)];
@@ -385,12 +704,30 @@ __global__ __launch_bounds__(PA_THREADS, 4) void paged_attn_s4_rows_kernel(Paged
   if (a.fill) paged_fill(b, lo, hi, static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
 }
 
+// Sequences of few rows and of many in one launch, 256 items of the one kind after 256 of the other as long as both last (as over the
+// int8 cache, where turns of 256 leave one of each kind to every CU).
+constexpr int S4_TURN = 256;
+template <int DP, int GROUPS, int OUT>
+__global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_s4_both_kernel(PagedAttn4 a, PagedCache4 c, PagedBatch b, PagedPlan rows,
+                                                                           PagedPlan tiles) {
+  __shared__ __attribute__((aligned(16))) char lds[s4_tiles_lds(DP) > s4_rows_lds(DP) ? s4_tiles_lds(DP) : s4_rows_lds(DP)];
+  if (a.fill) paged_fill(b, b.cu[0], b.cu[b.seqs], static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
+  const int i = blockIdx.x, each = (rows.slots < tiles.slots ? rows.slots : tiles.slots) & -S4_TURN, rest = i - 2 * each;
+  const bool many = rest < 0 ? (i & S4_TURN) == 0 : rest < tiles.slots - each;
+  const int index = rest < 0 ? i / (2 * S4_TURN) * S4_TURN + i % S4_TURN : each + rest - (many ? 0 : tiles.slots - each);
+  if (many) s4_tiles<DP, GROUPS, OUT>(a, c, b, tiles, index, lds);
+  else s4_rows<DP, GROUPS, OUT>(a, c, b, rows, index, lds);
+}
+
 // Joins slices that do not meet in the launch itself, EACH rows to a workgroup, in turns of eight items (as over the int8 cache).
 template <int ROWS, int EACH, int DP, int OUT>
 __global__ __launch_bounds__(PA_THREADS) void paged_attn_s4_join_kernel(PagedAttn4 a, PagedCache4 c, PagedBatch b, PagedPlan p) {
   __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
   constexpr int PIECES = ROWS / EACH;
-  const PagedItem it = paged_item<4, true, true>(b, c.page_shift, c.heads, ROWS, p, blockIdx.x / (8 * PIECES) * 8 + blockIdx.x % 8);
+  const int index = blockIdx.x / (8 * PIECES) * 8 + blockIdx.x % 8;
+  PagedItem it;
+  if constexpr (ROWS == ST_ROWS) it = paged_item<ST_PARTS, true>(b, c.page_shift, c.heads, ROWS, p, index);
+  else it = paged_item<4, true, true>(b, c.page_shift, c.heads, ROWS, p, index);
   if (!it.found || it.split != 0) return;
   join_slices<ROWS, EACH, DP, OUT, false, true>(PagedOut{a.out, a.q_heads, c.D, a.alpha_pv}, p, it, meet, blockIdx.x / 8 % PIECES * EACH);
 }
@@ -403,48 +740,79 @@ __global__ __launch_bounds__(PA_THREADS) void paged_attn_s4_join_kernel(PagedAtt
 constexpr int S4_TARGET = 768;
 
 // What a call of these sizes runs: bounds, since the lengths are on the device (see the int8 cache's).
-struct S4Shape {
+struct S4Kind {
   long long items;   // at most
-  long long slots;   // the same, slices included
+  long long slots;   // the same, slices included; 0: none of this kind
   long long places;  // slices of those that are cut
   int target;        // slices that the keys are cut into; 0: nothing is cut
-  bool meet;         // slices meet in the launch
+  void cut(int into, long long of_one) {
+    target = into;
+    // an item has at most as many slices as there are shortest ones in it, all together `target` more than items
+    const long long most = items * (of_one - 1);
+    slots += most < target + 8 ? most : target + 8;
+    places = slots < 2 * target + 8 ? slots : 2 * target + 8;
+  }
+};
+struct S4Shape {
+  S4Kind rows, tiles;
+  bool meet;  // slices of few rows meet in the launch
 };
 static S4Shape s4_shape(long long rows, long long seqs, long long group, long long heads, long long capacity) {
-  S4Shape s = {heads * (seqs + rows * group / PA_ROWS), 0, 0, 0, false};
-  s.slots = s.items;
-  if (seqs > 0 && capacity >= PA_MIN_SLICE + PA_MIN_SLICE / 2) {
-    s.target = S4_TARGET;
-    // slices of one item, and how many there are beyond one to each: those of the shortest length, or `target` in all
-    const long long of_one = capacity / PA_MIN_SLICE + 1, shared = s.target / s.items + 1, most = s.items * (of_one - 1);
-    const long long each = rows * group / seqs + 1 < PA_ROWS ? rows * group / seqs + 1 : PA_ROWS;
-    s.meet = (of_one < shared ? of_one : shared) * each * 520 <= 66560;
-    s.slots += most < s.target + 8 ? most : s.target + 8;
-    s.places = s.slots < 2 * s.target + 8 ? s.slots : 2 * s.target + 8;
+  S4Shape s = {};
+  const bool cut = seqs > 0 && capacity >= PA_MIN_SLICE + PA_MIN_SLICE / 2;
+  const long long of_one = capacity / PA_MIN_SLICE + 1;  // slices of one item
+  long long each = PA_ROWS;                              // rows of one
+  auto items = [](S4Kind& k, long long n) { k.items = k.slots = n; };
+  auto join_here = [&] {
+    const long long shared = s.rows.target / (s.rows.items > 0 ? s.rows.items : 1) + 1;
+    s.meet = s.rows.target > 0 && (of_one < shared ? of_one : shared) * each * 520 <= 66560;
+  };
+  if (rows * group <= PA_ROWS * seqs) {  // few rows to a sequence on average: all of them by that kernel
+    items(s.rows, heads * (seqs + rows * group / PA_ROWS));
+    each = rows * group / (seqs > 0 ? seqs : 1) + 1 < PA_ROWS ? rows * group / (seqs > 0 ? seqs : 1) + 1 : PA_ROWS;
+    if (cut) s.rows.cut(S4_TARGET, of_one);
+    join_here();
+    return s;
   }
+  // sequences with more than 16 rows are at most a 17th of all rows
+  const long long many = rows * group / (PA_ROWS + 1) < seqs ? rows * group / (PA_ROWS + 1) : seqs;
+  items(s.tiles, heads * (many + rows * group / ST_ROWS));
+  if (cut && s.tiles.items < ST_PLENTY) s.tiles.cut(PA_TARGET, of_one);
+  if (seqs == 1) return s;  // it has more than 16
+  items(s.rows, heads * seqs);
+  if (cut) s.rows.cut(PA_TARGET / 4, of_one);
+  join_here();
   return s;
 }
 static int s4_dp(long long D) { return D <= 64 ? 64 : 128; }
+static long long s4_bytes(const S4Kind& k, int rows, long long D) { return k.places * rows * (s4_dp(D) + 2) * 4; }
 
 long long paged_attn_s4_arrivals(long long rows, long long seqs, long long q_heads, long long heads, long long capacity) {
   const S4Shape s = s4_shape(rows, seqs, q_heads / heads, heads, capacity);
-  return s.meet ? s.places : 0;
+  return s.meet ? s.rows.places : 0;
 }
 long long paged_attn_s4_workspace_bytes(long long rows, long long seqs, long long q_heads, long long heads, long long D,
                                         long long capacity) {
-  return s4_shape(rows, seqs, q_heads / heads, heads, capacity).places * PA_ROWS * (s4_dp(D) + 2) * 4;
+  const S4Shape s = s4_shape(rows, seqs, q_heads / heads, heads, capacity);
+  return s4_bytes(s.rows, PA_ROWS, D) + s4_bytes(s.tiles, ST_ROWS, D);
 }
 
 template <int DP, int GROUPS, int OUT>
-static void launch_s4(const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, const PagedPlan& rows, long long items,
-                      hipStream_t stream) {
-  const unsigned grid = (unsigned)(rows.slots > 0 ? rows.slots : 1);
-  hipLaunchKernelGGL((paged_attn_s4_rows_kernel<DP, GROUPS, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows);
-  if (rows.target > 0 && rows.arrivals == nullptr) {
-    const unsigned cut = (unsigned)((items < rows.target ? (int)items : rows.target) + 7 & ~7);
-    hipLaunchKernelGGL((paged_attn_s4_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(cut * (PA_ROWS / 2)), dim3(PA_THREADS), 0, stream, a,
-                       c, b, rows);
-  }
+static void launch_s4(const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, const S4Shape& s, const PagedPlan& rows,
+                      const PagedPlan& tiles, hipStream_t stream) {
+  const unsigned grid = (unsigned)(rows.slots + tiles.slots > 0 ? rows.slots + tiles.slots : 1);
+  if (tiles.slots > 0)
+    hipLaunchKernelGGL((paged_attn_s4_both_kernel<DP, GROUPS, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows, tiles);
+  else
+    hipLaunchKernelGGL((paged_attn_s4_rows_kernel<DP, GROUPS, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows);
+  // an item that is cut has more than a target-th of all keys, so there are fewer than `target` of them
+  auto items = [](const S4Kind& k) { return (unsigned)((k.items < k.target ? (int)k.items : k.target) + 7 & ~7); };
+  if (rows.target > 0 && rows.arrivals == nullptr)
+    hipLaunchKernelGGL((paged_attn_s4_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(items(s.rows) * (PA_ROWS / 2)), dim3(PA_THREADS), 0,
+                       stream, a, c, b, rows);
+  if (tiles.target > 0)
+    hipLaunchKernelGGL((paged_attn_s4_join_kernel<ST_ROWS, ST_JOIN, DP, OUT>), dim3(items(s.tiles) * (ST_ROWS / ST_JOIN)), dim3(PA_THREADS),
+                       0, stream, a, c, b, tiles);
 }
 
 int launch_paged_attn_s4(int out_type, const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, void* workspace,
@@ -453,29 +821,38 @@ int launch_paged_attn_s4(int out_type, const PagedAttn4& a, const PagedCache4& c
   const int group = a.q_heads / c.heads;
   const long long capacity = (long long)b.per_seq << c.page_shift;
   S4Shape s = s4_shape(b.rows, b.seqs, group, c.heads, capacity);
-  if (workspace == nullptr || workspace_bytes < paged_attn_s4_workspace_bytes(b.rows, b.seqs, a.q_heads, c.heads, c.D, capacity))
-    s.target = 0, s.meet = false;
-  if (s.slots > 0x7fffff) return fail(TI_ERR_INVALID_ARG, "paged_attn_s4: %lld work items", s.slots);
-  PagedPlan rows;
-  rows.group = group;
-  rows.least = 0;
-  rows.most = 0x7fffffff;
-  rows.target = s.target;
-  rows.even = true;
-  rows.full = 0x7fffffff;
-  // with a window an item reads its own keys, the first ones, and what its tokens' windows are apart
-  const long long span = a.window > 0 ? (long long)a.window + ((a.sinks + 15) & ~15) + 16 + (PA_ROWS + group - 1) / group + 1 : 0x7fffffff;
-  rows.span = span < 0x7fffffff ? (int)span : 0x7fffffff;
-  rows.slots = (int)s.slots;
-  rows.places = (int)s.places;
-  rows.ws = static_cast<float*>(workspace);
+  const long long rows_bytes = s4_bytes(s.rows, PA_ROWS, c.D);
+  if (workspace == nullptr || workspace_bytes < rows_bytes + s4_bytes(s.tiles, ST_ROWS, c.D))
+    s.rows.target = s.tiles.target = 0, s.meet = false;
+  if (s.rows.slots + s.tiles.slots > 0x7fffff)
+    return fail(TI_ERR_INVALID_ARG, "paged_attn_s4: %lld work items", s.rows.slots + s.tiles.slots);
+  auto plan = [&](const S4Kind& k, int rows_of_item, int least, int most, char* ws) {
+    PagedPlan p;
+    p.group = group;
+    p.least = least;
+    p.most = most;
+    p.target = k.target;
+    p.full = 0x7fffffff;
+    p.even = true;
+    // with a window an item reads its own keys, the first ones, and what its tokens' windows are apart
+    const long long span = a.window > 0 ? (long long)a.window + ((a.sinks + 15) & ~15) + 16 + (rows_of_item + group - 1) / group + 1 : 0x7fffffff;
+    p.span = span < 0x7fffffff ? (int)span : 0x7fffffff;
+    p.slots = (int)k.slots;
+    p.places = (int)k.places;
+    p.ws = reinterpret_cast<float*>(ws);
+    p.arrivals = nullptr;
+    return p;
+  };
+  char* const ws = static_cast<char*>(workspace);
+  PagedPlan rows = plan(s.rows, PA_ROWS, 0, s.tiles.slots > 0 ? PA_ROWS : 0x7fffffff, ws);
+  const PagedPlan tiles = plan(s.tiles, ST_ROWS, s.rows.slots > 0 ? PA_ROWS : 0, 0x7fffffff, ws + (s.rows.target ? rows_bytes : 0));
   const bool meet = a.arrivals != nullptr && a.arrivals_count >= paged_attn_s4_arrivals(b.rows, b.seqs, a.q_heads, c.heads, capacity);
   rows.arrivals = meet && s.meet ? a.arrivals : nullptr;
   auto run = [&](auto dp, auto groups) {
     constexpr int DP = decltype(dp)::value, GROUPS = decltype(groups)::value;
-    if (out_type == PT_S8) launch_s4<DP, GROUPS, PT_S8>(a, c, b, rows, s.items, stream);
-    else if (out_type == PT_F16) launch_s4<DP, GROUPS, PT_F16>(a, c, b, rows, s.items, stream);
-    else launch_s4<DP, GROUPS, PT_BF16>(a, c, b, rows, s.items, stream);
+    if (out_type == PT_S8) launch_s4<DP, GROUPS, PT_S8>(a, c, b, s, rows, tiles, stream);
+    else if (out_type == PT_F16) launch_s4<DP, GROUPS, PT_F16>(a, c, b, s, rows, tiles, stream);
+    else launch_s4<DP, GROUPS, PT_BF16>(a, c, b, s, rows, tiles, stream);
   };
   using std::integral_constant;
   if (s4_dp(c.D) == 64) {
