@@ -27,18 +27,19 @@ struct PagedBatch {
 struct PagedSeq {
   int row0, T, len, end;  // first row, new tokens, cached positions that there are pages for, all positions
 };
-__device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int page_shift, int i) {
+__device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int page_shift, int lo, int hi, int len) {
   PagedSeq s;
   const int cap = b.per_seq << page_shift;
-  int lo = b.cu[i], hi = b.cu[i + 1];
   lo = lo < 0 ? 0 : lo > b.rows ? b.rows : lo;
   hi = hi < lo ? lo : hi > b.rows ? b.rows : hi;
-  const int len = b.lens[i];
   s.row0 = lo;
   s.T = hi - lo;
   s.end = len < 0 ? 0 : len < (1 << 30) ? len : 1 << 30;
   s.len = s.end > cap ? cap : s.end;
   return s;
+}
+__device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int page_shift, int i) {
+  return paged_seq(b, page_shift, b.cu[i], b.cu[i + 1], b.lens[i]);
 }
 
 enum PagedType : int { PT_F32 = 0, PT_F16 = 1, PT_BF16 = 2, PT_S8 = 3 };

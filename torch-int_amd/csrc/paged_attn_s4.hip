@@ -777,7 +777,7 @@ static S4Shape s4_shape(long long rows, long long seqs, long long group, long lo
   // sequences with more than 16 rows are at most a 17th of all rows
   const long long many = rows * group / (PA_ROWS + 1) < seqs ? rows * group / (PA_ROWS + 1) : seqs;
   items(s.tiles, heads * (many + rows * group / ST_ROWS));
-  if (cut && s.tiles.items < ST_PLENTY) s.tiles.cut(PA_TARGET, of_one);
+  if (cut && s.tiles.items < ST_PLENTY) s.tiles.cut(seqs == 1 ? PA_TARGET : PA_TARGET / 2, of_one);
   if (seqs == 1) return s;  // it has more than 16
   items(s.rows, heads * seqs);
   if (cut) s.rows.cut(PA_TARGET / 4, of_one);

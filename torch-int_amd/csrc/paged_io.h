@@ -89,4 +89,31 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedBatch& b, int page_
   return p;
 }
 
+// The same with fewer trips to memory: lane i of a wave asks for the end and the length of sequence i at once, so that of the first 64
+// sequences nothing has to be asked for when it is known which one a row belongs to.
+struct PagedAsked {
+  int first, end, len;
+};
+__device__ __forceinline__ PagedAsked paged_ask(const PagedBatch& b) {
+  const int lane = threadIdx.x & 63;
+  return PagedAsked{b.cu[0], b.cu[lane < b.seqs ? lane + 1 : b.seqs], lane < b.seqs ? b.lens[lane] : 0};
+}
+__device__ __forceinline__ PagedPlace paged_place(const PagedBatch& b, int page_shift, int row, const PagedAsked& asked) {
+  const int seq = paged_seq_of(b, row, asked.end);
+  PagedPlace p = {seq, -1, false};
+  if (seq < b.seqs) {
+    PagedSeq s;
+    if (seq < 64) {
+      s = paged_seq(b, page_shift, seq == 0 ? asked.first : __builtin_amdgcn_readlane(asked.end, seq - 1),
+                    __builtin_amdgcn_readlane(asked.end, seq), __builtin_amdgcn_readlane(asked.len, seq));
+    } else {
+      s = paged_seq(b, page_shift, seq);
+    }
+    p.mine = row >= s.row0 && row < s.row0 + s.T;
+    if (p.mine) p.position = s.end - s.T + (row - s.row0);
+    if (p.position >= s.len) p.position = -1;
+  }
+  return p;
+}
+
 }  // namespace ti
