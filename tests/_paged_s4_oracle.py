@@ -26,11 +26,17 @@ def quantise(y, groups):
     return u[..., :half] + 16 * u[..., half:], ((at << 4) + zero.long()).to(torch.int16)
 
 
+def parts(codes, words):
+    """fp64 steps, codes and zeros of every column [..., d] of codes [..., d / 2] and words [..., groups]."""
+    step, zero = STEPS[((words.int() & 0x7FF0) >> 4).long().clamp(max=len(STEPS) - 1)], (words & 15).double()
+    u = torch.cat([codes % 16, codes // 16], -1).double()
+    return step.repeat_interleave(u.shape[-1] // words.shape[-1], -1), u, zero.repeat_interleave(u.shape[-1] // words.shape[-1], -1)
+
+
 def values(codes, words):
     """fp64 values of codes [..., d / 2] and words [..., groups]."""
-    step, zero = STEPS[((words.int() & 0x7FF0) >> 4).long().clamp(max=len(STEPS) - 1)], (words & 15).double()
-    u = torch.cat([codes % 16, codes // 16], -1).double().unflatten(-1, (words.shape[-1], -1))
-    return (step[..., None] * (u - zero[..., None])).flatten(-2)
+    step, u, zero = parts(codes, words)
+    return step * (u - zero)
 
 
 def append(key, value, caches, block_table, context_lens, cu_new, alpha_k=1.0, alpha_v=1.0, query=None, alpha_q=1.0, cos_sin=None,
@@ -74,7 +80,8 @@ def attention(query, caches, block_table, context_lens, cu_new, alpha_qk, alpha_
     rows, q_heads, d = query.shape
     group = q_heads // heads
     out = torch.zeros(rows, q_heads, d, dtype=torch.float64)
-    size, light, keys = torch.zeros_like(out), torch.zeros_like(out), torch.zeros(rows, 1, 1, dtype=torch.float64)
+    size, light = torch.zeros_like(out), torch.zeros_like(out)
+    keys = torch.zeros(rows, 1, 1, dtype=torch.float64)
     most, mass = torch.zeros(rows, q_heads, 1, dtype=torch.float64), torch.zeros(rows, q_heads, 1, dtype=torch.float64)
     alpha_qk, alpha_pv = f32(alpha_qk), f32(alpha_pv)
     gathered = {}
@@ -86,43 +93,46 @@ def attention(query, caches, block_table, context_lens, cu_new, alpha_qk, alpha_
             at = block_table[b].long()[place // page]
             there = (at >= 0) & (at < pages)
             at = at.clamp(0, pages - 1)
-            gathered[b] = (values(k_cache[at, :, place % page], k_scale[at, :, place % page]),
-                           values(v_cache[at, :, place % page], v_scale[at, :, place % page]), there, place)
-        k, v, there, place = gathered[b]
+            gathered[b] = (*(parts(codes[at, :, place % page], words[at, :, place % page])
+                             for codes, words in ((k_cache, k_scale), (v_cache, v_scale))), there, place)
+        k_parts, v_parts, there, place = gathered[b]
         sees = there & (place <= p)
         if window:
             sees &= (p - place < window) | (place < sinks)
         if not bool(sees.any()):
             continue
-        k, v = k[sees].repeat_interleave(group, 1), v[sees].repeat_interleave(group, 1)
+        (ks, ku, kz), (vs, vu, vz) = ((x[sees].repeat_interleave(group, 1) for x in y) for y in (k_parts, v_parts))
+        k, v = ks * (ku - kz), vs * (vu - vz)
         terms = k * query[row].double()
         s = alpha_qk * terms.sum(-1)  # [positions, q_heads]
         w = torch.softmax(s, 0)
         out[row] = alpha_pv * (w[:, :, None] * v).sum(0)
         size[row] = abs(alpha_pv) * (w[:, :, None] * v.abs()).sum(0)
-        light[row] = abs(alpha_pv) * v.abs().sum(0)
+        light[row] = abs(alpha_pv) * ((vu - vz).abs() * vs.amax((0, 2))[:, None]).sum(0)
         most[row] = 1.4427 * s.abs().amax(0)[:, None]
-        mass[row] = 1.4427 * alpha_qk * terms.abs().sum(-1).amax(0)[:, None]
+        mass[row] = 1.4427 * alpha_qk * d * terms.abs().sum(-1).amax(0)[:, None]
         keys[row] = s.shape[0]
-    return out, (size, light, most, mass * d, keys)
+    return out, (size, light, most, mass, keys)
 
 
 def attention_error(got, want, about, weight_error):
     """Largest error over the bound that the arithmetic allows, which a right kernel keeps at 1 or below.
 
-    `about`: the sum of weight times |value|; of |value|; the largest |score| of a row in powers of two; head_dim times the largest
-    sum of |q k|, in powers of two as well; and the number of keys.
+    `about`: the sum of weight times |value|; of |value| where every step were the row's largest; the largest |score| of
+    a row in powers of two; head_dim times the largest sum of |q k|, in powers of two as well; the number of keys.
 
     A weight 2^(x c + m): x is a sum of head_dim products, exact ones, in fp32, off by head_dim 2^-24 of the sum of their sizes; c =
-    fp32(alpha log2 e) and the multiply-add are off by 2^-24 of the exponent each, and m has one too, so 2^-22 of it; both
-    times ln 2; the hardware's 2^x by 2^-22 more.  The weight is stored with a relative error of ``weight_error``, or, where it is
-    less than 2^-14, in multiples of 2^-24: off by 2^-25 where the row's largest weight counts 2^8 at least, so by 2^-33 of that,
-    which is no more than the denominator.  The same weights are in numerator and denominator, so the context is off by twice
-    these shares, of the sum of weight times |value| and of |value|; sums of `keys` terms in fp32 add at most their number times 2^-24,
-    rescalings and the final quotient 2^-20.  Then one rounding: half a step."""
+    fp32(alpha log2 e) and the multiply-add are off by 2^-24 of the exponent each, and m has one too, so 2^-22 of it; both times
+    ln 2; the hardware's 2^x by 2^-22 more.  The
+    weight, or its product with the value's step, is stored with a relative error of ``weight_error``, or, where it is less than
+    2^-14, in multiples of 2^-24: off by 2^-25, where the row's largest weight, times the next power of two to the largest step, counts
+    2^7 at least.  So a key's part is off by 2^-32 of its value in units of its step, times twice the largest step, in shares of the
+    largest weight, which is no more than the denominator.  Weights in numerator and denominator are off alike, so the context is
+    by twice these shares.  Sums of `keys` terms in fp32 add at most their number times 2^-24, rescalings and the final quotient
+    2^-20.  Then one rounding: half a step."""
     size, light, most, terms, keys = about
     share = 2 * ((most * 2.0 ** -22 + terms * 2.0 ** -24) * 0.7 + 2.0 ** -22 + weight_error) + keys * 2.0 ** -24 + 2.0 ** -20
-    off_by = share * size + 2.0 ** -32 * (light + keys * size)
+    off_by = share * size + 2.0 ** -30 * (light + keys * size)
     if got.dtype is torch.int8:
         bound = 0.5 + off_by
         want = want.clamp(-128, 127)

@@ -122,6 +122,19 @@ def test_attention_of_flat_and_of_peaked_scores(a_qk):
         _attend((a_qk, query), q, caches, table, lens, cu, a_qk, 0.5, out_dtype=torch.float16)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 0), (100, 5)])
+def test_keys_that_outweigh_those_before_them(window, sinks):
+    # peaked rows, whose reference moves by 20 powers of two and more from one block of keys to the next; where the heaviest keys'
+    # values are 0, as those of 4 bits often are, the context is what the keys before them have left
+    g = torch.Generator().manual_seed(1)
+    for lens, new in (([700], [300]), ([700, 90], [1, 2])):
+        cu, lens, table, pages, rows = _batch(g, lens, new, 16)
+        caches = _cache(g, pages, 2, 16, 128, 2)
+        q = _query(g, rows, 8, 128, torch.float16)
+        _attend((lens, new, window), q, caches, table, lens, cu, 3 * _alpha(128, torch.float16), 1.0, window, sinks,
+                ONE_FP16 if rows > 3 else TWO_FP16)
+
+
 @pytest.mark.parametrize("size", [2.0 ** -17, 2.0 ** -12, 3e-3, 300.0, 3000.0])
 def test_values_of_any_size(size):
     # steps from the smallest on, where keys and values are subnormal numbers of fp16, to the largest

@@ -810,6 +810,7 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
   rows.group = tiles.group = group;
   rows.span = tiles.span = 0x7fffffff;
   rows.full = tiles.full = PA_FULL;
+  rows.at_once = tiles.at_once = 0;
   rows.even = tiles.even = false;
   rows.least = 0;
   rows.most = s.tiles_slots > 0 ? PA_ROWS : 0x7fffffff;

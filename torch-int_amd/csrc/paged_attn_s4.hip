@@ -22,6 +22,21 @@ struct S4Bits {
   __device__ __forceinline__ unsigned low(unsigned c) const { return (c & low_mask) | low_one; }
   __device__ __forceinline__ unsigned high(unsigned c) const { return (c & high_mask) | high_one; }
 };
+// The same without the step: u - z.
+struct S4Zero {
+  v2h base[2];
+  __device__ __forceinline__ void set(const S4Bits& b, int nibble, unsigned word) {
+    base[nibble] = __builtin_bit_cast(v2h, b.low(word));
+    if (nibble) base[nibble] -= v2h{(_Float16)960.0f, (_Float16)960.0f};
+  }
+  __device__ __forceinline__ v2h code(const S4Bits& b, unsigned c, int nibble) const {
+    return __builtin_bit_cast(v2h, nibble ? b.high(c) : b.low(c)) - base[nibble];
+  }
+  __device__ __forceinline__ void codes(const S4Bits& b, unsigned c, v2h (&y)[4]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = code(b, i >> 1 ? c >> 8 : c, i & 1);
+  }
+};
 struct S4Two {
   v2h step[2], base[2];  // of low nibbles and of high ones: the step, and 1024 + z or 64 + z
   __device__ __forceinline__ void set(const S4Bits& b, int nibble, unsigned word) {  // `word`: a word in each half
@@ -40,6 +55,30 @@ struct S4Two {
 
 __device__ __forceinline__ v8h join8(v2h a, v2h b, v2h c, v2h d) {
   return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+typedef unsigned short v2us __attribute__((ext_vector_type(2)));
+
+// The sum over the four lanes n, n + 16, n + 32, n + 48, in all of them.
+__device__ __forceinline__ float rows_add(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+// The largest of all lanes, the same in all.
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+  auto step = [&](auto ctrl, auto rows) {
+    const unsigned y = (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    x = x > y ? x : y;
+  };
+  step(std::integral_constant<int, 0x111>(), std::integral_constant<int, 0xf>());
+  step(std::integral_constant<int, 0x112>(), std::integral_constant<int, 0xf>());
+  step(std::integral_constant<int, 0x114>(), std::integral_constant<int, 0xf>());
+  step(std::integral_constant<int, 0x118>(), std::integral_constant<int, 0xf>());
+  step(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());
+  step(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());
+  return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
 }
 
 // Eight neighbouring elements of a query as fp16, in the order 0 2 1 3 4 6 5 7 in which the nibbles of two dwords come apart.
@@ -386,6 +425,8 @@ constexpr int ST_ROWS = 128, ST_KEYS = 64;
 constexpr int ST_PARTS = 4;
 constexpr int ST_JOIN = 32;      // rows that a workgroup joins
 constexpr int ST_PLENTY = 2048;  // items from which on nothing is cut
+constexpr int ST_AT_ONCE = 512;  // workgroups on the chip
+constexpr int ST_TARGET = 1536;  // slices, at most about
 constexpr int s4_tiles_lds(int DP) { return 2 * 2 * ST_KEYS * DP * 2; }  // two steps of K, then of V
 template <int DP, int GROUPS, int OUT>
 __device__ __forceinline__ void s4_tiles(const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, const PagedPlan& p, int index,
@@ -414,11 +455,13 @@ __device__ __forceinline__ void s4_tiles(const PagedAttn4& a, const PagedCache4&
   const S4Span span(a, p0, p1);
   const int places = span.places();
   const int any_from = a.window > 0 ? p0 + 1 - a.window : -0x7fffffff;       // before it no row sees keys, but for first ones
-  const int wave_from = a.window > 0 ? w0 + 1 - a.window : -0x7fffffff;      // nor before this one of the wave
   const int wave_all_from = a.window > 0 ? w1 + 1 - a.window : -0x7fffffff;  // from here on all of its rows do
   const long long lo_ll = (long long)it.split * it.slice;
   const int lo = lo_ll < places ? (int)lo_ll : places;
   const int hi = lo_ll + it.slice < places ? (int)(lo_ll + it.slice) : places;
+
+  int keys = w1 + 1 - span.shift;  // places up to the wave's last key
+  keys = keys < 0 ? 0 : keys < hi ? keys : hi;
 
   v8h qf[KS];
 #pragma unroll
@@ -457,16 +500,18 @@ __device__ __forceinline__ void s4_tiles(const PagedAttn4& a, const PagedCache4&
   const unsigned vcol = (unsigned)(h * 4 * c.token) + (vbyte < half ? (unsigned)vbyte : 0u);
   int kreg[KW];
   unsigned vreg[8], ks, vs[2][2 * GROUPS];
-  bool dead = false;  // the step on its way has keys that no row sees
-  int dead_key = 0;   // its first key
-  int dead_at = 0;    // and place
+  bool dead = false;  // of the values on their way, no row sees some
+  int dead_at = 0, dead_key = 0;
   bool dead_page = false;
-  auto fetch = [&](int s0, int page) {
-    const int block = (s0 >> 4) + wave, key = key_of(block);
-    const bool on = have(page);
-    const unsigned long long at = on ? (unsigned)page : 0u;
-    const auto code = at * c.page + (unsigned)((key & mask) * c.token), word = at * c.scale_page + (unsigned)((key & mask) * (2 * GROUPS));
-    const auto rk = pool(kb + code), rv = pool(vb + code), rks = pool(ksb + word), rvs = pool(vsb + word);
+  auto code_at = [&](int key, int page) {
+    return (unsigned long long)(have(page) ? (unsigned)page : 0u) * c.page + (unsigned)((key & mask) * c.token);
+  };
+  auto word_at = [&](int key, int page) {
+    return (unsigned long long)(have(page) ? (unsigned)page : 0u) * c.scale_page + (unsigned)((key & mask) * (2 * GROUPS));
+  };
+  auto fetch_k = [&](int s0, int page) {
+    const int key = key_of((s0 >> 4) + wave);
+    const auto rk = pool(kb + code_at(key, page)), rks = pool(ksb + word_at(key, page));
     if constexpr (KW == 4) {
       const v4i x = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rk, kcol, 0, 0));
 #pragma unroll
@@ -477,6 +522,10 @@ __device__ __forceinline__ void s4_tiles(const PagedAttn4& a, const PagedCache4&
     }
     if constexpr (GROUPS == 2) ks = __builtin_amdgcn_raw_buffer_load_b32(rks, krow * 4, 0, 0);
     else ks = __builtin_amdgcn_raw_buffer_load_b16(rks, krow * 2, 0, 0);
+  };
+  auto fetch_v = [&](int s0, int page) {
+    const int block = (s0 >> 4) + wave, key = key_of(block);
+    const auto rv = pool(vb + code_at(key, page)), rvs = pool(vsb + word_at(key, page));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if constexpr (GROUPS == 2) {
@@ -493,28 +542,29 @@ __device__ __forceinline__ void s4_tiles(const PagedAttn4& a, const PagedCache4&
         else vreg[i * 4 + j] = __builtin_amdgcn_raw_buffer_load_b8(rv, vcol, (8 * i + j) * c.token, 0);
       }
     }
-    dead_at = block << 4, dead_key = key, dead_page = !on;
-    dead = !on || dead_at + 16 > hi || (key < any_from && key + 16 > a.sinks);
+    dead_at = block << 4, dead_key = key, dead_page = !have(page);
+    dead = dead_page || dead_at + 16 > hi || (key < any_from && key + 16 > a.sinks);
   };
+  // The numbers of keys, in KW / 2 parts, and of values: four parts for their pairs, NDB for the stores.
   auto swizzle = [](int r, int chunk) { return chunk ^ (r & 7); };
-  auto put_k = [&](int slot) {
-    S4Two two;
-    two.set(bits, 0, __builtin_amdgcn_perm(ks, ks, 0x01000100u));
-    two.set(bits, 1, __builtin_amdgcn_perm(ks, ks, GROUPS == 2 ? 0x03020302u : 0x01000100u));
-    const int r = wave * 16 + krow;
-    char* const to = lds + slot * BYTES + r * (DP * 2);
-#pragma unroll
-    for (int i = 0; i < KW / 2; ++i) {
-      v2h u[4], w[4];
-      two.values(bits, (unsigned)kreg[2 * i], u);
-      two.values(bits, (unsigned)kreg[2 * i + 1], w);
-      const int chunk = (kbyte >> 3) + i;
-      *reinterpret_cast<v8h*>(to + swizzle(r, chunk) * 16) = join8(u[0], u[2], w[0], w[2]);
-      *reinterpret_cast<v8h*>(to + swizzle(r, chunk + DP / 16) * 16) = join8(u[1], u[3], w[1], w[3]);
+  const int kto = (wave * 16 + krow) * (DP * 2);
+  S4Two ktwo;
+  auto put_k = [&](int slot, int part) {
+    if (part == 0) {
+      ktwo.set(bits, 0, __builtin_amdgcn_perm(ks, ks, 0x01000100u));
+      ktwo.set(bits, 1, __builtin_amdgcn_perm(ks, ks, GROUPS == 2 ? 0x03020302u : 0x01000100u));
     }
+    v2h u[4], w[4];
+    ktwo.values(bits, (unsigned)kreg[2 * part], u);
+    ktwo.values(bits, (unsigned)kreg[2 * part + 1], w);
+    const int chunk = (kbyte >> 3) + part;
+    char* const to = lds + slot * BYTES + kto;
+    *reinterpret_cast<v8h*>(to + swizzle(krow, chunk) * 16) = join8(u[0], u[2], w[0], w[2]);
+    *reinterpret_cast<v8h*>(to + swizzle(krow, chunk + DP / 16) * 16) = join8(u[1], u[3], w[1], w[3]);
   };
-  auto put_v = [&](int slot) {
-    if (__builtin_expect(dead, 0)) {  // what no row sees is not there: steps, which may be anything, become zeros
+  v2h vy[4][4];
+  auto dead_v = [&] {  // what no row sees is not there: steps, which may be anything, become zeros
+    if (__builtin_expect(dead, 0)) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int at = (i >> 2) * 8 + h * 4 + (i & 3), key = dead_key + at;
@@ -524,24 +574,22 @@ __device__ __forceinline__ void s4_tiles(const PagedAttn4& a, const PagedCache4&
         }
       }
     }
-    v2h y[4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned* const w = vs[j >> 1];
-      S4Two two;
-      if constexpr (GROUPS == 2) {
-        const unsigned first = w[2 * (j & 1)], second = w[2 * (j & 1) + 1];
-        two.set(bits, 0, __builtin_amdgcn_perm(second, first, 0x05040100u));
-        two.set(bits, 1, __builtin_amdgcn_perm(second, first, 0x07060302u));
-      } else {
-        two.set(bits, 0, w[j & 1]);
-        two.set(bits, 1, w[j & 1]);
-      }
-      two.values(bits, vreg[2 * j] | vreg[2 * j + 1] << 16, y[j]);
+  };
+  auto make_v = [&](int j) {
+    const unsigned* const w = vs[j >> 1];
+    S4Two two;
+    if constexpr (GROUPS == 2) {
+      const unsigned first = w[2 * (j & 1)], second = w[2 * (j & 1) + 1];
+      two.set(bits, 0, __builtin_amdgcn_perm(second, first, 0x05040100u));
+      two.set(bits, 1, __builtin_amdgcn_perm(second, first, 0x07060302u));
+    } else {
+      two.set(bits, 0, w[j & 1]);
+      two.set(bits, 1, w[j & 1]);
     }
-#pragma unroll
-    for (int i = 0; i < NDB; ++i)
-      *reinterpret_cast<v8h*>(lds + 2 * BYTES + slot * BYTES + ((wave * NDB + i) * 64 + lane) * 16) = join8(y[0][i], y[1][i], y[2][i], y[3][i]);
+    two.values(bits, vreg[2 * j] | vreg[2 * j + 1] << 16, vy[j]);
+  };
+  auto put_v = [&](int slot, int i) {
+    *reinterpret_cast<v8h*>(lds + 2 * BYTES + slot * BYTES + ((wave * NDB + i) * 64 + lane) * 16) = join8(vy[0][i], vy[1][i], vy[2][i], vy[3][i]);
   };
 
   float off = PA_EMPTY, den = 0.0f;
@@ -551,105 +599,209 @@ __device__ __forceinline__ void s4_tiles(const PagedAttn4& a, const PagedCache4&
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[i][r] = 0.0f;
 
+  // 32 keys: the softmax of their scores into their probabilities, beside it the scores of the next 32 and the products of the 32
+  // before, in bundles that the compiler keeps in order: a matrix instruction, then what runs beside it.  Their operands go
+  // through a ring of RING registers of 16 bytes a lane, read from the LDS RING - 1 bundles ahead.  Scores are two bundles ahead of
+  // the products at the end, so that their largest is there when the next 32 begin.
+  constexpr int BUNDLES = 2 * KS, RING = 4;
+  struct Half {
+    v16f x;     // scores
+    float top;  // the largest of them
+    v8h pr[2];  // probabilities
+  };
+  v8h op[RING];
+  const int klane = n * (DP * 2) + ((h ^ (n & 7)) << 4);
+  auto is_score = [](int m) { return m <= BUNDLES - 4 ? (m & 1) == 0 : m == BUNDLES - 3; };
+  auto number = [](int m) { return m <= BUNDLES - 4 ? m >> 1 : m == BUNDLES - 3 ? KS - 1 : m - KS; };
+  // operand m of the 32 keys whose scores come from the keys at `k` and whose products are of the values at `v`
+  auto read = [&](int m, int k, int v) {
+    if (is_score(m)) op[m % RING] = *reinterpret_cast<const v8h*>(lds + ((k + klane) ^ (number(m) << 5)));
+    else op[m % RING] = *reinterpret_cast<const v8h*>(lds + v + (number(m) * 64 + lane) * 16);
+  };
+  // `ahead`: whether the operands that the next 32 keys begin with may be read already, from k_next and v_next
+  auto run = [&](Half& now, Half& next, v8h (&before)[2], int k, int v, bool ahead, int k_next, int v_next, auto beside) {
+    if (__builtin_expect(__ballot(__builtin_fmaf(now.top, cl, off) > 15.0f) != 0, 0)) {
+      // A new reference.  It moves by a whole number, so that what is relative to the old one is scaled without rounding.
+      auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(now.top), __float_as_uint(now.top), false, false);
+      const float top = __builtin_fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
+      const float above = __builtin_fmaf(top, cl, off) - 8.0f;
+      const bool moves = above > 7.0f, first = off == PA_EMPTY;
+      const float by = moves ? __builtin_ceilf(above) : 0.0f;
+      const float scale = first && moves ? 0.0f : __builtin_amdgcn_exp2f(-by);
+      off = !moves ? off : first ? __builtin_fmaf(-top, cl, 8.0f) : off - by;
+      den *= scale;
+      // (in two steps: a probability of 2^15 is still one of fp16 where it is to become 2^-20, the factor for it is not)
+      const float part = __builtin_floorf(by * 0.5f);
+      const _Float16 scale_1 = (_Float16)__builtin_amdgcn_exp2f(-part), scale_2 = (_Float16)__builtin_amdgcn_exp2f(part - by);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) before[q] = before[q] * scale_1 * scale_2;
+#pragma unroll
+      for (int i = 0; i < NDB; ++i) acc[i] *= scale;
+    }
+    v16f t;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t[r] = 0.0f;
+    float e[16];
+    v2h two[8];
+    constexpr int EACH = 16 / BUNDLES;  // scores to a bundle
+    auto softmax = [&](int m) {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int r = m * EACH + i;
+        if (r < 16) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(now.x[r], cl, off));
+        if (r >= 3 && r < 19 && (r & 1)) {
+          const v2f pair = {e[r - 3], e[r - 2]};
+          two[(r - 3) >> 1] = __builtin_convertvector(pair, v2h);
+          asm volatile("" : "+v"(two[(r - 3) >> 1]));  // computed here, not where the next 32 keys need it
+        }
+        if (r >= 4 && r < 20 && !(r & 1)) den = __builtin_amdgcn_fdot2(two[(r - 4) >> 1], v2h{(_Float16)1.0f, (_Float16)1.0f}, den, false);
+      }
+    };
+#pragma unroll
+    for (int m = 0; m < BUNDLES; ++m) {
+      __builtin_amdgcn_sched_barrier(0);
+      const int i = number(m);
+      if (is_score(m)) t = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[m % RING], qf[i], t, 0, 0, 0);
+      else acc[i % NDB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(op[m % RING], before[i / NDB], acc[i % NDB], 0, 0, 0);
+      softmax(m);
+      if (m + RING - 1 < BUNDLES) read(m + RING - 1, k, v);
+      else if (ahead) read(m + RING - 1 - BUNDLES, k_next, v_next);
+      beside(m);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int m = BUNDLES; m * EACH < 20; ++m) softmax(m);
+    next.top = t[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) next.top = __builtin_fmaxf(next.top, t[r]);
+    asm volatile("" : "+v"(den), "+v"(next.top));
+    next.x = t;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) now.pr[q] = join8(two[4 * q], two[4 * q + 1], two[4 * q + 2], two[4 * q + 3]);
+  };
+
   if (lo < hi) {
     // whether the pool lacks any of the item's pages: looked at once, so that steps need not
     bool holes = false;
     for (int i = (lo >> 4) + lane; i <= last_block; i += 64) holes |= !have(table[key_of(i) >> c.page_shift]);
     holes = __ballot(holes) != 0;
+    // Pages are looked up a step ahead, by vector loads: these return in order, so that the wait for the keys and values in
+    // front of one is all the wait it needs (a scalar one would have to be over at every wait for the LDS).
+    int zero = 0;
+    asm("" : "+v"(zero));
+    auto ask = [&](int s0) { return b.table[(long long)it.seq * b.per_seq + (key_of((s0 >> 4) + wave) >> c.page_shift) + zero]; };
     auto page_at = [&](int s0) { return table[key_of((s0 >> 4) + wave) >> c.page_shift]; };
-    fetch(lo, page_at(lo));
-    int page = page_at(lo + ST_KEYS);
+    const int page0 = page_at(lo), page1 = page_at(lo + ST_KEYS);
+    int asked = ask(lo + 2 * ST_KEYS);
+    fetch_k(lo, page0);
+    fetch_v(lo, page0);
     if (c.D < DP) {  // chunks behind the head size are never written: zeros, as Q is there
       for (int i = threadIdx.x * 16; i < 2 * BYTES; i += PA_THREADS * 16) *reinterpret_cast<v4i*>(lds + i) = v4i{0, 0, 0, 0};
       __syncthreads();
     }
-    put_k(0);
-    put_v(0);
-    fetch(lo + ST_KEYS, page);
-    page = page_at(lo + 2 * ST_KEYS);
+#pragma unroll
+    for (int i = 0; i < KW / 2; ++i) put_k(0, i);
+    fetch_k(lo + ST_KEYS, page1);
+    dead_v();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) make_v(j);
+#pragma unroll
+    for (int i = 0; i < NDB; ++i) put_v(0, i);
+    fetch_v(lo + ST_KEYS, page1);
     __syncthreads();
-    int slot = 0;
-    for (int s0 = lo; s0 < hi; s0 += ST_KEYS) {
-      const char* const kl = lds + slot * BYTES;
-      const char* const vl = lds + 2 * BYTES + slot * BYTES;
-      // the places of the four blocks of 16 keys, and whether the wave's rows see all of them, or none
-      int key[4];
+    // keys whose scores do not count: masks, and pages that are lost
+    auto hide = [&](v16f& x, float& top, int s0) {
+      const int k0 = key_of(s0 >> 4), k1 = key_of((s0 >> 4) + 1);
+      if (__builtin_expect(s0 + 32 > hi || k1 + 15 > w0 || k0 < wave_all_from || holes, 0)) {
+        bool on[2] = {true, true};
+        if (holes) on[0] = have(table[k0 >> c.page_shift]), on[1] = have(table[k1 >> c.page_shift]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) key[i] = key_of((s0 >> 4) + i);
-      v16f x[2];
-      bool any[2];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        any[q] = s0 + 32 * q < hi && key[2 * q] <= w1 && (key[2 * q + 1] + 16 > wave_from || key[2 * q] < a.sinks);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[q][r] = 0.0f;
-        if (any[q]) {
-#pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            const v8h kf = *reinterpret_cast<const v8h*>(kl + (32 * q + n) * (DP * 2) + swizzle(n, 2 * i + h) * 16);
-            x[q] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[i], x[q], 0, 0, 0);
-          }
+        for (int r = 0; r < 16; ++r) {
+          const int at = (r & 3) + 8 * ((r >> 2) & 1) + 4 * h, mine = (r >> 3 ? k1 : k0) + at;
+          if (s0 + 16 * (r >> 3) + at >= hi || mine >= limit || !on[r >> 3] || (mine < from && mine >= a.sinks)) x[r] = -__builtin_inff();
         }
+        top = x[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = __builtin_fmaxf(top, x[r]);
       }
-      // the next step's keys and values, which have arrived, become numbers
-      put_k(slot ^ 1);
-      put_v(slot ^ 1);
-      fetch(s0 + 2 * ST_KEYS, page);
-      page = page_at(s0 + 3 * ST_KEYS);
+    };
+    Half even, odd;
+    {
+      v16f t;
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        if (!any[q]) continue;
-        if (__builtin_expect(s0 + 32 * q + 32 > hi || key[2 * q + 1] + 15 > w0 || key[2 * q] < wave_all_from || holes, 0)) {
-          bool on[2] = {true, true};
-          if (holes) {
+      for (int r = 0; r < 16; ++r) t[r] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) on[i] = have(table[key[2 * q + i] >> c.page_shift]);
-          }
+      for (int i = 0; i < KS; ++i)
+        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const v8h*>(lds + (klane ^ (i << 5))), qf[i], t, 0, 0, 0);
+      even.x = t;
+      even.top = t[0];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int at = (r & 3) + 8 * ((r >> 2) & 1) + 4 * h, mine = key[2 * q + (r >> 3)] + at;
-            if (s0 + 32 * q + 16 * (r >> 3) + at >= hi || mine >= limit || !on[r >> 3] || (mine < from && mine >= a.sinks))
-              x[q][r] = -__builtin_inff();
-          }
+      for (int r = 1; r < 16; ++r) even.top = __builtin_fmaxf(even.top, t[r]);
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) odd.pr[q][j] = (_Float16)0.0f;
+    // A step is 64 keys, in two halves.  Beside the first: the scores of the second, the products of the second half before it (in the
+    // first step of its own, times zero), and keys of the next step become numbers.  Beside the second: the scores of the next step's
+    // first half, the products of the first, and values of the next step become numbers.  Keys and values have two places each; the
+    // barrier between the halves makes sure that what the second reads is there, and that what is written behind it has been read.
+    constexpr int K_HALF = 32 * DP * 2, V0 = 2 * BYTES, V_HALF = BYTES / 2;
+    int slot = 0, v_before = V0 + V_HALF;
+#pragma unroll
+    for (int m = 0; m < RING - 1; ++m) read(m, K_HALF, v_before);
+    int s0 = lo, page = 0;
+    for (;;) {
+      const int other = slot ^ 1, k_other = other * BYTES, v_now = V0 + slot * BYTES;
+      // the same for all lanes: with the half behind its last keys a wave gathers those
+      const bool here = __builtin_amdgcn_readfirstlane(s0 < keys + 32) != 0;
+      auto stage_k = [&](int m) {
+        if (m == 0) page = __builtin_amdgcn_readfirstlane(asked);
+#pragma unroll
+        for (int i = 0; i < KW / 2; ++i)
+          if (m == KS / 2 + i * (KS / 4)) put_k(other, i);
+        if (m == BUNDLES - 2) {
+          fetch_k(s0 + 2 * ST_KEYS, page);
+          asked = ask(s0 + 3 * ST_KEYS);
         }
-        float top = x[q][0];
+      };
+      auto stage_v = [&](int m) {
+        if (m == KS / 4) dead_v();
 #pragma unroll
-        for (int r = 1; r < 16; ++r) top = __builtin_fmaxf(top, x[q][r]);
-        if (__builtin_expect(__ballot(__builtin_fmaf(top, cl, off) > 15.0f) != 0, 0)) {
-          auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-          top = __builtin_fmaxf(__uint_as_float(o[0]), __uint_as_float(o[1]));
-          if (__builtin_fmaf(top, cl, off) > 15.0f) {
-            const float fresh = 8.0f - top * cl;
-            const float scale = __builtin_amdgcn_exp2f(fresh - off);
-            off = fresh;
-            den *= scale;
+        for (int j = 0; j < 4; ++j)
+          if (m == KS / 4 + j * (KS / 4)) make_v(j);
 #pragma unroll
-            for (int i = 0; i < NDB; ++i) acc[i] *= scale;
-          }
-        }
-        v8h pr[2];
+        for (int i = 0; i < NDB; ++i)
+          if (m == KS + KS / 4 + (i * KS / 4) / (NDB / 2)) put_v(other, i);
+        if (m == BUNDLES - 1) fetch_v(s0 + 2 * ST_KEYS, page);
+      };
+      if (__builtin_expect(here, 1)) {
+        hide(even.x, even.top, s0);
+        run(even, odd, odd.pr, slot * BYTES + K_HALF, v_before, false, 0, 0, stage_k);
+      } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          v2h two[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const v2f e = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[q][8 * i + 2 * j], cl, off)),
-                           __builtin_amdgcn_exp2f(__builtin_fmaf(x[q][8 * i + 2 * j + 1], cl, off))};
-            two[j] = __builtin_convertvector(e, v2h);
-            den = __builtin_amdgcn_fdot2(two[j], v2h{(_Float16)1.0f, (_Float16)1.0f}, den, false);
-          }
-          pr[i] = join8(two[0], two[1], two[2], two[3]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < NDB; ++j) {
-            const v8h vf = *reinterpret_cast<const v8h*>(vl + (((2 * q + i) * NDB + j) * 64 + lane) * 16);
-            acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pr[i], acc[j], 0, 0, 0);
-          }
+        for (int m = 0; m < BUNDLES; ++m) stage_k(m);
       }
       __syncthreads();
-      slot ^= 1;
+      if (__builtin_expect(here, 1)) {
+#pragma unroll
+        for (int m = 0; m < RING - 1; ++m) read(m, k_other, v_now);
+        hide(odd.x, odd.top, s0 + 32);
+        run(odd, even, even.pr, k_other, v_now, true, k_other + K_HALF, v_now + V_HALF, stage_v);
+      } else {
+#pragma unroll
+        for (int m = 0; m < BUNDLES; ++m) stage_v(m);
+      }
+      v_before = v_now + V_HALF;
+      slot = other;
+      s0 += ST_KEYS;
+      if (s0 >= hi) break;
+    }
+    if (s0 < keys + 32) {  // nobody has gathered them: the wave's keys reach into the last half
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+        acc[i % NDB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const v8h*>(lds + v_before + (i * 64 + lane) * 16),
+                                                              odd.pr[i / NDB], acc[i % NDB], 0, 0, 0);
     }
   }
 
@@ -697,7 +849,7 @@ __device__ __forceinline__ void s4_tiles(const PagedAttn4& a, const PagedCache4&
 }
 
 template <int DP, int GROUPS, int OUT>
-__global__ __launch_bounds__(PA_THREADS, 4) void paged_attn_s4_rows_kernel(PagedAttn4 a, PagedCache4 c, PagedBatch b, PagedPlan rows) {
+__global__ __launch_bounds__(PA_THREADS, DP == 128 && GROUPS == 2 ? 3 : 4) void paged_attn_s4_rows_kernel(PagedAttn4 a, PagedCache4 c, PagedBatch b, PagedPlan rows) {
   __shared__ __attribute__((aligned(16))) char lds[s4_rows_lds(DP)];
   const int lo = b.cu[0], hi = b.cu[b.seqs];  // (on their way beside what the item needs)
   s4_rows<DP, GROUPS, OUT>(a, c, b, rows, blockIdx.x, lds);
@@ -777,7 +929,7 @@ static S4Shape s4_shape(long long rows, long long seqs, long long group, long lo
   // sequences with more than 16 rows are at most a 17th of all rows
   const long long many = rows * group / (PA_ROWS + 1) < seqs ? rows * group / (PA_ROWS + 1) : seqs;
   items(s.tiles, heads * (many + rows * group / ST_ROWS));
-  if (cut && s.tiles.items < ST_PLENTY) s.tiles.cut(seqs == 1 ? PA_TARGET : PA_TARGET / 2, of_one);
+  if (cut && s.tiles.items < ST_PLENTY) s.tiles.cut(ST_TARGET, of_one);
   if (seqs == 1) return s;  // it has more than 16
   items(s.rows, heads * seqs);
   if (cut) s.rows.cut(PA_TARGET / 4, of_one);
@@ -833,6 +985,7 @@ int launch_paged_attn_s4(int out_type, const PagedAttn4& a, const PagedCache4& c
     p.most = most;
     p.target = k.target;
     p.full = 0x7fffffff;
+    p.at_once = rows_of_item == ST_ROWS ? ST_AT_ONCE : 0;
     p.even = true;
     // with a window an item reads its own keys, the first ones, and what its tokens' windows are apart
     const long long span = a.window > 0 ? (long long)a.window + ((a.sinks + 15) & ~15) + 16 + (rows_of_item + group - 1) / group + 1 : 0x7fffffff;

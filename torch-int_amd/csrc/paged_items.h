@@ -16,6 +16,7 @@ constexpr int PA_ROWS = 16;
 constexpr int PA_TARGET = 512;     // slices that the keys of a batch are cut into, beyond one to each item
 constexpr int PA_FULL = 512;       // items that fill the chip
 constexpr int PA_MIN_SLICE = 512;  // keys of a slice, at least
+constexpr float PA_SORTED = 2048;  // items from which on they are not put in order
 constexpr float PA_EMPTY = 3.0e38f;  // offset of a row that has seen no key: 2^(-inf + PA_EMPTY) is 0
 
 // The sequences that one of the two kernels takes, by how many rows a key head has in them, and how their keys are cut.
@@ -24,6 +25,7 @@ struct PagedPlan {
   int least, most;  // rows of a sequence: more than `least`, up to `most`
   int target;       // slices that the keys are cut into; 0: nothing is cut
   int full;         // items that fill the chip
+  int at_once;      // workgroups that run at once, where slices are chosen for them to come out even; else 0
   bool even;        // slices of an item are of one length, up to half as long again, instead of the last one being what is left
   int span;         // keys that an item reads, at most
   int slots;        // work items at most, slices included: what the grid holds
@@ -93,6 +95,22 @@ __device__ __forceinline__ int paged_slice(float items, float total, int target,
   return slice < PA_MIN_SLICE ? PA_MIN_SLICE : slice;
 }
 
+// The same for items that take long, `at_once` of them at a time: cut into as many slices as make the last round of workgroups least
+// in vain.  A workgroup costs some 170 keys before and behind its own, one that is joined some 700.
+__device__ __forceinline__ int paged_slice_even(float items, float total, int target, int at_once) {
+  const float keys = total / __builtin_fmaxf(items, 1.0f);
+  float best = __builtin_ceilf(items / (float)at_once) * (keys + 170.0f);
+  float slice = 2.0f * keys;
+  for (int k = 2; k <= 16; ++k) {
+    const float n = items * (float)k;
+    if (n > (float)target || keys < (float)(k * PA_MIN_SLICE)) break;
+    const float cost = __builtin_ceilf(n / (float)at_once) * (keys / (float)k + 700.0f);
+    if (cost < best) best = cost, slice = keys / (float)k;
+  }
+  const int want = slice < 1.0e9f ? ((int)slice + 63) & ~63 : 1 << 30;
+  return want < PA_MIN_SLICE ? PA_MIN_SLICE : want;
+}
+
 // The work item with number `index`, in the order part, sequence, slice, tile of rows, head.  A sequence's tiles come from the
 // last, which has the most keys, to the first, in PARTS parts, so that the long items of all sequences begin before the short
 // ones.  SORTED: instead, in PARTS classes of sequences, those of long slices first.  CUT: the first slice of the `index`-th item
@@ -116,6 +134,7 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
     }
   };
   it.slice = 0x7fffffff;
+  float count = 2.0f * PA_SORTED;
   if (p.target != 0) {
     float items = 0.0f, total = 0.0f;
     for (int i0 = (b.seqs - 1) & ~63; i0 >= 0; i0 -= 64) {  // the first 64 come last and stay
@@ -123,7 +142,9 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
       items += wave_add((float)tiles);
       total += wave_add((float)tiles * (float)(s.len < p.span ? s.len : p.span));
     }
-    it.slice = paged_slice(items * (float)heads, total * (float)heads, p.target, p.full);
+    count = items * (float)heads;
+    it.slice = p.at_once != 0 ? paged_slice_even(items * (float)heads, total * (float)heads, p.target, p.at_once)
+                              : paged_slice(items * (float)heads, total * (float)heads, p.target, p.full);
   }
   int before = 0, before_cut = 0, before_sliced = 0;
   int splits = 1;
@@ -139,14 +160,17 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
     cut_up();
     if (CUT && cuts == 0) return it;
   }
-  for (int part = 0, i0 = 0; part < PARTS; i0 + 64 < b.seqs ? i0 += 64 : (i0 = 0, ++part)) {
+  // (of many items the last ones are a small part: they come as they are)
+  const bool sorted = SORTED && count < PA_SORTED;
+  const int parts = SORTED && !sorted ? 1 : PARTS;
+  for (int part = 0, i0 = 0; part < parts; i0 + 64 < b.seqs ? i0 += 64 : (i0 = 0, ++part)) {
     if (b.seqs > 64) {
       look(i0);
       cut_up();
     }
     const int behind = PARTS == 1 || SORTED ? 0 : (int)((long long)tiles * part / PARTS);  // tiles of the parts before
     int here = PARTS == 1 || SORTED ? tiles : (int)((long long)tiles * (part + 1) / PARTS) - behind;
-    if (SORTED) {  // (four classes)
+    if (sorted) {  // (four classes)
       const int keys = (s.len < p.span ? s.len : p.span) / splits, want = it.slice;
       const int mine = keys > want ? 0 : keys > (want >> 1) + (want >> 2) ? 1 : keys > want >> 1 ? 2 : 3;
       here = mine == part ? tiles : 0;
