@@ -125,7 +125,14 @@ struct S4Span {
   __device__ __forceinline__ int key(int place) const { return place < head ? place : place + shift; }
 };
 
-// Few rows: 16 to a workgroup, its four waves take 32 keys each in turn.
+// Few rows: 16 to a workgroup, its four waves take 32 keys each in turn.  A SIMD issues one instruction of any kind in four cycles, and
+// with one or a few rows to a key that is what bounds it, so what is done to a code is as little as can be: it becomes u - z, and
+// the steps are multiplied into scores and weights:
+//   q . k = s sum q (u - z),   sum_j p_j v_j = sum_j (p_j s_j) (u_j - z_j),
+// where the weights p s go in as two fp16 numbers (22 bits).  Two groups have sums and weights of their own.  Steps reach from 2^-20
+// to 2^13, so the reference M keeps p times the largest step of the keys so far at 2^15 or less.
+// (Codes as they are, subnormal fp16 numbers u 2^-24, and z times the sums of q and of weights taken off behind the products
+// would be a fifth less to issue, but the matrix pipe adds subnormal numbers with 2^-20 of their sum lost.)
 constexpr int s4_rows_lds(int DP) { return PA_WAVES * PA_ROWS * (DP + 4 + 2) * 4; }
 template <int DP, int GROUPS, int OUT>
 __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, const PagedPlan& p, int index,
@@ -178,55 +185,68 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
   const uint8_t* vb = c.v + it.head * c.head;
   const char* ksb = reinterpret_cast<const char*>(c.k_scale) + it.head * c.scale_head;
   const char* vsb = reinterpret_cast<const char*>(c.v_scale) + it.head * c.scale_head;
-  // The table through the constant address space: nothing writes to it while the kernel runs, and scalar loads are counted
-  // apart from the keys and values in flight, which a vector load would have to wait for.
-  const auto table = (const __attribute__((address_space(4))) int*)(b.table + (long long)it.seq * b.per_seq);
+  const int* const table = b.table + (long long)it.seq * b.per_seq;
   const int mask = (1 << c.page_shift) - 1, last_block = hi > 0 ? (hi - 1) >> 4 : 0;
   const int head_blocks = span.head >> 4, shift_blocks = span.shift >> 4;
 
-  const S4Bits bits;
-  float off = PA_EMPTY;
-  v4f acc[NB], dsum = {0, 0, 0, 0};
+  float off = PA_EMPTY, dsum = 0.0f, most = 35.0f;  // 2^most times the largest step so far is 2^15 (the smallest there is: 2^-20)
+  unsigned top_word = 15;                           // a word no less than those so far, bits of z set
+  v4f acc[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) acc[i] = v4f{0, 0, 0, 0};
-  v8h ones;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) ones[i] = (_Float16)1.0f;
 
-  // Two blocks of 16 keys: their first keys, their pages; where these are, and what a lane has of them.
-  struct Blocks {
-    int key[2], page[2];
+  // The places of the wave's next 64 blocks of 16 keys, two to a step, one to a lane: bytes from a pool's start, first key, and whether
+  // there is something to hide in it.  Blocks behind the last key are hidden, and read where there is memory.
+  constexpr int STRIDE = PA_WAVES * 32;
+  unsigned long long code = 0, word = 0, odd = 0, lost = 0;
+  int key = 0;
+  auto look = [&](int s0) {
+    const int place = (s0 >> 4) + (lane >> 1) * (STRIDE / 16) + (lane & 1);
+    int at = place < last_block ? place : last_block;
+    at = at < head_blocks ? at : at + shift_blocks;
+    key = at << 4;
+    const int page = table[key >> c.page_shift];
+    const bool have = (unsigned)page < (unsigned)c.pages;
+    const unsigned long long there = have ? (unsigned)page : 0u;
+    code = there * c.page + (unsigned)((key & mask) * c.token);
+    word = there * c.scale_page + (unsigned)((key & mask) * (2 * GROUPS));
+    lost = __ballot(!have);
+    odd = lost | __ballot((place << 4) + 16 > hi || key + 16 > p0 + 1 || key < all_from);
   };
-  auto blocks_at = [&](int s0) {  // asks for the pages; blocks behind the last key are masked, and read where there is memory
-    Blocks w;
-#pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
-      int at = (s0 >> 4) + blk;
-      at = at < last_block ? at : last_block;
-      at = at < head_blocks ? at : at + shift_blocks;
-      w.key[blk] = at << 4;
-      w.page[blk] = table[w.key[blk] >> c.page_shift];
-    }
-    return w;
-  };
-  auto have = [&](int page) { return (unsigned)page < (unsigned)c.pages; };
   // by buffer instructions: what a lane adds is one register, the block's place in scalar ones
   auto pool = [](const void* from) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(from), 0, -1, 0x00020000); };
-  auto code_place = [&](const Blocks& w, int blk) {
-    return (have(w.page[blk]) ? (unsigned)w.page[blk] : 0u) * c.page + (unsigned)((w.key[blk] & mask) * c.token);
-  };
-  auto word_place = [&](const Blocks& w, int blk) {
-    return (have(w.page[blk]) ? (unsigned)w.page[blk] : 0u) * c.scale_page + (unsigned)((w.key[blk] & mask) * (2 * GROUPS));
+  auto lane64 = [](unsigned long long x, int i) {
+    return (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32 | (unsigned)__builtin_amdgcn_readlane((int)x, i);
   };
   const unsigned kcol = (unsigned)(n * c.token) + (unsigned)kbyte;
   const int vbyte = (n * NB / 2) & ~3;
   const unsigned vcol = (unsigned)(kg * 4 * c.token) + (vbyte < half ? (unsigned)vbyte : 0u);
   int k[2][KW];
-  unsigned v[8], ks[2], vs[2][2 * GROUPS];
-  auto fetch_k = [&](const Blocks& w) {
+  unsigned v[8], kz[2], ks[2][2 * GROUPS], vs[2][2 * GROUPS];  // (words of K: of the lane's key, and of those whose scores it gets)
+  auto fetch_words = [&](unsigned (&w)[2 * GROUPS], const char* from) {
+    const auto r = pool(from);
+    if constexpr (GROUPS == 2) {
+      const v4i x = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, kg * 16, 0, 0));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = (unsigned)x[i];
+    } else {
+      const int2 x = __builtin_bit_cast(int2, __builtin_amdgcn_raw_buffer_load_b64(r, kg * 8, 0, 0));
+      w[0] = (unsigned)x.x, w[1] = (unsigned)x.y;
+    }
+  };
+  struct Places {
+    unsigned long long code[2], word[2];
+  };
+  auto places_of = [&](int i) {  // of step i of the 32 that have been looked up
+    Places w;
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) w.code[blk] = lane64(code, 2 * i + blk), w.word[blk] = lane64(word, 2 * i + blk);
+    return w;
+  };
+  auto fetch_k = [&](const Places& w) {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      const auto r = pool(kb + code_place(w, blk)), rw = pool(ksb + word_place(w, blk));
+      const auto r = pool(kb + w.code[blk]);
       if constexpr (KW == 4) {
         const v4i x = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(r, kcol, 0, 0));
 #pragma unroll
@@ -235,74 +255,91 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
         const int2 x = __builtin_bit_cast(int2, __builtin_amdgcn_raw_buffer_load_b64(r, kcol, 0, 0));
         k[blk][0] = x.x, k[blk][1] = x.y;
       }
-      if constexpr (GROUPS == 2) ks[blk] = __builtin_amdgcn_raw_buffer_load_b32(rw, n * 4, 0, 0);
-      else ks[blk] = __builtin_amdgcn_raw_buffer_load_b16(rw, n * 2, 0, 0);
+      fetch_words(ks[blk], ksb + w.word[blk]);
+      if constexpr (GROUPS == 2) kz[blk] = __builtin_amdgcn_raw_buffer_load_b32(pool(ksb + w.word[blk]), n * 4, 0, 0);
+      else kz[blk] = __builtin_amdgcn_raw_buffer_load_b16(pool(ksb + w.word[blk]), n * 2, 0, 0);
     }
   };
-  auto fetch_v = [&](const Blocks& w) {
+  auto fetch_v = [&](const Places& w) {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      const auto r = pool(vb + code_place(w, blk)), rw = pool(vsb + word_place(w, blk));
-      if constexpr (GROUPS == 2) {
-        const v4i x = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, kg * 16, 0, 0));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vs[blk][i] = (unsigned)x[i];
-      } else {
-        const int2 x = __builtin_bit_cast(int2, __builtin_amdgcn_raw_buffer_load_b64(rw, kg * 8, 0, 0));
-        vs[blk][0] = (unsigned)x.x, vs[blk][1] = (unsigned)x.y;
-      }
+      fetch_words(vs[blk], vsb + w.word[blk]);
+      const auto r = pool(vb + w.code[blk]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[blk * 4 + j] = __builtin_amdgcn_raw_buffer_load_b32(r, vcol, j * c.token, 0);
     }
   };
-  const unsigned vpick = DP == 128 || (n & 1) == 0 ? 0x05040100u : 0x07060302u;  // the half of a dword of V that this lane has
+  const S4Bits bits;
+  unsigned steps = 0x7ff07ff0u;
+  float minus = -1.0f;  // (kept out of the compiler's sight, as the zero is put in its way, for one instruction instead of two)
+  asm("" : "+s"(steps), "+v"(minus));
+  auto halves = [](unsigned x) { return __builtin_bit_cast(v2h, x); };
+  auto times = [](_Float16 s, float x) { return __builtin_fmaf((float)s, x, 0.0f); };
   auto scores = [&](float (&x)[8]) {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      S4Two two;
-      two.set(bits, 0, __builtin_amdgcn_perm(ks[blk], ks[blk], 0x01000100u));
-      two.set(bits, 1, __builtin_amdgcn_perm(ks[blk], ks[blk], GROUPS == 2 ? 0x03020302u : 0x01000100u));
-      v4f s = {0, 0, 0, 0};
+      S4Zero zero;
+      zero.set(bits, 0, __builtin_amdgcn_perm(kz[blk], kz[blk], 0x01000100u));
+      zero.set(bits, 1, __builtin_amdgcn_perm(kz[blk], kz[blk], GROUPS == 2 ? 0x03020302u : 0x01000100u));
+      v4f d0 = {0, 0, 0, 0}, d1 = {0, 0, 0, 0};  // of low nibbles and of high ones
 #pragma unroll
       for (int i = 0; i < KW / 2; ++i) {
         v2h u[4], w[4];
-        two.values(bits, (unsigned)k[blk][2 * i], u);
-        two.values(bits, (unsigned)k[blk][2 * i + 1], w);
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(join8(u[0], u[2], w[0], w[2]), qf[i], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(join8(u[1], u[3], w[1], w[3]), qf[KW / 2 + i], s, 0, 0, 0);
+        zero.codes(bits, (unsigned)k[blk][2 * i], u);
+        zero.codes(bits, (unsigned)k[blk][2 * i + 1], w);
+        d0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(join8(u[0], u[2], w[0], w[2]), qf[i], d0, 0, 0, 0);
+        v4f& high = GROUPS == 2 ? d1 : d0;
+        high = __builtin_amdgcn_mfma_f32_16x16x32_f16(join8(u[1], u[3], w[1], w[3]), qf[KW / 2 + i], high, 0, 0, 0);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[blk * 4 + r] = s[r];
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (GROUPS == 2) {
+          const v2h s = halves(ks[blk][r] & steps);
+          x[blk * 4 + r] = __builtin_fmaf((float)s[0], d0[r], times(s[1], d1[r]));
+        } else {
+          x[blk * 4 + r] = times(halves(ks[blk][r >> 1] & steps)[r & 1], d0[r]);
+        }
+      }
     }
   };
-  auto work = [&](float (&x)[8], int s0, const Blocks& at) {
-    const int key0 = at.key[0], key1 = at.key[1];
-    const bool on[2] = {have(at.page[0]), have(at.page[1])};
-    if (s0 + 32 > hi || key1 + 16 > p0 + 1 || key0 < all_from || !on[0] || !on[1]) {
+  const unsigned vpick = DP == 128 || (n & 1) == 0 ? 0x05040100u : 0x07060302u;  // the half of a dword of V that this lane has
+  auto work = [&](float (&x)[8], int s0, int i0) {
+    if (odd >> (2 * i0) & 3) {
       // What no row sees is not there: its values' steps, which may be anything, become zeros.
-      auto dead = [&](int i) {
-        const int key = (i >> 2 ? key1 : key0) + kg * 4 + (i & 3);
-        return s0 + (i >> 2) * 16 + kg * 4 + (i & 3) >= hi || !on[i >> 2] || (key < any_from && key >= a.sinks);
-      };
+      const int key0 = __builtin_amdgcn_readlane(key, 2 * i0), key1 = __builtin_amdgcn_readlane(key, 2 * i0 + 1);
+      const bool gone[2] = {(lost >> (2 * i0) & 1) != 0, (lost >> (2 * i0) & 2) != 0};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int key = (i >> 2 ? key1 : key0) + kg * 4 + (i & 3);
-        if (dead(i) || key >= limit || (key < from && key >= a.sinks)) x[i] = -__builtin_inff();
+        const int mine = (i >> 2 ? key1 : key0) + kg * 4 + (i & 3);
+        const bool dead = s0 + (i >> 2) * 16 + kg * 4 + (i & 3) >= hi || gone[i >> 2] || (mine < any_from && mine >= a.sinks);
+        if (dead || mine >= limit || (mine < from && mine >= a.sinks)) x[i] = -__builtin_inff();
         if (GROUPS == 2) {
-          if (dead(i)) vs[i >> 2][i & 3] = 0;
-        } else if (dead(i)) {
+          if (dead) vs[i >> 2][i & 3] = 0;
+        } else if (dead) {
           vs[i >> 2][(i & 3) >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
         }
       }
     }
     float top = x[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = x[i] > top ? x[i] : top;
-    // a new reference only where a probability would pass 2^15: it starts at 2^8, fp16 ends at 2^16
-    if (__ballot(__builtin_fmaf(top, cl, off) > 15.0f) != 0) {
+    for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, x[i]);
+    // the largest word of the lane's, both halves; where one is larger than all before, p has to be less
+    v2us larger = __builtin_bit_cast(v2us, vs[0][0]);
+#pragma unroll
+    for (int i = 1; i < 4 * GROUPS; ++i) larger = __builtin_elementwise_max(larger, __builtin_bit_cast(v2us, vs[i / (2 * GROUPS)][i % (2 * GROUPS)]));
+    const unsigned largest = larger[0] > larger[1] ? larger[0] : larger[1];
+    if (__ballot(largest > top_word) != 0) {
+      // (the top bit and those of z are no part of a step; the next power of two)
+      const unsigned all = wave_max(largest) & 0x7fffu;
+      top_word = top_word > (all | 0x3ff) ? top_word : all | 0x3ff;
+      const int exponent = (int)(top_word >> 10) - 14;
+      most = 15.0f - (float)(exponent < -20 ? -20 : exponent);
+    }
+    // a new reference only where a weight could pass 2^15: it starts at 2^8, fp16 ends at 2^16
+    if (__ballot(__builtin_fmaf(top, cl, off) > most) != 0) {
       top = rows_max(top);
-      if (__builtin_fmaf(top, cl, off) > 15.0f) {
-        const float fresh = 8.0f - top * cl;
+      if (__builtin_fmaf(top, cl, off) > most) {
+        const float fresh = most - 7.0f - top * cl;
         const float scale = __builtin_amdgcn_exp2f(fresh - off);
         off = fresh;
 #pragma unroll
@@ -310,62 +347,85 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
         dsum *= scale;
       }
     }
-    v2h hi2[4], lo2[4];
+    float e[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const v2f e = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], cl, off)), __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], cl, off))};
-      hi2[i] = __builtin_convertvector(e, v2h);
-      const v2f rest = {__builtin_fmaf((float)hi2[i][0], -1.0f, e[0]), __builtin_fmaf((float)hi2[i][1], -1.0f, e[1])};
-      lo2[i] = __builtin_convertvector(rest, v2h);
+    for (int i = 0; i < 8; ++i) {
+      e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], cl, off));
+      dsum += e[i];
     }
-    const v8h hi_p = join8(hi2[0], hi2[1], hi2[2], hi2[3]), lo_p = join8(lo2[0], lo2[1], lo2[2], lo2[3]);
-    dsum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, hi_p, dsum, 0, 0, 0);
-    dsum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, lo_p, dsum, 0, 0, 0);
-    S4Two two[4];  // of the keys' pairs
+    // pairs of keys side by side, of a dword's lower half and its upper one
+    unsigned pairs[NB / 4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned* const w = vs[j >> 1];
-      if constexpr (GROUPS == 2) {
-        const unsigned first = w[2 * (j & 1)], second = w[2 * (j & 1) + 1];
-        two[j].set(bits, 0, __builtin_amdgcn_perm(second, first, 0x05040100u));
-        two[j].set(bits, 1, __builtin_amdgcn_perm(second, first, 0x07060302u));
-      } else {
-        two[j].set(bits, 0, w[j & 1]);
-        two[j].set(bits, 1, w[j & 1]);
+    for (int h = 0; h < NB / 4; ++h)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pairs[h][j] = __builtin_amdgcn_perm(v[2 * j + 1], v[2 * j], h ? 0x07060302u : vpick);
+    S4Zero zero[4];  // of the pairs
+#pragma unroll
+    for (int q = 0; q < GROUPS; ++q) {
+      v2h hi2[4], lo2[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        unsigned both = vs[j >> 1][j & 1];
+        if constexpr (GROUPS == 2)
+          both = __builtin_amdgcn_perm(vs[j >> 1][2 * (j & 1) + 1], vs[j >> 1][2 * (j & 1)], q ? 0x07060302u : 0x05040100u);
+        if (GROUPS == 2) zero[j].set(bits, q, both);
+        else zero[j].set(bits, 0, both), zero[j].set(bits, 1, both);
+        const v2h s = halves(both & steps);
+        const v2f y = {times(s[0], e[2 * j]), times(s[1], e[2 * j + 1])};
+        hi2[j] = __builtin_convertvector(y, v2h);
+        const v2f rest = {__builtin_fmaf((float)hi2[j][0], minus, y[0]), __builtin_fmaf((float)hi2[j][1], minus, y[1])};
+        lo2[j] = __builtin_convertvector(rest, v2h);
       }
-    }
+      const v8h hi_w = join8(hi2[0], hi2[1], hi2[2], hi2[3]), lo_w = join8(lo2[0], lo2[1], lo2[2], lo2[3]);
 #pragma unroll
-    for (int h = 0; h < NB / 4; ++h) {
-      v2h y[4][4];
+      for (int h = 0; h < NB / 4; ++h)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) two[j].values(bits, __builtin_amdgcn_perm(v[2 * j + 1], v[2 * j], h ? 0x07060302u : vpick), y[j]);
+        for (int i = 0; i < 4; ++i) {
+          if (GROUPS == 2 && (i & 1) != q) continue;
+          v2h y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const v8h vf = join8(y[0][i], y[1][i], y[2][i], y[3][i]);
-        acc[4 * h + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, hi_p, acc[4 * h + i], 0, 0, 0);
-        acc[4 * h + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, lo_p, acc[4 * h + i], 0, 0, 0);
-      }
+          for (int j = 0; j < 4; ++j) y[j] = zero[j].code(bits, i >> 1 ? pairs[h][j] >> 8 : pairs[h][j], i & 1);
+          const v8h vf = join8(y[0], y[1], y[2], y[3]);
+          acc[4 * h + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, hi_w, acc[4 * h + i], 0, 0, 0);
+          acc[4 * h + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, lo_w, acc[4 * h + i], 0, 0, 0);
+        }
     }
   };
 
-  // A step's keys are asked for as soon as those of the step before have become numbers, its values when those have.
+  // A step's keys are asked for as soon as those of the step before have become scores, its values when those have become sums.
   int s0 = lo + wave * 32;
   if (s0 < hi) {
-    constexpr int STRIDE = PA_WAVES * 32;
-    Blocks here = blocks_at(s0);
-    fetch_k(here);
-    fetch_v(here);
-    Blocks next = blocks_at(s0 + STRIDE);
-    for (;;) {  // (loads are issued without a branch around them, so that the waits can count them)
+    // Waits count loads, in the order in which they were issued: keys before values on every way into the loop, which the barriers keep
+    // so, or the wait for keys would be one for the values behind them as well.
+    look(s0);
+    Places next = places_of(0);
+    fetch_k(next);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_v(next);
+    __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0;; ++i) {
       float x[8];
       scores(x);
+      // (the places behind the 32nd step's are not known yet: its own again, which nobody uses)
+      next = places_of(i + 1 < 32 ? i + 1 : 31);
+      __builtin_amdgcn_sched_barrier(0);
       fetch_k(next);
-      const Blocks after = blocks_at(s0 + 2 * STRIDE);
-      work(x, s0, here);
+      __builtin_amdgcn_sched_barrier(0);
+      work(x, s0, i);
+      __builtin_amdgcn_sched_barrier(0);
       fetch_v(next);
-      here = next, next = after;
+      __builtin_amdgcn_sched_barrier(0);
       s0 += STRIDE;
       if (s0 >= hi) break;
+      if (i == 31) {
+        look(s0);
+        next = places_of(0);
+        fetch_k(next);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_v(next);
+        __builtin_amdgcn_sched_barrier(0);
+        i = -1;
+      }
     }
   }
 
@@ -379,9 +439,10 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
       if constexpr (NB == 8) *reinterpret_cast<v4f*>(to) = v4f{acc[nib][r], acc[2 + nib][r], acc[4 + nib][r], acc[6 + nib][r]};
       else *reinterpret_cast<v2f*>(to) = v2f{acc[nib][r], acc[2 + nib][r]};
     }
+  dsum = rows_add(dsum);
   if (kg == 0) {
     offs[wave][n] = off;
-    den[wave][n] = dsum[0];
+    den[wave][n] = dsum;
   }
   __syncthreads();
   const PagedOut to = {a.out, a.q_heads, c.D, a.alpha_pv};
