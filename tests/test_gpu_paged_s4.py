@@ -95,6 +95,11 @@ ATTENTION = [
     (2, 2, 64, 1, 16, [1000, 300], [500, 300], 17, 0),
     (4, 1, 80, 2, 32, [2000], [130], 700, 40),
     (1, 1, 128, 1, 64, [900], [900], 300, 300),
+    # some tens of rows to a sequence, and one over the line
+    (8, 2, 128, 2, 16, [300, 77, 12], [12, 11, 12], 0, 0),
+    (6, 1, 64, 1, 32, [500], [8], 0, 0),
+    (7, 1, 64, 1, 32, [500], [7], 0, 0),
+    (12, 4, 80, 2, 64, [200, 90], [16, 15], 60, 3),
 ]
 
 
@@ -449,10 +454,35 @@ def test_the_same_inputs_give_the_same_bits_on_any_stream():
     assert all(torch.equal(x, first) for x in got)
 
 
+@pytest.mark.parametrize("seqs,low,high,long,chunks,window", [
+    (65, 1, 200, 0, 0, 0), (70, 1000, 5000, 0, 0, 0), (130, 0, 300, 9000, 0, 0), (256, 1500, 2700, 0, 0, 700),
+    (257, 0, 300, 6000, 0, 0), (90, 100, 4000, 9000, 8, 0), (300, 0, 200, 5000, 5, 150), (520, 0, 60, 2000, 0, 0)])
+def test_more_sequences_than_a_wave_looks_at(seqs, low, high, long, chunks, window, monkeypatch):
+    # short and long ones, some without tokens or keys, one of `long` keys in their middle, chunks among single tokens: against
+    # fp64, and the same bits when slices are joined behind the launch
+    P = _paged()
+    g = torch.Generator().manual_seed(seqs)
+    lens = torch.randint(low, high + 1, (seqs,), generator=g).tolist()
+    new = torch.randint(0, 3, (seqs,), generator=g).tolist()
+    if long:
+        lens[seqs // 2], new[seqs // 2] = long, 1
+    for i in range(chunks):
+        new[(i + 1) * seqs // (chunks + 2)] = 40 + 30 * i
+    cu, lens, table, pages, rows = _batch(g, lens, new, 16)
+    caches = _cache(g, pages, 2, 16, 32, 1)
+    q = _query(g, rows, 6, 32, torch.bfloat16)
+    a_qk, sinks = _alpha(32, torch.bfloat16), 3 if window else 0
+    first = _attend(("many", seqs), q, caches, table, lens, cu, a_qk, 1.0, window, sinks, ONE_FP16).to(DEV)
+    args = (q.to(DEV), *_device(caches), table.to(DEV), lens.to(DEV), cu.to(DEV), a_qk, 1.0, window, sinks)
+    monkeypatch.setattr(P, "_arrivals", lambda *a: (None, 0))
+    assert torch.equal(P.paged_attn_s4(*args), first)
+
+
 @pytest.mark.parametrize("hq,hk,d,lens,new,window", [
     (1, 1, 128, [70000], [1], 0), (8, 1, 64, [9000, 2, 700], [1, 1, 1], 0), (4, 2, 80, [3000, 2900], [9, 1], 0),
     (32, 2, 128, [5000, 40, 6001], [1, 1, 2], 0), (12, 12, 64, [1025], [1], 0), (4, 2, 128, [4000, 70], [100, 1], 0),
-    (1, 1, 64, [3000], [200], 0), (8, 8, 80, [1500], [33], 0), (2, 1, 128, [9000, 50], [1, 1], 5000), (4, 2, 64, [4000, 3000], [70, 3], 2000)])
+    (1, 1, 64, [3000], [200], 0), (8, 8, 80, [1500], [33], 0), (2, 1, 128, [9000, 50], [1, 1], 5000), (4, 2, 64, [4000, 3000], [70, 3], 2000),
+    (8, 2, 128, [4000, 900], [12, 7], 0), (12, 4, 64, [6000], [16], 0), (8, 2, 80, [5000, 4000, 3], [15, 9, 3], 3000)])
 def test_slices_that_meet_in_the_launch_or_behind_it(hq, hk, d, lens, new, window, monkeypatch):
     # the same bits with the counters, without them (a second launch), again and again, and after calls whose tables hold
     # nonsense: the counters are zero behind every call; against fp64 as well

@@ -133,6 +133,11 @@ struct S4Span {
 // to 2^13, so the reference M keeps p times the largest step of the keys so far at 2^15 or less.
 // (Codes as they are, subnormal fp16 numbers u 2^-24, and z times the sums of q and of weights taken off behind the products
 // would be a fifth less to issue, but the matrix pipe adds subnormal numbers with 2^-20 of their sum lost.)
+// One token to each of 28 sequences of 1500 keys, 40 heads of 128: 39 us, 3.4 TB/s; 75 of up to 7003, 32 heads on 8: 75 us, 3.9 TB/s;
+// one of 200000, 64 heads on 8: 57 us, 3.8 TB/s.  40 % of the issue slots of a 32-key step are codes becoming numbers (2.25 instructions
+// to two), a third scores, steps and weights, a sixth addresses; half of the waves that fit are there on average, as workgroups begin
+// (item, table, addresses, first keys: 5 us) and end.
+constexpr int S4_HELD = 4;  // times 64 sequences
 constexpr int s4_rows_lds(int DP) { return PA_WAVES * PA_ROWS * (DP + 4 + 2) * 4; }
 template <int DP, int GROUPS, int OUT>
 __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, const PagedPlan& p, int index,
@@ -143,7 +148,7 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
   const auto offs = reinterpret_cast<float(*)[PA_ROWS]>(lds + PA_WAVES * PA_ROWS * (DP + 4) * 4);
   const auto den = offs + PA_WAVES;
 
-  const PagedItem it = paged_item<4, false, true>(b, c.page_shift, c.heads, PA_ROWS, p, index);
+  const PagedItem it = paged_item<4, false, true, S4_HELD>(b, c.page_shift, c.heads, PA_ROWS, p, index);
   if (!it.found) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -482,12 +487,20 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
 // nibbles, or high ones) exchanged by the row; values in the order in which MFMA operands are read, of eight keys, chosen as
 // S^T = K Q^T leaves them in a lane, one column in 16 bytes, lane after lane.  One unpacking then serves 128 rows.
 // Column block i of V holds, of lane m's NDB / 2 bytes of a row, byte i / 2's low nibble or high one.
+//
+// A step is two halves of 32 keys with a barrier behind each.  The instructions of a half are laid out as bundles of one matrix
+// instruction and what fits beside it: the scores of the next half and the sums of the one before are on their way while this one's
+// become weights and the next step's codes numbers.  1536 rows over 12288 keys, 32 heads on 8: 448 us with one after the other, 397 so,
+// 715 TFLOP/s.  Two workgroups to a CU fill the LDS and the registers; of the time the matrix pipe is busy for 28 %, the vector ALUs for 43, the
+// LDS for 29, and what bounds it is issue.
+// A weight is one fp16 number, 11 bits: a second one would be 16 matrix instructions more to the 32 of a step, and the sum of the
+// rounding errors, at most 2^-11 of sum w |v| / sum w, is no more than what rounding such an output to fp16 costs, an eighth of what bf16 does.
 constexpr int ST_ROWS = 128, ST_KEYS = 64;
 constexpr int ST_PARTS = 4;
 constexpr int ST_JOIN = 32;      // rows that a workgroup joins
-constexpr int ST_PLENTY = 2048;  // items from which on nothing is cut
+constexpr int ST_PLENTY = 2048;  // items from which on nothing is cut: four rounds, whose last one is a small part
 constexpr int ST_AT_ONCE = 512;  // workgroups on the chip
-constexpr int ST_TARGET = 1536;  // slices, at most about
+constexpr int ST_TARGET = 1536;  // slices, at most about (1536 rows over 12288 keys 397 us; with 768 424, which is two rounds of 384 at best)
 constexpr int s4_tiles_lds(int DP) { return 2 * 2 * ST_KEYS * DP * 2; }  // two steps of K, then of V
 template <int DP, int GROUPS, int OUT>
 __device__ __forceinline__ void s4_tiles(const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, const PagedPlan& p, int index,
@@ -497,7 +510,7 @@ __device__ __forceinline__ void s4_tiles(const PagedAttn4& a, const PagedCache4&
   constexpr int KW = DP / 32;   // dwords of a key row that a thread brings
   constexpr int BYTES = ST_KEYS * DP * 2;  // of a step of K, or of V
 
-  const PagedItem it = paged_item<ST_PARTS>(b, c.page_shift, c.heads, ST_ROWS, p, index);
+  const PagedItem it = paged_item<ST_PARTS, false, false, S4_HELD>(b, c.page_shift, c.heads, ST_ROWS, p, index);
   if (!it.found) return;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -909,8 +922,10 @@ __device__ __forceinline__ void s4_tiles(const PagedAttn4& a, const PagedCache4&
     *reinterpret_cast<v2f*>(p.ws + (long long)p.places * ST_ROWS * DP + (place * ST_ROWS + wave * 32 + n) * 2) = v2f{off, den};
 }
 
+// (two groups of a wide head take 144 registers, three waves to a SIMD; four would spill)
 template <int DP, int GROUPS, int OUT>
-__global__ __launch_bounds__(PA_THREADS, DP == 128 && GROUPS == 2 ? 3 : 4) void paged_attn_s4_rows_kernel(PagedAttn4 a, PagedCache4 c, PagedBatch b, PagedPlan rows) {
+__global__ __launch_bounds__(PA_THREADS, DP == 128 && GROUPS == 2 ? 3 : 4) void paged_attn_s4_rows_kernel(PagedAttn4 a, PagedCache4 c,
+                                                                                                         PagedBatch b, PagedPlan rows) {
   __shared__ __attribute__((aligned(16))) char lds[s4_rows_lds(DP)];
   const int lo = b.cu[0], hi = b.cu[b.seqs];  // (on their way beside what the item needs)
   s4_rows<DP, GROUPS, OUT>(a, c, b, rows, blockIdx.x, lds);
@@ -939,8 +954,8 @@ __global__ __launch_bounds__(PA_THREADS) void paged_attn_s4_join_kernel(PagedAtt
   constexpr int PIECES = ROWS / EACH;
   const int index = blockIdx.x / (8 * PIECES) * 8 + blockIdx.x % 8;
   PagedItem it;
-  if constexpr (ROWS == ST_ROWS) it = paged_item<ST_PARTS, true>(b, c.page_shift, c.heads, ROWS, p, index);
-  else it = paged_item<4, true, true>(b, c.page_shift, c.heads, ROWS, p, index);
+  if constexpr (ROWS == ST_ROWS) it = paged_item<ST_PARTS, true, false, S4_HELD>(b, c.page_shift, c.heads, ROWS, p, index);
+  else it = paged_item<4, true, true, S4_HELD>(b, c.page_shift, c.heads, ROWS, p, index);
   if (!it.found || it.split != 0) return;
   join_slices<ROWS, EACH, DP, OUT, false, true>(PagedOut{a.out, a.q_heads, c.D, a.alpha_pv}, p, it, meet, blockIdx.x / 8 % PIECES * EACH);
 }
@@ -951,6 +966,13 @@ __global__ __launch_bounds__(PA_THREADS) void paged_attn_s4_join_kernel(PagedAtt
 // longer), 83 without that exception, 75 with even ones, long ones first; 512, 768 and 1024 slices of them 80, 75 and 75, 20 x 4 tokens
 // in windows of 1024 keys 29, 29 and 34 (where 768 leave 640 items whole).
 constexpr int S4_TARGET = 768;
+
+// Rows to a sequence, on average, up to which all of a batch go to the kernel of 16 rows: it reads a sequence's keys once for every 16,
+// but starts sooner, spreads further and has three or four waves to a SIMD.  All by it, and by tiles: 16 sequences of 500 to 4000 keys, 32
+// heads on 8, 8 tokens each (32 rows) 28 and 55 us, 12 (48) 32 and 58, 16 (64) 38 and 59.  A batch whose average is a chunk among single tokens
+// loses less than that: 250, 500 and 900 tokens beside 60 single ones (21, 37, 63 rows on average) 79, 106 and 147, and 92, 97 and 121 by
+// both.
+constexpr int S4_FEW_MEAN = 48;
 
 // What a call of these sizes runs: bounds, since the lengths are on the device (see the int8 cache's).
 struct S4Kind {
@@ -980,7 +1002,7 @@ static S4Shape s4_shape(long long rows, long long seqs, long long group, long lo
     const long long shared = s.rows.target / (s.rows.items > 0 ? s.rows.items : 1) + 1;
     s.meet = s.rows.target > 0 && (of_one < shared ? of_one : shared) * each * 520 <= 66560;
   };
-  if (rows * group <= PA_ROWS * seqs) {  // few rows to a sequence on average: all of them by that kernel
+  if (rows * group <= S4_FEW_MEAN * seqs) {  // few rows to a sequence on average: all of them by that kernel
     items(s.rows, heads * (seqs + rows * group / PA_ROWS));
     each = rows * group / (seqs > 0 ? seqs : 1) + 1 < PA_ROWS ? rows * group / (seqs > 0 ? seqs : 1) + 1 : PA_ROWS;
     if (cut) s.rows.cut(S4_TARGET, of_one);

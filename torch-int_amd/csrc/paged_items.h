@@ -16,7 +16,12 @@ constexpr int PA_ROWS = 16;
 constexpr int PA_TARGET = 512;     // slices that the keys of a batch are cut into, beyond one to each item
 constexpr int PA_FULL = 512;       // items that fill the chip
 constexpr int PA_MIN_SLICE = 512;  // keys of a slice, at least
-constexpr float PA_SORTED = 2048;  // items from which on they are not put in order
+// Items are put in order where there are fewer than PA_SORTED of PA_LONG keys or more on average: finding one's own in four classes
+// takes 1 to 4 us, which long items win back where few of them would end last.  Over the 4-bit cache, in order and as they come: 75 tokens
+// over 50 to 7003 keys, 8 key heads, 75 and 82 us; 120 over 50 to 5000, 16 heads, 147 and 150; 64 over 3000 to 4000, 4 heads, 37.7 and 38.3; but
+// 250 over 500 to 3000, 2 heads, 43 and 39; 200 over 20 to 3000, 8 heads, 88 and 86; 120 over 50 to 900, 8 heads, 28 and 26; 300 (which are
+// looked at again for every class) over 20 to 1000, 8 heads, 98 and 62.
+constexpr float PA_SORTED = 2048, PA_LONG = 2048;
 constexpr float PA_EMPTY = 3.0e38f;  // offset of a row that has seen no key: 2^(-inf + PA_EMPTY) is 0
 
 // The sequences that one of the two kernels takes, by how many rows a key head has in them, and how their keys are cut.
@@ -95,8 +100,13 @@ __device__ __forceinline__ int paged_slice(float items, float total, int target,
   return slice < PA_MIN_SLICE ? PA_MIN_SLICE : slice;
 }
 
-// The same for items that take long, `at_once` of them at a time: cut into as many slices as make the last round of workgroups least
-// in vain.  A workgroup costs some 170 keys before and behind its own, one that is joined some 700.
+// The same for items of about one length that take long, `at_once` of them at a time: cut into as many slices as make the last round
+// of workgroups least in vain.  A workgroup costs some 170 keys before and behind its own, one that is joined some 700.  Over the 4-bit cache, so and cut
+// into `target` parts as above: 1536 rows over 6000 keys, 32 heads, 212 and 226 us; 700 over 13000, 28 heads on 4, 195 and 210; 300 rows and 31
+// tokens over 600 to 2007, 32 heads on 8, 49.5 and 58; but 64 rows over 8000 53.7 and 51.8, 4 x 1000 rows over 4000 to 16000 931 and 847: of
+// unequal items the longest ends last.  Those are cut into `target` parts, but none of fewer keys than make one round of all, nor of 2048:
+// slices of at least 1024, 2048 and 4096 keys take 3 x 400 rows over 1500 to 5000 keys 123, 115 and 164 us, 2 x 200 over 5000 to 30000 223,
+// 215 and 212; 16 x 24 rows over 500 to 4000 take 105 with 2048, 62 with a round's; 16 x 100 over 400 to 900 83 without any, 61 so.
 __device__ __forceinline__ int paged_slice_even(float items, float total, int target, int at_once) {
   const float keys = total / __builtin_fmaxf(items, 1.0f);
   float best = __builtin_ceilf(items / (float)at_once) * (keys + 170.0f);
@@ -114,8 +124,9 @@ __device__ __forceinline__ int paged_slice_even(float items, float total, int ta
 // The work item with number `index`, in the order part, sequence, slice, tile of rows, head.  A sequence's tiles come from the
 // last, which has the most keys, to the first, in PARTS parts, so that the long items of all sequences begin before the short
 // ones.  SORTED: instead, in PARTS classes of sequences, those of long slices first.  CUT: the first slice of the `index`-th item
-// among those that are cut.
-template <int PARTS, bool CUT = false, bool SORTED = false>
+// among those that are cut.  HELD: 64 times so many sequences stay in registers, asked for together; of more, or with 1, 64 are
+// looked at again at a time (over the 4-bit cache, 120 tokens over 50 to 900 keys, 8 key heads: 30 us, and 28 with 4).
+template <int PARTS, bool CUT = false, bool SORTED = false, int HELD = 1>
 __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_shift, int heads, int rows_per_tile, const PagedPlan& p,
                                                 int index) {
   PagedItem it;
@@ -133,18 +144,51 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
       tiles = p.tiles(s, rows_per_tile);
     }
   };
-  it.slice = 0x7fffffff;
-  float count = 2.0f * PA_SORTED;
-  if (p.target != 0) {
-    float items = 0.0f, total = 0.0f;
-    for (int i0 = (b.seqs - 1) & ~63; i0 >= 0; i0 -= 64) {  // the first 64 come last and stay
-      look(i0);
-      items += wave_add((float)tiles);
-      total += wave_add((float)tiles * (float)(s.len < p.span ? s.len : p.span));
+  PagedSeq held[HELD];
+  int held_tiles[HELD];
+  const bool all = HELD > 1 && b.seqs <= 64 * HELD;
+  if (all) {
+    int lo[HELD], hi[HELD], len[HELD];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      const int i = h * 64 + lane < b.seqs ? h * 64 + lane : b.seqs - 1;
+      lo[h] = b.cu[i], hi[h] = b.cu[i + 1], len[h] = b.lens[i];
     }
-    count = items * (float)heads;
-    it.slice = p.at_once != 0 ? paged_slice_even(items * (float)heads, total * (float)heads, p.target, p.at_once)
-                              : paged_slice(items * (float)heads, total * (float)heads, p.target, p.full);
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      held[h] = paged_seq(b, page_shift, lo[h], hi[h], len[h]);
+      held_tiles[h] = h * 64 + lane < b.seqs ? p.tiles(held[h], rows_per_tile) : 0;
+    }
+    s = held[0], tiles = held_tiles[0];
+  }
+  it.slice = 0x7fffffff;
+  bool sorted = false;
+  if (p.target != 0) {
+    auto keys_of = [&](const PagedSeq& s) { return (float)(s.len < p.span ? s.len : p.span); };
+    float items = 0.0f, total = 0.0f;
+    if (all) {
+#pragma unroll
+      for (int h = 0; h < HELD; ++h) items += (float)held_tiles[h], total += (float)held_tiles[h] * keys_of(held[h]);
+      items = wave_add(items), total = wave_add(total);
+    } else {
+      for (int i0 = (b.seqs - 1) & ~63; i0 >= 0; i0 -= 64) {  // the first 64 come last and stay
+        look(i0);
+        items += wave_add((float)tiles);
+        total += wave_add((float)tiles * keys_of(s));
+      }
+    }
+    bool alike = p.at_once != 0 && all;  // no item is longer than the average by more than a quarter
+    if (alike)
+#pragma unroll
+      for (int h = 0; h < HELD; ++h) alike = alike && __ballot(held_tiles[h] > 0 && keys_of(held[h]) * items > 1.25f * total) == 0;
+    const float count = items * (float)heads, keys = total * (float)heads;
+    it.slice = alike ? paged_slice_even(count, keys, p.target, p.at_once) : paged_slice(count, keys, p.target, p.full);
+    if (p.at_once != 0 && !alike) {  // (a joined slice costs 700)
+      const float round = 1.25f * keys / (float)p.at_once;
+      const int least = round < 4.0f * PA_MIN_SLICE ? (int)round & ~63 : 4 * PA_MIN_SLICE;
+      it.slice = it.slice < least ? least : it.slice;
+    }
+    sorted = SORTED && count < PA_SORTED && total >= PA_LONG * items;
   }
   int before = 0, before_cut = 0, before_sliced = 0;
   int splits = 1;
@@ -156,16 +200,20 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
     cuts = __ballot(splits > 1 && tiles > 0);
   };
   if (b.seqs <= 64) {
-    if (p.target == 0) look(0);
+    if (p.target == 0 && !all) look(0);
     cut_up();
     if (CUT && cuts == 0) return it;
   }
-  // (of many items the last ones are a small part: they come as they are)
-  const bool sorted = SORTED && count < PA_SORTED;
   const int parts = SORTED && !sorted ? 1 : PARTS;
   for (int part = 0, i0 = 0; part < parts; i0 + 64 < b.seqs ? i0 += 64 : (i0 = 0, ++part)) {
     if (b.seqs > 64) {
-      look(i0);
+      if (all) {
+#pragma unroll
+        for (int h = 0; h < HELD; ++h)
+          if (i0 == h * 64) s = held[h], tiles = held_tiles[h];
+      } else {
+        look(i0);
+      }
       cut_up();
     }
     const int behind = PARTS == 1 || SORTED ? 0 : (int)((long long)tiles * part / PARTS);  // tiles of the parts before
@@ -176,8 +224,8 @@ __device__ __forceinline__ PagedItem paged_item(const PagedBatch& b, int page_sh
       here = mine == part ? tiles : 0;
     }
     // a cu_new that descends can count rows many times over: no sum of items passes the range of int
-    const long long whole = (long long)here * heads, all = whole * splits;
-    const int n = all > 0x800000 ? 0x800000 : (int)all;
+    const long long whole = (long long)here * heads, slices = whole * splits;
+    const int n = slices > 0x800000 ? 0x800000 : (int)slices;
     const int cut = splits == 1 ? 0 : whole > 0x800000 ? 0x800000 : (int)whole;
     const int upto = wave_scan(n), upto_cut = CUT ? wave_scan(cut) : 0;
     // what those of some lanes that are cut have of n, whose sum `all` is; mostly all of them are, or none
