@@ -1,0 +1,64 @@
+"""The 4-bit paged cache's attention: which weights have 22 bits, on inputs where weights of 11 bits break the bound
+(tests/_paged_s4_cancelling.py, shown on the CPU by tests/test_host_paged_s4_weights.py)."""
+import pytest
+import torch
+
+from tests import _paged_oracle as orc
+from tests import _paged_s4_cancelling as data
+from tests.test_gpu_paged import _batch, _s8
+from tests.test_gpu_paged_s4 import DEV, TWO_FP16, _cache, _device, _paged
+
+pytestmark = pytest.mark.gpu
+
+
+def _cancelling(g, hq, hk, d, groups, lens, new, heavy, pad=0, chunk=0):
+    """A batch of such sequences, ``pad`` rows of nobody behind them and, where asked, a chunk of another kind of keys: the
+    arguments of a call but for its window, and what the sequences' rows are to be."""
+    cu, lens_t, table, pages, rows = _batch(g, lens + [chunk] * (chunk > 0), new + [chunk] * (chunk > 0), 16, pad=pad)
+    caches = _cache(g, pages, hk, 16, d, groups)
+    q = _s8(g, rows, hq, d, spread=30)
+    wants = []
+    for b, (n, t) in enumerate(zip(lens, new)):
+        mine = slice(int(cu[b]), int(cu[b + 1]))
+        q[mine], k, v, at = data.sequence(g, n, heavy, t, hq, d)
+        pos = torch.arange(n)
+        where = table[b].long()[pos // 16], slice(None), pos % 16
+        for codes, words, x, step in ((caches[0], caches[2], k, data.K_STEP), (caches[1], caches[3], v, data.V_STEP)):
+            codes[where], words[where] = data.codes(x)[:, None], data.word(step)
+        wants.append((mine, data.wanted(q[mine], k, v, at)))
+    return (q, caches, table, lens_t, cu), wants
+
+
+def _check(case, args, wants, heavy, query, monkeypatch):
+    P = _paged()
+    q, caches, table, lens, cu = args
+    call = (q.to(query).to(DEV), *_device(caches), table.to(DEV), lens.to(DEV), cu.to(DEV), data.ALPHA, 1.0)
+    for where in ("in the launch", "behind it"):
+        got = P.paged_attn_s4(*call, out_dtype=torch.float16).cpu()
+        for mine, (want, size, most) in wants:
+            worst = orc.attention_error(got[mine], want, size, most, heavy, TWO_FP16)
+            print("22 bits", case, where, "rows", mine, "error over its bound", worst, flush=True)
+            assert worst <= 1.0
+        assert (got[int(cu[-1]):] == 0).all()
+        monkeypatch.setattr(P, "_arrivals", lambda *a: (None, 0))
+
+
+# query heads, key heads, head size, context lengths, new tokens, a chunk
+EXACT = [
+    (8, 8, 64, [64], [1], 0),
+    (8, 1, 128, [160, 64, 90], [1, 1, 2], 0),           # up to 16 rows
+    (16, 1, 80, [3000], [1], 0),                        # 16 rows, in slices
+    (8, 2, 96, [3000, 700, 5000], [1, 4, 2], 0),
+    (8, 1, 64, [3000, 500], [2, 1], 40),                # up to 16 rows beside a chunk
+    (8, 1, 128, [300, 200], [5, 6], 0),                 # 40 and 48 rows, 44 on average
+    (8, 2, 64, [4000, 80, 90, 100], [30, 1, 1, 1], 0),  # 120 rows, 33 on average
+    (4, 4, 80, [130], [40], 0),
+]
+
+
+@pytest.mark.parametrize("groups", [1, 2])
+@pytest.mark.parametrize("i", range(len(EXACT)))
+def test_weights_of_22_bits(i, groups, monkeypatch):
+    hq, hk, d, lens, new, chunk = EXACT[i]
+    args, wants = _cancelling(torch.Generator().manual_seed(i), hq, hk, d, groups, lens, new, 64, 0, chunk)
+    _check((EXACT[i], groups), args, wants, 64, [torch.int8, torch.float16, torch.bfloat16][i % 3], monkeypatch)
