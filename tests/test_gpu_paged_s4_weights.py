@@ -6,7 +6,7 @@ import torch
 from tests import _paged_oracle as orc
 from tests import _paged_s4_cancelling as data
 from tests.test_gpu_paged import _batch, _s8
-from tests.test_gpu_paged_s4 import DEV, TWO_FP16, _cache, _device, _paged
+from tests.test_gpu_paged_s4 import DEV, ONE_FP16, TWO_FP16, _attend, _cache, _device, _paged
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,40 @@ def test_weights_of_22_bits(i, groups, monkeypatch):
     hq, hk, d, lens, new, chunk = EXACT[i]
     args, wants = _cancelling(torch.Generator().manual_seed(i), hq, hk, d, groups, lens, new, 64, 0, chunk)
     _check((EXACT[i], groups), args, wants, 64, [torch.int8, torch.float16, torch.bfloat16][i % 3], monkeypatch)
+
+
+# query heads, key heads, head size, context lengths, new tokens, rows of nobody: more than 48 rows to a sequence, as the host counts
+SPARE = [
+    (16, 1, 128, [400], [1], 3),
+    (16, 1, 64, [20000], [1], 3),
+    (64, 8, 128, [5000], [1], 6),
+    (28, 4, 80, [3000], [2], 7),
+    (8, 1, 96, [3000], [2], 5),
+    (4, 4, 64, [200], [16], 60),
+    (16, 1, 128, [3000, 90], [1, 1], 5),
+    (8, 1, 64, [700, 3000, 66], [1, 1, 2], 17),
+    (2, 1, 64, [100], [1], 3000),
+]
+
+
+@pytest.mark.parametrize("groups", [1, 2])
+@pytest.mark.parametrize("i", range(len(SPARE)))
+def test_spare_rows_do_not_take_bits_from_weights(i, groups, monkeypatch):
+    # rows of nobody behind a recorded step's sequences: those still have up to 16 rows, and weights of 22 bits
+    hq, hk, d, lens, new, pad = SPARE[i]
+    assert (sum(new) + pad) * hq > 48 * len(lens) * hk and max(new) * hq <= 16 * hk
+    args, wants = _cancelling(torch.Generator().manual_seed(50 + i), hq, hk, d, groups, lens, new, 64, pad)
+    _check((SPARE[i], groups), args, wants, 64, [torch.int8, torch.float16, torch.bfloat16][i % 3], monkeypatch)
+
+
+@pytest.mark.parametrize("hq,hk,d,groups,n,new,pad,window,sinks", [
+    (16, 1, 128, 2, 6000, 1, 4, 0, 0), (8, 1, 80, 1, 2000, 2, 30, 700, 5), (28, 4, 64, 1, 1, 1, 8, 0, 0), (64, 8, 128, 2, 40, 0, 7, 0, 0),
+    (8, 1, 128, 1, 3000, 40, 9, 0, 0), (4, 2, 64, 2, 900, 300, 40, 100, 3)])
+def test_one_sequence_and_spare_rows(hq, hk, d, groups, n, new, pad, window, sinks):
+    g = torch.Generator().manual_seed(n + pad)
+    cu, lens, table, pages, rows = _batch(g, [n], [new], 16, pad=pad)
+    caches = _cache(g, pages, hk, 16, d, groups)
+    q = torch.randn(rows, hq, d, generator=g).half()
+    got = _attend((hq, hk, d, n, new, pad), q, caches, table, lens, cu, 2.0 / d ** 0.5, 1.0, window, sinks,
+                  TWO_FP16 if new * hq <= 16 * hk else ONE_FP16, out_dtype=torch.bfloat16)
+    assert (got[new:] == 0).all()

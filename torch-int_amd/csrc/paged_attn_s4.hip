@@ -947,17 +947,26 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_s4_both_kernel(Paged
   else s4_rows<DP, GROUPS, OUT>(a, c, b, rows, index, lds);
 }
 
-// Joins slices that do not meet in the launch itself, EACH rows to a workgroup, in turns of eight items (as over the int8 cache).
+// Joins slices that do not meet in the launch itself, EACH rows to a workgroup, in turns of eight items (as over the int8 cache): the
+// many rows', which take longer, in the first `tile_blocks` workgroups, the few rows' in the others.
+constexpr int S4_JOIN = 2;
 template <int ROWS, int EACH, int DP, int OUT>
-__global__ __launch_bounds__(PA_THREADS) void paged_attn_s4_join_kernel(PagedAttn4 a, PagedCache4 c, PagedBatch b, PagedPlan p) {
-  __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
+__device__ __forceinline__ void s4_join(const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, const PagedPlan& p, int block, float* meet) {
   constexpr int PIECES = ROWS / EACH;
-  const int index = blockIdx.x / (8 * PIECES) * 8 + blockIdx.x % 8;
+  const int index = block / (8 * PIECES) * 8 + block % 8;
   PagedItem it;
   if constexpr (ROWS == ST_ROWS) it = paged_item<ST_PARTS, true, false, S4_HELD>(b, c.page_shift, c.heads, ROWS, p, index);
   else it = paged_item<4, true, true, S4_HELD>(b, c.page_shift, c.heads, ROWS, p, index);
   if (!it.found || it.split != 0) return;
-  join_slices<ROWS, EACH, DP, OUT, false, true>(PagedOut{a.out, a.q_heads, c.D, a.alpha_pv}, p, it, meet, blockIdx.x / 8 % PIECES * EACH);
+  join_slices<ROWS, EACH, DP, OUT, false, true>(PagedOut{a.out, a.q_heads, c.D, a.alpha_pv}, p, it, meet, block / 8 % PIECES * EACH);
+}
+template <int DP, int OUT>
+__global__ __launch_bounds__(PA_THREADS) void paged_attn_s4_join_kernel(PagedAttn4 a, PagedCache4 c, PagedBatch b, PagedPlan rows,
+                                                                        PagedPlan tiles, int tile_blocks) {
+  __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
+  const int block = blockIdx.x;
+  if (block < tile_blocks) s4_join<ST_ROWS, ST_JOIN, DP, OUT>(a, c, b, tiles, block, meet);
+  else s4_join<PA_ROWS, S4_JOIN, DP, OUT>(a, c, b, rows, block - tile_blocks, meet);
 }
 
 // Slices that the keys of a batch are cut into, about: three to a CU.  An item is cut where it has one and a half times as many keys or
@@ -973,6 +982,14 @@ constexpr int S4_TARGET = 768;
 // loses less than that: 250, 500 and 900 tokens beside 60 single ones (21, 37, 63 rows on average) 79, 106 and 147, and 92, 97 and 121 by
 // both.
 constexpr int S4_FEW_MEAN = 48;
+
+// Sequences of a batch of the other kind up to which those of few rows are cut into S4_TARGET slices as well; of more, into 128, since
+// they share the chip with tiles.  So few can be all there is, the rest being rows of nobody behind a recorded step: one token over 200000
+// keys and 3 such rows, 16 heads on 1, 35 us, 349 when one sequence went to the tiles; 4 tokens over 50000 and 30 rows, 64 on 8, 70 us, 123
+// in 128 slices; 8 over 20000 and 50 rows 58 and 101.  Beside a chunk over 20000 keys, 32 heads on 8, it pays
+// for 7 single tokens too (chunks of 100, 512 and 2000 tokens 129, 253 and 776 us; 185, 315 and 776), for 15 it depends (900 tokens 424 and
+// 472, 2500 tokens 1012 and 991).
+constexpr int S4_LONE = 8;
 
 // What a call of these sizes runs: bounds, since the lengths are on the device (see the int8 cache's).
 struct S4Kind {
@@ -1002,7 +1019,7 @@ static S4Shape s4_shape(long long rows, long long seqs, long long group, long lo
     const long long shared = s.rows.target / (s.rows.items > 0 ? s.rows.items : 1) + 1;
     s.meet = s.rows.target > 0 && (of_one < shared ? of_one : shared) * each * 520 <= 66560;
   };
-  if (rows * group <= S4_FEW_MEAN * seqs) {  // few rows to a sequence on average: all of them by that kernel
+  if (rows * group <= S4_FEW_MEAN * seqs) {  // few rows to a sequence on average, nobody's counted: all of them by that kernel
     items(s.rows, heads * (seqs + rows * group / PA_ROWS));
     each = rows * group / (seqs > 0 ? seqs : 1) + 1 < PA_ROWS ? rows * group / (seqs > 0 ? seqs : 1) + 1 : PA_ROWS;
     if (cut) s.rows.cut(S4_TARGET, of_one);
@@ -1013,9 +1030,9 @@ static S4Shape s4_shape(long long rows, long long seqs, long long group, long lo
   const long long many = rows * group / (PA_ROWS + 1) < seqs ? rows * group / (PA_ROWS + 1) : seqs;
   items(s.tiles, heads * (many + rows * group / ST_ROWS));
   if (cut && s.tiles.items < ST_PLENTY) s.tiles.cut(ST_TARGET, of_one);
-  if (seqs == 1) return s;  // it has more than 16
+  // Rows can be nobody's: one sequence too may have 16 of them or fewer.
   items(s.rows, heads * seqs);
-  if (cut) s.rows.cut(PA_TARGET / 4, of_one);
+  if (cut) s.rows.cut(seqs <= S4_LONE ? S4_TARGET : PA_TARGET / 4, of_one);
   join_here();
   return s;
 }
@@ -1042,12 +1059,11 @@ static void launch_s4(const PagedAttn4& a, const PagedCache4& c, const PagedBatc
     hipLaunchKernelGGL((paged_attn_s4_rows_kernel<DP, GROUPS, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows);
   // an item that is cut has more than a target-th of all keys, so there are fewer than `target` of them
   auto items = [](const S4Kind& k) { return (unsigned)((k.items < k.target ? (int)k.items : k.target) + 7 & ~7); };
-  if (rows.target > 0 && rows.arrivals == nullptr)
-    hipLaunchKernelGGL((paged_attn_s4_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(items(s.rows) * (PA_ROWS / 2)), dim3(PA_THREADS), 0,
-                       stream, a, c, b, rows);
-  if (tiles.target > 0)
-    hipLaunchKernelGGL((paged_attn_s4_join_kernel<ST_ROWS, ST_JOIN, DP, OUT>), dim3(items(s.tiles) * (ST_ROWS / ST_JOIN)), dim3(PA_THREADS),
-                       0, stream, a, c, b, tiles);
+  const unsigned row_blocks = rows.target > 0 && rows.arrivals == nullptr ? items(s.rows) * (PA_ROWS / S4_JOIN) : 0;
+  const unsigned tile_blocks = tiles.target > 0 ? items(s.tiles) * (ST_ROWS / ST_JOIN) : 0;
+  if (row_blocks + tile_blocks > 0)
+    hipLaunchKernelGGL((paged_attn_s4_join_kernel<DP, OUT>), dim3(row_blocks + tile_blocks), dim3(PA_THREADS), 0, stream, a, c, b, rows, tiles,
+                       (int)tile_blocks);
 }
 
 int launch_paged_attn_s4(int out_type, const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, void* workspace,

@@ -245,9 +245,10 @@ def paged_attn_s4(query, k_cache, v_cache, k_scale, v_scale, block_table, contex
     that is handed in, which must not share memory with the inputs.  ``alpha_qk`` is from 1e-30 to 1e4.
 
     Keys, values and queries are computed with as they are (bf16 queries as fp16), sums and softmax in fp32.
-    Weights have 22 bits in sequences of up to 16 rows (new tokens times ``q_heads // heads``) and, as long as a batch has no more
-    than 48 on average, in all; longer sequences of other batches have weights of 11 bits.  The same batch gives the same bits on any stream and in a recorded graph; beside other sequences the last bits of a token's
-    context can differ."""
+    Weights have 22 bits in sequences of up to 16 rows (new tokens times ``q_heads // heads``) and, as long as ``query`` has no more
+    than 48 to a sequence on average (rows of no sequence counted), in all; longer sequences of other batches have weights of 11
+    bits.  The same batch gives the same bits on any stream and in a recorded graph; beside other sequences the last bits of a
+    token's context can differ."""
     op = "paged_attn_s4"
     q_code = _QUERIES.get(query.dtype) if isinstance(query, torch.Tensor) else None
     if q_code is None or query.dim() != 3:
