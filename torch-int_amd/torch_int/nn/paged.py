@@ -62,7 +62,7 @@ class PagedAttn_S8(ScalarCacheMixin, torch.nn.Module):
 class PagedKVAppend_S4(ScalarCacheMixin, torch.nn.Module):
     """Writes new keys and values into their pages in 4 bits and, where there are some, rotates the queries beside them.  ``a_k`` and
     ``a_v`` are factors of the inputs (int8 inputs' steps); ``a_q`` is one over the step of int8 queries (for int8 inputs, their step
-    over it), or a factor of those in ``query_dtype`` fp16 or bf16."""
+    over it), or a factor of those in ``query_dtype`` fp16 or bf16 (int8 inputs' step)."""
 
     def __init__(self, alpha_k=1.0, alpha_v=1.0, alpha_q=1.0, neighbours=False, query_dtype=torch.int8):
         super().__init__()
@@ -79,11 +79,12 @@ class PagedKVAppend_S4(ScalarCacheMixin, torch.nn.Module):
                                            self.query_dtype, query_out)
 
     @staticmethod
-    def from_scale(q_scale=None, k_input_scale=1.0, v_input_scale=1.0, neighbours=False, query_dtype=torch.float16):
-        """From the step of int8 queries (without one they are made in ``query_dtype``) and, for int8 keys and values, their inputs'."""
+    def from_scale(q_scale=None, k_input_scale=1.0, v_input_scale=1.0, neighbours=False, query_dtype=torch.float16, q_input_scale=1.0):
+        """From the step of int8 queries (without one they are made in ``query_dtype``) and, for int8 keys, values and queries, their
+        inputs'."""
         mod = PagedKVAppend_S4(neighbours=neighbours, query_dtype=query_dtype if q_scale is None else torch.int8)
         mod.a_k, mod.a_v = _as_tensor(k_input_scale), _as_tensor(v_input_scale)
-        mod.a_q = _as_tensor(1.0 if q_scale is None else 1.0 / q_scale)
+        mod.a_q = _as_tensor(q_input_scale if q_scale is None else q_input_scale / q_scale)
         return mod
 
 
