@@ -103,6 +103,12 @@ __device__ __forceinline__ v8h query8(const void* q, int type, long long at) {
         w[i] = __builtin_bit_cast(unsigned, __builtin_convertvector(y, v2h));
       }
     }
+    // an infinity becomes NaN: scores of minus infinity alone would make a row that has seen no key
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const v2h y = __builtin_bit_cast(v2h, w[i]);
+      w[i] = __builtin_bit_cast(unsigned, y + (y - y));
+    }
   }
   return join8(__builtin_bit_cast(v2h, w[0]), __builtin_bit_cast(v2h, w[1]), __builtin_bit_cast(v2h, w[2]), __builtin_bit_cast(v2h, w[3]));
 }
