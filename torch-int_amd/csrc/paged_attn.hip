@@ -692,23 +692,32 @@ __global__ __launch_bounds__(PA_THREADS, DP == 64 ? 3 : 2) void paged_attn_both_
   __shared__ __attribute__((aligned(16))) char lds[tiles_lds(DP) > rows_lds(DP) ? tiles_lds(DP) : rows_lds(DP)];
   if (a.fill) paged_fill(b, b.cu[0], b.cu[b.seqs], static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
   const int i = blockIdx.x, each = (rows.slots < tiles.slots ? rows.slots : tiles.slots) & -TURN, rest = i - 2 * each;
-  const bool many = rest < 0 ? (i & TURN) == 0 : rest < tiles.slots - each;
-  const int index = rest < 0 ? i / (2 * TURN) * TURN + i % TURN : each + rest - (many ? 0 : tiles.slots - each);
+  bool many = rest < 0 ? (i & TURN) == 0 : rest < tiles.slots - each;
+  int index = rest < 0 ? i / (2 * TURN) * TURN + i % TURN : each + rest - (many ? 0 : tiles.slots - each);
+  if (b.seqs == 1) many = paged_seq(b, c.page_shift, 0).T * rows.group > PA_ROWS, index = i;  // of one kind
   if (many) paged_tiles<DP, OUT>(a, c, b, tiles, index, lds);
   else paged_rows<DP, OUT>(a, c, b, rows, index, lds);
 }
 
 // Joins slices that do not meet in the launch itself: an item that was cut to ROWS / EACH workgroups, EACH of its rows to one.
 // Eight items take turns, so that what there is to join comes first and goes to all CUs, and that an item whose number leaves the
-// same rest by 8 as its slices' (as where key heads come in eights) is read by the XCD that has written it.
+// same rest by 8 as its slices' (as where key heads come in eights) is read by the XCD that has written it.  The many rows' slices
+// are joined by the first `tile_blocks` workgroups, the few rows' by the others.
+constexpr int PA_JOIN = 2;
 template <int ROWS, int EACH, int DP, int OUT>
-__global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan p) {
-  __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
+__device__ __forceinline__ void paged_join(const PagedAttn& a, const PagedCache& c, const PagedBatch& b, const PagedPlan& p, int block, float* meet) {
   constexpr int PIECES = ROWS / EACH;
-  const PagedItem it = paged_item<ROWS == PT_ROWS ? PT_PARTS : 1, true>(b, c.page_shift, c.heads, ROWS, p,
-                                                                                 blockIdx.x / (8 * PIECES) * 8 + blockIdx.x % 8);
+  const PagedItem it = paged_item<ROWS == PT_ROWS ? PT_PARTS : 1, true>(b, c.page_shift, c.heads, ROWS, p, block / (8 * PIECES) * 8 + block % 8);
   if (!it.found || it.split != 0) return;
-  join_slices<ROWS, EACH, DP, OUT, false>(paged_out(a, c), p, it, meet, blockIdx.x / 8 % PIECES * EACH);
+  join_slices<ROWS, EACH, DP, OUT, false>(paged_out(a, c), p, it, meet, block / 8 % PIECES * EACH);
+}
+template <int DP, int OUT>
+__global__ __launch_bounds__(PA_THREADS) void paged_attn_join_kernel(PagedAttn a, PagedCache c, PagedBatch b, PagedPlan rows, PagedPlan tiles,
+                                                                     int tile_blocks) {
+  __shared__ __attribute__((aligned(16))) float meet[PA_THREADS * 8];
+  const int block = blockIdx.x;
+  if (block < tile_blocks) paged_join<PT_ROWS, PT_JOIN, DP, OUT>(a, c, b, tiles, block, meet);
+  else paged_join<PA_ROWS, PA_JOIN, DP, OUT>(a, c, b, rows, block - tile_blocks, meet);
 }
 
 // What a call of these sizes runs.  The lengths are on the device, so the grids and the workspace are bounds.  The grid: one item to
@@ -748,14 +757,17 @@ static PagedShape paged_shape(long long rows, long long seqs, long long group, l
   const long long many = rows * group / (PA_ROWS + 1) < seqs ? rows * group / (PA_ROWS + 1) : seqs;
   s.tiles_slots = heads * (many + rows * group / PT_ROWS);
   const bool cut_tiles = cut && s.tiles_slots < PT_PLENTY;
-  if (seqs == 1) {  // it has more than 16
+  s.rows_slots = heads * seqs;
+  // One sequence is of one kind or the other, which only the device knows: rows can be nobody's, as behind a recorded step (a token over
+  // 100000 keys and 2 such rows, 16 heads on 1: 25 us, and 146 when one sequence always went to the tiles, in 16 workgroups).
+  if (seqs == 1) {
     if (cut_tiles) s.cut_tiles(PA_TARGET);
+    if (cut) s.cut_rows(PA_TARGET, PA_ROWS);
     return s;
   }
   // Where both kinds share the chip, a place on each CU for the tiles, and few cuts for the others, which have the time: 512 rows over
   // 600 to 2007 keys beside 31 sequences of one row took 58.8 us with 512 slices of each kind, 48.3 with 256 of each, 44.4 with
   // 256 of tiles and 128 of the others.
-  s.rows_slots = heads * seqs;
   if (cut_tiles) s.cut_tiles(PA_TARGET / 2);
   if (cut) s.cut_rows(PA_TARGET / 4, PA_ROWS);
   return s;
@@ -770,13 +782,16 @@ long long paged_attn_arrivals(long long rows, long long seqs, long long q_heads,
 long long paged_attn_workspace_bytes(long long rows, long long seqs, long long q_heads, long long heads, long long D,
                                      long long capacity) {
   const PagedShape s = paged_shape(rows, seqs, q_heads / heads, heads, capacity);
-  return (s.rows_target ? paged_bytes(s.rows_places, PA_ROWS, D) : 0) + (s.tiles_target ? paged_bytes(s.tiles_places, PT_ROWS, D) : 0);
+  const long long few = s.rows_target ? paged_bytes(s.rows_places, PA_ROWS, D) : 0;
+  const long long many = s.tiles_target ? paged_bytes(s.tiles_places, PT_ROWS, D) : 0;
+  return seqs > 1 ? few + many : few > many ? few : many;  // (one sequence is of one kind)
 }
 
 template <int DP, int OUT>
 static void launch_attn(const PagedAttn& a, const PagedCache& c, const PagedBatch& b, const PagedPlan& rows, const PagedPlan& tiles,
                         hipStream_t stream) {
-  const unsigned grid = (unsigned)(rows.slots + tiles.slots > 0 ? rows.slots + tiles.slots : 1);
+  const int slots = b.seqs != 1 ? rows.slots + tiles.slots : rows.slots < tiles.slots ? tiles.slots : rows.slots;
+  const unsigned grid = (unsigned)(slots > 0 ? slots : 1);
   if (tiles.slots > 0)
     hipLaunchKernelGGL((paged_attn_both_kernel<DP, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows, tiles);
   else
@@ -786,12 +801,11 @@ static void launch_attn(const PagedAttn& a, const PagedCache& c, const PagedBatc
     const int most = p.slots - p.target - 8;
     return (unsigned)((most < p.target ? most : p.target) + 7 & ~7);
   };
-  if (rows.target > 0 && rows.arrivals == nullptr)
-    hipLaunchKernelGGL((paged_attn_join_kernel<PA_ROWS, 2, DP, OUT>), dim3(items(rows) * (PA_ROWS / 2)), dim3(PA_THREADS), 0,
-                       stream, a, c, b, rows);
-  if (tiles.target > 0)
-    hipLaunchKernelGGL((paged_attn_join_kernel<PT_ROWS, PT_JOIN, DP, OUT>), dim3(items(tiles) * (PT_ROWS / PT_JOIN)), dim3(PA_THREADS),
-                       0, stream, a, c, b, tiles);
+  const unsigned row_blocks = rows.target > 0 && rows.arrivals == nullptr ? items(rows) * (PA_ROWS / PA_JOIN) : 0;
+  const unsigned tile_blocks = tiles.target > 0 ? items(tiles) * (PT_ROWS / PT_JOIN) : 0;
+  if (row_blocks + tile_blocks > 0)
+    hipLaunchKernelGGL((paged_attn_join_kernel<DP, OUT>), dim3(row_blocks + tile_blocks), dim3(PA_THREADS), 0, stream, a, c, b, rows, tiles,
+                       (int)tile_blocks);
 }
 
 int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, const PagedBatch& b, void* workspace,
@@ -824,7 +838,7 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
   tiles.slots = (int)s.tiles_slots;
   tiles.places = (int)s.tiles_places;
   tiles.target = s.tiles_target;
-  tiles.ws = reinterpret_cast<float*>(ws + (s.rows_target ? paged_bytes(s.rows_places, PA_ROWS, c.D) : 0));
+  tiles.ws = reinterpret_cast<float*>(ws + (s.rows_target && b.seqs > 1 ? paged_bytes(s.rows_places, PA_ROWS, c.D) : 0));
   tiles.arrivals = nullptr;  // slices of 66 KB: many workgroups join them, in a launch of their own
   auto run = [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
