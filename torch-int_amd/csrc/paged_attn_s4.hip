@@ -947,8 +947,9 @@ __global__ __launch_bounds__(PA_THREADS, 2) void paged_attn_s4_both_kernel(Paged
   __shared__ __attribute__((aligned(16))) char lds[s4_tiles_lds(DP) > s4_rows_lds(DP) ? s4_tiles_lds(DP) : s4_rows_lds(DP)];
   if (a.fill) paged_fill(b, b.cu[0], b.cu[b.seqs], static_cast<char*>(a.out), (long long)a.q_heads * c.D * (OUT == PT_S8 ? 1 : 2));
   const int i = blockIdx.x, each = (rows.slots < tiles.slots ? rows.slots : tiles.slots) & -S4_TURN, rest = i - 2 * each;
-  const bool many = rest < 0 ? (i & S4_TURN) == 0 : rest < tiles.slots - each;
-  const int index = rest < 0 ? i / (2 * S4_TURN) * S4_TURN + i % S4_TURN : each + rest - (many ? 0 : tiles.slots - each);
+  bool many = rest < 0 ? (i & S4_TURN) == 0 : rest < tiles.slots - each;
+  int index = rest < 0 ? i / (2 * S4_TURN) * S4_TURN + i % S4_TURN : each + rest - (many ? 0 : tiles.slots - each);
+  if (b.seqs == 1) many = paged_seq(b, c.page_shift, 0).T * rows.group > PA_ROWS, index = i;  // of one kind
   if (many) s4_tiles<DP, GROUPS, OUT>(a, c, b, tiles, index, lds);
   else s4_rows<DP, GROUPS, OUT>(a, c, b, rows, index, lds);
 }
@@ -991,7 +992,7 @@ constexpr int S4_FEW_MEAN = 48;
 
 // Sequences of a batch of the other kind up to which those of few rows are cut into S4_TARGET slices as well; of more, into 128, since
 // they share the chip with tiles.  So few can be all there is, the rest being rows of nobody behind a recorded step: one token over 200000
-// keys and 3 such rows, 16 heads on 1, 35 us, 349 when one sequence went to the tiles; 4 tokens over 50000 and 30 rows, 64 on 8, 70 us, 123
+// keys and 3 such rows, 16 heads on 1, 32 us, 349 when one sequence went to the tiles; 4 tokens over 50000 and 30 rows, 64 on 8, 70 us, 123
 // in 128 slices; 8 over 20000 and 50 rows 58 and 101.  Beside a chunk over 20000 keys, 32 heads on 8, it pays
 // for 7 single tokens too (chunks of 100, 512 and 2000 tokens 129, 253 and 776 us; 185, 315 and 776), for 15 it depends (900 tokens 424 and
 // 472, 2500 tokens 1012 and 991).
@@ -1058,7 +1059,8 @@ long long paged_attn_s4_workspace_bytes(long long rows, long long seqs, long lon
 template <int DP, int GROUPS, int OUT>
 static void launch_s4(const PagedAttn4& a, const PagedCache4& c, const PagedBatch& b, const S4Shape& s, const PagedPlan& rows,
                       const PagedPlan& tiles, hipStream_t stream) {
-  const unsigned grid = (unsigned)(rows.slots + tiles.slots > 0 ? rows.slots + tiles.slots : 1);
+  const int slots = b.seqs != 1 ? rows.slots + tiles.slots : rows.slots < tiles.slots ? tiles.slots : rows.slots;
+  const unsigned grid = (unsigned)(slots > 0 ? slots : 1);
   if (tiles.slots > 0)
     hipLaunchKernelGGL((paged_attn_s4_both_kernel<DP, GROUPS, OUT>), dim3(grid), dim3(PA_THREADS), 0, stream, a, c, b, rows, tiles);
   else
