@@ -450,9 +450,12 @@ __device__ __forceinline__ void paged_tiles(const PagedAttn& a, const PagedCache
       const float scale = first && moves ? 0.0f : __builtin_amdgcn_exp2f(-by);
       off = !moves ? off : first ? __builtin_fmaf(-top, cl, 8.0f) : off - by;
       den *= scale;
-      const _Float16 scale_h = (_Float16)scale;
+      // (in two steps: a probability of 2^8 to 2^15 is still one of fp16 where it is to become less than 2^-16, the factor for it, below
+      // 2^-24, is not)
+      const float part = by < 24.0f ? by : 24.0f;
+      const _Float16 scale_1 = (_Float16)__builtin_amdgcn_exp2f(-part), scale_2 = (_Float16)__builtin_amdgcn_exp2f(part - by);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) before[q] *= scale_h;
+      for (int q = 0; q < 2; ++q) before[q] = before[q] * scale_1 * scale_2;
 #pragma unroll
       for (int i = 0; i < NDB; ++i) acc[i] *= scale;
     }
