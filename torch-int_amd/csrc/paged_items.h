@@ -104,18 +104,23 @@ __device__ __forceinline__ int paged_slice(float items, float total, int target,
 // of workgroups least in vain.  A workgroup costs some 170 keys before and behind its own, one that is joined some 700.  Over the 4-bit cache, so and cut
 // into `target` parts as above: 1536 rows over 6000 keys, 32 heads, 212 and 226 us; 700 over 13000, 28 heads on 4, 195 and 210; 300 rows and 31
 // tokens over 600 to 2007, 32 heads on 8, 49.5 and 58; but 64 rows over 8000 53.7 and 51.8, 4 x 1000 rows over 4000 to 16000 931 and 847: of
-// unequal items the longest ends last.  Those are cut into `target` parts, but none of fewer keys than make one round of all, nor of 2048:
-// slices of at least 1024, 2048 and 4096 keys take 3 x 400 rows over 1500 to 5000 keys 123, 115 and 164 us, 2 x 200 over 5000 to 30000 223,
-// 215 and 212; 16 x 24 rows over 500 to 4000 take 105 with 2048, 62 with a round's; 16 x 100 over 400 to 900 83 without any, 61 so.
+// unequal items the longest ends last (and of more than 64 x HELD sequences nobody looks whether they are).  Those are cut into `target`
+// parts, but none of fewer keys than make one round of all, nor of 2048: slices of at least 1024, 2048 and 4096 keys take 3 x 400 rows over
+// 1500 to 5000 keys 123, 115 and 164 us, 2 x 200 over 5000 to 30000 223, 215 and 212; 16 x 24 rows over 500 to 4000 take 105 with 2048, 62
+// with a round's; 16 x 100 over 400 to 900 83 without any, 61 so.
+// Of items that are alike too, more than 16 slices have 2048 keys or more, as a join reads them one after another: 4 tokens over 200000 keys, 16
+// heads on 1, 198 us, 289 with 1024, 375 with 16 slices at most; 32 tokens, 32 heads on 8, 237, 237 and 430; 8 x 40000, 16 on 1, 101, 98 and 112.
 __device__ __forceinline__ int paged_slice_even(float items, float total, int target, int at_once) {
   const float keys = total / __builtin_fmaxf(items, 1.0f);
   float best = __builtin_ceilf(items / (float)at_once) * (keys + 170.0f);
   float slice = 2.0f * keys;
-  for (int k = 2; k <= 16; ++k) {
-    const float n = items * (float)k;
-    if (n > (float)target || keys < (float)(k * PA_MIN_SLICE)) break;
-    const float cost = __builtin_ceilf(n / (float)at_once) * (keys / (float)k + 700.0f);
-    if (cost < best) best = cost, slice = keys / (float)k;
+  // as many as there can be: of 512 keys up to 16, of PA_LONG beyond
+  float most = __builtin_fmaxf(__builtin_fminf(keys / (float)PA_MIN_SLICE, 16.0f), keys / PA_LONG);
+  most = __builtin_fminf(most, (float)target / __builtin_fmaxf(items, 1.0f));
+  for (int rounds = 1; (rounds - 1) * at_once < target; ++rounds) {  // of all numbers that take as many rounds the largest costs least
+    const float k = __builtin_floorf(__builtin_fminf((float)(rounds * at_once) / items, most));
+    const float cost = __builtin_ceilf(items * k / (float)at_once) * (keys / k + 700.0f);
+    if (k >= 2.0f && cost < best) best = cost, slice = keys / k;
   }
   const int want = slice < 1.0e9f ? ((int)slice + 63) & ~63 : 1 << 30;
   return want < PA_MIN_SLICE ? PA_MIN_SLICE : want;
