@@ -718,9 +718,11 @@ int ti_paged_kv_read_s4(const TiPagedCacheS4* cache, const TiPagedBatch* batch, 
  * token of a call sees may hold anything, and their entries of the block table may be anything.
  * q of `q_type` (TI_TYPE_S8, TI_TYPE_F16, TI_TYPE_BF16; bf16 is computed with as fp16: beyond 65504 it is infinite, below 2^-14 its bits
  * get fewer), strides in elements, multiples of 16 bytes; alpha_qk in [1e-30, 1e4].  Scores, alpha_qk * q . k, are meant to stay below
- * 2^24, beyond which fp32 no longer tells them apart; a row whose query holds an infinity or a NaN has NaN (int8: 0), unless it sees nothing.  Products are exact
- * or fp32's; weights have 22 bits in sequences of up to 16 rows (tokens times q_heads / heads) and in batches of up to 48 to a sequence on
- * average (rows of no sequence counted), 11 bits in other sequences. */
+ * 2^24, beyond which fp32 no longer tells them apart; a row whose query holds an infinity or a NaN has NaN (int8: 0), unless it sees
+ * nothing.  Products are exact or fp32's; weights have 22 bits in sequences of up to 16 rows (tokens times q_heads / heads) and in
+ * batches of up to 48 to a sequence on average (rows of no sequence counted), 11 bits in other sequences.  Of the former each goes in
+ * times its value's step: where that is less than 2^-10 of the largest step among the keys that the 16 rows computed together see, a
+ * weight is off by 2^-32 of the row's largest weight times the largest step over its own, which can be more than 2^-22 of it. */
 typedef struct {
   const void* q;
   int64_t q_row, q_head, q_heads;

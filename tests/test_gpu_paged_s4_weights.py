@@ -99,3 +99,26 @@ def test_one_sequence_and_spare_rows(hq, hk, d, groups, n, new, pad, window, sin
     got = _attend((hq, hk, d, n, new, pad), q, caches, table, lens, cu, 2.0 / d ** 0.5, 1.0, window, sinks,
                   TWO_FP16 if new * hq <= 16 * hk else ONE_FP16, out_dtype=torch.bfloat16)
     assert (got[new:] == 0).all()
+
+
+@pytest.mark.parametrize("hq,hk,d,groups,lens,new", [(8, 2, 64, 2, [300], [2]), (16, 1, 128, 1, [3000, 90], [1, 1]), (4, 4, 96, 2, [200], [30])])
+@pytest.mark.parametrize("powers", [3, 10, 14, 17])
+def test_values_of_larger_steps_beside_take_bits_that_are_stated(powers, hq, hk, d, groups, lens, new):
+    # a light key in front of the others whose values' step is 2^powers of theirs: a weight is off by 2^-22 of itself, or by 2^-32 of the
+    # largest weight times that, which here is as large as all the others but for some powers of two
+    P = _paged()
+    (q, caches, table, lens_t, cu), wants = _cancelling(torch.Generator().manual_seed(powers), hq, hk, d, groups, lens, new, 64)
+    heavy = 64
+    for b in range(len(lens)):
+        at = heavy // 2           # behind the first heavy keys
+        caches[3][int(table[b, at // 16]), :, at % 16] = data.word(data.V_STEP * 2.0 ** (powers - 10))
+        pos = [j for j in range(lens[b]) if j != at]
+        for j in pos:
+            caches[3][int(table[b, j // 16]), :, j % 16] = data.word(data.V_STEP * 2.0 ** -10)
+    got = P.paged_attn_s4(q.to(DEV), *_device(caches), table.to(DEV), lens_t.to(DEV), cu.to(DEV), data.ALPHA, 1024.0, out_dtype=torch.float16).cpu()
+    for mine, (want, size, most) in wants:
+        # (scores are within 2^(3 * 16 * 15 / 256) = 2^2.9 of one another, so the sum of weights is 64 / 2^2.9 of the largest at least)
+        error = max(TWO_FP16, 2.0 ** -32 * 2.0 ** powers * 2.0 ** 2.9)
+        worst = orc.attention_error(got[mine], want, size, most, heavy, error)
+        print("steps", powers, hq, d, "error over its bound", worst, flush=True)
+        assert worst <= 1.0

@@ -136,7 +136,9 @@ struct S4Span {
 // the steps are multiplied into scores and weights:
 //   q . k = s sum q (u - z),   sum_j p_j v_j = sum_j (p_j s_j) (u_j - z_j),
 // where the weights p s go in as two fp16 numbers (22 bits).  Two groups have sums and weights of their own.  Steps reach from 2^-20
-// to 2^13, so the reference M keeps p times the largest step of the keys so far at 2^15 or less.
+// to 2^13, so the reference M keeps p times the largest step of the keys so far at 2^15 or less, and the row's largest p times it at 2^8 or
+// more.  The second fp16 number ends at 2^-24, so p is off by 2^-32 of the largest p times the largest step over its own at most: more
+// than 22 bits' worth where a heavy key's step is 2^-10 of the largest or less.
 // (Codes as they are, subnormal fp16 numbers u 2^-24, and z times the sums of q and of weights taken off behind the products
 // would be a fifth less to issue, but the matrix pipe adds subnormal numbers with 2^-20 of their sum lost.)
 // One token to each of 28 sequences of 1500 keys, 40 heads of 128: 39 us, 3.4 TB/s; 75 of up to 7003, 32 heads on 8: 75 us, 3.9 TB/s;
@@ -497,10 +499,12 @@ __device__ __forceinline__ void s4_rows(const PagedAttn4& a, const PagedCache4& 
 // A step is two halves of 32 keys with a barrier behind each.  The instructions of a half are laid out as bundles of one matrix
 // instruction and what fits beside it: the scores of the next half and the sums of the one before are on their way while this one's
 // become weights and the next step's codes numbers.  1536 rows over 12288 keys, 32 heads on 8: 448 us with one after the other, 397 so,
-// 715 TFLOP/s.  Two workgroups to a CU fill the LDS and the registers; of the time the matrix pipe is busy for 28 %, the vector ALUs for 43, the
-// LDS for 29, and what bounds it is issue.
-// A weight is one fp16 number, 11 bits: a second one would be 16 matrix instructions more to the 32 of a step, and the sum of the
-// rounding errors, at most 2^-11 of sum w |v| / sum w, is no more than what rounding such an output to fp16 costs, an eighth of what bf16 does.
+// 712 TFLOP/s.  Two workgroups to a CU fill the LDS and the registers; the matrix pipe is busy for 32 % of the clocks, the vector ALUs for 49, 8
+// are LDS conflicts, and what bounds it is issue.
+// A weight is one fp16 number, 11 bits: a second one would be 16 matrix instructions more to the 32 of a step.  A context is off by 2^-11 of
+// sum w |v| / sum w at most, by far less where many keys count, as their errors are independent: against 64 bits, 3 x 700 tokens of normal
+// values, 40 heads, fp16 out, by 0.00024 of its norm, of which rounding the output alone is 0.00021; bf16 out 0.0017 with and without.
+// Where values cancel it can be more than the output's rounding, which is 2^-11 of what is left of them.
 constexpr int ST_ROWS = 128, ST_KEYS = 64;
 constexpr int ST_PARTS = 4;
 constexpr int ST_JOIN = 32;      // rows that a workgroup joins
@@ -985,9 +989,12 @@ constexpr int S4_TARGET = 768;
 
 // Rows to a sequence, on average, up to which all of a batch go to the kernel of 16 rows: it reads a sequence's keys once for every 16,
 // but starts sooner, spreads further and has three or four waves to a SIMD.  All by it, and by tiles: 16 sequences of 500 to 4000 keys, 32
-// heads on 8, 8 tokens each (32 rows) 28 and 55 us, 12 (48) 32 and 58, 16 (64) 38 and 59.  A batch whose average is a chunk among single tokens
-// loses less than that: 250, 500 and 900 tokens beside 60 single ones (21, 37, 63 rows on average) 79, 106 and 147, and 92, 97 and 121 by
-// both.
+// heads on 8, 8 tokens each (32 rows) 28 and 55 us, 12 (48) 32 and 58, 16 (64) 38 and 59.  A chunk among single tokens, which this sends to the
+// same kernel, gains where it is short or its keys are few, and loses otherwise: all by this kernel, and by both, 32 heads on 8, 250 and 500
+// tokens beside 60 over up to 3000 keys 73 and 105 us, and 87 and 97, 512 beside 63 over 2000, 6000 and 12000 80, 199 and 379, and 84, 168 and 288;
+// own keys, 40 heads, 700 beside 31 over 2000, 6000 and 12000 119, 319 and 638, and 137, 293 and 519; 32 heads, 300 beside 15 over 4000 and 13000 91
+// and 262, and 101 and 242, 700 beside 15 146 and 448, and 130 and 345.  A line that also knows the longest sequence would take the better of
+// the two; the host knows no lengths.
 constexpr int S4_FEW_MEAN = 48;
 
 // Sequences of a batch of the other kind up to which those of few rows are cut into S4_TARGET slices as well; of more, into 128, since

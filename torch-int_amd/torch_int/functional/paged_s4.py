@@ -244,10 +244,11 @@ def paged_attn_s4(query, k_cache, v_cache, k_scale, v_scale, block_table, contex
     layer behind it).  A token that sees nothing gets zeros; rows of no sequence are zeros too, or left as they are in an ``out``
     that is handed in, which must not share memory with the inputs.  ``alpha_qk`` is from 1e-30 to 1e4.
 
-    Keys, values and queries are computed with as they are (bf16 queries as fp16), sums and softmax in fp32.
+    Keys, values and queries are computed with as they are, but for bf16 queries, which become fp16 (infinite beyond 65504, with fewer
+    bits below 2^-14); sums and softmax are fp32.  A query that holds an infinity or a NaN gives NaN (0 in int8), in its own row and head.
     Weights have 22 bits in sequences of up to 16 rows (new tokens times ``q_heads // heads``) and, as long as ``query`` has no more
-    than 48 to a sequence on average (rows of no sequence counted), in all; longer sequences of other batches have weights of 11
-    bits.  The same batch gives the same bits on any stream and in a recorded graph; beside other sequences the last bits of a
+    than 48 to a sequence on average (rows of no sequence counted), in all, some fewer beside values of more than 2^10 times their
+    step (``include/torch_int_hip.h``); longer sequences of other batches have weights of 11 bits.  The same batch gives the same bits on any stream and in a recorded graph; beside other sequences the last bits of a
     token's context can differ."""
     op = "paged_attn_s4"
     q_code = _QUERIES.get(query.dtype) if isinstance(query, torch.Tensor) else None
