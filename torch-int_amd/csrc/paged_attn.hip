@@ -819,8 +819,8 @@ int launch_paged_attn_s8(int out_type, const PagedAttn& a, const PagedCache& c, 
   PagedShape s = paged_shape(b.rows, b.seqs, group, c.heads, capacity);
   if (workspace == nullptr || workspace_bytes < paged_attn_workspace_bytes(b.rows, b.seqs, a.q_heads, c.heads, c.D, capacity))
     s.rows_target = s.tiles_target = 0, s.rows_meet = false;
-  if (s.rows_slots + s.tiles_slots > 0x7fffff)
-    return fail(TI_ERR_INVALID_ARG, "paged_attn_s8: %lld work items", s.rows_slots + s.tiles_slots);
+  const long long items = b.seqs != 1 ? s.rows_slots + s.tiles_slots : s.rows_slots < s.tiles_slots ? s.tiles_slots : s.rows_slots;
+  if (items > 0x7fffff) return fail(TI_ERR_INVALID_ARG, "paged_attn_s8: %lld work items", items);
   const bool meet = a.arrivals != nullptr && a.arrivals_count >= paged_attn_arrivals(b.rows, b.seqs, a.q_heads, c.heads, capacity);
   char* ws = static_cast<char*>(workspace);
   PagedPlan rows, tiles;

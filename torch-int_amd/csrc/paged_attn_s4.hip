@@ -1090,8 +1090,8 @@ int launch_paged_attn_s4(int out_type, const PagedAttn4& a, const PagedCache4& c
   const long long rows_bytes = s4_bytes(s.rows, PA_ROWS, c.D);
   if (workspace == nullptr || workspace_bytes < rows_bytes + s4_bytes(s.tiles, ST_ROWS, c.D))
     s.rows.target = s.tiles.target = 0, s.meet = false;
-  if (s.rows.slots + s.tiles.slots > 0x7fffff)
-    return fail(TI_ERR_INVALID_ARG, "paged_attn_s4: %lld work items", s.rows.slots + s.tiles.slots);
+  const long long items = b.seqs != 1 ? s.rows.slots + s.tiles.slots : s.rows.slots < s.tiles.slots ? s.tiles.slots : s.rows.slots;
+  if (items > 0x7fffff) return fail(TI_ERR_INVALID_ARG, "paged_attn_s4: %lld work items", items);
   auto plan = [&](const S4Kind& k, int rows_of_item, int least, int most, char* ws) {
     PagedPlan p;
     p.group = group;
