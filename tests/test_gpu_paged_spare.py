@@ -48,3 +48,38 @@ def test_one_sequence_and_spare_rows(hq, hk, d, n, new, pad):
     got = _attend((hq, hk, d, n, new, pad), _s8(g, rows, hq, d, spread=30), k, v, table, lens, cu, 2.0 / (900 * d ** 0.5), 0.02,
                   EXACT_WEIGHTS if new * hq <= 16 * hk else FP16_WEIGHTS, out_dtype=torch.bfloat16)
     assert (got[new:] == 0).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_recorded_step_of_one_sequence_is_of_either_kind_when_it_replays(bits):
+    # 40 rows, of which a replay's sequence has one, some or all: eager calls, two graphs and their replays in turn
+    g = torch.Generator().manual_seed(bits)
+    rows, hq, hk, d, page, per = 40, 8, 1, 128, 16, 400
+    table = torch.randperm(per, generator=g).int().view(1, per).to(DEV)
+    lens, cu = torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
+    q = _s8(g, rows, hq, d, spread=30).to(DEV)
+    if bits == 8:
+        k, v = (_s8(g, per, hk, page, d, spread=30).to(DEV) for _ in range(2))
+        step = lambda: _paged().paged_attn_s8(q, k, v, table, lens, cu, 2e-4, 0.02, out_dtype=torch.float16)  # noqa: E731
+    else:
+        from tests.test_gpu_paged_s4 import _cache, _device
+        from torch_int.functional import paged_s4
+        pools = _device(_cache(g, per, hk, page, d, 2))
+        step = lambda: paged_s4.paged_attn_s4(q, *pools, table, lens, cu, 6e-3)  # noqa: E731
+    step()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out))
+    for n, new in ((6000, 1), (6000, 40), (700, 2), (6400, 3), (40, 40), (5000, 0), (6399, 17), (1, 1)):
+        lens.fill_(n)
+        cu[1] = new
+        want = step()
+        torch.cuda.synchronize()
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert (want[new:] == 0).all() and all(torch.equal(out, want) for _, out in graphs), (n, new)
+        assert bool(want[:new].any()) or new == 0
